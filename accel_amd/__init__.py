@@ -109,6 +109,26 @@ class Selection:
 
 SELECT_BIAS, SELECT_BF16_OUT = 1, 2
 
+KV_NONE = 0xffffffff
+
+
+class KVCacheDesc(ctypes.Structure):
+    """accel_kv_cache_t."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+                ("refs", ctypes.c_void_p), ("tables", ctypes.c_void_p),
+                ("lens", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("layers", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("sequences", ctypes.c_int64),
+                ("slots", ctypes.c_int64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """accel_attention_t."""
+    _fields_ = [("scale", ctypes.c_float), ("window", ctypes.c_int64),
+                ("sinks", ctypes.c_int64)]
+
+
 QFMT_AWQ, QFMT_GPTQ, QFMT_GPTQ_V2 = 1, 2, 3
 
 
@@ -199,6 +219,20 @@ SIGNATURES = {
     "accel_swiglu": ([_i, _vp, _P(Tensor), _P(Tensor), _P(Tensor)], _i),
     "accel_rmsnorm": ([_i, _vp, _P(Tensor), _P(Tensor), ctypes.c_float, _P(Tensor)], _i),
     "accel_matvec_f32_f16": ([_i, _vp, _P(Tensor), _P(Tensor), _P(Tensor)], _i),
+    "accel_kv_clear": ([_i, _vp, _P(KVCacheDesc)], _i),
+    "accel_kv_reserve": ([_i, _vp, _P(KVCacheDesc), _P(Tensor), _P(Tensor)], _i),
+    "accel_kv_append": ([_i, _vp, _P(KVCacheDesc), ctypes.c_int64, _P(Tensor), _P(Tensor),
+                         _P(Tensor), _P(Tensor)], _i),
+    "accel_kv_fork": ([_i, _vp, _P(KVCacheDesc), _P(Tensor), _P(Tensor)], _i),
+    "accel_kv_trim": ([_i, _vp, _P(KVCacheDesc), _P(Tensor), ctypes.c_int64, ctypes.c_int64],
+                      _i),
+    "accel_kv_free": ([_i, _vp, _P(KVCacheDesc), _P(Tensor)], _i),
+    "accel_kv_compact": ([_i, _vp, _P(KVCacheDesc), _P(Tensor)], _i),
+    "accel_kv_copy": ([_i, _vp, _P(KVCacheDesc), _P(Tensor), _P(Tensor)], _i),
+    "accel_paged_attention": ([_i, _vp, _P(Tensor), _P(KVCacheDesc), ctypes.c_int64, _P(Tensor),
+                               _P(AttentionDesc), _P(Tensor)], _i),
+    "accel_paged_prefill": ([_i, _vp, _P(Tensor), _P(Tensor), _P(KVCacheDesc), ctypes.c_int64,
+                             _P(Tensor), _P(AttentionDesc), _P(Tensor)], _i),
     "accel_quant_matmul": ([_i, _vp, _P(Tensor), _P(Tensor), _P(Tensor), _P(Tensor)], _i),
     "accel_int8_quantize": ([_vp, ctypes.c_int64, _vp, _vp], _i),
     "accel_int8_dequantize": ([_vp, _vp, ctypes.c_int64, _vp], _i),
@@ -469,6 +503,47 @@ class Int4Weights:
         for b in (self.codes, self.scales, self.zeros):
             if b:
                 b.free()
+
+
+@dataclass
+class KVCache:
+    """accel_kv_cache_t over device buffers: keys and values [layers, pages,
+    kv_heads, page_size, head_dim] (F16 or BF16), refs u32 [pages], tables u32
+    [sequences, slots], lens u32 [sequences].  Device.kv_cache allocates one."""
+    device: "Device"
+    keys: Buffer
+    values: Buffer
+    refs: Buffer
+    tables: Buffer
+    lens: Buffer
+
+    def __post_init__(self):
+        k = self.keys.shape
+        if len(k) != 5 or tuple(self.values.shape) != tuple(k) or \
+                self.values.dtype != self.keys.dtype:
+            raise ValueError(f"keys {k} and values {self.values.shape}: both are [layers, pages, "
+                             "kv_heads, page_size, head_dim] of one type")
+        t = self.tables.shape
+        if len(t) != 2 or tuple(self.refs.shape) != (k[1],) or \
+                tuple(self.lens.shape) != (t[0],) or \
+                any(b.dtype != U32 for b in (self.refs, self.tables, self.lens)):
+            raise ValueError(f"refs {self.refs.shape}, tables {t} and lens {self.lens.shape}: "
+                             f"u32 [{k[1]}], [sequences, slots] and [sequences]")
+        self._desc = KVCacheDesc(self.keys.ptr, self.values.ptr, self.refs.ptr, self.tables.ptr,
+                                 self.lens.ptr, self.keys.dtype, k[2], k[3], k[4], k[0], k[1],
+                                 t[0], t[1])
+
+    def desc(self) -> KVCacheDesc:
+        return self._desc
+
+    def free(self) -> None:
+        for b in (self.keys, self.values, self.refs, self.tables, self.lens):
+            b.free()
+
+
+def _opt(buffer):
+    """A buffer's tensor by reference, or NULL."""
+    return ctypes.byref(buffer.tensor()) if buffer is not None else None
 
 
 class Device:
@@ -807,6 +882,74 @@ class Device:
         tx, tg, to = x.tensor(), gain.tensor(), out.tensor()
         _check(_lib.accel_rmsnorm(self.index, stream, ctypes.byref(tx), ctypes.byref(tg),
                                   ctypes.c_float(eps), ctypes.byref(to)))
+
+    # ---- paged key-value cache and attention ----------------------------------
+    def kv_cache(self, layers: int, pages: int, kv_heads: int, page_size: int, head_dim: int,
+                 sequences: int, slots: int, dtype: int = BF16, stream=None) -> KVCache:
+        """Allocates a cache and clears it (accel_kv_clear)."""
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        c = KVCache(self, self.alloc(shape, dtype), self.alloc(shape, dtype),
+                    self.alloc((pages,), U32), self.alloc((sequences, slots), U32),
+                    self.alloc((sequences,), U32))
+        self.KVClear(c, stream)
+        return c
+
+    def KVClear(self, cache: KVCache, stream=None) -> None:
+        _check(_lib.accel_kv_clear(self.index, stream, ctypes.byref(cache.desc())))
+
+    def KVReserve(self, cache: KVCache, grow: Buffer, seqs: Buffer = None, stream=None) -> None:
+        """Pages for the positions sequences grow by (accel_kv_reserve)."""
+        _check(_lib.accel_kv_reserve(self.index, stream, ctypes.byref(cache.desc()), _opt(seqs),
+                                     _opt(grow)))
+
+    def KVAppend(self, cache: KVCache, layer: int, k: Buffer, v: Buffer, seqs: Buffer = None,
+                 offsets: Buffer = None, stream=None) -> None:
+        """New rows of keys and values at the sequences' last positions
+        (accel_kv_append)."""
+        _check(_lib.accel_kv_append(self.index, stream, ctypes.byref(cache.desc()), layer,
+                                    _opt(k), _opt(v), _opt(seqs), _opt(offsets)))
+
+    def KVFork(self, cache: KVCache, parents: Buffer, children: Buffer, stream=None) -> None:
+        """Branches of sequences that share their whole pages (accel_kv_fork)."""
+        _check(_lib.accel_kv_fork(self.index, stream, ctypes.byref(cache.desc()), _opt(parents),
+                                  _opt(children)))
+
+    def KVTrim(self, cache: KVCache, window: int, sinks: int = 0, seqs: Buffer = None,
+               stream=None) -> None:
+        """Gives back the pages behind a window (accel_kv_trim)."""
+        _check(_lib.accel_kv_trim(self.index, stream, ctypes.byref(cache.desc()), _opt(seqs),
+                                  window, sinks))
+
+    def KVFree(self, cache: KVCache, seqs: Buffer = None, stream=None) -> None:
+        """Empties sequences (accel_kv_free)."""
+        _check(_lib.accel_kv_free(self.index, stream, ctypes.byref(cache.desc()), _opt(seqs)))
+
+    def KVCompact(self, cache: KVCache, live: Buffer = None, stream=None) -> None:
+        """Moves the pages in use to the lowest numbers (accel_kv_compact)."""
+        _check(_lib.accel_kv_compact(self.index, stream, ctypes.byref(cache.desc()), _opt(live)))
+
+    def KVCopy(self, cache: KVCache, src: Buffer, dst: Buffer, stream=None) -> None:
+        """Copies pages in every layer (accel_kv_copy)."""
+        _check(_lib.accel_kv_copy(self.index, stream, ctypes.byref(cache.desc()), _opt(src),
+                                  _opt(dst)))
+
+    def PagedAttention(self, q: Buffer, cache: KVCache, out: Buffer, layer: int = 0,
+                       seqs: Buffer = None, scale: float = 0.0, window: int = 0, sinks: int = 0,
+                       stream=None) -> None:
+        """Attention of one new token a sequence (accel_paged_attention)."""
+        opt = AttentionDesc(scale, window, sinks)
+        _check(_lib.accel_paged_attention(self.index, stream, _opt(q),
+                                          ctypes.byref(cache.desc()), layer, _opt(seqs),
+                                          ctypes.byref(opt), _opt(out)))
+
+    def PagedPrefill(self, q: Buffer, offsets: Buffer, cache: KVCache, out: Buffer,
+                     layer: int = 0, seqs: Buffer = None, scale: float = 0.0, window: int = 0,
+                     sinks: int = 0, stream=None) -> None:
+        """Attention of the new tokens of prompts or chunks (accel_paged_prefill)."""
+        opt = AttentionDesc(scale, window, sinks)
+        _check(_lib.accel_paged_prefill(self.index, stream, _opt(q), _opt(offsets),
+                                        ctypes.byref(cache.desc()), layer, _opt(seqs),
+                                        ctypes.byref(opt), _opt(out)))
 
     def QuantMatMul(self, x: Buffer, quants: Buffer, scales: Buffer, out: Buffer,
                     stream=None) -> None:

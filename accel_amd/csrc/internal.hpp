@@ -23,6 +23,10 @@ void clear_error();
 // Bits of the device fault word: what a kernel reports when it gives up
 // instead of producing its result.
 constexpr uint32_t kFaultWaitGaveUp = 1u;     // a split-K hand-off's bounded wait ran out
+constexpr uint32_t kFaultKvRoom = 2u;         // no free page, or no slot left in a table
+constexpr uint32_t kFaultKvPage = 4u;         // no page where a position is read or written
+constexpr uint32_t kFaultKvSequence = 8u;     // a sequence or page index that cannot be served
+constexpr uint32_t kFaultKv = kFaultKvRoom | kFaultKvPage | kFaultKvSequence;
 
 // Per-device state: the open flag, sticky loss, fault injection, the
 // library-owned workspace and the fault word.
@@ -398,6 +402,52 @@ bool int4_ragged_shape(const void* a, const void* codes, int K, int N);
 bool int4_ragged_rows_supported(const void* a, const void* codes, int M, int K, int N);
 hipError_t launch_int4_ragged_rows(const Device* d, hipStream_t st, const void* a, bool bf16,
                                    Int4Planes w, void* out, int M, int K, int N, Epilogue ep);
+
+// The paged cache on the device (kvpages.hip, attention.hip): the arrays of
+// accel_kv_cache_t with the page size as a shift.
+struct KvCache {
+    uint16_t* keys;
+    uint16_t* values;
+    uint32_t* refs;
+    uint32_t* tables;
+    uint32_t* lens;
+    int64_t layers;
+    uint32_t pages, sequences, slots;
+    int heads, shift, dim;      // key-value heads; page size 1 << shift
+    bool bf16;
+    __host__ __device__ size_t page_elems() const { return ((size_t)heads << shift) * dim; }
+};
+hipError_t launch_kv_clear(hipStream_t st, const KvCache& c);
+hipError_t launch_kv_reserve(Device* d, hipStream_t st, const KvCache& c, const uint32_t* seqs,
+                             const uint32_t* grow, int n, int* status);
+hipError_t launch_kv_append(Device* d, hipStream_t st, const KvCache& c, int64_t layer,
+                            const void* k, const void* v, int32_t dtype, const uint32_t* seqs,
+                            const uint32_t* offsets, int n, int rows);
+hipError_t launch_kv_fork(Device* d, hipStream_t st, const KvCache& c, const uint32_t* parents,
+                          const uint32_t* children, int n, int* status);
+// Empties the sequences (window 0), or gives back the pages behind the window.
+hipError_t launch_kv_free(Device* d, hipStream_t st, const KvCache& c, const uint32_t* seqs,
+                          int n, int64_t window, int64_t sinks);
+hipError_t launch_kv_compact(Device* d, hipStream_t st, const KvCache& c, uint32_t* live,
+                             int* status);
+hipError_t launch_kv_copy(Device* d, hipStream_t st, const KvCache& c, const uint32_t* src,
+                          const uint32_t* dst, int n);
+
+// What an attention call sees and where it reads and writes.  q and out are
+// [rows, heads, dim]; q_f32: f32, else the cache's type.
+struct Attention {
+    const void* q;
+    void* out;
+    const uint32_t* seqs;      // [n] or null
+    const uint32_t* offsets;   // [n + 1], or null: one row an entry
+    int n, rows, heads;
+    int64_t layer;
+    bool q_f32;
+    float scale;
+    uint32_t window, sinks;    // window 0: all
+};
+hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
+                                  const Attention& a, int* status);
 
 // Device quantizer.
 hipError_t launch_int4_quantize(hipStream_t st, const float* w, int64_t n,

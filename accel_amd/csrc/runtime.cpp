@@ -183,6 +183,31 @@ int take_fault(Device* d) {
     if (!d->fault_host) return ACCEL_OK;
     const uint32_t f = __atomic_exchange_n(d->fault_host, 0u, __ATOMIC_ACQ_REL);
     if (!f) return ACCEL_OK;
+    const struct {
+        uint32_t bit;
+        const char* text;
+    } known[] = {
+        {kFaultWaitGaveUp, "a split-K hand-off's bounded wait gave up"},
+        {kFaultKvRoom, "a key-value pool had no free page, or a table no slot left"},
+        {kFaultKvPage, "a key-value table names no page for a position read or written"},
+        {kFaultKvSequence, "a sequence or page index cannot be served"},
+    };
+    char what[320] = "";
+    uint32_t rest = f;
+    for (const auto& k : known) {
+        if (!(f & k.bit)) continue;
+        rest &= ~k.bit;
+        const size_t at = strlen(what);
+        snprintf(what + at, sizeof what - at, "%s%s", at ? "; " : "", k.text);
+    }
+    if (rest) {
+        const size_t at = strlen(what);
+        snprintf(what + at, sizeof what - at, "%sunknown fault bits", at ? "; " : "");
+    }
+    if (!(f & ~kFaultKv))
+        return fail(ACCEL_E_HIP,
+                    "accel_hip: device fault word 0x%x (%s): the entries concerned were left out",
+                    f, what);
     // A kernel that gave up left its hand-off counters mid-way: wait for the
     // device, then clear the counters of every workspace.
     (void)hipDeviceSynchronize();
@@ -192,8 +217,6 @@ int take_fault(Device* d) {
         for (const auto& r : d->retired) (void)hipMemset(r.ptr, 0, kWorkspaceCounterBytes);
         if (d->scratch) (void)hipMemset(d->scratch, 0, kWorkspaceCounterBytes);
     }
-    const char* what = f == kFaultWaitGaveUp ? "a split-K hand-off's bounded wait gave up"
-                                              : "unknown fault bits";
     return fail(ACCEL_E_HIP,
                 "accel_hip: device fault word 0x%x (%s): the results of the work waited on "
                 "are undefined",

@@ -593,6 +593,136 @@ int accel_rmsnorm(int dev, void* stream, const accel_tensor_t* x,
 int accel_matvec_f32_f16(int dev, void* stream, const accel_tensor_t* x,
                          const accel_tensor_t* w, accel_tensor_t* out);
 
+/* ---- paged key-value cache and attention -------------------------------- */
+
+/* A table entry that names no page, and a sequence index that stands for a
+ * padded row of a batch. */
+#define ACCEL_KV_NONE 0xffffffffu
+
+/* The keys and values of a decoder's layers in pages, shared by sequences.
+ * Position p of sequence s is slot p % page_size of page
+ * tables[s][p / page_size]; one table serves every layer.  All of it is device
+ * memory that the caller owns; the operators below are the only ones that need
+ * to change refs, tables and lens.  An operator that changes them must not run
+ * beside another on the same cache. */
+typedef struct accel_kv_cache {
+    void* keys;          /* [layers, pages, kv_heads, page_size, head_dim], 16-byte aligned */
+    void* values;        /* the same */
+    uint32_t* refs;      /* [pages] table entries that name the page; 0: free */
+    uint32_t* tables;    /* [sequences, slots] pages, or ACCEL_KV_NONE */
+    uint32_t* lens;      /* [sequences] positions held */
+    int32_t dtype;       /* ACCEL_BF16 or ACCEL_F16 */
+    int32_t kv_heads;
+    int32_t page_size;   /* a power of two, 8 .. 4096 */
+    int32_t head_dim;    /* a multiple of 8, 8 .. 256 */
+    int64_t layers, pages, sequences, slots;
+} accel_kv_cache_t;
+
+/* What the kernels of this section find wrong on the device (a sequence index
+ * outside the cache, a pool without a free page, a table without a page where
+ * a position is read or written) reaches the host as the device's fault word,
+ * at the next wait (Faults above).  Nothing outside the cache's arrays is read
+ * or written for it: the sequence, row or key concerned is left out as said at
+ * each operator, and the others are served. */
+
+/* An empty cache: refs and lens 0, tables ACCEL_KV_NONE.  keys and values are
+ * left as they are: no operator reads a position that was not written. */
+int accel_kv_clear(int dev, void* stream, const accel_kv_cache_t* cache);
+
+/* Sequence seqs[i] (u32 [n]; NULL: i, n = sequences) grows by grow[i] (u32
+ * [n]) positions: its length, and a page for each slot of its table that they
+ * reach, the lowest free pages first, entry by entry in the list's order.  An
+ * entry for which the pool or the table has no room is left unchanged and
+ * reported, and so are the second of two entries with one sequence and a
+ * sequence index outside the cache; ACCEL_KV_NONE is skipped. */
+int accel_kv_reserve(int dev, void* stream, const accel_kv_cache_t* cache,
+                     const accel_tensor_t* seqs, const accel_tensor_t* grow);
+
+/* New rows of keys and values, k and v [T, kv_heads, head_dim] in f32, f16 or
+ * bf16 (rounded to the cache's type, nearest even), of `layer` (0 .. layers -
+ * 1): entry i's are rows [offsets[i], offsets[i+1]) and go to the last
+ * positions of sequence seqs[i], as accel_kv_reserve left its length.  offsets
+ * u32 [n+1], ascending from 0; NULL: one row an entry, n = T.  seqs u32 [n];
+ * NULL: i.  Rows past the last offset and rows of ACCEL_KV_NONE are skipped.
+ * A position before the sequence's first, or without a page, is skipped and
+ * reported. */
+int accel_kv_append(int dev, void* stream, const accel_kv_cache_t* cache, int64_t layer,
+                    const accel_tensor_t* k, const accel_tensor_t* v,
+                    const accel_tensor_t* seqs, const accel_tensor_t* offsets);
+
+/* Sequence children[i] becomes a branch of parents[i] (u32 [n] each): its
+ * length and its whole pages, shared (refs counts them once more), and where
+ * the last page is partly full a copy of it in every layer, in the lowest free
+ * pages in the list's order, so that both may append.  One parent may be named
+ * many times; a child has to be empty and named once.  An entry that breaks
+ * this, that names a sequence outside the cache or that finds no free page
+ * leaves its child empty and is reported; an entry with an ACCEL_KV_NONE is
+ * skipped.  Parents are read as they were before the call.  A parent's slot
+ * without a page (accel_kv_trim) has none in the branch. */
+int accel_kv_fork(int dev, void* stream, const accel_kv_cache_t* cache,
+                  const accel_tensor_t* parents, const accel_tensor_t* children);
+
+/* Gives back the pages of seqs (u32 [n]; NULL: all sequences) that no query at
+ * or after the sequence's last position sees with this window and these sinks
+ * (accel_attention_t; window >= 1): their entries become ACCEL_KV_NONE.  The
+ * length stays. */
+int accel_kv_trim(int dev, void* stream, const accel_kv_cache_t* cache,
+                  const accel_tensor_t* seqs, int64_t window, int64_t sinks);
+
+/* Empties seqs (u32 [n]; NULL: all sequences): every page given back, the row
+ * ACCEL_KV_NONE, the length 0.  A sequence named twice is emptied once. */
+int accel_kv_free(int dev, void* stream, const accel_kv_cache_t* cache,
+                  const accel_tensor_t* seqs);
+
+/* Moves the pages in use to the lowest numbers: with L pages in use, the pages
+ * at or past L that are in use move, in order, into the free ones below L, in
+ * order, in every layer; refs and tables follow.  live (u32 [1], or NULL)
+ * receives L. */
+int accel_kv_compact(int dev, void* stream, const accel_kv_cache_t* cache, accel_tensor_t* live);
+
+/* Copies page src[i] to page dst[i] (u32 [n] each) in every layer; refs and
+ * tables stay.  A pair with an ACCEL_KV_NONE is skipped; one with a page
+ * outside the cache is skipped and reported.  No page may be the target of two
+ * pairs, or of one and the source of another: what such a page receives is not
+ * specified. */
+int accel_kv_copy(int dev, void* stream, const accel_kv_cache_t* cache,
+                  const accel_tensor_t* src, const accel_tensor_t* dst);
+
+/* What a query sees.  The query at position p of a sequence sees the keys at
+ * positions j <= p with, where window is not 0, p - j < window or j < sinks. */
+typedef struct accel_attention {
+    float scale;      /* of a query's product with a key; 0: 1 / sqrt(head_dim) */
+    int64_t window;   /* positions seen, its own among them; 0: all */
+    int64_t sinks;    /* first positions that stay visible past the window */
+} accel_attention_t;
+
+/* Attention of one new token a sequence: row i of q [n, heads, head_dim] is
+ * the query at the last position of sequence seqs[i] (u32 [n]; NULL: i, n <=
+ * sequences), and out (q's shape and type) is sum_j softmax_j(scale * q . k_j)
+ * v_j over the keys of `layer` that it sees.  heads is a multiple of kv_heads;
+ * query head h reads key-value head h / (heads / kv_heads).  q is f32, or the
+ * cache's type; products, softmax and sums are f32 (f32 queries and weights
+ * are not rounded to the cache's type).  A query that sees no key (an empty
+ * sequence, ACCEL_KV_NONE) gives zeros.  A page missing where the query would
+ * see it is left out of the softmax and reported.  q and out 16-byte aligned.
+ * opt may be NULL (all zero). */
+int accel_paged_attention(int dev, void* stream, const accel_tensor_t* q,
+                          const accel_kv_cache_t* cache, int64_t layer,
+                          const accel_tensor_t* seqs, const accel_attention_t* opt,
+                          accel_tensor_t* out);
+
+/* The same for the new tokens of prompts, or of chunks of prompts: entry i's
+ * queries are rows [offsets[i], offsets[i+1]) of q [T, heads, head_dim], at the
+ * last positions of sequence seqs[i] (its length counts them; their keys and
+ * values are in the cache already).  offsets u32 [n+1], ascending from 0.  Rows
+ * past the last offset are left as they were.  For a 16-bit q the softmax
+ * weights are rounded to the cache's type before the product with the values
+ * (their sum is not). */
+int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q,
+                        const accel_tensor_t* offsets, const accel_kv_cache_t* cache,
+                        int64_t layer, const accel_tensor_t* seqs,
+                        const accel_attention_t* opt, accel_tensor_t* out);
+
 /* ---- int8 weights ------------------------------------------------------ */
 
 /* tensor.QuantMatMul (tensor/quantized.go:72-163): x f32 or f16 [M,K] times
