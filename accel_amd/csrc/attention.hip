@@ -5,36 +5,577 @@
 // m the largest score, over the keys j <= p with p - j < window or j < sinks
 // (all j <= p without a window).
 //
-// One workgroup a query row and head; the softmax's running maximum and sum
-// are carried over blocks of 256 keys, so the keys are read once.
+// One new token a sequence (paged_decode_kernel).  The bytes of the keys and
+// values bound it: each is read once, for all the query heads of its group.
+// A wave takes 32 keys at a time against up to 16 query heads as
+// S^T = K Q^T and O^T += V^T P^T on the matrix cores, everything in registers:
+//
+// - K goes from memory to the A operand as it is (a lane 16 bytes of one key a
+//   step).  Which key is which row is free, and is chosen so that a lane's
+//   eight scores (C layout: column = query, rows 4 (lane / 16) + i of two
+//   tiles) are eight consecutive keys: exactly its part of P^T's B operand.
+// - A lane loads V for those eight keys, DIM / 16 consecutive dims of each, and
+//   turns the block by byte permutes (half an instruction an element) into A
+//   operands with the eight keys along k; which dim is which row is free too.
+// - The running maximum is only moved when some score exceeds it by 2^8 (sums
+//   and weights stay far inside f32 and the 16-bit types' ranges), so most
+//   steps have no exchange between lanes.  A lane sums its own weights.
+//
+// Weights are split into two 16-bit terms (f32 queries: three bf16 or two f16
+// terms, queries too), so a 16-bit call rounds only its result and an f32 call
+// keeps 2^-22 of each; the matrix cores have the time.
+//
+// The work is cut evenly over the workgroups whatever the lengths: all tiles of
+// 32 keys of all (head, sequence) pairs in one line, a workgroup an equal
+// stretch of it, its four waves every fourth tile.  A pair that crosses
+// stretches is joined by the workgroup that finishes last, in the stretches'
+// order, so the result does not depend on the schedule.
 #include <hip/hip_runtime.h>
 
+#include "bf16split.hpp"
 #include "internal.hpp"
 #include "kvcache.hpp"
+#include "splitk.hpp"
 
 namespace accel {
 namespace {
 
-__device__ __forceinline__ float widen(uint16_t h, bool bf16) {
-    if (bf16) return __uint_as_float((uint32_t)h << 16);
-    _Float16 v;
-    __builtin_memcpy(&v, &h, 2);
-    return (float)v;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <bool BF16>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__global__ __launch_bounds__(256) void paged_attention_kernel(KvCache c, Attention a,
-                                                              uint32_t* fault) {
+// Two f32 values as TERMS pairs of 16-bit values whose sum they are, up to the
+// last term's rounding.
+template <bool BF16, int TERMS>
+__device__ __forceinline__ void terms16(float a, float b, uint32_t (&t)[TERMS]) {
+    if constexpr (BF16) {
+        split_terms<TERMS>(a, b, t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < TERMS; i++) {
+            const f16x2 h = {(_Float16)a, (_Float16)b};
+            t[i] = __builtin_bit_cast(uint32_t, h);
+            a -= (float)h[0];
+            b -= (float)h[1];
+        }
+    }
+}
+
+__device__ __forceinline__ float widen(uint16_t h, bool bf16) {
+    if (bf16) return __uint_as_float((uint32_t)h << 16);
+    return half_bits_to_float(h);
+}
+
+__device__ __forceinline__ void store_result(const KvCache& c, const Attention& a, size_t i,
+                                             float v) {
+    if (a.q_f32) static_cast<float*>(a.out)[i] = v;
+    else if (c.bf16) static_cast<__bf16*>(a.out)[i] = (__bf16)v;
+    else static_cast<_Float16*>(a.out)[i] = (_Float16)v;
+}
+
+// ---- one new token a sequence ---------------------------------------------------
+
+constexpr int kWaves = 4;             // waves a workgroup
+constexpr int kTile = 32;             // keys a wave step
+constexpr float kLift = 8.0f;         // how far scores may exceed the running maximum
+constexpr float kLowest = -3.0e38f;   // the maximum before any key
+// Pairs of at most this many tiles are not cut: a join costs more than it
+// brings there.
+constexpr uint32_t kWhole = 16;
+
+// The keys a query at position n - 1 sees: [0, first) and [lo, n); the tiles
+// that hold them, in order.
+struct Span {
+    uint32_t n, lo, first, sink_tiles, start, tiles;
+};
+__device__ __forceinline__ Span span_of(const Attention& a, uint32_t n) {
+    Span s;
+    s.n = n;
+    s.lo = a.window && n > a.window ? n - a.window : 0;
+    s.first = a.sinks < s.lo ? a.sinks : s.lo;
+    s.sink_tiles = (s.first + kTile - 1) / kTile;
+    s.start = s.lo / kTile > s.sink_tiles ? s.lo / kTile : s.sink_tiles;
+    const uint32_t end = (n + kTile - 1) / kTile;
+    s.tiles = s.sink_tiles + (end > s.start ? end - s.start : 0);
+    return s;
+}
+
+__device__ __forceinline__ uint32_t decode_tiles(const KvCache& c, const Attention& a, int i,
+                                                 uint32_t* fault, uint32_t* len) {
+    const uint32_t s = sequence_of(c, a.seqs, i, fault);
+    *len = s == kNoSequence ? 0 : length_of(c, s);
+    return span_of(a, *len).tiles;
+}
+
+// The entries' tiles summed up, for more entries than a wave has lanes:
+// sums[i] = tiles of entries 0 .. i.  One workgroup.
+__global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a, uint32_t* sums,
+                                                          uint32_t* fault) {
+    __shared__ uint32_t sh[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (int base = 0; base < a.n; base += 1024) {
+        const int i = base + threadIdx.x;
+        uint32_t len, v = i < a.n ? decode_tiles(c, a, i, fault, &len) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(v, d, 64);
+            if (lane >= d) v += up;
+        }
+        __syncthreads();
+        if (lane == 63) sh[wave] = v;
+        __syncthreads();
+        uint32_t before = carry;
+        for (int w = 0; w < 16; w++) {
+            before += w < wave ? sh[w] : 0u;
+            carry += sh[w];
+        }
+        if (i < a.n) sums[i] = before + v;
+    }
+}
+
+// Where the line of tiles is cut.
+struct Cut {
+    uint32_t per_head;      // tiles of all entries, for one head
+    uint32_t lane_sum;      // up to 64 entries: this lane's entry's running sum
+    uint64_t chunk;         // tiles a workgroup
+    const uint32_t* sums;   // more entries: the running sums
+    int n;
+};
+
+// The entry whose tiles hold x of one head's line; *start its first tile.
+__device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* start) {
+    const int lane = threadIdx.x & 63;
+    if (!k.sums) {
+        const int i = __popcll(__ballot(lane < k.n && k.lane_sum <= x));
+        *start = i ? __shfl(k.lane_sum, i - 1, 64) : 0;
+        return __builtin_amdgcn_readfirstlane(i);
+    }
+    // 64 ways a step
+    int lo = 0, size = k.n;
+    while (size > 64) {
+        const int step = (size + 63) / 64;
+        const int at = lo + (lane + 1) * step - 1;
+        const uint64_t below = __ballot(at < lo + size && at < k.n && k.sums[at] <= x);
+        const int skip = __popcll(below) * step;
+        lo += skip;
+        size = size - skip < step ? size - skip : step;
+    }
+    const uint64_t below = __ballot(lane < size && k.sums[lo + lane] <= x);
+    const int i = lo + __popcll(below);
+    *start = i ? k.sums[i - 1] : 0;
+    return __builtin_amdgcn_readfirstlane(i);
+}
+
+// A boundary inside a pair that is not worth cutting moves to its start.
+__device__ __forceinline__ uint64_t snap(const Cut& k, const KvCache& c, const Attention& a,
+                                         uint64_t u, uint64_t total) {
+    if (u >= total) return total;
+    const uint64_t head = u / k.per_head;
+    const uint32_t x = (uint32_t)(u - head * k.per_head);
+    uint32_t start, len;
+    const int i = find_entry(k, x, &start);
+    if (start == x) return u;
+    const uint32_t tiles = decode_tiles(c, a, i, nullptr, &len);
+    return tiles <= kWhole ? head * k.per_head + start : u;
+}
+
+template <bool BF16, int QT, int PT, int DIM, bool FULL>
+__global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_kernel(
+    KvCache c, Attention a, const uint32_t* sums, uint32_t workgroups, uint32_t* tickets,
+    uint32_t ticket_stride, float* parts, uint32_t* fault) {
+    constexpr int NJ = DIM / 32;       // steps of 32 dims of a score
+    constexpr int VD = DIM / 16;       // dims of a value a lane holds
+    constexpr int VW = VD / 2;         // and words
+    constexpr bool F32 = QT > 1;
+    // f16 terms of f32 weights: 2^7 keeps the last one's steps below 2^-30
+    constexpr float kWeightGain = !BF16 ? 128.0f : 1.0f;
+    __shared__ float acc_sh[kWaves][16][DIM + 4];
+    __shared__ float max_sh[kWaves][16], sum_sh[kWaves][16];
+    __shared__ int last_sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, quad = lane >> 4;
+    const int dim = FULL ? DIM : c.dim;
+    const int group = a.heads / c.heads;
+    const int group_tiles = (group + 15) / 16;
+    const uint32_t head_count = (uint32_t)(c.heads * group_tiles);
+
+    // the line of tiles
+    Cut cut;
+    cut.n = a.n;
+    cut.sums = sums;
+    if (!sums) {
+        uint32_t len, v = 0;
+        if (lane < a.n) v = decode_tiles(c, a, lane, blockIdx.x ? nullptr : fault, &len);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(v, d, 64);
+            if (lane >= d) v += up;
+        }
+        cut.lane_sum = v;
+        cut.per_head = __builtin_amdgcn_readfirstlane(__shfl(v, 63, 64));
+    } else {
+        cut.lane_sum = 0;
+        cut.per_head = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
+    }
+    // entries that see nothing
+    for (int i = blockIdx.x; i < a.n; i += workgroups) {
+        uint32_t len;
+        if (decode_tiles(c, a, i, nullptr, &len) == 0)
+            for (int x = threadIdx.x; x < a.heads * dim; x += 64 * kWaves)
+                store_result(c, a, (size_t)i * a.heads * dim + x, 0.0f);
+    }
+    const uint64_t total = (uint64_t)cut.per_head * head_count;
+    const uint64_t even = (total + workgroups - 1) / workgroups;
+    cut.chunk = even > kWhole ? even : kWhole;
+    uint64_t u = snap(cut, c, a, blockIdx.x * cut.chunk, total);
+    const uint64_t u_end = snap(cut, c, a, (blockIdx.x + 1) * cut.chunk, total);
+
+    const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
+    while (u < u_end) {
+        const uint32_t hx = (uint32_t)(u / cut.per_head);
+        const uint32_t x = (uint32_t)(u - (uint64_t)hx * cut.per_head);
+        uint32_t item;
+        const int entry = find_entry(cut, x, &item);
+        item = __builtin_amdgcn_readfirstlane(item);
+        const uint32_t head = hx / group_tiles;
+        const int g0 = (int)(hx - head * group_tiles) * 16;
+        const int cols = group - g0 < 16 ? group - g0 : 16;
+        const uint32_t seq = a.seqs ? a.seqs[entry] : (uint32_t)entry;
+        const Span sp = span_of(a, length_of(c, seq));
+        const uint32_t t0 = x - item;
+        const uint64_t left = u_end - u;
+        const uint32_t t1 = sp.tiles - t0 <= left ? sp.tiles : t0 + (uint32_t)left;
+        const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
+
+        // queries: the B operand, column = query head
+        u32x4 q[QT][NJ];
+        float factor = a.scale * 1.44269504088896340736f;
+        if constexpr (F32) {
+            const float* src = static_cast<const float*>(a.q) + qrow + (size_t)col * dim;
+            float v[NJ][8];
+            float top = 0;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const int d = j * 32 + quad * 8;
+                const bool in = col < cols && d < dim;
+                f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+                if (in) {
+                    lo = *reinterpret_cast<const f32x4*>(src + d);
+                    hi = *reinterpret_cast<const f32x4*>(src + d + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[j][e] = e < 4 ? lo[e] : hi[e - 4];
+                    top = fmaxf(top, fabsf(v[j][e]));
+                }
+            }
+            if constexpr (!BF16) {
+                // f16 terms: the row's largest value goes to [2^14, 2^15)
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const int ex = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+                factor *= ldexpf(1.0f, -ex);
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[j][e] = ldexpf(v[j][e], ex);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t t[QT];
+                    terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
+#pragma unroll
+                    for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
+                }
+        } else {
+            const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow + (size_t)col * dim;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const int d = j * 32 + quad * 8;
+                q[0][j] = col < cols && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
+                                                : (u32x4){0, 0, 0, 0};
+            }
+        }
+
+        f32x4 o[VD];
+#pragma unroll
+        for (int e = 0; e < VD; e++) o[e] = (f32x4){0, 0, 0, 0};
+        float m = kLowest, sum = 0;
+
+        const uint32_t* table = c.tables + (size_t)seq * c.slots;
+        const uint32_t row_mask = (1u << c.shift) - 1;
+        const uint32_t kv_row = head << c.shift;      // rows before this head's in a page
+        const int k_block = col >> 2;
+        // first position of tile t
+        const auto tile_pos = [&](uint32_t t) {
+            return (t < sp.sink_tiles ? t : sp.start + (t - sp.sink_tiles)) * kTile;
+        };
+        // the page of eight positions from pos (a multiple of 8) on, where a
+        // key among them is seen; ~0 where it names none
+        const auto seen8 = [&](uint32_t pos) {
+            return pos < sp.n && (pos + 8 > sp.lo || pos < sp.first);
+        };
+        const auto page_of = [&](uint32_t pos) {
+            uint32_t p = 0;
+            if (seen8(pos)) p = table[pos >> c.shift];
+            return p;
+        };
+        const auto k_rows = [&](uint32_t page, uint32_t pos) {
+            const uint32_t p = page < c.pages ? page : 0;
+            return c.keys + layer +
+                   ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                    ((pos + k_block * 8 + (col & 3)) & row_mask)) * dim + quad * 8;
+        };
+        const auto v_rows = [&](uint32_t page, uint32_t pos) {
+            const uint32_t p = page < c.pages ? page : 0;
+            const int d = FULL || col * VD < dim ? col * VD : 0;
+            return c.values + layer +
+                   ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                    ((pos + quad * 8) & row_mask)) * dim + d;
+        };
+        u32x4 k[2][NJ];
+        uint32_t v[8][VW];
+        const auto load_k = [&](uint32_t page, uint32_t pos) {
+            const uint16_t* p = k_rows(page, pos);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    if (FULL || j * 32 + quad * 8 < dim)
+                        k[t][j] = *reinterpret_cast<const u32x4*>(p + t * 4 * dim + j * 32);
+                    else
+                        k[t][j] = (u32x4){0, 0, 0, 0};
+                }
+        };
+        const auto load_v = [&](uint32_t page, uint32_t pos) {
+            const uint16_t* p = v_rows(page, pos);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (VW == 2) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(p + i * dim);
+                    v[i][0] = w[0], v[i][1] = w[1];
+                } else {
+#pragma unroll
+                    for (int h = 0; h < VW / 4; h++) {
+                        // a head may end inside a lane's sixteen dims
+                        const int d = FULL || h == 0 || col * VD + h * 8 < dim ? h * 8 : 0;
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + i * dim + d);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[i][4 * h + e] = w[e];
+                    }
+                }
+            }
+        };
+
+        uint32_t t = t0 + wave;
+        uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
+        if (t < t1) {
+            pos = tile_pos(t);
+            k_page = page_of(pos + k_block * 8);
+            v_page = page_of(pos + quad * 8);
+            if (t + kWaves < t1) {
+                k_next = page_of(tile_pos(t + kWaves) + k_block * 8);
+                v_next = page_of(tile_pos(t + kWaves) + quad * 8);
+            }
+            load_k(k_page, pos);
+            load_v(v_page, pos);
+        }
+        for (; t < t1; t += kWaves) {
+            const bool more = t + kWaves < t1;
+            const uint32_t pos_next = more ? tile_pos(t + kWaves) : 0;
+            // scores
+            f32x4 s[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                s[i] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int x = QT - 1; x >= 0; x--) s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
+            }
+            const uint32_t page_now = v_page;
+            if (more) load_k(k_next, pos_next);
+            // which of them are seen
+            const bool all = pos + kTile <= sp.n && (pos >= sp.lo || pos + kTile <= sp.first) &&
+                             !__any(page_now >= c.pages);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
+            uint32_t hidden = 0;
+            if (!all) {
+                const uint32_t p0 = pos + quad * 8;
+                if (page_now >= c.pages) report(fault, kFaultKvPage);
+                // selects without a branch: written with && and ||, this
+                // compiler left y[0] of a key behind the window as it was
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool ok = (p0 + e < sp.n) & ((p0 + e >= sp.lo) | (p0 + e < sp.first)) &
+                                    (page_now < c.pages);
+                    hidden |= ok ? 0u : 1u << e;
+                    y[e] = ok ? y[e] : -INFINITY;
+                }
+            }
+            float top = y[0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
+            if (__any(top > m + kLift)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float up = fmaxf(m, top);
+                const float keep = __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                sum *= keep;
+#pragma unroll
+                for (int e = 0; e < VD; e++) o[e] *= keep;
+            }
+            u32x4 w[PT];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
+                const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
+                sum += a0 + a1;
+                uint32_t x[PT];
+                terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
+#pragma unroll
+                for (int i = 0; i < PT; i++) w[i][e] = x[i];
+            }
+            // values of keys that are not seen count as 0, whatever they hold
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (hidden >> i & 1) {
+#pragma unroll
+                        for (int e = 0; e < VW; e++) v[i][e] = 0;
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < VD; e++) {
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    f[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], sel);
+#pragma unroll
+                for (int i = PT - 1; i >= 0; i--) o[e] = mfma16<BF16>(f, w[i], o[e]);
+            }
+            if (more) {
+                load_v(v_next, pos_next);
+                v_page = v_next;
+                pos = pos_next;
+                if (t + 2 * kWaves < t1) {
+                    const uint32_t after = tile_pos(t + 2 * kWaves);
+                    k_next = page_of(after + k_block * 8);
+                    v_next = page_of(after + quad * 8);
+                }
+            }
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+
+        // the waves' parts of this pair
+        __syncthreads();
+        if (col < cols) {
+            if (quad == 0) max_sh[wave][col] = m, sum_sh[wave][col] = sum;
+#pragma unroll
+            for (int e = 0; e < VD; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc_sh[wave][col][(quad * 4 + i) * VD + e] = o[e][i] * (1.0f / kWeightGain);
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == sp.tiles;
+        const uint32_t per = (uint32_t)(cols * dim);
+        // the pair's first and last stretch, and this stretch's place
+        const uint64_t begin = u - t0;
+        const uint32_t w0 = (uint32_t)(begin / cut.chunk);
+        const uint32_t w1 = (uint32_t)((begin + sp.tiles - 1) / cut.chunk);
+        const uint32_t slot_size = (uint32_t)((group < 16 ? group : 16) * (dim + 2));
+        float* part = parts + (size_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * slot_size;
+        for (uint32_t i = threadIdx.x; i < per; i += 64 * kWaves) {
+            const int g = (int)(i / dim), d = (int)(i - g * dim);
+            float top = max_sh[0][g];
+#pragma unroll
+            for (int x = 1; x < kWaves; x++) top = fmaxf(top, max_sh[x][g]);
+            float den = 0, num = 0;
+#pragma unroll
+            for (int x = 0; x < kWaves; x++) {
+                const float f = __builtin_amdgcn_exp2f(max_sh[x][g] - top);
+                den += f * sum_sh[x][g];
+                num += f * acc_sh[x][g][d];
+            }
+            if (whole) {
+                store_result(c, a, qrow + (size_t)g * dim + d, den == 0 ? 0.0f : num / den);
+            } else {
+                store_device(part + 2 * cols + i, num);
+                if (d == 0) {
+                    store_device(part + 2 * g, top);
+                    store_device(part + 2 * g + 1, den);
+                }
+            }
+        }
+        if (!whole) {
+            // the last stretch to arrive joins them all
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_s_waitcnt(0);
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __syncthreads();
+            uint32_t* ticket = tickets + (size_t)w0 * ticket_stride;
+            if (threadIdx.x == 0)
+                last_sh = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT) == w1 - w0;
+            __syncthreads();
+            if (last_sh) {
+                const auto slot = [&](uint32_t w) {
+                    return parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * slot_size;
+                };
+                for (uint32_t i = threadIdx.x; i < per; i += 64 * kWaves) {
+                    const int g = (int)(i / dim), d = (int)(i - g * dim);
+                    float top = kLowest;
+                    for (uint32_t w = w0; w <= w1; w++)
+                        top = fmaxf(top, load_device(slot(w) + 2 * g));
+                    float den = 0, num = 0;
+                    for (uint32_t w = w0; w <= w1; w++) {
+                        const float f = __builtin_amdgcn_exp2f(load_device(slot(w) + 2 * g) - top);
+                        den += f * load_device(slot(w) + 2 * g + 1);
+                        num += f * load_device(slot(w) + 2 * cols + i);
+                    }
+                    store_result(c, a, qrow + (size_t)g * dim + d, den == 0 ? 0.0f : num / den);
+                }
+                if (threadIdx.x == 0)
+                    __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        u += t1 - t0;
+    }
+}
+
+// ---- prompts ------------------------------------------------------------------------
+
+// One workgroup a query row and head; the softmax's running maximum and sum
+// are carried over blocks of 256 keys, so the keys are read once.
+__global__ __launch_bounds__(256) void paged_prefill_kernel(KvCache c, Attention a,
+                                                            uint32_t* fault) {
     __shared__ float q[256], e[256], red[4];
     __shared__ uint32_t at[256];
     const int tid = threadIdx.x;
     const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x - row * a.heads;
-    int entry = (int)row;
-    uint32_t left = 1;
-    if (a.offsets) {
-        entry = entry_of(a.offsets, a.n, row);
-        if (entry < 0) return;
-        left = a.offsets[entry + 1] - row;
-    }
+    const int entry = entry_of(a.offsets, a.n, row);
+    if (entry < 0) return;
+    const uint32_t left = a.offsets[entry + 1] - row;
     const uint32_t s = sequence_of(c, a.seqs, entry, fault);
     const uint32_t len = s == kNoSequence ? 0 : length_of(c, s);
     // keys [0, sinks) and [lo, n)
@@ -94,21 +635,73 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(KvCache c, Attenti
             }
         }
     }
-    if (tid < c.dim) {
-        const float o = sum > 0 || sum != sum ? acc / sum : 0.f;
-        if (a.q_f32) static_cast<float*>(a.out)[qrow + tid] = o;
-        else if (c.bf16) static_cast<__bf16*>(a.out)[qrow + tid] = (__bf16)o;
-        else static_cast<_Float16*>(a.out)[qrow + tid] = (_Float16)o;
-    }
+    if (tid < c.dim) store_result(c, a, qrow + tid, sum > 0 || sum != sum ? acc / sum : 0.f);
+}
+
+template <bool BF16, int QT, int PT, int DIM, bool FULL>
+void decode(Device* d, hipStream_t st, const KvCache& c, const Attention& a, const uint32_t* sums,
+            uint32_t workgroups, uint32_t* tickets, float* parts) {
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, QT, PT, DIM, FULL>), dim3(workgroups),
+                       dim3(64 * kWaves), 0, st, c, a, sums, workgroups, tickets,
+                       (uint32_t)(kWorkspaceCounterBytes / 4) / workgroups, parts, d->fault_dev);
+}
+
+template <bool BF16, int QT, int PT>
+void decode_dims(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
+                 const uint32_t* sums, uint32_t workgroups, uint32_t* tickets, float* parts) {
+    const auto go = [&](auto f) { f(d, st, c, a, sums, workgroups, tickets, parts); };
+    if (c.dim == 64) go(decode<BF16, QT, PT, 64, true>);
+    else if (c.dim < 64) go(decode<BF16, QT, PT, 64, false>);
+    else if (c.dim == 128) go(decode<BF16, QT, PT, 128, true>);
+    else if (c.dim < 128) go(decode<BF16, QT, PT, 128, false>);
+    else if (c.dim == 256) go(decode<BF16, QT, PT, 256, true>);
+    else go(decode<BF16, QT, PT, 256, false>);
 }
 
 }  // namespace
 
+bool paged_attention_counts(const KvCache& c, const Attention& a) {
+    const uint64_t tiles = (((uint64_t)c.slots << c.shift) + 2 * kTile - 1) / kTile + 1;
+    return (uint64_t)a.n * tiles <= 0xffffffffu;
+}
+
 hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
                                   const Attention& a, int* status) {
     *status = ACCEL_OK;
-    hipLaunchKernelGGL(paged_attention_kernel, dim3((unsigned)(a.rows * a.heads)), dim3(256), 0,
-                       st, c, a, d->fault_dev);
+    const int group = a.heads / c.heads;
+    // two workgroups a CU (one past 128 dims) hold as many loads in flight as
+    // the memory answers; the counters have a ticket for each
+    const uint32_t workgroups = (uint32_t)d->cu_count * (c.dim > 128 ? 1 : 2);
+    const size_t slot = (size_t)(group < 16 ? group : 16) * (c.dim + 2);
+    const bool summed = a.n > 64;
+    const size_t sums_words = summed ? (((size_t)a.n + 63) & ~(size_t)63) : 0;
+    char* ws = static_cast<char*>(
+        workspace(d, st, (sums_words + 2 * workgroups * slot) * 4, status));
+    if (!ws) return hipSuccess;
+    uint32_t* sums = reinterpret_cast<uint32_t*>(ws + kWorkspaceCounterBytes);
+    float* parts = reinterpret_cast<float*>(sums + sums_words);
+    if (summed)
+        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, sums,
+                           d->fault_dev);
+    const auto go = [&](auto f) {
+        f(d, st, c, a, summed ? sums : nullptr, workgroups, reinterpret_cast<uint32_t*>(ws),
+          parts);
+    };
+    if (a.q_f32) {
+        if (c.bf16) go(decode_dims<true, 3, 3>);
+        else go(decode_dims<false, 2, 2>);
+    } else {
+        if (c.bf16) go(decode_dims<true, 1, 2>);
+        else go(decode_dims<false, 1, 2>);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
+                                int* status) {
+    *status = ACCEL_OK;
+    hipLaunchKernelGGL(paged_prefill_kernel, dim3((unsigned)(a.rows * a.heads)), dim3(256), 0, st,
+                       c, a, d->fault_dev);
     return hipGetLastError();
 }
 

@@ -446,8 +446,12 @@ struct Attention {
     float scale;
     uint32_t window, sinks;    // window 0: all
 };
+// n entries' tiles of 32 keys have to be counted in 32 bits.
+bool paged_attention_counts(const KvCache& c, const Attention& a);
 hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
                                   const Attention& a, int* status);
+hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
+                                int* status);
 
 // Device quantizer.
 hipError_t launch_int4_quantize(hipStream_t st, const float* w, int64_t n,

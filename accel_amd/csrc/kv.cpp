@@ -389,17 +389,20 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
         a.offsets = static_cast<const uint32_t*>(offsets->data);
     }
     if ((rc = check_seqs(op, seqs, c, &n, &a.seqs)) != ACCEL_OK) return rc;
+    a.n = (int)n;
+    if (!ragged && !paged_attention_counts(c, a))
+        return refuse(op, "more entries of such tables than 32 bits count the tiles of");
     Device* d;
     if ((rc = begin(dev, &d)) != ACCEL_OK || n == 0 || T == 0) return rc;
     a.q = q->data;
     a.out = out->data;
-    a.n = (int)n;
     a.rows = (int)T;
     a.heads = (int)H;
     a.layer = layer;
     a.q_f32 = q->dtype == ACCEL_F32;
     int status = ACCEL_OK;
-    const hipError_t e = launch_paged_attention(d, (hipStream_t)stream, c, a, &status);
+    const hipError_t e = ragged ? launch_paged_prefill(d, (hipStream_t)stream, c, a, &status)
+                                : launch_paged_attention(d, (hipStream_t)stream, c, a, &status);
     return done(d, e, status, op);
 }
 

@@ -14,13 +14,13 @@ __device__ __forceinline__ void report(uint32_t* fault, uint32_t bit) {
 }
 
 // Entry i's sequence: its index, or kNoSequence for a padded row and for an
-// index outside the cache (which is reported).
+// index outside the cache (reported where fault is not null).
 constexpr uint32_t kNoSequence = ACCEL_KV_NONE;
 __device__ __forceinline__ uint32_t sequence_of(const KvCache& c, const uint32_t* seqs, int i,
                                                 uint32_t* fault) {
     const uint32_t s = seqs ? seqs[i] : (uint32_t)i;
     if (s < c.sequences) return s;
-    if (s != ACCEL_KV_NONE) report(fault, kFaultKvSequence);
+    if (s != ACCEL_KV_NONE && fault) report(fault, kFaultKvSequence);
     return kNoSequence;
 }
 
