@@ -111,11 +111,14 @@ __device__ __forceinline__ Span span_of(const Attention& a, uint32_t n) {
     return s;
 }
 
-__device__ __forceinline__ uint32_t decode_tiles(const KvCache& c, const Attention& a, int i,
-                                                 uint32_t* fault, uint32_t* len) {
+// Entry i's sequence and what its table holds of it (0: nothing to see).
+struct Held {
+    uint32_t seq, len;
+};
+__device__ __forceinline__ Held held_by(const KvCache& c, const Attention& a, int i,
+                                        uint32_t* fault) {
     const uint32_t s = sequence_of(c, a.seqs, i, fault);
-    *len = s == kNoSequence ? 0 : length_of(c, s);
-    return span_of(a, *len).tiles;
+    return {s, s == kNoSequence ? 0 : length_of(c, s)};
 }
 
 // The entries' tiles summed up, for more entries than a wave has lanes:
@@ -127,7 +130,7 @@ __global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a
     uint32_t carry = 0;
     for (int base = 0; base < a.n; base += 1024) {
         const int i = base + threadIdx.x;
-        uint32_t len, v = i < a.n ? decode_tiles(c, a, i, fault, &len) : 0;
+        uint32_t v = i < a.n ? span_of(a, held_by(c, a, i, fault).len).tiles : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
@@ -145,22 +148,29 @@ __global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a
     }
 }
 
-// Where the line of tiles is cut.
+// Where the line of tiles is cut.  Up to 64 entries: what is known of an entry
+// is in the lane of its number, read once; more: in memory, the tiles summed up
+// by the launch before.
 struct Cut {
     uint32_t per_head;      // tiles of all entries, for one head
-    uint32_t lane_sum;      // up to 64 entries: this lane's entry's running sum
+    uint32_t lane_sum;      // up to 64 entries: the running sum of this lane's
+    Held lane_held;         // and its sequence
     uint64_t chunk;         // tiles a workgroup
     const uint32_t* sums;   // more entries: the running sums
     int n;
 };
+
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
 
 // The entry whose tiles hold x of one head's line; *start its first tile.
 __device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* start) {
     const int lane = threadIdx.x & 63;
     if (!k.sums) {
         const int i = __popcll(__ballot(lane < k.n && k.lane_sum <= x));
-        *start = i ? __shfl(k.lane_sum, i - 1, 64) : 0;
-        return __builtin_amdgcn_readfirstlane(i);
+        *start = i ? lane_value(k.lane_sum, i - 1) : 0;
+        return i;
     }
     // 64 ways a step
     int lo = 0, size = k.n;
@@ -173,22 +183,111 @@ __device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* st
         size = size - skip < step ? size - skip : step;
     }
     const uint64_t below = __ballot(lane < size && k.sums[lo + lane] <= x);
-    const int i = lo + __popcll(below);
-    *start = i ? k.sums[i - 1] : 0;
-    return __builtin_amdgcn_readfirstlane(i);
+    const int i = __builtin_amdgcn_readfirstlane(lo + __popcll(below));
+    *start = i ? __builtin_amdgcn_readfirstlane(k.sums[i - 1]) : 0;
+    return i;
+}
+
+__device__ __forceinline__ Held entry_held(const Cut& k, const KvCache& c, const Attention& a,
+                                           int i) {
+    if (!k.sums) return {lane_value(k.lane_held.seq, i), lane_value(k.lane_held.len, i)};
+    const Held h = held_by(c, a, i, nullptr);
+    return {(uint32_t)__builtin_amdgcn_readfirstlane(h.seq),
+            (uint32_t)__builtin_amdgcn_readfirstlane(h.len)};
+}
+
+// u / per and u % per; the line is rarely longer than 32 bits count.
+__device__ __forceinline__ uint32_t split_line(uint64_t u, uint32_t per, uint32_t* rest) {
+    if (u >> 32) {
+        const uint32_t q = (uint32_t)(u / per);
+        *rest = (uint32_t)(u - (uint64_t)q * per);
+        return q;
+    }
+    const uint32_t q = (uint32_t)u / per;
+    *rest = (uint32_t)u - q * per;
+    return q;
 }
 
 // A boundary inside a pair that is not worth cutting moves to its start.
 __device__ __forceinline__ uint64_t snap(const Cut& k, const KvCache& c, const Attention& a,
                                          uint64_t u, uint64_t total) {
     if (u >= total) return total;
-    const uint64_t head = u / k.per_head;
-    const uint32_t x = (uint32_t)(u - head * k.per_head);
-    uint32_t start, len;
+    uint32_t x, start;
+    split_line(u, k.per_head, &x);
     const int i = find_entry(k, x, &start);
     if (start == x) return u;
-    const uint32_t tiles = decode_tiles(c, a, i, nullptr, &len);
-    return tiles <= kWhole ? head * k.per_head + start : u;
+    return span_of(a, entry_held(k, c, a, i).len).tiles <= kWhole ? u - (x - start) : u;
+}
+
+// The join of a pair's parts, by the whole workgroup: sum and values scaled to
+// the largest maximum and added in the parts' order.  A part is (maximum, sum)
+// of each column, then the columns' values.  The maxima of all parts are read
+// at once and the parts' factors kept in LDS (`room` floats), then a lane takes
+// two dims of a column, BATCH parts' loads in flight.
+template <int BATCH>
+__device__ void join_parts(const KvCache& c, const Attention& a, float* parts, uint32_t slot_size,
+                           uint32_t w0, int count, int cols, int dim, size_t qrow, float* sh,
+                           int room) {
+    const auto slot = [&](int p) {
+        return parts + (size_t)(2 * (w0 + p) + (p == 0 ? 1 : 0)) * slot_size;
+    };
+    const auto load2 = [](float* p) {
+        return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<uint64_t*>(p),
+                                                           __ATOMIC_RELAXED,
+                                                           __HIP_MEMORY_SCOPE_AGENT));
+    };
+    const int half = dim / 2;
+    // as many columns a pass as the factors fit
+    const int fit = room / (count + 1);
+    for (int g0 = 0; g0 < cols; g0 += fit) {
+        const int gs = cols - g0 < fit ? cols - g0 : fit;
+        float* factor = sh;                // [gs][count]
+        float* den = sh + gs * count;      // [gs]
+        __syncthreads();
+        for (int g = threadIdx.x >> 6; g < gs; g += kWaves) {
+            // a wave a column
+            const int lane = threadIdx.x & 63;
+            float top = kLowest;
+            for (int p = lane; p < count; p += 64)
+                top = fmaxf(top, load2(slot(p) + 2 * (g0 + g))[0]);
+            for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+            float sum = 0;
+            for (int p0 = 0; p0 < count; p0 += 64) {
+                const int p = p0 + lane;
+                float term = 0;
+                if (p < count) {
+                    const f32x2 ml = load2(slot(p) + 2 * (g0 + g));
+                    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+                    factor[g * count + p] = f;
+                    term = f * ml[1];
+                }
+                for (int x = 32; x; x >>= 1) term += __shfl_xor(term, x, 64);
+                sum += term;
+            }
+            if (lane == 0) den[g] = sum;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < gs * half; i += 64 * kWaves) {
+            const int g = i / half, d = (i - g * half) * 2;
+            const uint32_t at = (uint32_t)(2 * cols + (g0 + g) * dim + d);
+            f32x2 num = {0, 0};
+            for (int p0 = 0; p0 < count; p0 += BATCH) {
+                f32x2 v[BATCH];
+#pragma unroll
+                for (int x = 0; x < BATCH; x++) v[x] = load2(slot(p0 + x < count ? p0 + x : p0) + at);
+#pragma unroll
+                for (int x = 0; x < BATCH; x++) {
+                    const float f = p0 + x < count ? factor[g * count + p0 + x] : 0.0f;
+                    num[0] += p0 + x < count ? f * v[x][0] : 0.0f;
+                    num[1] += p0 + x < count ? f * v[x][1] : 0.0f;
+                }
+            }
+            const float l = den[g];
+            const size_t o = qrow + (size_t)(g0 + g) * dim + d;
+            store_result(c, a, o, l == 0 ? 0.0f : num[0] / l);
+            store_result(c, a, o + 1, l == 0 ? 0.0f : num[1] / l);
+        }
+    }
 }
 
 template <bool BF16, int QT, int PT, int DIM, bool FULL>
@@ -216,44 +315,41 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
     cut.n = a.n;
     cut.sums = sums;
     if (!sums) {
-        uint32_t len, v = 0;
-        if (lane < a.n) v = decode_tiles(c, a, lane, blockIdx.x ? nullptr : fault, &len);
+        cut.lane_held = {kNoSequence, 0};
+        if (lane < a.n) cut.lane_held = held_by(c, a, lane, blockIdx.x ? nullptr : fault);
+        uint32_t v = span_of(a, cut.lane_held.len).tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
             if (lane >= d) v += up;
         }
         cut.lane_sum = v;
-        cut.per_head = __builtin_amdgcn_readfirstlane(__shfl(v, 63, 64));
+        cut.per_head = lane_value(v, 63);
     } else {
-        cut.lane_sum = 0;
         cut.per_head = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
     }
     // entries that see nothing
-    for (int i = blockIdx.x; i < a.n; i += workgroups) {
-        uint32_t len;
-        if (decode_tiles(c, a, i, nullptr, &len) == 0)
+    for (int i = blockIdx.x; i < a.n; i += workgroups)
+        if (entry_held(cut, c, a, i).len == 0)
             for (int x = threadIdx.x; x < a.heads * dim; x += 64 * kWaves)
                 store_result(c, a, (size_t)i * a.heads * dim + x, 0.0f);
-    }
     const uint64_t total = (uint64_t)cut.per_head * head_count;
     const uint64_t even = (total + workgroups - 1) / workgroups;
-    cut.chunk = even > kWhole ? even : kWhole;
+    cut.chunk = even > kWaves ? even : kWaves;
     uint64_t u = snap(cut, c, a, blockIdx.x * cut.chunk, total);
     const uint64_t u_end = snap(cut, c, a, (blockIdx.x + 1) * cut.chunk, total);
 
     const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
     while (u < u_end) {
-        const uint32_t hx = (uint32_t)(u / cut.per_head);
-        const uint32_t x = (uint32_t)(u - (uint64_t)hx * cut.per_head);
-        uint32_t item;
+        uint32_t x, item;
+        const uint32_t hx = split_line(u, cut.per_head, &x);
         const int entry = find_entry(cut, x, &item);
-        item = __builtin_amdgcn_readfirstlane(item);
         const uint32_t head = hx / group_tiles;
         const int g0 = (int)(hx - head * group_tiles) * 16;
         const int cols = group - g0 < 16 ? group - g0 : 16;
-        const uint32_t seq = a.seqs ? a.seqs[entry] : (uint32_t)entry;
-        const Span sp = span_of(a, length_of(c, seq));
+        const Held held = entry_held(cut, c, a, entry);
+        const uint32_t seq = held.seq;
+        const Span sp = span_of(a, held.len);
         const uint32_t t0 = x - item;
         const uint64_t left = u_end - u;
         const uint32_t t1 = sp.tiles - t0 <= left ? sp.tiles : t0 + (uint32_t)left;
@@ -539,22 +635,8 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
                                                  __HIP_MEMORY_SCOPE_AGENT) == w1 - w0;
             __syncthreads();
             if (last_sh) {
-                const auto slot = [&](uint32_t w) {
-                    return parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * slot_size;
-                };
-                for (uint32_t i = threadIdx.x; i < per; i += 64 * kWaves) {
-                    const int g = (int)(i / dim), d = (int)(i - g * dim);
-                    float top = kLowest;
-                    for (uint32_t w = w0; w <= w1; w++)
-                        top = fmaxf(top, load_device(slot(w) + 2 * g));
-                    float den = 0, num = 0;
-                    for (uint32_t w = w0; w <= w1; w++) {
-                        const float f = __builtin_amdgcn_exp2f(load_device(slot(w) + 2 * g) - top);
-                        den += f * load_device(slot(w) + 2 * g + 1);
-                        num += f * load_device(slot(w) + 2 * cols + i);
-                    }
-                    store_result(c, a, qrow + (size_t)g * dim + d, den == 0 ? 0.0f : num / den);
-                }
+                join_parts<16>(c, a, parts, slot_size, w0, (int)(w1 - w0) + 1, cols, dim, qrow,
+                               &acc_sh[0][0][0], kWaves * 16 * (DIM + 4));
                 if (threadIdx.x == 0)
                     __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
