@@ -25,11 +25,11 @@
 // terms, queries too), so a 16-bit call rounds only its result and an f32 call
 // keeps 2^-22 of each; the matrix cores have the time.
 //
-// The work is cut evenly over the workgroups whatever the lengths: all tiles of
-// 32 keys of all (head, sequence) pairs in one line, a workgroup an equal
-// stretch of it, its four waves every fourth tile.  A pair that crosses
-// stretches is joined by the workgroup that finishes last, in the stretches'
-// order, so the result does not depend on the schedule.
+// The work is cut evenly over the workgroups whatever the lengths: the tiles of
+// 32 keys of all sequences in one line a key-value head, a workgroup an equal
+// stretch of a head's line, its waves the tiles in turn.  A sequence that
+// crosses stretches is joined by the workgroup that finishes last, in the
+// stretches' order, so the result does not depend on the schedule.
 #include <hip/hip_runtime.h>
 
 #include "bf16split.hpp"
@@ -86,13 +86,12 @@ __device__ __forceinline__ void store_result(const KvCache& c, const Attention& 
 
 // ---- one new token a sequence ---------------------------------------------------
 
-constexpr int kWaves = 4;             // waves a workgroup
 constexpr int kTile = 32;             // keys a wave step
 constexpr float kLift = 8.0f;         // how far scores may exceed the running maximum
 constexpr float kLowest = -3.0e38f;   // the maximum before any key
-// Pairs of at most this many tiles are not cut: a join costs more than it
-// brings there.
-constexpr uint32_t kWhole = 16;
+// A cut this near to a sequence's first or last tile moves there: a join (about
+// 4 us) costs more than three steps of eight waves.
+constexpr uint32_t kNear = 24;
 
 // The keys a query at position n - 1 sees: [0, first) and [lo, n); the tiles
 // that hold them, in order.
@@ -152,10 +151,10 @@ __global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a
 // is in the lane of its number, read once; more: in memory, the tiles summed up
 // by the launch before.
 struct Cut {
-    uint32_t per_head;      // tiles of all entries, for one head
+    uint32_t tiles;         // of all entries
+    uint32_t chunk;         // tiles a workgroup
     uint32_t lane_sum;      // up to 64 entries: the running sum of this lane's
     Held lane_held;         // and its sequence
-    uint64_t chunk;         // tiles a workgroup
     const uint32_t* sums;   // more entries: the running sums
     int n;
 };
@@ -164,7 +163,7 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-// The entry whose tiles hold x of one head's line; *start its first tile.
+// The entry whose tiles hold x of the line; *start its first tile.
 __device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* start) {
     const int lane = threadIdx.x & 63;
     if (!k.sums) {
@@ -196,40 +195,29 @@ __device__ __forceinline__ Held entry_held(const Cut& k, const KvCache& c, const
             (uint32_t)__builtin_amdgcn_readfirstlane(h.len)};
 }
 
-// u / per and u % per; the line is rarely longer than 32 bits count.
-__device__ __forceinline__ uint32_t split_line(uint64_t u, uint32_t per, uint32_t* rest) {
-    if (u >> 32) {
-        const uint32_t q = (uint32_t)(u / per);
-        *rest = (uint32_t)(u - (uint64_t)q * per);
-        return q;
-    }
-    const uint32_t q = (uint32_t)u / per;
-    *rest = (uint32_t)u - q * per;
-    return q;
-}
-
-// A boundary inside a pair that is not worth cutting moves to its start.
-__device__ __forceinline__ uint64_t snap(const Cut& k, const KvCache& c, const Attention& a,
-                                         uint64_t u, uint64_t total) {
-    if (u >= total) return total;
-    uint32_t x, start;
-    split_line(u, k.per_head, &x);
+// Where cut w of the line is made.
+__device__ __forceinline__ uint32_t cut_at(const Cut& k, const KvCache& c, const Attention& a,
+                                           uint64_t w) {
+    if (w * k.chunk >= k.tiles) return k.tiles;
+    const uint32_t x = (uint32_t)(w * k.chunk);
+    uint32_t start;
     const int i = find_entry(k, x, &start);
-    if (start == x) return u;
-    return span_of(a, entry_held(k, c, a, i).len).tiles <= kWhole ? u - (x - start) : u;
+    const uint32_t end = start + span_of(a, entry_held(k, c, a, i).len).tiles;
+    return x - start <= kNear ? start : end - x <= kNear ? end : x;
 }
 
-// The join of a pair's parts, by the whole workgroup: sum and values scaled to
+// The join of a sequence's parts (of workgroups w0, w0 + 1 .. of the head) by the
+// whole workgroup: sum and values scaled to
 // the largest maximum and added in the parts' order.  A part is (maximum, sum)
 // of each column, then the columns' values.  The maxima of all parts are read
 // at once and the parts' factors kept in LDS (`room` floats), then a lane takes
 // two dims of a column, BATCH parts' loads in flight.
-template <int BATCH>
-__device__ void join_parts(const KvCache& c, const Attention& a, float* parts, uint32_t slot_size,
-                           uint32_t w0, int count, int cols, int dim, size_t qrow, float* sh,
+template <int WAVES, int BATCH>
+__device__ void join_parts(const KvCache& c, const Attention& a, float* parts, size_t slot_size,
+                           uint32_t w0, uint32_t heads, uint32_t head, int count, int cols, int dim, size_t qrow, float* sh,
                            int room) {
     const auto slot = [&](int p) {
-        return parts + (size_t)(2 * (w0 + p) + (p == 0 ? 1 : 0)) * slot_size;
+        return parts + (2 * ((w0 + p) * (size_t)heads + head) + (p == 0 ? 1 : 0)) * slot_size;
     };
     const auto load2 = [](float* p) {
         return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<uint64_t*>(p),
@@ -244,7 +232,7 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, u
         float* factor = sh;                // [gs][count]
         float* den = sh + gs * count;      // [gs]
         __syncthreads();
-        for (int g = threadIdx.x >> 6; g < gs; g += kWaves) {
+        for (int g = threadIdx.x >> 6; g < gs; g += WAVES) {
             // a wave a column
             const int lane = threadIdx.x & 63;
             float top = kLowest;
@@ -267,7 +255,7 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, u
             if (lane == 0) den[g] = sum;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < gs * half; i += 64 * kWaves) {
+        for (int i = threadIdx.x; i < gs * half; i += 64 * WAVES) {
             const int g = i / half, d = (i - g * half) * 2;
             const uint32_t at = (uint32_t)(2 * cols + (g0 + g) * dim + d);
             f32x2 num = {0, 0};
@@ -290,25 +278,35 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, u
     }
 }
 
+// Waves a workgroup, one workgroup a CU: eight, as the registers of up to 128
+// dims allow; past that four.
+template <int DIM>
+constexpr int kWaves = DIM > 128 ? 4 : 8;
+
 template <bool BF16, int QT, int PT, int DIM, bool FULL>
-__global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_kernel(
-    KvCache c, Attention a, const uint32_t* sums, uint32_t workgroups, uint32_t* tickets,
+__global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
+    KvCache c, Attention a, const uint32_t* sums, uint32_t stretches, uint32_t* tickets,
     uint32_t ticket_stride, float* parts, uint32_t* fault) {
+    constexpr int W = kWaves<DIM>;
     constexpr int NJ = DIM / 32;       // steps of 32 dims of a score
     constexpr int VD = DIM / 16;       // dims of a value a lane holds
     constexpr int VW = VD / 2;         // and words
     constexpr bool F32 = QT > 1;
     // f16 terms of f32 weights: 2^7 keeps the last one's steps below 2^-30
     constexpr float kWeightGain = !BF16 ? 128.0f : 1.0f;
-    __shared__ float acc_sh[kWaves][16][DIM + 4];
-    __shared__ float max_sh[kWaves][16], sum_sh[kWaves][16];
+    __shared__ float acc_sh[W][16][DIM + 4];
+    __shared__ float max_sh[W][16], sum_sh[W][16];
     __shared__ int last_sh;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, quad = lane >> 4;
     const int dim = FULL ? DIM : c.dim;
     const int group = a.heads / c.heads;
     const int group_tiles = (group + 15) / 16;
-    const uint32_t head_count = (uint32_t)(c.heads * group_tiles);
+    const uint32_t heads = (uint32_t)(c.heads * group_tiles);
+    const uint32_t stretch = blockIdx.x / heads, head_tile = blockIdx.x - stretch * heads;
+    const uint32_t head = head_tile / group_tiles;
+    const int g0 = (int)(head_tile - head * group_tiles) * 16;
+    const int cols = group - g0 < 16 ? group - g0 : 16;
 
     // the line of tiles
     Cut cut;
@@ -324,35 +322,38 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
             if (lane >= d) v += up;
         }
         cut.lane_sum = v;
-        cut.per_head = lane_value(v, 63);
+        cut.tiles = lane_value(v, 63);
     } else {
-        cut.per_head = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
+        cut.tiles = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
     }
     // entries that see nothing
-    for (int i = blockIdx.x; i < a.n; i += workgroups)
-        if (entry_held(cut, c, a, i).len == 0)
-            for (int x = threadIdx.x; x < a.heads * dim; x += 64 * kWaves)
-                store_result(c, a, (size_t)i * a.heads * dim + x, 0.0f);
-    const uint64_t total = (uint64_t)cut.per_head * head_count;
-    const uint64_t even = (total + workgroups - 1) / workgroups;
-    cut.chunk = even > kWaves ? even : kWaves;
-    uint64_t u = snap(cut, c, a, blockIdx.x * cut.chunk, total);
-    const uint64_t u_end = snap(cut, c, a, (blockIdx.x + 1) * cut.chunk, total);
+    for (int base = wave * 64; stretch + (uint64_t)stretches * base < (uint64_t)a.n;
+         base += 64 * W) {
+        const uint64_t i = stretch + (uint64_t)stretches * (base + lane);
+        uint32_t len = 1;
+        if (!sums) len = __shfl(cut.lane_held.len, (int)i & 63, 64);
+        else if (i < (uint64_t)a.n) len = held_by(c, a, (int)i, nullptr).len;
+        for (uint64_t none = __ballot(i < (uint64_t)a.n && len == 0); none; none &= none - 1) {
+            const size_t row = stretch + (size_t)stretches * (base + __builtin_ctzll(none));
+            for (int x = lane; x < cols * dim; x += 64)
+                store_result(c, a, (row * a.heads + head * group + g0) * dim + x, 0.0f);
+        }
+    }
+    // a tile a wave at least
+    const uint32_t even = (uint32_t)(((uint64_t)cut.tiles + stretches - 1) / stretches);
+    cut.chunk = even > W ? even : W;
+    uint32_t u = cut_at(cut, c, a, stretch);
+    const uint32_t u_end = cut_at(cut, c, a, stretch + 1);
 
     const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
     while (u < u_end) {
-        uint32_t x, item;
-        const uint32_t hx = split_line(u, cut.per_head, &x);
-        const int entry = find_entry(cut, x, &item);
-        const uint32_t head = hx / group_tiles;
-        const int g0 = (int)(hx - head * group_tiles) * 16;
-        const int cols = group - g0 < 16 ? group - g0 : 16;
+        uint32_t item;
+        const int entry = find_entry(cut, u, &item);
         const Held held = entry_held(cut, c, a, entry);
         const uint32_t seq = held.seq;
         const Span sp = span_of(a, held.len);
-        const uint32_t t0 = x - item;
-        const uint64_t left = u_end - u;
-        const uint32_t t1 = sp.tiles - t0 <= left ? sp.tiles : t0 + (uint32_t)left;
+        const uint32_t t0 = u - item;
+        const uint32_t t1 = sp.tiles - t0 <= u_end - u ? sp.tiles : t0 + (u_end - u);
         const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
 
         // queries: the B operand, column = query head
@@ -483,16 +484,16 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
             pos = tile_pos(t);
             k_page = page_of(pos + k_block * 8);
             v_page = page_of(pos + quad * 8);
-            if (t + kWaves < t1) {
-                k_next = page_of(tile_pos(t + kWaves) + k_block * 8);
-                v_next = page_of(tile_pos(t + kWaves) + quad * 8);
+            if (t + W < t1) {
+                k_next = page_of(tile_pos(t + W) + k_block * 8);
+                v_next = page_of(tile_pos(t + W) + quad * 8);
             }
             load_k(k_page, pos);
             load_v(v_page, pos);
         }
-        for (; t < t1; t += kWaves) {
-            const bool more = t + kWaves < t1;
-            const uint32_t pos_next = more ? tile_pos(t + kWaves) : 0;
+        for (; t < t1; t += W) {
+            const bool more = t + W < t1;
+            const uint32_t pos_next = more ? tile_pos(t + W) : 0;
             // scores
             f32x4 s[2];
 #pragma unroll
@@ -572,8 +573,8 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
                 load_v(v_next, pos_next);
                 v_page = v_next;
                 pos = pos_next;
-                if (t + 2 * kWaves < t1) {
-                    const uint32_t after = tile_pos(t + 2 * kWaves);
+                if (t + 2 * W < t1) {
+                    const uint32_t after = tile_pos(t + 2 * W);
                     k_next = page_of(after + k_block * 8);
                     v_next = page_of(after + quad * 8);
                 }
@@ -595,20 +596,16 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
         __syncthreads();
         const bool whole = t0 == 0 && t1 == sp.tiles;
         const uint32_t per = (uint32_t)(cols * dim);
-        // the pair's first and last stretch, and this stretch's place
-        const uint64_t begin = u - t0;
-        const uint32_t w0 = (uint32_t)(begin / cut.chunk);
-        const uint32_t w1 = (uint32_t)((begin + sp.tiles - 1) / cut.chunk);
-        const uint32_t slot_size = (uint32_t)((group < 16 ? group : 16) * (dim + 2));
-        float* part = parts + (size_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * slot_size;
-        for (uint32_t i = threadIdx.x; i < per; i += 64 * kWaves) {
+        const size_t slot_size = (size_t)(group < 16 ? group : 16) * (dim + 2);
+        float* part = parts + (2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * slot_size;
+        for (uint32_t i = threadIdx.x; i < per; i += 64 * W) {
             const int g = (int)(i / dim), d = (int)(i - g * dim);
             float top = max_sh[0][g];
 #pragma unroll
-            for (int x = 1; x < kWaves; x++) top = fmaxf(top, max_sh[x][g]);
+            for (int x = 1; x < W; x++) top = fmaxf(top, max_sh[x][g]);
             float den = 0, num = 0;
 #pragma unroll
-            for (int x = 0; x < kWaves; x++) {
+            for (int x = 0; x < W; x++) {
                 const float f = __builtin_amdgcn_exp2f(max_sh[x][g] - top);
                 den += f * sum_sh[x][g];
                 num += f * acc_sh[x][g][d];
@@ -624,19 +621,24 @@ __global__ __launch_bounds__(64 * kWaves, DIM > 128 ? 1 : 2) void paged_decode_k
             }
         }
         if (!whole) {
-            // the last stretch to arrive joins them all
+            // the stretches that hold a part: w0, whose end is the first cut
+            // farther than kNear from the sequence's ends, to w1, whose start
+            // is the last; the one to arrive last joins them all
+            const uint64_t end = (uint64_t)item + sp.tiles;
+            const uint32_t w0 = (uint32_t)(((uint64_t)item + kNear) / cut.chunk);
+            const uint32_t w1 = (uint32_t)((end - kNear + cut.chunk - 1) / cut.chunk) - 1;
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
             __builtin_amdgcn_s_waitcnt(0);
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
             __syncthreads();
-            uint32_t* ticket = tickets + (size_t)w0 * ticket_stride;
+            uint32_t* ticket = tickets + ((size_t)w0 * heads + head_tile) * ticket_stride;
             if (threadIdx.x == 0)
                 last_sh = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
                                                  __HIP_MEMORY_SCOPE_AGENT) == w1 - w0;
             __syncthreads();
             if (last_sh) {
-                join_parts<16>(c, a, parts, slot_size, w0, (int)(w1 - w0) + 1, cols, dim, qrow,
-                               &acc_sh[0][0][0], kWaves * 16 * (DIM + 4));
+                join_parts<W, 16>(c, a, parts, slot_size, w0, heads, head_tile, (int)(w1 - w0) + 1,
+                                  cols, dim, qrow, &acc_sh[0][0][0], W * 16 * (DIM + 4));
                 if (threadIdx.x == 0)
                     __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
@@ -722,16 +724,18 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel(KvCache c, Attention
 
 template <bool BF16, int QT, int PT, int DIM, bool FULL>
 void decode(Device* d, hipStream_t st, const KvCache& c, const Attention& a, const uint32_t* sums,
-            uint32_t workgroups, uint32_t* tickets, float* parts) {
-    hipLaunchKernelGGL((paged_decode_kernel<BF16, QT, PT, DIM, FULL>), dim3(workgroups),
-                       dim3(64 * kWaves), 0, st, c, a, sums, workgroups, tickets,
-                       (uint32_t)(kWorkspaceCounterBytes / 4) / workgroups, parts, d->fault_dev);
+            uint32_t heads, uint32_t stretches, uint32_t* tickets, float* parts) {
+    const uint32_t grid = heads * stretches;
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, QT, PT, DIM, FULL>), dim3(grid),
+                       dim3(64 * kWaves<DIM>), 0, st, c, a, sums, stretches, tickets,
+                       (uint32_t)(kWorkspaceCounterBytes / 4) / grid, parts, d->fault_dev);
 }
 
 template <bool BF16, int QT, int PT>
 void decode_dims(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
-                 const uint32_t* sums, uint32_t workgroups, uint32_t* tickets, float* parts) {
-    const auto go = [&](auto f) { f(d, st, c, a, sums, workgroups, tickets, parts); };
+                 const uint32_t* sums, uint32_t heads, uint32_t stretches, uint32_t* tickets,
+                 float* parts) {
+    const auto go = [&](auto f) { f(d, st, c, a, sums, heads, stretches, tickets, parts); };
     if (c.dim == 64) go(decode<BF16, QT, PT, 64, true>);
     else if (c.dim < 64) go(decode<BF16, QT, PT, 64, false>);
     else if (c.dim == 128) go(decode<BF16, QT, PT, 128, true>);
@@ -751,14 +755,17 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
                                   const Attention& a, int* status) {
     *status = ACCEL_OK;
     const int group = a.heads / c.heads;
-    // two workgroups a CU (one past 128 dims) hold as many loads in flight as
-    // the memory answers; the counters have a ticket for each
-    const uint32_t workgroups = (uint32_t)d->cu_count * (c.dim > 128 ? 1 : 2);
+    // a workgroup a CU holds as many loads in flight as the memory answers;
+    // one a head is never cut, so past as many heads as CUs there are no joins
+    // and no tickets
+    const uint32_t heads = (uint32_t)(c.heads * ((group + 15) / 16));
+    const uint32_t stretches = (uint32_t)d->cu_count > heads ? (uint32_t)d->cu_count / heads : 1;
     const size_t slot = (size_t)(group < 16 ? group : 16) * (c.dim + 2);
+    const size_t part_words = stretches > 1 ? 2 * (size_t)heads * stretches * slot : 0;
     const bool summed = a.n > 64;
     const size_t sums_words = summed ? (((size_t)a.n + 63) & ~(size_t)63) : 0;
     char* ws = static_cast<char*>(
-        workspace(d, st, (sums_words + 2 * workgroups * slot) * 4, status));
+        workspace(d, st, (sums_words + part_words) * 4, status));
     if (!ws) return hipSuccess;
     uint32_t* sums = reinterpret_cast<uint32_t*>(ws + kWorkspaceCounterBytes);
     float* parts = reinterpret_cast<float*>(sums + sums_words);
@@ -766,8 +773,8 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
         hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, sums,
                            d->fault_dev);
     const auto go = [&](auto f) {
-        f(d, st, c, a, summed ? sums : nullptr, workgroups, reinterpret_cast<uint32_t*>(ws),
-          parts);
+        f(d, st, c, a, summed ? sums : nullptr, heads, stretches,
+          reinterpret_cast<uint32_t*>(ws), parts);
     };
     if (a.q_f32) {
         if (c.bf16) go(decode_dims<true, 3, 3>);
