@@ -32,6 +32,8 @@
 // stretches' order, so the result does not depend on the schedule.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "bf16split.hpp"
 #include "internal.hpp"
 #include "kvcache.hpp"
@@ -120,16 +122,31 @@ __device__ __forceinline__ Held held_by(const KvCache& c, const Attention& a, in
     return {s, s == kNoSequence ? 0 : length_of(c, s)};
 }
 
+// A prompt entry's rows of q: [first, first + count).
+struct Rows {
+    uint32_t first, count;
+};
+__device__ __forceinline__ Rows rows_of(const Attention& a, int i) {
+    const uint32_t all = (uint32_t)a.rows;
+    const uint32_t x = a.offsets[i], y = a.offsets[i + 1];
+    const uint32_t lo = x < all ? x : all, hi = y < all ? y : all;
+    return {lo, hi > lo ? hi - lo : 0};
+}
+
 // The entries' tiles summed up, for more entries than a wave has lanes:
-// sums[i] = tiles of entries 0 .. i.  One workgroup.
-__global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a, uint32_t* sums,
-                                                          uint32_t* fault) {
+// sums[i] = tiles of entries 0 .. i, of keys (tokens 0) or of so many of a
+// prompt's tokens.  One workgroup.
+__global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a, uint32_t tokens,
+                                                          uint32_t* sums, uint32_t* fault) {
     __shared__ uint32_t sh[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t carry = 0;
     for (int base = 0; base < a.n; base += 1024) {
         const int i = base + threadIdx.x;
-        uint32_t v = i < a.n ? span_of(a, held_by(c, a, i, fault).len).tiles : 0;
+        uint32_t v = 0;
+        if (i < a.n)
+            v = tokens ? (rows_of(a, i).count + tokens - 1) / tokens
+                       : span_of(a, held_by(c, a, i, fault).len).tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
@@ -648,78 +665,429 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
 }
 
 // ---- prompts ------------------------------------------------------------------------
+//
+// A workgroup takes 128 rows, 32 a wave: (token, query head of one group) pairs,
+// as many whole tokens as fit, so a tile of keys and values serves the group's
+// heads at once.  Tiles of KT keys go through LDS, staged a tile ahead through
+// registers: K as it lies, V turned by byte permutes into rows of dims with
+// the keys along them.  A wave computes S^T = K Q^T and O^T += V^T P^T with
+// 32 x 32 x 16 MFMAs; a lane has one row's scores and sums (its column), half
+// of the keys, and the other half is 32 lanes on.  As in the decode kernel the
+// keys' order in K's rows is chosen so that a lane's scores are its part of P^T's
+// operand, and the running maximum moves only when scores exceed it by 2^8.
+//
+// LDS words are laid out in 16-byte chunks, a row's chunks exchanged by an
+// exclusive or with the row so that the sixteen rows a read takes at once lie
+// in different banks.
 
-// One workgroup a query row and head; the softmax's running maximum and sum
-// are carried over blocks of 256 keys, so the keys are read once.
-__global__ __launch_bounds__(256) void paged_prefill_kernel(KvCache c, Attention a,
-                                                            uint32_t* fault) {
-    __shared__ float q[256], e[256], red[4];
-    __shared__ uint32_t at[256];
-    const int tid = threadIdx.x;
-    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x - row * a.heads;
-    const int entry = entry_of(a.offsets, a.n, row);
-    if (entry < 0) return;
-    const uint32_t left = a.offsets[entry + 1] - row;
-    const uint32_t s = sequence_of(c, a.seqs, entry, fault);
-    const uint32_t len = s == kNoSequence ? 0 : length_of(c, s);
-    // keys [0, sinks) and [lo, n)
-    const uint32_t n = left <= len ? len - left + 1 : 0;
-    const uint32_t lo = a.window && n > a.window ? n - a.window : 0;
-    const uint32_t first = a.sinks < lo ? a.sinks : lo;
-    const uint32_t seen = first + n - lo;
-    const size_t qrow = ((size_t)row * a.heads + head) * c.dim;
-    if (tid < c.dim)
-        q[tid] = a.scale * (a.q_f32 ? static_cast<const float*>(a.q)[qrow + tid]
-                                    : widen(static_cast<const uint16_t*>(a.q)[qrow + tid], c.bf16));
-    const uint32_t kvh = head / (a.heads / c.heads);
-    const size_t base = (size_t)a.layer * c.pages * c.page_elems();
-    float m = -INFINITY, sum = 0, acc = 0;
-    for (uint32_t k0 = 0; k0 < seen; k0 += 256) {
-        const uint32_t k = k0 + tid;
-        float score = -INFINITY;
-        uint32_t page = ACCEL_KV_NONE, pos = 0;
-        if (k < seen) {
-            pos = k < first ? k : lo + (k - first);
-            page = c.tables[(size_t)s * c.slots + (pos >> c.shift)];
-            if (page >= c.pages) report(fault, kFaultKvPage);
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool BF16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kRows = 128;            // rows a workgroup
+
+// Tokens of a tile of rows, and the query heads of one.
+__host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
+__host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
+
+template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT>
+__global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
+    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t* fault) {
+    constexpr int NS = DIM / 16;            // MFMA steps of a score
+    constexpr int NC = DIM / 8;             // 16-byte chunks of a key
+    constexpr int SUB = KT / 32;            // 32-key parts of a tile
+    constexpr int DT = DIM / 32;            // 32-dim parts of a row of values
+    constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
+    constexpr int KL = KT * NC / 128;       // chunks of K a staging lane loads
+    constexpr int VB = KT * DIM / 1024;     // dims of V a staging lane loads of 8 keys
+    constexpr int CK = KT / 8;              // chunks of a row of V^T
+    constexpr bool F32 = QT > 1;
+    constexpr float kWeightGain = F32 && !BF16 ? 128.0f : 1.0f;
+    __shared__ u32x4 k_sh[2][KT * NC];
+    __shared__ u32x4 v_sh[2][DIM * CK];
+    __shared__ uint32_t odd_sh[2][2];       // keys of a tile with values that are not finite
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 31, half = lane >> 5;
+    const int dim = FULL ? DIM : c.dim;
+    const int group = a.heads / c.heads;
+    const int per = prompt_heads(group), tokens = prompt_tokens(group);
+    const int group_tiles = (group + per - 1) / per;
+    const uint32_t heads = (uint32_t)(c.heads * group_tiles);
+    const uint32_t order = blockIdx.x / heads, head_tile = blockIdx.x - order * heads;
+    const uint32_t head = head_tile / group_tiles;
+    const int g0 = (int)(head_tile - head * group_tiles) * per;
+    const int gs = group - g0 < per ? group - g0 : per;
+
+    // this workgroup's tile of rows: the longest (last) ones first; where all
+    // tiles run at once, two a CU, the second half of them shortest first, so
+    // that a long one shares its CU with a short one
+    Cut cut;
+    cut.n = a.n;
+    cut.sums = sums;
+    if (!sums) {
+        uint32_t v = lane < a.n ? (rows_of(a, lane).count + tokens - 1) / tokens : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(v, d, 64);
+            if (lane >= d) v += up;
         }
-        __syncthreads();
-        at[tid] = page < c.pages ? page : ACCEL_KV_NONE;
-        if (page < c.pages) {
-            const uint16_t* kr = c.keys + base +
-                ((((size_t)page * c.heads + kvh) << c.shift) + (pos & ((1u << c.shift) - 1))) * c.dim;
-            score = 0;
-            for (int d = 0; d < c.dim; d++) score += q[d] * widen(kr[d], c.bf16);
+        cut.lane_sum = v;
+        cut.tiles = lane_value(v, 63);
+    } else {
+        cut.tiles = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
+    }
+    if (order >= cut.tiles) return;
+    const uint32_t tile = cut.tiles <= 2 * fold && order >= fold ? order - fold
+                                                                 : cut.tiles - 1 - order;
+    uint32_t item;
+    const int entry = find_entry(cut, tile, &item);
+    const Rows rows = rows_of(a, entry);
+    const uint32_t tok0 = (tile - item) * tokens;
+    const uint32_t toks = rows.count - tok0 < (uint32_t)tokens ? rows.count - tok0 : tokens;
+    const Held held = held_by(c, a, entry, threadIdx.x ? nullptr : fault);
+    // the position of the tile's first token; below 0 it sees nothing
+    const int base = (int)held.len - (int)rows.count + (int)tok0;
+    const int window = a.window ? (int)a.window : 0x7fffffff;
+    const int sinks = a.window ? (int)a.sinks : 0;
+
+    // this lane's row
+    const int r = wave * 32 + col;
+    const int tok = r / per, g = r - tok * per;
+    const bool real = tok < (int)toks && g < gs;
+    const int p = real && base + tok > -1 ? base + tok : -1;
+    const size_t qrow = ((size_t)(rows.first + tok0 + (real ? tok : 0)) * a.heads + head * group +
+                         g0 + (real ? g : 0)) * dim;
+    // the wave's first and last position, and the workgroup's
+    const int tok_a = wave * 32 / per, tok_b = (wave * 32 + 31) / per;
+    const bool busy = tok_a < (int)toks;
+    const int p_a = base + tok_a > -1 ? base + tok_a : -1;
+    const int p_last = base + (tok_b < (int)toks ? tok_b : (int)toks - 1);
+    const int p_b = p_last > -1 ? p_last : -1;
+    const int p_end = base + (int)toks;           // past the workgroup's last
+
+    // queries: the B operand, column = row
+    u32x4 q[QT][NS];
+    float factor = a.scale * 1.44269504088896340736f;
+    if constexpr (F32) {
+        const float* src = static_cast<const float*>(a.q) + qrow;
+        float top = 0;
+        if constexpr (!BF16) {
+            // f16 terms: the row's largest value goes to [2^14, 2^15)
+#pragma unroll
+            for (int j = 0; j < NS; j++) {
+                const int d = j * 16 + half * 8;
+                if (real && d < dim)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(src[d + e]));
+            }
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
         }
-        float top = score;
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(m, fmaxf(red[0], red[1])), fmaxf(red[2], red[3]));
-        const float keep = top == -INFINITY ? 0.f : expf(m - top);
-        const float mine = page < c.pages ? expf(score - top) : 0.f;
-        e[tid] = mine;
-        float part = mine;
-        for (int x = 32; x; x >>= 1) part += __shfl_xor(part, x, 64);
-        __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = part;
-        __syncthreads();
-        sum = sum * keep + (red[0] + red[1] + red[2] + red[3]);
-        acc *= keep;
-        m = top;
-        if (tid < c.dim) {
-            const uint32_t end = seen - k0 < 256 ? seen - k0 : 256;
-            for (uint32_t j = 0; j < end; j++) {
-                if (at[j] == ACCEL_KV_NONE) continue;
-                const uint32_t pj = k0 + j < first ? k0 + j : lo + (k0 + j - first);
-                const uint16_t* vr = c.values + base +
-                    ((((size_t)at[j] * c.heads + kvh) << c.shift) + (pj & ((1u << c.shift) - 1))) *
-                        c.dim;
-                acc += e[j] * widen(vr[tid], c.bf16);
+        const int ex = !BF16 && top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top)
+                                                          : 0;
+        if constexpr (!BF16) factor *= ldexpf(1.0f, -ex);
+#pragma unroll
+        for (int j = 0; j < NS; j++) {
+            const int d = j * 16 + half * 8;
+            f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if (real && d < dim) {
+                x[0] = *reinterpret_cast<const f32x4*>(src + d);
+                x[1] = *reinterpret_cast<const f32x4*>(src + d + 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                float y0 = x[e >> 1][2 * (e & 1)], y1 = x[e >> 1][2 * (e & 1) + 1];
+                if constexpr (!BF16) y0 = ldexpf(y0, ex), y1 = ldexpf(y1, ex);
+                uint32_t t[QT];
+                terms16<BF16, QT>(y0, y1, t);
+#pragma unroll
+                for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
             }
         }
+    } else {
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow;
+#pragma unroll
+        for (int j = 0; j < NS; j++) {
+            const int d = j * 16 + half * 8;
+            q[0][j] = real && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
+                                      : (u32x4){0, 0, 0, 0};
+        }
     }
-    if (tid < c.dim) store_result(c, a, qrow + tid, sum > 0 || sum != sum ? acc / sum : 0.f);
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int e = 0; e < DT; e++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[e][i] = 0;
+    float m = kLowest, sum = 0;
+
+    // tiles of keys: those of the sinks, then those from the first window's
+    // start to the last position
+    const int lo = base + 1 > window ? base + 1 - window : 0;
+    const int near = sinks < lo ? sinks : lo;
+    const int sink_tiles = (near + KT - 1) / KT;
+    const int start = lo / KT > sink_tiles ? lo / KT : sink_tiles;
+    const int last = p_end > 0 ? (p_end - 1) / KT + 1 : 0;
+    const int count = p_end > 0 ? sink_tiles + (last > start ? last - start : 0) : 0;
+    const auto tile_pos = [&](int t) {
+        return (t < sink_tiles ? t : start + (t - sink_tiles)) * KT;
+    };
+    const uint32_t* table = c.tables + (size_t)held.seq * c.slots;
+    const size_t page_size = (size_t)c.heads << c.shift;
+    const uint32_t row_mask = (1u << c.shift) - 1;
+    const size_t head_row = (size_t)head << c.shift;
+    const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
+    // the page of the eight positions from pos on, for a lane a block; one that
+    // some row of the workgroup sees has to name a page
+    const auto page_of = [&](int pos) {
+        uint32_t page = 0;
+        const int x = pos + (lane & (BLOCKS - 1)) * 8;
+        if (x < p_end && (x + 8 > lo || x < near)) page = table[(uint32_t)x >> c.shift];
+        return page;
+    };
+    const bool stages_v = wave < 2;
+    const int st = threadIdx.x & 127;
+    // staging lanes: K chunks st, st + 128 ..; V block (eight keys, VB dims)
+    const int v_block = st / (DIM / VB), v_dim = (st % (DIM / VB)) * VB;
+    u32x4 k_in[KL];
+    uint32_t v_in[8][VB / 2];
+    const auto load = [&](uint32_t pages, int pos) {
+        if (stages_v) {
+            const uint32_t page = __shfl(pages, v_block, 64);
+            const size_t at = (page < c.pages ? page : 0) * page_size + head_row +
+                              ((pos + v_block * 8) & row_mask);
+            const uint16_t* src = c.values + layer + at * dim + (FULL || v_dim < dim ? v_dim : 0);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (VB == 4) {
+                    const u32x2 w = *reinterpret_cast<const u32x2*>(src + i * dim);
+                    v_in[i][0] = w[0], v_in[i][1] = w[1];
+                } else {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * dim);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v_in[i][e] = w[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KL; i++) {
+                const int key = (st + 128 * i) / NC, ch = (st + 128 * i) % NC;
+                const uint32_t page = __shfl(pages, key / 8, 64);
+                const size_t at = (page < c.pages ? page : 0) * page_size + head_row +
+                                  ((pos + key) & row_mask);
+                k_in[i] = FULL || ch * 8 < dim
+                              ? *reinterpret_cast<const u32x4*>(c.keys + layer + at * dim + ch * 8)
+                              : (u32x4){0, 0, 0, 0};
+            }
+        }
+    };
+    const auto k_at = [](int key, int ch) {
+        return key * NC + (ch ^ (NC >= 16 ? key & 15 : key >> 1 & 7));
+    };
+    const auto v_at = [](int d, int ck) {
+        return d * CK + (ck ^ ((CK == 8 ? (d >> 1) ^ (d >> 4) : (d >> 2) ^ (d >> 4)) & (CK - 1)));
+    };
+    // whether every row of the workgroup sees all of the tile
+    const auto plain = [&](int pos) {
+        return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
+    };
+    const auto store = [&](uint32_t pages, int pos, int buf) {
+        if (stages_v) {
+            if (!plain(pos) || __any(pages >= c.pages)) {
+                // values no row sees count as 0, whatever they hold; those that
+                // are not finite are left out of the product, where a row that
+                // does not see them would meet them, and added apart
+                const uint32_t page = __shfl(pages, v_block, 64);
+                uint32_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int x = pos + v_block * 8 + i;
+                    const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
+#pragma unroll
+                    for (int e = 0; e < VB / 2; e++) {
+                        constexpr uint32_t kEnd = BF16 ? 0x7f80u : 0x7c00u;
+                        uint32_t w = seen ? v_in[i][e] : 0u;
+                        const bool b0 = (w & kEnd) == kEnd, b1 = (w >> 16 & kEnd) == kEnd;
+                        w &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu);
+                        bad |= (b0 | b1) ? 1u << i : 0u;
+                        v_in[i][e] = w;
+                    }
+                }
+                if (bad)
+                    atomicOr(&odd_sh[buf][v_block >> 2], bad << (v_block & 3) * 8);
+            }
+#pragma unroll
+            for (int e = 0; e < VB; e++) {
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    w[i] = __builtin_amdgcn_perm(v_in[2 * i + 1][e >> 1], v_in[2 * i][e >> 1], sel);
+                v_sh[buf][v_at(v_dim + e, v_block)] = w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+                k_sh[buf][k_at((st + 128 * i) / NC, (st + 128 * i) % NC)] = k_in[i];
+        }
+    };
+
+    uint32_t pages = 0, pages_next = 0;
+    if (threadIdx.x < 4) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    __syncthreads();
+    if (count) {
+        pages = page_of(tile_pos(0));
+        if (count > 1) pages_next = page_of(tile_pos(1));
+        load(pages, tile_pos(0));
+        store(pages, tile_pos(0), 0);
+    }
+    bool unnamed = false;       // a page some row sees and the table does not name
+    for (int t = 0; t < count; t++) {
+        const int pos = tile_pos(t), buf = t & 1;
+        const bool more = t + 1 < count;
+        unnamed |= pages >= c.pages;
+        __syncthreads();
+        const uint32_t odd0 = odd_sh[buf][0], odd1 = odd_sh[buf][1];
+        if (more) load(pages_next, tile_pos(t + 1));
+        // a wave none of whose rows sees the tile only stages
+        if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
+            f32x16 s[SUB];
+#pragma unroll
+            for (int i = 0; i < SUB; i++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[i][e] = 0;
+                // row 8 x + 4 h + b holds key 16 (x / 2) + 8 h + 4 (x % 2) + b
+                const int key = i * 32 + 16 * (col >> 4) + 8 * (col >> 2 & 1) +
+                                4 * (col >> 3 & 1) + (col & 3);
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    const u32x4 kf = k_sh[buf][k_at(key, 2 * j + half)];
+#pragma unroll
+                    for (int x = QT - 1; x >= 0; x--) s[i] = mfma32<BF16>(kf, q[x][j], s[i]);
+                }
+            }
+            const bool missing = __any(pages >= c.pages);
+            if (pos + KT > p_a + 1 || !(pos > p_b - window || pos + KT <= sinks) || missing ||
+                pos + KT > p_end) {
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int x = pos + i * 32 + (e >> 3) * 16 + half * 8 + (e & 7);
+                        bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                        if (missing)
+                            ok &= __shfl(pages, i * 4 + (e >> 3) * 2 + half, 64) < c.pages;
+                        s[i][e] = ok ? s[i][e] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, s[i][e]);
+            top *= factor;
+            if (__any(top > m + kLift)) {
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float up = fmaxf(m, top);
+                const float keep = __builtin_amdgcn_exp2f(m - up);
+                m = up;
+                sum *= keep;
+#pragma unroll
+                for (int e = 0; e < DT; e++) o[e] *= keep;
+            }
+            u32x4 w[PT][SUB][2];
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
+                    const float w1 =
+                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
+                    sum += w0 + w1;
+                    s[i][2 * e] = w0, s[i][2 * e + 1] = w1;
+                    uint32_t x[PT];
+                    terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
+#pragma unroll
+                    for (int k = 0; k < PT; k++) w[k][i][e >> 2][e & 3] = x[k];
+                }
+#pragma unroll
+            for (int e = 0; e < DT; e++)
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const u32x4 vf = v_sh[buf][v_at(e * 32 + col, i * 4 + j * 2 + half)];
+#pragma unroll
+                        for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
+                    }
+            if (odd0 | odd1) {
+                // the values that are not finite, for the rows that see them
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int k = i * 32 + (e >> 3) * 16 + h * 8 + (e & 7);
+                            if (!((k < 32 ? odd0 : odd1) >> (k & 31) & 1)) continue;
+                            const float weight = __shfl(s[i][e], col + 32 * h, 64) * kWeightGain;
+                            const int x = pos + k;
+                            const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                            const uint32_t page = table[(uint32_t)x >> c.shift];
+                            const uint16_t* src =
+                                c.values + layer +
+                                ((page < c.pages ? page : 0) * page_size + head_row +
+                                 ((uint32_t)x & row_mask)) * dim;
+#pragma unroll
+                            for (int y = 0; y < DT; y++)
+#pragma unroll
+                                for (int z = 0; z < 16; z++) {
+                                    const int d = y * 32 + 8 * (z >> 2) + 4 * half + (z & 3);
+                                    const float f = d < dim ? widen(src[d], BF16) : 0.0f;
+                                    const bool take = ok & !(fabsf(f) < INFINITY);
+                                    o[y][z] = take ? o[y][z] + weight * f : o[y][z];
+                                }
+                        }
+            }
+        }
+        if (more) {
+            // every wave has passed the barrier above, so none reads this buffer
+            if (threadIdx.x < 2) odd_sh[buf ^ 1][threadIdx.x] = 0;
+            pages = pages_next;
+            store(pages, tile_pos(t + 1), buf ^ 1);
+            if (t + 2 < count) pages_next = page_of(tile_pos(t + 2));
+        }
+    }
+    if (unnamed && wave == 0) report(fault, kFaultKvPage);
+    if (!real) return;
+    sum += __shfl_xor(sum, 32, 64);
+    const float scale = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
+#pragma unroll
+    for (int e = 0; e < DT; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = e * 32 + 8 * i + 4 * half;
+            if (!FULL && d >= dim) continue;
+            f32x4 v;
+#pragma unroll
+            for (int x = 0; x < 4; x++) v[x] = sum == 0 ? 0.0f : o[e][4 * i + x] * scale;
+            if constexpr (F32) {
+                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + qrow + d) = v;
+            } else {
+                uint32_t x[2][1];
+                terms16<BF16, 1>(v[0], v[1], x[0]);
+                terms16<BF16, 1>(v[2], v[3], x[1]);
+                *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + qrow + d) =
+                    (u32x2){x[0][0], x[1][0]};
+            }
+        }
 }
 
 template <bool BF16, int QT, int PT, int DIM, bool FULL>
@@ -770,7 +1138,7 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
     uint32_t* sums = reinterpret_cast<uint32_t*>(ws + kWorkspaceCounterBytes);
     float* parts = reinterpret_cast<float*>(sums + sums_words);
     if (summed)
-        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, sums,
+        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, 0u, sums,
                            d->fault_dev);
     const auto go = [&](auto f) {
         f(d, st, c, a, summed ? sums : nullptr, heads, stretches,
@@ -789,8 +1157,49 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
 hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
                                 int* status) {
     *status = ACCEL_OK;
-    hipLaunchKernelGGL(paged_prefill_kernel, dim3((unsigned)(a.rows * a.heads)), dim3(256), 0, st,
-                       c, a, d->fault_dev);
+    const int group = a.heads / c.heads;
+    const int per = prompt_heads(group), tokens = prompt_tokens(group);
+    const uint32_t heads = (uint32_t)(c.heads * ((group + per - 1) / per));
+    // an entry's last tile may be partly filled
+    const uint64_t tiles = (uint64_t)a.rows / tokens + (a.n < a.rows ? a.n : a.rows);
+    const bool summed = a.n > 64;
+    uint32_t* sums = nullptr;
+    if (summed) {
+        char* ws = static_cast<char*>(workspace(d, st, (size_t)a.n * 4, status));
+        if (!ws) return hipSuccess;
+        sums = reinterpret_cast<uint32_t*>(ws + kWorkspaceCounterBytes);
+        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
+                           sums, d->fault_dev);
+    }
+    const uint32_t fold = (uint32_t)d->cu_count / heads;
+    const dim3 grid((unsigned)(tiles * heads));
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, a, sums, fold, d->fault_dev);
+    };
+    const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
+    const auto dims = [&](auto bf16, auto qt, auto pt) {
+        constexpr bool B = decltype(bf16)::value;
+        constexpr int Q = decltype(qt)::value, P = decltype(pt)::value;
+        if (c.dim <= 64)
+            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64>)
+                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64>);
+        else if (c.dim <= 128)
+            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64>)
+                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64>);
+        else
+            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32>)
+                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32>);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 3> three;
+    if (a.q_f32) {
+        if (c.bf16) dims(std::true_type(), three, three);
+        else dims(std::false_type(), two, two);
+    } else {
+        if (c.bf16) dims(std::true_type(), one, one);
+        else dims(std::false_type(), one, one);
+    }
     return hipGetLastError();
 }
 

@@ -49,8 +49,9 @@ int check_cache(const char* op, const accel_kv_cache_t* c, KvCache* out) {
                  (long long)c->slots);
         return refuse(op, buf);
     }
-    // positions, and a table's entries, are counted in 31 bits
-    if (c->slots > INT32_MAX / c->page_size || c->sequences > INT32_MAX / c->slots) {
+    // positions (with a tile's past the last) and a table's entries are counted
+    // in 31 bits
+    if (c->slots > (INT32_MAX - 65535) / c->page_size || c->sequences > INT32_MAX / c->slots) {
         snprintf(buf, sizeof buf,
                  "tables of %lld sequences x %lld slots of %d positions are more than 31 bits "
                  "count",
