@@ -706,8 +706,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int SUB = KT / 32;            // 32-key parts of a tile
     constexpr int DT = DIM / 32;            // 32-dim parts of a row of values
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
-    constexpr int KL = KT * NC / 128;       // chunks of K a staging lane loads
-    constexpr int VB = KT * DIM / 1024;     // dims of V a staging lane loads of 8 keys
+    constexpr int KL = KT * NC / 256;       // chunks of K a lane stages
+    constexpr int VB = KT * DIM / 1024;     // dims of V a lane stages, of four keys
+    constexpr int VW = VB / 2;              // in words
     constexpr int CK = KT / 8;              // chunks of a row of V^T
     constexpr bool F32 = QT > 1;
     constexpr float kWeightGain = F32 && !BF16 ? 128.0f : 1.0f;
@@ -852,100 +853,100 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (x < p_end && (x + 8 > lo || x < near)) page = table[(uint32_t)x >> c.shift];
         return page;
     };
-    const bool stages_v = wave < 2;
-    const int st = threadIdx.x & 127;
-    // staging lanes: K chunks st, st + 128 ..; V block (eight keys, VB dims)
-    const int v_block = st / (DIM / VB), v_dim = (st % (DIM / VB)) * VB;
-    u32x4 k_in[KL];
-    uint32_t v_in[8][VB / 2];
-    const auto load = [&](uint32_t pages, int pos) {
-        if (stages_v) {
-            const uint32_t page = __shfl(pages, v_block, 64);
-            const size_t at = (page < c.pages ? page : 0) * page_size + head_row +
-                              ((pos + v_block * 8) & row_mask);
-            const uint16_t* src = c.values + layer + at * dim + (FULL || v_dim < dim ? v_dim : 0);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (VB == 4) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(src + i * dim);
-                    v_in[i][0] = w[0], v_in[i][1] = w[1];
-                } else {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * dim);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v_in[i][e] = w[e];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < KL; i++) {
-                const int key = (st + 128 * i) / NC, ch = (st + 128 * i) % NC;
-                const uint32_t page = __shfl(pages, key / 8, 64);
-                const size_t at = (page < c.pages ? page : 0) * page_size + head_row +
-                                  ((pos + key) & row_mask);
-                k_in[i] = FULL || ch * 8 < dim
-                              ? *reinterpret_cast<const u32x4*>(c.keys + layer + at * dim + ch * 8)
-                              : (u32x4){0, 0, 0, 0};
-            }
-        }
-    };
     const auto k_at = [](int key, int ch) {
         return key * NC + (ch ^ (NC >= 16 ? key & 15 : key >> 1 & 7));
     };
+    // V^T: 256 bytes hold two rows of eight chunks, or four of four; lanes that
+    // read take consecutive dims, lanes that write every VB-th
     const auto v_at = [](int d, int ck) {
-        return d * CK + (ck ^ ((CK == 8 ? (d >> 1) ^ (d >> 4) : (d >> 2) ^ (d >> 4)) & (CK - 1)));
+        return CK == 8 ? (d ^ (d >> 3 & 1)) * CK + (ck ^ (((d >> 1) ^ (d >> 4)) & 7))
+                       : d * CK + (ck ^ (((d >> 2) ^ (d >> 4)) & 3));
+    };
+    // what a lane stages: K's chunks straight to LDS, a wave 64 consecutive ones
+    // a step (what the lane reads follows from where it lands); four keys' VB
+    // dims of V through registers
+    const int v_four = threadIdx.x / (DIM / VB), v_dim = (threadIdx.x % (DIM / VB)) * VB;
+    uint32_t in[4 * VW];
+    const auto load = [&](uint32_t pages, int pos, int buf) {
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            const int at = (wave * KL + i) * 64;
+            const int key = (at + lane) / NC;
+            const int ch = (at + lane) % NC ^ (NC >= 16 ? key & 15 : key >> 1 & 7);
+            // a step's keys lie in one block of eight
+            const uint32_t page = lane_value(pages, __builtin_amdgcn_readfirstlane(at / NC / 8));
+            const size_t row = (page < c.pages ? page : 0) * page_size + head_row +
+                               ((pos + key) & row_mask);
+            if (FULL || ch * 8 < dim)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)(c.keys + layer + row * dim +
+                                                                    ch * 8),
+                    (__attribute__((address_space(3))) void*)&k_sh[buf][at], 16, 0, 0);
+        }
+        const uint32_t page = __shfl(pages, v_four >> 1, 64);
+        const size_t row = (page < c.pages ? page : 0) * page_size + head_row +
+                           ((pos + v_four * 4) & row_mask);
+        const uint16_t* src = c.values + layer + row * dim + (FULL || v_dim < dim ? v_dim : 0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (VB == 4) {
+                const u32x2 w = *reinterpret_cast<const u32x2*>(src + i * dim);
+                in[2 * i] = w[0], in[2 * i + 1] = w[1];
+            } else {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * dim);
+#pragma unroll
+                for (int e = 0; e < 4; e++) in[4 * i + e] = w[e];
+            }
+        }
     };
     // whether every row of the workgroup sees all of the tile
     const auto plain = [&](int pos) {
         return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
     };
     const auto store = [&](uint32_t pages, int pos, int buf) {
-        if (stages_v) {
-            if (!plain(pos) || __any(pages >= c.pages)) {
-                // values no row sees count as 0, whatever they hold; those that
-                // are not finite are left out of the product, where a row that
-                // does not see them would meet them, and added apart
-                const uint32_t page = __shfl(pages, v_block, 64);
-                uint32_t bad = 0;
+        if (!plain(pos) || __any(pages >= c.pages)) {
+            // values no row sees count as 0, whatever they hold; those that are
+            // not finite are left out of the product, where a row that does not
+            // see them would meet them, and added apart
+            const uint32_t page = __shfl(pages, v_four >> 1, 64);
+            uint32_t bad = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int x = pos + v_block * 8 + i;
-                    const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
+            for (int i = 0; i < 4; i++) {
+                const int x = pos + v_four * 4 + i;
+                const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
 #pragma unroll
-                    for (int e = 0; e < VB / 2; e++) {
-                        constexpr uint32_t kEnd = BF16 ? 0x7f80u : 0x7c00u;
-                        uint32_t w = seen ? v_in[i][e] : 0u;
-                        const bool b0 = (w & kEnd) == kEnd, b1 = (w >> 16 & kEnd) == kEnd;
-                        w &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu);
-                        bad |= (b0 | b1) ? 1u << i : 0u;
-                        v_in[i][e] = w;
-                    }
+                for (int e = 0; e < VW; e++) {
+                    constexpr uint32_t kEnd = BF16 ? 0x7f80u : 0x7c00u;
+                    uint32_t w = seen ? in[i * VW + e] : 0u;
+                    const bool b0 = (w & kEnd) == kEnd, b1 = (w >> 16 & kEnd) == kEnd;
+                    w &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu);
+                    bad |= (b0 | b1) ? 1u << i : 0u;
+                    in[i * VW + e] = w;
                 }
-                if (bad)
-                    atomicOr(&odd_sh[buf][v_block >> 2], bad << (v_block & 3) * 8);
             }
+            if (bad) atomicOr(&odd_sh[buf][v_four >> 3], bad << (v_four & 7) * 4);
+        }
 #pragma unroll
-            for (int e = 0; e < VB; e++) {
-                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 w;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w[i] = __builtin_amdgcn_perm(v_in[2 * i + 1][e >> 1], v_in[2 * i][e >> 1], sel);
-                v_sh[buf][v_at(v_dim + e, v_block)] = w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < KL; i++)
-                k_sh[buf][k_at((st + 128 * i) / NC, (st + 128 * i) % NC)] = k_in[i];
+        for (int e = 0; e < VB; e++) {
+            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+            const u32x2 w = {
+                __builtin_amdgcn_perm(in[VW + (e >> 1)], in[e >> 1], sel),
+                __builtin_amdgcn_perm(in[3 * VW + (e >> 1)], in[2 * VW + (e >> 1)], sel)};
+            reinterpret_cast<u32x2*>(&v_sh[buf][v_at(v_dim + e, v_four >> 1)])[v_four & 1] = w;
         }
     };
 
+    // dims past the head's: K's chunks there are no load's target and stay 0
+    if constexpr (!FULL) {
+        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256) (&k_sh[0][0])[i] = (u32x4){0, 0, 0, 0};
+    }
     uint32_t pages = 0, pages_next = 0;
     if (threadIdx.x < 4) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     __syncthreads();
     if (count) {
         pages = page_of(tile_pos(0));
         if (count > 1) pages_next = page_of(tile_pos(1));
-        load(pages, tile_pos(0));
+        load(pages, tile_pos(0), 0);
         store(pages, tile_pos(0), 0);
     }
     bool unnamed = false;       // a page some row sees and the table does not name
@@ -955,7 +956,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         unnamed |= pages >= c.pages;
         __syncthreads();
         const uint32_t odd0 = odd_sh[buf][0], odd1 = odd_sh[buf][1];
-        if (more) load(pages_next, tile_pos(t + 1));
+        if (more) load(pages_next, tile_pos(t + 1), buf ^ 1);
         // a wave none of whose rows sees the tile only stages
         if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
             f32x16 s[SUB];
@@ -973,17 +974,21 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     for (int x = QT - 1; x >= 0; x--) s[i] = mfma32<BF16>(kf, q[x][j], s[i]);
                 }
             }
-            const bool missing = __any(pages >= c.pages);
-            if (pos + KT > p_a + 1 || !(pos > p_b - window || pos + KT <= sinks) || missing ||
-                pos + KT > p_end) {
+            const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
+            if (pos + KT > p_a + 1 || !(pos > p_b - window || pos + KT <= sinks) ||
+                ~named & ((1ull << BLOCKS) - 1)) {
+                const uint32_t mine = (uint32_t)named >> half;
+                // a key's place in the tile against these
+                const int here = pos + half * 8;
+                const int until = p - here, kept = sinks - here;
 #pragma unroll
                 for (int i = 0; i < SUB; i++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const int x = pos + i * 32 + (e >> 3) * 16 + half * 8 + (e & 7);
-                        bool ok = (x <= p) & ((x > p - window) | (x < sinks));
-                        if (missing)
-                            ok &= __shfl(pages, i * 4 + (e >> 3) * 2 + half, 64) < c.pages;
+                        const int x = i * 32 + (e >> 3) * 16 + (e & 7);
+                        const bool ok = (x <= until) &
+                                        (((uint32_t)(until - x) < (uint32_t)window) | (x < kept)) &
+                                        ((mine >> (i * 4 + (e >> 3) * 2) & 1) != 0);
                         s[i][e] = ok ? s[i][e] : -INFINITY;
                     }
             }
@@ -1011,7 +1016,6 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     const float w1 =
                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
                     sum += w0 + w1;
-                    s[i][2 * e] = w0, s[i][2 * e + 1] = w1;
                     uint32_t x[PT];
                     terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
 #pragma unroll
@@ -1027,34 +1031,28 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
                         for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
                     }
-            if (odd0 | odd1) {
-                // the values that are not finite, for the rows that see them
+            // the values that are not finite, for the rows that see them: whatever
+            // the weight, the sum is what they are
+            for (uint64_t odd = odd0 | (uint64_t)odd1 << 32; odd; odd &= odd - 1) {
+                const int x = pos + (int)__builtin_ctzll(odd);
+                const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                const uint32_t page = table[(uint32_t)x >> c.shift];
+                const uint16_t* src = c.values + layer +
+                                      ((page < c.pages ? page : 0) * page_size + head_row +
+                                       ((uint32_t)x & row_mask)) * dim;
 #pragma unroll
-                for (int i = 0; i < SUB; i++)
+                for (int y = 0; y < DT; y++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
+                    for (int z = 0; z < 4; z++) {
+                        const int d = y * 32 + 8 * z + 4 * half;
+                        u32x2 f = {0, 0};
+                        if (FULL || d < dim) f = *reinterpret_cast<const u32x2*>(src + d);
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int k = i * 32 + (e >> 3) * 16 + h * 8 + (e & 7);
-                            if (!((k < 32 ? odd0 : odd1) >> (k & 31) & 1)) continue;
-                            const float weight = __shfl(s[i][e], col + 32 * h, 64) * kWeightGain;
-                            const int x = pos + k;
-                            const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
-                            const uint32_t page = table[(uint32_t)x >> c.shift];
-                            const uint16_t* src =
-                                c.values + layer +
-                                ((page < c.pages ? page : 0) * page_size + head_row +
-                                 ((uint32_t)x & row_mask)) * dim;
-#pragma unroll
-                            for (int y = 0; y < DT; y++)
-#pragma unroll
-                                for (int z = 0; z < 16; z++) {
-                                    const int d = y * 32 + 8 * (z >> 2) + 4 * half + (z & 3);
-                                    const float f = d < dim ? widen(src[d], BF16) : 0.0f;
-                                    const bool take = ok & !(fabsf(f) < INFINITY);
-                                    o[y][z] = take ? o[y][z] + weight * f : o[y][z];
-                                }
+                        for (int e = 0; e < 4; e++) {
+                            const float v = widen((uint16_t)(f[e >> 1] >> 16 * (e & 1)), BF16);
+                            o[y][4 * z + e] += ok && !(fabsf(v) < INFINITY) ? v : 0.0f;
                         }
+                    }
             }
         }
         if (more) {
