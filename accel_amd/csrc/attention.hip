@@ -712,10 +712,13 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int CK = KT / 8;              // chunks of a row of V^T
     constexpr bool F32 = QT > 1;
     constexpr float kWeightGain = F32 && !BF16 ? 128.0f : 1.0f;
-    __shared__ u32x4 k_sh[2][KT * NC];
-    __shared__ u32x4 v_sh[2][DIM * CK];
-    __shared__ uint32_t odd_sh[2][2];       // keys of a tile with values that are not finite
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
+    __shared__ __attribute__((aligned(256))) char v_sh[2][DIM * CK * 16];
+    // keys of a tile with values that are not finite: tile t's in place t % 3,
+    // which is cleared two steps before it is read, a barrier before it is set
+    __shared__ uint32_t odd_sh[3][2];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int dim = FULL ? DIM : c.dim;
     const int group = a.heads / c.heads;
@@ -853,40 +856,54 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (x < p_end && (x + 8 > lo || x < near)) page = table[(uint32_t)x >> c.shift];
         return page;
     };
-    const auto k_at = [](int key, int ch) {
-        return key * NC + (ch ^ (NC >= 16 ? key & 15 : key >> 1 & 7));
+    // Where chunks lie: linear in the bits of their numbers under exclusive or,
+    // so a lane's address is its own part, exchanged with a constant's.  V^T: 256
+    // bytes hold two rows of eight chunks, or four of four; lanes that read take
+    // consecutive dims, lanes that write every VB-th.
+    const auto k_byte = [](int key, int ch) {
+        return (key * NC + (ch ^ (NC >= 16 ? key & 15 : key >> 1 & 7))) * 16;
     };
-    // V^T: 256 bytes hold two rows of eight chunks, or four of four; lanes that
-    // read take consecutive dims, lanes that write every VB-th
-    const auto v_at = [](int d, int ck) {
-        return CK == 8 ? (d ^ (d >> 3 & 1)) * CK + (ck ^ (((d >> 1) ^ (d >> 4)) & 7))
-                       : d * CK + (ck ^ (((d >> 2) ^ (d >> 4)) & 3));
+    const auto v_byte = [](int d, int ck) {
+        return CK == 8 ? ((d ^ (d >> 3 & 1)) * CK + (ck ^ (((d >> 1) ^ (d >> 4)) & 7))) * 16
+                       : (d * CK + (ck ^ (((d >> 2) ^ (d >> 4)) & 3))) * 16;
     };
     // what a lane stages: K's chunks straight to LDS, a wave 64 consecutive ones
     // a step (what the lane reads follows from where it lands); four keys' VB
     // dims of V through registers
-    const int v_four = threadIdx.x / (DIM / VB), v_dim = (threadIdx.x % (DIM / VB)) * VB;
+    uint32_t k_off[KL];                     // bytes from the row of a block's first key
+#pragma unroll
+    for (int i = 0; i < KL; i++) {
+        const int at = (wave * KL + i) * 64, key = (at + lane) / NC;
+        const int ch = (at + lane) % NC ^ (NC >= 16 ? key & 15 : key >> 1 & 7);
+        k_off[i] = ch * 8 < dim ? (uint32_t)((key & 7) * dim + ch * 8) * 2 : 0xffffffffu;
+    }
+    constexpr int VL = DIM / VB;            // lanes across a row of V
+    const int v_four = threadIdx.x / VL, v_dim = (threadIdx.x % VL) * VB;
+    const uint32_t v_off = (uint32_t)((v_four & 1) * 4 * dim + (FULL || v_dim < dim ? v_dim : 0));
+    const int v_to = v_byte(v_dim, v_four >> 1) + (v_four & 1) * 8;
     uint32_t in[4 * VW];
-    const auto load = [&](uint32_t pages, int pos, int buf) {
+    // element offset of block b's first row (b uniform)
+    const auto block_row = [&](uint32_t pages, int pos, int b) {
+        const uint32_t page = lane_value(pages, b);
+        return ((page < c.pages ? page : 0) * page_size + head_row +
+                (((uint32_t)pos + b * 8) & row_mask)) * dim;
+    };
+    const auto load = [&](uint32_t pages, int pos, auto buf) {
 #pragma unroll
         for (int i = 0; i < KL; i++) {
             const int at = (wave * KL + i) * 64;
-            const int key = (at + lane) / NC;
-            const int ch = (at + lane) % NC ^ (NC >= 16 ? key & 15 : key >> 1 & 7);
-            // a step's keys lie in one block of eight
-            const uint32_t page = lane_value(pages, __builtin_amdgcn_readfirstlane(at / NC / 8));
-            const size_t row = (page < c.pages ? page : 0) * page_size + head_row +
-                               ((pos + key) & row_mask);
-            if (FULL || ch * 8 < dim)
+            const char* row = reinterpret_cast<const char*>(
+                c.keys + layer + block_row(pages, pos, at / NC / 8));
+            if (FULL || k_off[i] != 0xffffffffu)
                 __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(c.keys + layer + row * dim +
-                                                                    ch * 8),
-                    (__attribute__((address_space(3))) void*)&k_sh[buf][at], 16, 0, 0);
+                    (const __attribute__((address_space(1))) void*)(row + k_off[i]),
+                    (__attribute__((address_space(3))) void*)(k_sh[decltype(buf)::value] + at * 16),
+                    16, 0, 0);
         }
-        const uint32_t page = __shfl(pages, v_four >> 1, 64);
-        const size_t row = (page < c.pages ? page : 0) * page_size + head_row +
-                           ((pos + v_four * 4) & row_mask);
-        const uint16_t* src = c.values + layer + row * dim + (FULL || v_dim < dim ? v_dim : 0);
+        // a wave's lanes hold one block of keys (VL 32) or two
+        const size_t row0 = block_row(pages, pos, VL == 32 ? wave : 2 * wave);
+        const size_t row1 = VL == 32 ? row0 : block_row(pages, pos, 2 * wave + 1);
+        const uint16_t* src = c.values + layer + (VL == 32 || lane < 32 ? row0 : row1) + v_off;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (VB == 4) {
@@ -903,7 +920,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const auto plain = [&](int pos) {
         return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
     };
-    const auto store = [&](uint32_t pages, int pos, int buf) {
+    const auto store = [&](uint32_t pages, int pos, int odd, auto buf) {
+        constexpr int B = decltype(buf)::value;
         if (!plain(pos) || __any(pages >= c.pages)) {
             // values no row sees count as 0, whatever they hold; those that are
             // not finite are left out of the product, where a row that does not
@@ -924,7 +942,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     in[i * VW + e] = w;
                 }
             }
-            if (bad) atomicOr(&odd_sh[buf][v_four >> 3], bad << (v_four & 7) * 4);
+            if (bad) atomicOr(&odd_sh[odd][v_four >> 3], bad << (v_four & 7) * 4);
         }
 #pragma unroll
         for (int e = 0; e < VB; e++) {
@@ -932,31 +950,43 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             const u32x2 w = {
                 __builtin_amdgcn_perm(in[VW + (e >> 1)], in[e >> 1], sel),
                 __builtin_amdgcn_perm(in[3 * VW + (e >> 1)], in[2 * VW + (e >> 1)], sel)};
-            reinterpret_cast<u32x2*>(&v_sh[buf][v_at(v_dim + e, v_four >> 1)])[v_four & 1] = w;
+            *reinterpret_cast<u32x2*>(v_sh[B] + (v_to ^ v_byte(e, 0))) = w;
         }
     };
 
     // dims past the head's: K's chunks there are no load's target and stay 0
     if constexpr (!FULL) {
-        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256) (&k_sh[0][0])[i] = (u32x4){0, 0, 0, 0};
+        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
+            reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
     }
     uint32_t pages = 0, pages_next = 0;
-    if (threadIdx.x < 4) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+    if (threadIdx.x < 6) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     __syncthreads();
     if (count) {
         pages = page_of(tile_pos(0));
         if (count > 1) pages_next = page_of(tile_pos(1));
-        load(pages, tile_pos(0), 0);
-        store(pages, tile_pos(0), 0);
+        load(pages, tile_pos(0), std::integral_constant<int, 0>());
+        store(pages, tile_pos(0), 0, std::integral_constant<int, 0>());
     }
+    // the lane's part of what it reads: row 8 x + 4 h + b of K's operand holds
+    // key 16 (x / 2) + 8 h + 4 (x % 2) + b
+    const int k_from = k_byte(16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3),
+                              half);
+    const int v_from = v_byte(col, half);
+    int odd_at = 0;
     bool unnamed = false;       // a page some row sees and the table does not name
-    for (int t = 0; t < count; t++) {
-        const int pos = tile_pos(t), buf = t & 1;
+    const auto step = [&](int t, auto buf) {
+        constexpr int B = decltype(buf)::value;
+        const std::integral_constant<int, B ^ 1> other;
+        const int pos = tile_pos(t);
         const bool more = t + 1 < count;
         unnamed |= pages >= c.pages;
         __syncthreads();
-        const uint32_t odd0 = odd_sh[buf][0], odd1 = odd_sh[buf][1];
-        if (more) load(pages_next, tile_pos(t + 1), buf ^ 1);
+        const uint32_t odd0 = odd_sh[odd_at][0], odd1 = odd_sh[odd_at][1];
+        const int odd_next = odd_at == 2 ? 0 : odd_at + 1;
+        if (threadIdx.x < 2) odd_sh[odd_next == 2 ? 0 : odd_next + 1][threadIdx.x] = 0;
+        odd_at = odd_next;
+        if (more) load(pages_next, tile_pos(t + 1), other);
         // a wave none of whose rows sees the tile only stages
         if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
             f32x16 s[SUB];
@@ -964,12 +994,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             for (int i = 0; i < SUB; i++) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[i][e] = 0;
-                // row 8 x + 4 h + b holds key 16 (x / 2) + 8 h + 4 (x % 2) + b
-                const int key = i * 32 + 16 * (col >> 4) + 8 * (col >> 2 & 1) +
-                                4 * (col >> 3 & 1) + (col & 3);
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
-                    const u32x4 kf = k_sh[buf][k_at(key, 2 * j + half)];
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(
+                        k_sh[B] + (k_from ^ k_byte(0, 2 * j)) + k_byte(i * 32, 0));
 #pragma unroll
                     for (int x = QT - 1; x >= 0; x--) s[i] = mfma32<BF16>(kf, q[x][j], s[i]);
                 }
@@ -1027,7 +1055,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 for (int i = 0; i < SUB; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const u32x4 vf = v_sh[buf][v_at(e * 32 + col, i * 4 + j * 2 + half)];
+                        constexpr int kLow = CK * 16 - 1;    // a row's chunks
+                        const int at = v_byte(e * 32, i * 4 + j * 2);
+                        const u32x4 vf = *reinterpret_cast<const u32x4*>(
+                            v_sh[B] + (v_from ^ (at & kLow)) + (at & ~kLow));
 #pragma unroll
                         for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
                     }
@@ -1057,11 +1088,14 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         }
         if (more) {
             // every wave has passed the barrier above, so none reads this buffer
-            if (threadIdx.x < 2) odd_sh[buf ^ 1][threadIdx.x] = 0;
             pages = pages_next;
-            store(pages, tile_pos(t + 1), buf ^ 1);
+            store(pages, tile_pos(t + 1), odd_next, other);
             if (t + 2 < count) pages_next = page_of(tile_pos(t + 2));
         }
+    };
+    for (int t = 0; t < count; t += 2) {
+        step(t, std::integral_constant<int, 0>());
+        if (t + 1 < count) step(t + 1, std::integral_constant<int, 1>());
     }
     if (unnamed && wave == 0) report(fault, kFaultKvPage);
     if (!real) return;
