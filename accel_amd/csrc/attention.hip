@@ -694,6 +694,9 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 
 constexpr int kRows = 128;            // rows a workgroup
 
+// s_waitcnt vmcnt(0), as an instruction that the compiler counts itself.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // Tokens of a tile of rows, and the query heads of one.
 __host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
 __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
@@ -922,6 +925,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     };
     const auto store = [&](uint32_t pages, int pos, int odd, auto buf) {
         constexpr int B = decltype(buf)::value;
+        // K's chunks are in LDS before the barrier that follows
+        wait_loads();
         if (!plain(pos) || __any(pages >= c.pages)) {
             // values no row sees count as 0, whatever they hold; those that are
             // not finite are left out of the product, where a row that does not
@@ -973,6 +978,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int k_from = k_byte(16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3),
                               half);
     const int v_from = v_byte(col, half);
+    // the queries have arrived: without this the loop's first product waits for
+    // every load in flight, each time
+    wait_loads();
     int odd_at = 0;
     bool unnamed = false;       // a page some row sees and the table does not name
     const auto step = [&](int t, auto buf) {
@@ -987,6 +995,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (threadIdx.x < 2) odd_sh[odd_next == 2 ? 0 : odd_next + 1][threadIdx.x] = 0;
         odd_at = odd_next;
         if (more) load(pages_next, tile_pos(t + 1), other);
+        // a whole step ahead of its use
+        const uint32_t pages_after = t + 2 < count ? page_of(tile_pos(t + 2)) : 0;
         // a wave none of whose rows sees the tile only stages
         if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
             f32x16 s[SUB];
@@ -1090,7 +1100,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             // every wave has passed the barrier above, so none reads this buffer
             pages = pages_next;
             store(pages, tile_pos(t + 1), odd_next, other);
-            if (t + 2 < count) pages_next = page_of(tile_pos(t + 2));
+            pages_next = pages_after;
         }
     };
     for (int t = 0; t < count; t += 2) {
