@@ -847,10 +847,12 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         return (t < sink_tiles ? t : start + (t - sink_tiles)) * KT;
     };
     const uint32_t* table = c.tables + (size_t)held.seq * c.slots;
-    const size_t page_size = (size_t)c.heads << c.shift;
+    const uint64_t page_bytes = c.page_elems() * 2;
     const uint32_t row_mask = (1u << c.shift) - 1;
-    const size_t head_row = (size_t)head << c.shift;
+    const uint32_t head_row = head << c.shift;    // below 2^24
     const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
+    const char* keys = reinterpret_cast<const char*>(c.keys + layer);
+    const char* values = reinterpret_cast<const char*>(c.values + layer);
     // the page of the eight positions from pos on, for a lane a block; one that
     // some row of the workgroup sees has to name a page
     const auto page_of = [&](int pos) {
@@ -882,21 +884,27 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     }
     constexpr int VL = DIM / VB;            // lanes across a row of V
     const int v_four = threadIdx.x / VL, v_dim = (threadIdx.x % VL) * VB;
-    const uint32_t v_off = (uint32_t)((v_four & 1) * 4 * dim + (FULL || v_dim < dim ? v_dim : 0));
+    const uint32_t v_off = ((v_four & 1) * 4 * dim + (FULL || v_dim < dim ? v_dim : 0)) * 2;
     const int v_to = v_byte(v_dim, v_four >> 1) + (v_four & 1) * 8;
     uint32_t in[4 * VW];
-    // element offset of block b's first row (b uniform)
-    const auto block_row = [&](uint32_t pages, int pos, int b) {
-        const uint32_t page = lane_value(pages, b);
-        return ((page < c.pages ? page : 0) * page_size + head_row +
-                (((uint32_t)pos + b * 8) & row_mask)) * dim;
+    // the lanes of blocks 0 .. hold the byte offset of their block's first row
+    // in a plane, from which a load's uniform part is read
+    const uint32_t row_bytes = (uint32_t)dim * 2;
+    const auto block_rows = [&](uint32_t pages, int pos) {
+        const uint32_t at = (uint32_t)head_row +
+                            (((uint32_t)pos + (lane & (BLOCKS - 1)) * 8) & row_mask);
+        return (pages < c.pages ? pages : 0) * page_bytes + (uint64_t)at * row_bytes;
+    };
+    const auto block_row = [&](uint64_t rows, int b) {
+        return (uint64_t)lane_value((uint32_t)rows, b) |
+               (uint64_t)lane_value((uint32_t)(rows >> 32), b) << 32;
     };
     const auto load = [&](uint32_t pages, int pos, auto buf) {
+        const uint64_t rows = block_rows(pages, pos);
 #pragma unroll
         for (int i = 0; i < KL; i++) {
             const int at = (wave * KL + i) * 64;
-            const char* row = reinterpret_cast<const char*>(
-                c.keys + layer + block_row(pages, pos, at / NC / 8));
+            const char* row = keys + block_row(rows, at / NC / 8);
             if (FULL || k_off[i] != 0xffffffffu)
                 __builtin_amdgcn_global_load_lds(
                     (const __attribute__((address_space(1))) void*)(row + k_off[i]),
@@ -904,9 +912,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     16, 0, 0);
         }
         // a wave's lanes hold one block of keys (VL 32) or two
-        const size_t row0 = block_row(pages, pos, VL == 32 ? wave : 2 * wave);
-        const size_t row1 = VL == 32 ? row0 : block_row(pages, pos, 2 * wave + 1);
-        const uint16_t* src = c.values + layer + (VL == 32 || lane < 32 ? row0 : row1) + v_off;
+        const uint64_t row0 = block_row(rows, VL == 32 ? wave : 2 * wave);
+        const uint64_t row1 = VL == 32 ? row0 : block_row(rows, 2 * wave + 1);
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(
+            values + (VL == 32 || lane < 32 ? row0 : row1) + v_off);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (VB == 4) {
@@ -1078,9 +1087,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 const int x = pos + (int)__builtin_ctzll(odd);
                 const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
                 const uint32_t page = table[(uint32_t)x >> c.shift];
-                const uint16_t* src = c.values + layer +
-                                      ((page < c.pages ? page : 0) * page_size + head_row +
-                                       ((uint32_t)x & row_mask)) * dim;
+                const uint16_t* src = reinterpret_cast<const uint16_t*>(
+                    values + (page < c.pages ? page : 0) * page_bytes +
+                    (uint64_t)(head_row + ((uint32_t)x & row_mask)) * row_bytes);
 #pragma unroll
                 for (int y = 0; y < DT; y++)
 #pragma unroll
