@@ -939,24 +939,37 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (!plain(pos) || __any(pages >= c.pages)) {
             // values no row sees count as 0, whatever they hold; those that are
             // not finite are left out of the product, where a row that does not
-            // see them would meet them, and added apart
+            // see them would meet them, and added apart.  A 16-bit value whose
+            // exponent is all ones carries into the sign's place.
+            constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+            constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
             const uint32_t page = __shfl(pages, v_four >> 1, 64);
-            uint32_t bad = 0;
+            uint32_t carry[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int x = pos + v_four * 4 + i;
                 const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
+                const uint32_t keep = seen ? 0xffffffffu : 0u;
+                carry[i] = 0;
 #pragma unroll
                 for (int e = 0; e < VW; e++) {
-                    constexpr uint32_t kEnd = BF16 ? 0x7f80u : 0x7c00u;
-                    uint32_t w = seen ? in[i * VW + e] : 0u;
-                    const bool b0 = (w & kEnd) == kEnd, b1 = (w >> 16 & kEnd) == kEnd;
-                    w &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu);
-                    bad |= (b0 | b1) ? 1u << i : 0u;
-                    in[i * VW + e] = w;
+                    in[i * VW + e] &= keep;
+                    carry[i] |= (in[i * VW + e] & kExp) + kOne;
                 }
             }
-            if (bad) atomicOr(&odd_sh[odd][v_four >> 3], bad << (v_four & 7) * 4);
+            if ((carry[0] | carry[1] | carry[2] | carry[3]) & 0x80008000u) {
+                uint32_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    bad |= carry[i] & 0x80008000u ? 1u << i : 0u;
+#pragma unroll
+                    for (int e = 0; e < VW; e++) {
+                        const uint32_t over = ((in[i * VW + e] & kExp) + kOne) & 0x80008000u;
+                        in[i * VW + e] &= ~((over >> 15) * 0xffffu);
+                    }
+                }
+                atomicOr(&odd_sh[odd][v_four >> 3], bad << (v_four & 7) * 4);
+            }
         }
 #pragma unroll
         for (int e = 0; e < VB; e++) {
@@ -1021,30 +1034,43 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     for (int x = QT - 1; x >= 0; x--) s[i] = mfma32<BF16>(kf, q[x][j], s[i]);
                 }
             }
-            const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
-            if (pos + KT > p_a + 1 || !(pos > p_b - window || pos + KT <= sinks) ||
-                ~named & ((1ull << BLOCKS) - 1)) {
-                const uint32_t mine = (uint32_t)named >> half;
-                // a key's place in the tile against these
-                const int here = pos + half * 8;
-                const int until = p - here, kept = sinks - here;
+            // keys a row does not see, by a key's place x in the tile: past the
+            // row's position, behind its window, on a page without a number
+            const int here = pos + half * 8;
+            const int until = p - here;
+            const auto hide = [&](auto seen) {
 #pragma unroll
                 for (int i = 0; i < SUB; i++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int x = i * 32 + (e >> 3) * 16 + (e & 7);
-                        const bool ok = (x <= until) &
-                                        (((uint32_t)(until - x) < (uint32_t)window) | (x < kept)) &
-                                        ((mine >> (i * 4 + (e >> 3) * 2) & 1) != 0);
-                        s[i][e] = ok ? s[i][e] : -INFINITY;
-                    }
+                    for (int e = 0; e < 16; e++)
+                        s[i][e] = seen(i * 32 + (e >> 3) * 16 + (e & 7)) ? s[i][e] : -INFINITY;
+            };
+            if (pos + KT > p_a + 1) hide([&](int x) { return x <= until; });
+            if (!(pos > p_b - window || pos + KT <= sinks)) {
+                // the first place the row's window holds; none where it is all past
+                const int from = until < window ? -KT : until - window + 1;
+                if (pos >= sinks) {
+                    hide([&](int x) { return x >= from; });
+                } else {
+                    const int kept = sinks - here;
+                    hide([&](int x) { return (x >= from) | (x < kept); });
+                }
             }
-            float top = s[0][0];
+            const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
+            if (~named & ((1ull << BLOCKS) - 1)) {
+                const uint32_t mine = (uint32_t)named >> half;
+                hide([&](int x) { return (mine >> (x >> 3) & 1) != 0; });
+            }
+            // two chains of three-way maxima
+            float top = s[0][0], top1 = s[0][1];
 #pragma unroll
             for (int i = 0; i < SUB; i++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, s[i][e]);
-            top *= factor;
+                for (int e = 0; e < 16; e += 4) {
+                    top = fmaxf(fmaxf(top, s[i][e]), s[i][e + 1]);
+                    top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
+                }
+            top = fmaxf(top, top1) * factor;
             if (__any(top > m + kLift)) {
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float up = fmaxf(m, top);
@@ -1055,6 +1081,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 for (int e = 0; e < DT; e++) o[e] *= keep;
             }
             u32x4 w[PT][SUB][2];
+            float part[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < SUB; i++)
 #pragma unroll
@@ -1062,12 +1089,13 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
                     const float w1 =
                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
-                    sum += w0 + w1;
+                    part[e & 3] += w0 + w1;
                     uint32_t x[PT];
                     terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
 #pragma unroll
                     for (int k = 0; k < PT; k++) w[k][i][e >> 2][e & 3] = x[k];
                 }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
             for (int e = 0; e < DT; e++)
 #pragma unroll
