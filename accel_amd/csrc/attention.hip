@@ -668,17 +668,13 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
 //
 // A workgroup takes 128 rows, 32 a wave: (token, query head of one group) pairs,
 // as many whole tokens as fit, so a tile of keys and values serves the group's
-// heads at once.  Tiles of KT keys go through LDS, staged a tile ahead through
-// registers: K as it lies, V turned by byte permutes into rows of dims with
-// the keys along them.  A wave computes S^T = K Q^T and O^T += V^T P^T with
-// 32 x 32 x 16 MFMAs; a lane has one row's scores and sums (its column), half
-// of the keys, and the other half is 32 lanes on.  As in the decode kernel the
-// keys' order in K's rows is chosen so that a lane's scores are its part of P^T's
-// operand, and the running maximum moves only when scores exceed it by 2^8.
-//
-// LDS words are laid out in 16-byte chunks, a row's chunks exchanged by an
-// exclusive or with the row so that the sixteen rows a read takes at once lie
-// in different banks.
+// heads at once.  Tiles of KT keys go through LDS as they lie, loaded straight
+// there a tile ahead; V is read turned (ds_read_b64_tr_b16).  A wave computes
+// S^T = K Q^T and O^T += V^T P^T with 32 x 32 x 16 MFMAs; a lane has one row's
+// scores and sums (its column), half of the keys, and the other half is 32
+// lanes on.  As in the decode kernel the keys' order in K's rows is chosen so that
+// a lane's scores are its part of P^T's operand, and the running maximum moves
+// only when scores exceed it by 2^8.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -697,6 +693,13 @@ constexpr int kRows = 128;            // rows a workgroup
 // s_waitcnt vmcnt(0), as an instruction that the compiler counts itself.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
+// Four keys of one dim: see the kernel's v_from.
+__device__ __forceinline__ u32x2 read_turned(const char* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s16x4*)p));
+}
+
 // Tokens of a tile of rows, and the query heads of one.
 __host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
 __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
@@ -709,14 +712,11 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int SUB = KT / 32;            // 32-key parts of a tile
     constexpr int DT = DIM / 32;            // 32-dim parts of a row of values
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
-    constexpr int KL = KT * NC / 256;       // chunks of K a lane stages
-    constexpr int VB = KT * DIM / 1024;     // dims of V a lane stages, of four keys
-    constexpr int VW = VB / 2;              // in words
-    constexpr int CK = KT / 8;              // chunks of a row of V^T
+    constexpr int KL = KT * NC / 256;       // chunks of K, and of V, a lane stages
     constexpr bool F32 = QT > 1;
     constexpr float kWeightGain = F32 && !BF16 ? 128.0f : 1.0f;
     __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
-    __shared__ __attribute__((aligned(256))) char v_sh[2][DIM * CK * 16];
+    __shared__ __attribute__((aligned(256))) char v_sh[2][KT * NC * 16];
     // keys of a tile with values that are not finite: tile t's in place t % 3,
     // which is cleared two steps before it is read, a barrier before it is set
     __shared__ uint32_t odd_sh[3][2];
@@ -862,31 +862,25 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         return page;
     };
     // Where chunks lie: linear in the bits of their numbers under exclusive or,
-    // so a lane's address is its own part, exchanged with a constant's.  V^T: 256
-    // bytes hold two rows of eight chunks, or four of four; lanes that read take
-    // consecutive dims, lanes that write every VB-th.
-    const auto k_byte = [](int key, int ch) {
-        return (key * NC + (ch ^ (NC >= 16 ? key & 15 : key >> 1 & 7))) * 16;
-    };
-    const auto v_byte = [](int d, int ck) {
-        return CK == 8 ? ((d ^ (d >> 3 & 1)) * CK + (ck ^ (((d >> 1) ^ (d >> 4)) & 7))) * 16
-                       : (d * CK + (ck ^ (((d >> 2) ^ (d >> 4)) & 3))) * 16;
-    };
-    // what a lane stages: K's chunks straight to LDS, a wave 64 consecutive ones
-    // a step (what the lane reads follows from where it lands); four keys' VB
-    // dims of V through registers
-    uint32_t k_off[KL];                     // bytes from the row of a block's first key
+    // so a lane's address is its own part, exchanged with a constant's.  K's
+    // sixteen rows a read takes at once, and V's four times 64 bytes, fall in
+    // different banks.
+    const auto k_swap = [](int key) { return NC >= 16 ? key & 15 : key >> 1 & 7; };
+    const auto v_swap = [](int key) { return NC >= 16 ? (key & 3) << 2 : (key >> 1 & 1) << 2; };
+    const auto k_byte = [&](int key, int ch) { return (key * NC + (ch ^ k_swap(key))) * 16; };
+    const auto v_byte = [&](int key, int ch) { return (key * NC + (ch ^ v_swap(key))) * 16; };
+    // what a lane stages, straight to LDS: a wave 64 consecutive chunks a step
+    // (what the lane reads follows from where it lands); bytes from the row of
+    // the block's first key, or none past the head's dims
+    constexpr uint32_t kNoChunk = 0xffffffffu;
+    uint32_t k_off[KL], v_off[KL];
 #pragma unroll
     for (int i = 0; i < KL; i++) {
-        const int at = (wave * KL + i) * 64, key = (at + lane) / NC;
-        const int ch = (at + lane) % NC ^ (NC >= 16 ? key & 15 : key >> 1 & 7);
-        k_off[i] = ch * 8 < dim ? (uint32_t)((key & 7) * dim + ch * 8) * 2 : 0xffffffffu;
+        const int at = (wave * KL + i) * 64 + lane, key = at / NC;
+        const int kc = at % NC ^ k_swap(key), vc = at % NC ^ v_swap(key);
+        k_off[i] = FULL || kc * 8 < dim ? (uint32_t)((key & 7) * dim + kc * 8) * 2 : kNoChunk;
+        v_off[i] = FULL || vc * 8 < dim ? (uint32_t)((key & 7) * dim + vc * 8) * 2 : kNoChunk;
     }
-    constexpr int VL = DIM / VB;            // lanes across a row of V
-    const int v_four = threadIdx.x / VL, v_dim = (threadIdx.x % VL) * VB;
-    const uint32_t v_off = ((v_four & 1) * 4 * dim + (FULL || v_dim < dim ? v_dim : 0)) * 2;
-    const int v_to = v_byte(v_dim, v_four >> 1) + (v_four & 1) * 8;
-    uint32_t in[4 * VW];
     // the lanes of blocks 0 .. hold the byte offset of their block's first row
     // in a plane, from which a load's uniform part is read
     const uint32_t row_bytes = (uint32_t)dim * 2;
@@ -899,85 +893,58 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         return (uint64_t)lane_value((uint32_t)rows, b) |
                (uint64_t)lane_value((uint32_t)(rows >> 32), b) << 32;
     };
+    const auto to_lds = [](const char* from, char* to) {
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)from,
+            (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+    };
     const auto load = [&](uint32_t pages, int pos, auto buf) {
+        constexpr int B = decltype(buf)::value;
         const uint64_t rows = block_rows(pages, pos);
 #pragma unroll
         for (int i = 0; i < KL; i++) {
+            // a step's keys lie in one block of eight
             const int at = (wave * KL + i) * 64;
-            const char* row = keys + block_row(rows, at / NC / 8);
-            if (FULL || k_off[i] != 0xffffffffu)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(row + k_off[i]),
-                    (__attribute__((address_space(3))) void*)(k_sh[decltype(buf)::value] + at * 16),
-                    16, 0, 0);
-        }
-        // a wave's lanes hold one block of keys (VL 32) or two
-        const uint64_t row0 = block_row(rows, VL == 32 ? wave : 2 * wave);
-        const uint64_t row1 = VL == 32 ? row0 : block_row(rows, 2 * wave + 1);
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(
-            values + (VL == 32 || lane < 32 ? row0 : row1) + v_off);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (VB == 4) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(src + i * dim);
-                in[2 * i] = w[0], in[2 * i + 1] = w[1];
-            } else {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * dim);
-#pragma unroll
-                for (int e = 0; e < 4; e++) in[4 * i + e] = w[e];
-            }
+            const uint64_t row = block_row(rows, at / NC / 8);
+            if (FULL || k_off[i] != kNoChunk) to_lds(keys + row + k_off[i], k_sh[B] + at * 16);
+            if (FULL || v_off[i] != kNoChunk) to_lds(values + row + v_off[i], v_sh[B] + at * 16);
         }
     };
     // whether every row of the workgroup sees all of the tile
     const auto plain = [&](int pos) {
         return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
     };
-    const auto store = [&](uint32_t pages, int pos, int odd, auto buf) {
+    const auto arrive = [&](uint32_t pages, int pos, int odd, auto buf) {
         constexpr int B = decltype(buf)::value;
-        // K's chunks are in LDS before the barrier that follows
+        // what this wave staged is in LDS before the barrier that follows
         wait_loads();
-        if (!plain(pos) || __any(pages >= c.pages)) {
-            // values no row sees count as 0, whatever they hold; those that are
-            // not finite are left out of the product, where a row that does not
-            // see them would meet them, and added apart.  A 16-bit value whose
-            // exponent is all ones carries into the sign's place.
-            constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
-            constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
-            const uint32_t page = __shfl(pages, v_four >> 1, 64);
-            uint32_t carry[4];
+        if (plain(pos) && !__any(pages >= c.pages)) return;
+        // values no row sees count as 0, whatever they hold; those that are not
+        // finite are left out of the product, where a row that does not see them
+        // would meet them, and added apart.  A 16-bit value whose exponent is
+        // all ones carries into the sign's place.
+        constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+        constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int x = pos + v_four * 4 + i;
-                const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
-                const uint32_t keep = seen ? 0xffffffffu : 0u;
-                carry[i] = 0;
+        for (int i = 0; i < KL; i++) {
+            const int at = (wave * KL + i) * 64 + lane, key = at / NC;
+            const int x = pos + key;
+            const uint32_t page = __shfl(pages, key >> 3, 64);
+            const bool seen = (x < p_end) & ((x >= lo) | (x < near)) & (page < c.pages);
+            u32x4* chunk = reinterpret_cast<u32x4*>(v_sh[B] + at * 16);
+            if (!FULL && v_off[i] == kNoChunk) continue;
+            u32x4 w = {0, 0, 0, 0};
+            if (seen) {
+                w = *chunk;
+                u32x4 over;
 #pragma unroll
-                for (int e = 0; e < VW; e++) {
-                    in[i * VW + e] &= keep;
-                    carry[i] |= (in[i * VW + e] & kExp) + kOne;
-                }
+                for (int e = 0; e < 4; e++) over[e] = ((w[e] & kExp) + kOne) & 0x80008000u;
+                if ((over[0] | over[1] | over[2] | over[3]) == 0) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] &= ~((over[e] >> 15) * 0xffffu);
+                atomicOr(&odd_sh[odd][key >> 5], 1u << (key & 31));
             }
-            if ((carry[0] | carry[1] | carry[2] | carry[3]) & 0x80008000u) {
-                uint32_t bad = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    bad |= carry[i] & 0x80008000u ? 1u << i : 0u;
-#pragma unroll
-                    for (int e = 0; e < VW; e++) {
-                        const uint32_t over = ((in[i * VW + e] & kExp) + kOne) & 0x80008000u;
-                        in[i * VW + e] &= ~((over >> 15) * 0xffffu);
-                    }
-                }
-                atomicOr(&odd_sh[odd][v_four >> 3], bad << (v_four & 7) * 4);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < VB; e++) {
-            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-            const u32x2 w = {
-                __builtin_amdgcn_perm(in[VW + (e >> 1)], in[e >> 1], sel),
-                __builtin_amdgcn_perm(in[3 * VW + (e >> 1)], in[2 * VW + (e >> 1)], sel)};
-            *reinterpret_cast<u32x2*>(v_sh[B] + (v_to ^ v_byte(e, 0))) = w;
+            *chunk = w;
         }
     };
 
@@ -993,13 +960,16 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         pages = page_of(tile_pos(0));
         if (count > 1) pages_next = page_of(tile_pos(1));
         load(pages, tile_pos(0), std::integral_constant<int, 0>());
-        store(pages, tile_pos(0), 0, std::integral_constant<int, 0>());
+        arrive(pages, tile_pos(0), 0, std::integral_constant<int, 0>());
     }
     // the lane's part of what it reads: row 8 x + 4 h + b of K's operand holds
     // key 16 (x / 2) + 8 h + 4 (x % 2) + b
     const int k_from = k_byte(16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3),
                               half);
-    const int v_from = v_byte(col, half);
+    // values through the transposing read: of sixteen lanes four take 32 bytes
+    // of one key's dims, and each receives one dim of the four keys
+    const int v_from = v_byte(half * 8 + (col >> 2 & 3), (col >> 4) * 2 + (col >> 1 & 1)) +
+                       (col & 1) * 8;
     // the queries have arrived: without this the loop's first product waits for
     // every load in flight, each time
     wait_loads();
@@ -1023,16 +993,20 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
             f32x16 s[SUB];
 #pragma unroll
-            for (int i = 0; i < SUB; i++) {
+            for (int i = 0; i < SUB; i++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[i][e] = 0;
 #pragma unroll
-                for (int j = 0; j < NS; j++) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(
+            for (int j = 0; j < NS; j++) {
+                u32x4 kf[SUB];
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+                    kf[i] = *reinterpret_cast<const u32x4*>(
                         k_sh[B] + (k_from ^ k_byte(0, 2 * j)) + k_byte(i * 32, 0));
 #pragma unroll
-                    for (int x = QT - 1; x >= 0; x--) s[i] = mfma32<BF16>(kf, q[x][j], s[i]);
-                }
+                for (int x = QT - 1; x >= 0; x--)
+#pragma unroll
+                    for (int i = 0; i < SUB; i++) s[i] = mfma32<BF16>(kf[i], q[x][j], s[i]);
             }
             // keys a row does not see, by a key's place x in the tile: past the
             // row's position, behind its window, on a page without a number
@@ -1097,15 +1071,17 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 }
             sum += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-            for (int e = 0; e < DT; e++)
+            for (int i = 0; i < SUB; i++)
 #pragma unroll
-                for (int i = 0; i < SUB; i++)
+                for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        constexpr int kLow = CK * 16 - 1;    // a row's chunks
-                        const int at = v_byte(e * 32, i * 4 + j * 2);
-                        const u32x4 vf = *reinterpret_cast<const u32x4*>(
-                            v_sh[B] + (v_from ^ (at & kLow)) + (at & ~kLow));
+                    for (int e = 0; e < DT; e++) {
+                        u32x2 part[2];
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            part[x] = read_turned(v_sh[B] + (v_from ^ v_byte(0, e * 4)) +
+                                                  (i * 32 + j * 16 + x * 4) * NC * 16);
+                        const u32x4 vf = {part[0][0], part[0][1], part[1][0], part[1][1]};
 #pragma unroll
                         for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
                     }
@@ -1136,7 +1112,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         if (more) {
             // every wave has passed the barrier above, so none reads this buffer
             pages = pages_next;
-            store(pages, tile_pos(t + 1), odd_next, other);
+            arrive(pages, tile_pos(t + 1), odd_next, other);
             pages_next = pages_after;
         }
     };
