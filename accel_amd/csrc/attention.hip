@@ -1008,6 +1008,16 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
                     for (int i = 0; i < SUB; i++) s[i] = mfma32<BF16>(kf[i], q[x][j], s[i]);
             }
+            // reads three products ahead of their use
+            if constexpr (QT == 1) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 3 * SUB, 0);
+#pragma unroll
+                for (int j = 0; j < NS - 3; j++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, SUB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, SUB, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 3 * SUB, 0);
+            }
             // keys a row does not see, by a key's place x in the tile: past the
             // row's position, behind its window, on a page without a number
             const int here = pos + half * 8;
