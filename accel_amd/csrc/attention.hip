@@ -700,13 +700,20 @@ __device__ __forceinline__ u32x2 read_turned(const char* p) {
                                          (__attribute__((address_space(3))) s16x4*)p));
 }
 
+// Tiles of keys that are worth a workgroup and its part of a join (5 tokens after
+// 8192, 16-bit: 48 us with two, 31 with four, 29 with eight; 42 tokens a tile of
+// 8 tiles: 25.4 with four, 26.4 with eight).
+template <bool F32>
+constexpr int kTilesAShare = F32 ? 2 : 4;
+
 // Tokens of a tile of rows, and the query heads of one.
 __host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
 __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
 
 template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT>
 __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
-    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t* fault) {
+    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t splits,
+    uint32_t* tickets, uint32_t ticket_stride, float* parts, uint32_t* fault) {
     constexpr int NS = DIM / 16;            // MFMA steps of a score
     constexpr int NC = DIM / 8;             // 16-byte chunks of a key
     constexpr int SUB = KT / 32;            // 32-key parts of a tile
@@ -728,7 +735,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int per = prompt_heads(group), tokens = prompt_tokens(group);
     const int group_tiles = (group + per - 1) / per;
     const uint32_t heads = (uint32_t)(c.heads * group_tiles);
-    const uint32_t order = blockIdx.x / heads, head_tile = blockIdx.x - order * heads;
+    // shares are the slow index: those that have nothing to do come last
+    const uint32_t places = gridDim.x / splits;
+    const uint32_t split = blockIdx.x / places, place = blockIdx.x - split * places;
+    const uint32_t order = place / heads, head_tile = place - order * heads;
     const uint32_t head = head_tile / group_tiles;
     const int g0 = (int)(head_tile - head * group_tiles) * per;
     const int gs = group - g0 < per ? group - g0 : per;
@@ -843,6 +853,16 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int start = lo / KT > sink_tiles ? lo / KT : sink_tiles;
     const int last = p_end > 0 ? (p_end - 1) / KT + 1 : 0;
     const int count = p_end > 0 ? sink_tiles + (last > start ? last - start : 0) : 0;
+    // this workgroup's share of them: where the rows are few, a tile of rows has
+    // several workgroups, each with at least kShare tiles of keys
+    constexpr int kShare = kTilesAShare<F32>;
+    const int shares = count / kShare < (int)splits ? (count / kShare > 0 ? count / kShare : 1)
+                                                    : (int)splits;
+    const int share = (count + shares - 1) / shares;
+    const int held_shares = count > 0 ? (count + share - 1) / share : 1;
+    if ((int)split >= held_shares) return;
+    const int t_begin = (int)split * share;
+    const int t_end = t_begin + share < count ? t_begin + share : count;
     const auto tile_pos = [&](int t) {
         return (t < sink_tiles ? t : start + (t - sink_tiles)) * KT;
     };
@@ -956,11 +976,11 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     uint32_t pages = 0, pages_next = 0;
     if (threadIdx.x < 6) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
     __syncthreads();
-    if (count) {
-        pages = page_of(tile_pos(0));
-        if (count > 1) pages_next = page_of(tile_pos(1));
-        load(pages, tile_pos(0), std::integral_constant<int, 0>());
-        arrive(pages, tile_pos(0), 0, std::integral_constant<int, 0>());
+    if (t_begin < t_end) {
+        pages = page_of(tile_pos(t_begin));
+        if (t_begin + 1 < t_end) pages_next = page_of(tile_pos(t_begin + 1));
+        load(pages, tile_pos(t_begin), std::integral_constant<int, 0>());
+        arrive(pages, tile_pos(t_begin), 0, std::integral_constant<int, 0>());
     }
     // the lane's part of what it reads: row 8 x + 4 h + b of K's operand holds
     // key 16 (x / 2) + 8 h + 4 (x % 2) + b
@@ -979,7 +999,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         constexpr int B = decltype(buf)::value;
         const std::integral_constant<int, B ^ 1> other;
         const int pos = tile_pos(t);
-        const bool more = t + 1 < count;
+        const bool more = t + 1 < t_end;
         unnamed |= pages >= c.pages;
         __syncthreads();
         const uint32_t odd0 = odd_sh[odd_at][0], odd1 = odd_sh[odd_at][1];
@@ -988,7 +1008,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         odd_at = odd_next;
         if (more) load(pages_next, tile_pos(t + 1), other);
         // a whole step ahead of its use
-        const uint32_t pages_after = t + 2 < count ? page_of(tile_pos(t + 2)) : 0;
+        const uint32_t pages_after = t + 2 < t_end ? page_of(tile_pos(t + 2)) : 0;
         // a wave none of whose rows sees the tile only stages
         if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
             f32x16 s[SUB];
@@ -1126,11 +1146,79 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             pages_next = pages_after;
         }
     };
-    for (int t = 0; t < count; t += 2) {
+    for (int t = t_begin; t < t_end; t += 2) {
         step(t, std::integral_constant<int, 0>());
-        if (t + 1 < count) step(t + 1, std::integral_constant<int, 1>());
+        if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>());
     }
     if (unnamed && wave == 0) report(fault, kFaultKvPage);
+    if (held_shares > 1) {
+        // a share's maximum, sum and values as the lanes hold them; the share to
+        // arrive last adds them all, in the shares' order
+        constexpr int kWords = DT * 16 + 2;
+        const auto part = [&](int x) {
+            return reinterpret_cast<uint64_t*>(parts) +
+                   ((size_t)place * splits + x) * (kWords / 2 * 256) + threadIdx.x;
+        };
+        const auto put = [](uint64_t* p, float x, float y) {
+            __hip_atomic_store(p, __builtin_bit_cast(uint64_t, (f32x2){x, y}), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        };
+        const auto get = [](uint64_t* p) {
+            return __builtin_bit_cast(
+                f32x2, __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        };
+        uint64_t* mine = part((int)split);
+        if (real) {
+            put(mine, m, sum);
+#pragma unroll
+            for (int e = 0; e < DT; e++)
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    put(mine + (1 + e * 8 + x) * 256, o[e][2 * x], o[e][2 * x + 1]);
+        }
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __syncthreads();
+        uint32_t* ticket = tickets + (size_t)place * ticket_stride;
+        if (threadIdx.x == 0)
+            odd_sh[0][0] = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (odd_sh[0][0] != (uint32_t)held_shares - 1) return;
+        if (threadIdx.x == 0)
+            __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!real) return;
+        m = kLowest;
+        for (int x = 0; x < held_shares; x++) m = fmaxf(m, get(part(x))[0]);
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < DT; e++)
+#pragma unroll
+            for (int z = 0; z < 16; z++) o[e][z] = 0;
+        // two shares' loads in flight
+        for (int x = 0; x < held_shares; x += 2) {
+            uint64_t* from[2] = {part(x), part(x + 1 < held_shares ? x + 1 : x)};
+            f32x2 ml[2], v[2][DT * 8];
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                ml[y] = get(from[y]);
+#pragma unroll
+                for (int z = 0; z < DT * 8; z++) v[y][z] = get(from[y] + (1 + z) * 256);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                if (x + y >= held_shares) break;
+                const float f = __builtin_amdgcn_exp2f(ml[y][0] - m);
+                sum += f * ml[y][1];
+#pragma unroll
+                for (int z = 0; z < DT * 8; z++) {
+                    o[z >> 3][2 * (z & 7)] += f * v[y][z][0];
+                    o[z >> 3][2 * (z & 7) + 1] += f * v[y][z][1];
+                }
+            }
+        }
+    }
     if (!real) return;
     sum += __shfl_xor(sum, 32, 64);
     const float scale = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
@@ -1227,19 +1315,43 @@ hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, con
     const uint32_t heads = (uint32_t)(c.heads * ((group + per - 1) / per));
     // an entry's last tile may be partly filled
     const uint64_t tiles = (uint64_t)a.rows / tokens + (a.n < a.rows ? a.n : a.rows);
+    const uint64_t bound = tiles * heads;
+    // two workgroups a CU of a 16-bit type up to 128 dims, else one; with fewer
+    // tiles of rows than that, several workgroups share one
+    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 ? 2 : 1);
+    uint32_t splits = bound < slots ? (uint32_t)(slots / bound) : 1;
+    // as many as the longest sequence's keys can be worth
+    const int64_t kt = c.dim <= 128 ? 64 : 32;
+    int64_t most = ((int64_t)c.slots << c.shift) / kt + 1;
+    if (a.window) {
+        const int64_t near = ((int64_t)a.window + tokens) / kt + a.sinks / kt + 3;
+        most = near < most ? near : most;
+    }
+    const int64_t worth = most / (a.q_f32 ? kTilesAShare<true> : kTilesAShare<false>);
+    splits = worth < (int64_t)splits ? (uint32_t)(worth > 1 ? worth : 1) : splits;
+    const int wide = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    const size_t part_words =
+        splits > 1 ? (size_t)(bound * splits) * 256 * (wide / 32 * 16 + 2) : 0;
     const bool summed = a.n > 64;
-    uint32_t* sums = nullptr;
-    if (summed) {
-        char* ws = static_cast<char*>(workspace(d, st, (size_t)a.n * 4, status));
+    const size_t sums_words = summed ? ((size_t)a.n + 1) & ~(size_t)1 : 0;
+    uint32_t *tickets = nullptr, *sums = nullptr;
+    float* parts = nullptr;
+    if (part_words + sums_words) {
+        char* ws = static_cast<char*>(workspace(d, st, (part_words + sums_words) * 4, status));
         if (!ws) return hipSuccess;
-        sums = reinterpret_cast<uint32_t*>(ws + kWorkspaceCounterBytes);
+        tickets = reinterpret_cast<uint32_t*>(ws);
+        parts = reinterpret_cast<float*>(ws + kWorkspaceCounterBytes);
+        if (summed) sums = reinterpret_cast<uint32_t*>(parts + part_words);
+    }
+    if (summed)
         hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
                            sums, d->fault_dev);
-    }
-    const uint32_t fold = (uint32_t)d->cu_count / heads;
-    const dim3 grid((unsigned)(tiles * heads));
+    const uint32_t fold = slots > (uint32_t)d->cu_count ? (uint32_t)d->cu_count / heads : 0;
+    const dim3 grid((unsigned)(bound * splits));
+    const uint32_t stride = (uint32_t)(kWorkspaceCounterBytes / 4) / slots;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, a, sums, fold, d->fault_dev);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, a, sums, fold, splits, tickets,
+                           stride, parts, d->fault_dev);
     };
     const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
     const auto dims = [&](auto bf16, auto qt, auto pt) {

@@ -422,6 +422,28 @@ def test_prompt_values_that_are_not_finite_reach_only_who_sees_them(dev, q, kv, 
         c.free()
 
 
+@types
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1500, 30)])
+def test_prompt_few_rows_after_a_long_prefix(dev, q, kv, window, sinks):
+    """Tiles of rows that several workgroups share, joined in a fixed order."""
+    c = Case(dev, [3000, 700, 2100, 0], new=[5, 64, 1, 0], heads=4, kv_heads=2, q=q, kv=kv)
+    c.check(window=window, sinks=sinks)
+    c.upload()
+    first = None
+    for _ in range(4):
+        c.call(window=window, sinks=sinks)
+        dev.sync()
+        got = c.out.numpy()
+        assert first is None or np.array_equal(first, got)
+        first = got
+    c.free()
+
+
+def test_prompt_few_rows_heads_of_256(dev):
+    Case(dev, [1500, 900], new=[7, 40], heads=6, kv_heads=2, dim=256).check()
+    Case(dev, [1500, 900], new=[7, 40], heads=6, kv_heads=2, dim=200, q=F32).check()
+
+
 def test_a_long_prompt_in_blocks(dev):
     """Rows of a prompt of several tiles against the same prompt in chunks."""
     n = 1100
