@@ -52,24 +52,40 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_
 // to `most`); returns how many there are, or most once there are as many.  A
 // wave tests 64 consecutive pages a step, so the loads are whole lines and a
 // page's rank is a population count of the wave's ballot.
+// `ahead` are the first step's counts, where they have been read already.
+struct Counts {
+    uint32_t r[kScan];
+};
+__device__ __forceinline__ Counts read_counts(const uint32_t* refs, uint32_t base, uint32_t last,
+                                              uint32_t past) {
+    Counts c;
+#pragma unroll
+    for (int j = 0; j < kScan; j++) {
+        const uint32_t page =
+            base + (threadIdx.x >> 6) * 64 * kScan + j * 64 + (threadIdx.x & 63);
+        c.r[j] = page < last ? refs[page] : past;
+    }
+    return c;
+}
+// The pool's first counts, which a search for free pages starts from: asked for
+// before what the call needs is known, so the two wait for memory together.
+__device__ __forceinline__ Counts read_ahead(const KvCache& c) {
+    return read_counts(c.refs, 0, c.pages, 1);
+}
 template <bool FREE>
 __device__ uint32_t list_pages(const uint32_t* refs, uint32_t first, uint32_t last, uint32_t* list,
-                               uint32_t most, uint32_t* sh) {
+                               uint32_t most, uint32_t* sh, const Counts* ahead = nullptr) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t found = 0;
     for (uint32_t base = first; base < last && found < most; base += kPlan * kScan) {
         uint64_t hit[kScan];
         uint32_t count = 0;
         const uint32_t at = base + (uint32_t)wave * 64 * kScan;
-        uint32_t r[kScan];
+        const Counts c = ahead && base == first
+                             ? *ahead : read_counts(refs, base, last, FREE ? 1u : 0u);
 #pragma unroll
         for (int j = 0; j < kScan; j++) {
-            const uint32_t page = at + j * 64 + lane;
-            r[j] = page < last ? refs[page] : (FREE ? 1u : 0u);
-        }
-#pragma unroll
-        for (int j = 0; j < kScan; j++) {
-            hit[j] = __ballot(FREE ? r[j] == 0 : r[j] != 0);
+            hit[j] = __ballot(FREE ? c.r[j] == 0 : c.r[j] != 0);
             count += __popcll(hit[j]);
         }
         uint32_t total;
@@ -88,19 +104,44 @@ __device__ uint32_t list_pages(const uint32_t* refs, uint32_t first, uint32_t la
     return found < most ? found : most;
 }
 
-// Whether entry i is the first to name sequence s.  mark [sequences]; the
-// whole workgroup calls it for all entries at once.
-__device__ void mark_first(const KvCache& c, const uint32_t* seqs, int n, uint32_t* mark) {
-    for (int i = threadIdx.x; i < n; i += kPlan)
-        if (seqs[i] < c.sequences)
-            __hip_atomic_store(mark + seqs[i], 0xffffffffu, __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kPlan)
-        if (seqs[i] < c.sequences)
-            __hip_atomic_fetch_min(mark + seqs[i], (uint32_t)i, __ATOMIC_RELAXED,
+// A planning workgroup's scratch in LDS, for calls small enough: each round trip
+// to memory it saves is most of a microsecond.
+constexpr uint32_t kNearMarks = 4096, kNearList = 2048;
+struct PlanScratch {
+    uint32_t sums[kPlanWaves];
+    uint32_t marks[kNearMarks];
+    uint32_t list[kNearList];
+};
+
+// For each sequence the first entry that names it, in sh or `far` [sequences];
+// the whole workgroup calls it for all entries at once.
+struct Marks {
+    PlanScratch* sh;
+    uint32_t* far;
+    bool near;
+    __device__ uint32_t first(uint32_t s) const { return near ? sh->marks[s] : load_fresh(far + s); }
+};
+__device__ Marks mark_first(const KvCache& c, const uint32_t* seqs, int n, PlanScratch* sh,
+                            uint32_t* far) {
+    const Marks m = {sh, far, c.sequences <= kNearMarks};
+    if (m.near) {
+        for (uint32_t s = threadIdx.x; s < c.sequences; s += kPlan) sh->marks[s] = 0xffffffffu;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kPlan)
+            if (seqs[i] < c.sequences) atomicMin(&sh->marks[seqs[i]], (uint32_t)i);
+    } else {
+        for (int i = threadIdx.x; i < n; i += kPlan)
+            if (seqs[i] < c.sequences)
+                __hip_atomic_store(far + seqs[i], 0xffffffffu, __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kPlan)
+            if (seqs[i] < c.sequences)
+                __hip_atomic_fetch_min(far + seqs[i], (uint32_t)i, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+    }
     __syncthreads();
+    return m;
 }
 
 __global__ __launch_bounds__(256) void kv_fill_kernel(uint32_t* p, size_t n, uint32_t v) {
@@ -114,9 +155,11 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
                                                            const uint32_t* grow, int n,
                                                            uint32_t* list, uint32_t* first,
                                                            uint32_t* mark, uint32_t* fault) {
-    __shared__ uint32_t sh[kPlanWaves];
+    __shared__ PlanScratch sh;
     const uint32_t cap = c.slots << c.shift, up = (1u << c.shift) - 1;
-    if (seqs) mark_first(c, seqs, n, mark);
+    const Counts ahead = read_ahead(c);
+    Marks marks = {};
+    if (seqs) marks = mark_first(c, seqs, n, &sh, mark);
     // what each entry needs, and where its pages begin in the list; an entry
     // that cannot be served is marked and needs none
     constexpr uint32_t kLeftOut = 0xffffffffu;
@@ -128,7 +171,7 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
         if (i < n) {
             const uint32_t s = sequence_of(c, seqs, i, fault);
             if (s != kNoSequence) {
-                if (seqs && load_fresh(mark + s) != (uint32_t)i) {
+                if (seqs && marks.first(s) != (uint32_t)i) {
                     report(fault, kFaultKvSequence);
                 } else {
                     const uint32_t len = c.lens[s], g = grow[i];
@@ -143,13 +186,15 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
         }
         // the sum stays below sequences * slots, which is below 2^31
         uint32_t total;
-        const uint32_t at = needed + block_scan(need, sh, &total);
+        const uint32_t at = needed + block_scan(need, sh.sums, &total);
         if (i < n) first[i] = ok ? at : kLeftOut;
         needed += total;
     }
     const uint32_t want = needed < c.pages ? needed : c.pages;
+    if (want <= kNearList) list = sh.list;
     __syncthreads();
-    const uint32_t found = want ? list_pages<true>(c.refs, 0, c.pages, list, want, sh) : 0;
+    const uint32_t found =
+        want ? list_pages<true>(c.refs, 0, c.pages, list, want, sh.sums, &ahead) : 0;
     __syncthreads();
     // a wave an entry: the slots of a long prompt are filled side by side
     const int lane = threadIdx.x & 63;
@@ -253,7 +298,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, size_t layer_
 }
 
 // A branch as planned: how many whole pages it shares, and the copy of the
-// last one (from, to; ACCEL_KV_NONE: none).
+// last one (from, to; ACCEL_KV_NONE: none).  ok: its length and one, 0 for an
+// entry left out.
 struct Branch {
     uint32_t whole, from, to, ok;
 };
@@ -264,20 +310,22 @@ __global__ __launch_bounds__(kPlan) void kv_fork_plan_kernel(KvCache c, const ui
                                                              const uint32_t* children, int n,
                                                              uint32_t* list, Branch* plan,
                                                              uint32_t* mark, uint32_t* fault) {
-    __shared__ uint32_t sh[kPlanWaves];
-    mark_first(c, children, n, mark);
-    uint32_t needed = 0;
+    __shared__ PlanScratch sh;
+    const Counts ahead = read_ahead(c);
+    const Marks marks = mark_first(c, children, n, &sh, mark);
+    uint32_t needed = 0, child = kNoSequence;
+    Branch b = {};
     for (int base = 0; base < n; base += kPlan) {
         const int i = base + threadIdx.x;
-        Branch b = {0, ACCEL_KV_NONE, ACCEL_KV_NONE, 0};
+        b = {0, ACCEL_KV_NONE, ACCEL_KV_NONE, 0};
         if (i < n) {
-            const uint32_t p = parents[i], s = children[i];
+            const uint32_t p = parents[i], s = child = children[i];
             if (p < c.sequences && s < c.sequences) {
-                if (load_fresh(mark + s) != (uint32_t)i || c.lens[s] != 0) {
+                if (marks.first(s) != (uint32_t)i || c.lens[s] != 0) {
                     report(fault, kFaultKvSequence);
                 } else {
                     const uint32_t len = length_of(c, p);
-                    b.ok = 1;
+                    b.ok = len + 1;
                     b.whole = len >> c.shift;
                     if (len & ((1u << c.shift) - 1)) {
                         const uint32_t last = c.tables[(size_t)p * c.slots + b.whole];
@@ -292,36 +340,36 @@ __global__ __launch_bounds__(kPlan) void kv_fork_plan_kernel(KvCache c, const ui
         }
         uint32_t total;
         const bool wants = b.ok && b.from != ACCEL_KV_NONE;
-        const uint32_t at = needed + block_scan(wants ? 1u : 0u, sh, &total);
+        const uint32_t at = needed + block_scan(wants ? 1u : 0u, sh.sums, &total);
         // the place in the list until the list is there
         if (i < n) {
             b.to = wants ? at : ACCEL_KV_NONE;
-            plan[i] = b;
+            if (n > kPlan) plan[i] = b;
         }
         needed += total;
     }
     const uint32_t want = needed < c.pages ? needed : c.pages;
+    if (want <= kNearList) list = sh.list;
     __syncthreads();
-    const uint32_t found = want ? list_pages<true>(c.refs, 0, c.pages, list, want, sh) : 0;
+    const uint32_t found =
+        want ? list_pages<true>(c.refs, 0, c.pages, list, want, sh.sums, &ahead) : 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kPlan) {
-        Branch b = plan[i];
-        if (!b.ok) continue;
-        uint32_t len = length_of(c, parents[i]);
-        if (b.to != ACCEL_KV_NONE) {
+        if (n > kPlan) {
+            b = plan[i];
+            child = children[i];
+        }
+        if (b.ok && b.to != ACCEL_KV_NONE) {
             if (b.to < found) {
                 b.to = list[b.to];
                 c.refs[b.to] = 1;
             } else {
                 report(fault, kFaultKvRoom);
                 b = {0, ACCEL_KV_NONE, ACCEL_KV_NONE, 0};
-                len = 0;
             }
-            plan[i] = b;
         }
-        // a child was empty, so no other entry's parent reads another length
-        // than the one it had
-        if (len) c.lens[children[i]] = len;
+        plan[i] = b;
+        if (b.ok > 1) c.lens[child] = b.ok - 1;
     }
 }
 

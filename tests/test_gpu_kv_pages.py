@@ -185,6 +185,20 @@ def test_many_sequences(dev):
     b.compact()
 
 
+def test_more_branches_than_a_workgroup_plans_at_once(dev):
+    """Entries past the planning workgroup's lanes; a child that a later entry
+    names as its parent counts as empty there; more marks and pages than LDS holds."""
+    b = Both(dev, layers=1, pages=9000, kv_heads=1, page=8, dim=8, sequences=6000, slots=3)
+    b.reserve([5, 17, 8], [0, 1, 2])
+    kids = list(range(10, 2300))
+    parents = [k % 3 for k in kids]
+    parents[1500] = kids[3]
+    b.fork(parents, kids)
+    b.reserve([9] * 2400, list(range(2400)))
+    b.free(kids[::2])
+    b.compact()
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_lives(dev, seed):
     rng = np.random.default_rng(seed)
