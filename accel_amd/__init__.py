@@ -539,6 +539,7 @@ class KVCache:
     def free(self) -> None:
         for b in (self.keys, self.values, self.refs, self.tables, self.lens):
             b.free()
+        self._desc = KVCacheDesc()       # refused by every operator
 
 
 def _opt(buffer):

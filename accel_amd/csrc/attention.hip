@@ -180,11 +180,13 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-// The entry whose tiles hold x of the line; *start its first tile.
+// The entry whose tiles hold x of the line (an entry in any case: sums over
+// offsets that do not ascend may wrap); *start its first tile.
 __device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* start) {
     const int lane = threadIdx.x & 63;
     if (!k.sums) {
-        const int i = __popcll(__ballot(lane < k.n && k.lane_sum <= x));
+        int i = __popcll(__ballot(lane < k.n && k.lane_sum <= x));
+        i = i < k.n ? i : k.n - 1;
         *start = i ? lane_value(k.lane_sum, i - 1) : 0;
         return i;
     }
@@ -199,7 +201,8 @@ __device__ __forceinline__ int find_entry(const Cut& k, uint32_t x, uint32_t* st
         size = size - skip < step ? size - skip : step;
     }
     const uint64_t below = __ballot(lane < size && k.sums[lo + lane] <= x);
-    const int i = __builtin_amdgcn_readfirstlane(lo + __popcll(below));
+    int i = __builtin_amdgcn_readfirstlane(lo + __popcll(below));
+    i = i < k.n ? i : k.n - 1;
     *start = i ? __builtin_amdgcn_readfirstlane(k.sums[i - 1]) : 0;
     return i;
 }
@@ -768,6 +771,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int entry = find_entry(cut, tile, &item);
     const Rows rows = rows_of(a, entry);
     const uint32_t tok0 = (tile - item) * tokens;
+    if (tok0 >= rows.count) return;      // offsets that do not ascend
     const uint32_t toks = rows.count - tok0 < (uint32_t)tokens ? rows.count - tok0 : tokens;
     const Held held = held_by(c, a, entry, threadIdx.x ? nullptr : fault);
     // the position of the tile's first token; below 0 it sees nothing

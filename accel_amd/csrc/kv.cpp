@@ -364,7 +364,8 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
     if (!valid_tensor(out) || out->dtype != q->dtype || out->rank != 3 || !same_rows(out, q))
         return refuse(op, "the output must have the queries' shape and type");
     const int64_t T = q->shape[0], H = q->shape[1];
-    if (H > 65536 || T > INT32_MAX / H)
+    // a prompt's tiles of rows are at most two a row
+    if (H > 65536 || T > INT32_MAX / 2 / H)
         return refuse(op, "more rows than a launch's 31-bit grid indexes");
     if (T && (!q->data || !out->data)) return refuse(op, "an operand is missing");
     if (!aligned16(q->data) || !aligned16(out->data))

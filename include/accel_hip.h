@@ -645,7 +645,8 @@ int accel_kv_reserve(int dev, void* stream, const accel_kv_cache_t* cache,
  * u32 [n+1], ascending from 0; NULL: one row an entry, n = T.  seqs u32 [n];
  * NULL: i.  Rows past the last offset and rows of ACCEL_KV_NONE are skipped.
  * A position before the sequence's first, or without a page, is skipped and
- * reported. */
+ * reported.  Of two entries with one sequence it is not specified whose rows
+ * stay. */
 int accel_kv_append(int dev, void* stream, const accel_kv_cache_t* cache, int64_t layer,
                     const accel_tensor_t* k, const accel_tensor_t* v,
                     const accel_tensor_t* seqs, const accel_tensor_t* offsets);

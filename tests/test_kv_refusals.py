@@ -172,6 +172,20 @@ def test_attention_types_options_and_lists():
             "queries are missing")
 
 
+def test_a_freed_cache_is_refused():
+    class Held:
+        ptr, dtype, shape = A, BF16, (1, 4, 2, 16, 64)
+
+        def free(self):
+            self.ptr = 0
+
+    k = Held()
+    b = lambda shape: accel_amd.Buffer(None, 0, 0, U32, shape)  # noqa: E731
+    c = accel_amd.KVCache(None, k, k, b((4,)), b((3, 2)), b((3,)))
+    c.free()
+    refused(L.accel_kv_clear(0, None, R(c.desc())), "needs keys")
+
+
 def test_a_closed_device_is_named():
     rc = L.accel_kv_clear(63, None, R(cache()))
     assert rc == accel_amd.E_NO_DEVICE, accel_amd.last_error()
