@@ -753,6 +753,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     cut.n = a.n;
     cut.sums = sums;
     if (!sums) {
+        // lengths are asked for beside the offsets, not after them
+        cut.lane_held = {kNoSequence, 0};
+        if (lane < a.n) cut.lane_held = held_by(c, a, lane, blockIdx.x ? nullptr : fault);
         uint32_t v = lane < a.n ? (rows_of(a, lane).count + tokens - 1) / tokens : 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -773,7 +776,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const uint32_t tok0 = (tile - item) * tokens;
     if (tok0 >= rows.count) return;      // offsets that do not ascend
     const uint32_t toks = rows.count - tok0 < (uint32_t)tokens ? rows.count - tok0 : tokens;
-    const Held held = held_by(c, a, entry, threadIdx.x ? nullptr : fault);
+    const Held held = sums ? held_by(c, a, entry, threadIdx.x ? nullptr : fault)
+                           : entry_held(cut, c, a, entry);
     // the position of the tile's first token; below 0 it sees nothing
     const int base = (int)held.len - (int)rows.count + (int)tok0;
     const int window = a.window ? (int)a.window : 0x7fffffff;
