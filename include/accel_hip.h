@@ -28,8 +28,9 @@
  * []uint16", internal/kernels/differential_darwin_test.go:242-244).
  *
  * Workspace.  Kernels that reduce across workgroups (the decode product's
- * K split) and the grouped products (segment offsets, tile lists) use a
- * per-device workspace owned by the library.  Two operator calls that run
+ * K split, the joins of paged attention), the grouped products (segment
+ * offsets, tile lists) and the paged cache's planning use a per-device
+ * workspace owned by the library.  Two operator calls that run
  * concurrently on different streams of one device race on it; serialize
  * them or use one stream per device.  The workspace grows on demand outside
  * graph capture; a call that would need it to grow on a capturing stream is
@@ -38,7 +39,8 @@
  * executable stays valid across later, larger eager calls.
  *
  * Faults.  A kernel that gives up instead of producing its result (a
- * split-K hand-off whose bounded wait runs out) records it in the device's
+ * split-K hand-off whose bounded wait runs out), or that leaves out an entry
+ * of a paged cache's call that cannot be served, records it in the device's
  * fault word; the next
  * stream_sync, event_sync or event_query that completes reports it as
  * ACCEL_E_HIP with a message, and clears it (the analogue of the
