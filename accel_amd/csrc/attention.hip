@@ -35,9 +35,8 @@
 // 1 to 8192 tokens in bf16 194 us, 5.5 TB/s of keys and values (a copy of 4 GiB
 // moves 4.6); one of 32768 in f32 35 us, 3.9 TB/s; one of 200 tokens 8 us, four
 // dependent reads of memory (length, table, keys, then the way out through
-// LDS).  Many sequences of a few tiles are bound by that chain too: a workgroup
-// walks its sequences one after the other (200 of 1 to 300 tokens: 56 us, the
-// bytes 27).
+// LDS).  Many sequences of a few tiles are bound by that chain too, so runs of
+// them go to a wave each (kAlone).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -104,6 +103,12 @@ constexpr float kLowest = -3.0e38f;   // the maximum before any key
 // us with 24, 15.5 with 12 or 8; 33 sequences seen through a window of 1000, 33
 // tiles each: 13.7, 14.3 and 15.5.
 constexpr uint32_t kNear = 12;
+
+// Sequences of up to this many tiles are taken by a wave each where as many of
+// them follow each other (256 of 50 to 150 tokens 59 -> 37 us; 200 of 1 to 300
+// 56 -> 45 with up to 8 tiles, 40 with 12 or 16).
+constexpr uint32_t kAlone = 12;
+constexpr int kManyAlone = 3;
 
 // The keys a query at position n - 1 sees: [0, first) and [lo, n); the tiles
 // that hold them, in order.
@@ -313,7 +318,8 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, s
 template <int DIM>
 constexpr int kWaves = DIM > 128 ? 4 : 8;
 
-template <bool BF16, int QT, int PT, int DIM, bool FULL>
+// MANY: a workgroup may have a run of short sequences.
+template <bool BF16, int QT, int PT, int DIM, bool FULL, bool MANY>
 __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
     KvCache c, Attention a, const uint32_t* sums, uint32_t stretches, uint32_t* tickets,
     uint32_t ticket_stride, float* parts, uint32_t* fault) {
@@ -378,12 +384,53 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
     const size_t layer = (size_t)a.layer * c.pages * c.page_elems();
     while (u < u_end) {
         uint32_t item;
-        const int entry = find_entry(cut, u, &item);
-        const Held held = entry_held(cut, c, a, entry);
+        int entry = find_entry(cut, u, &item);
+        Held held = entry_held(cut, c, a, entry);
+        Span sp = span_of(a, held.len);
+        uint32_t t0 = u - item;
+        uint32_t t1 = sp.tiles - t0 <= u_end - u ? sp.tiles : t0 + (u_end - u);
+        uint32_t u_next = u + (t1 - t0);
+        // Short sequences one after the other: a wave each, so that the waves'
+        // chains of reads run side by side.  A lane an entry from this one on:
+        // those up to the first that is too long, or not wholly in the stretch.
+        uint64_t mine = 1;
+        bool alone = false;
+        Held lane_held = {kNoSequence, 0};
+        if (MANY && t0 == 0 && t1 == sp.tiles && sp.tiles <= kAlone && u_next < u_end) {
+            const int e = entry + lane;
+            if (!sums)
+                lane_held = {__shfl(cut.lane_held.seq, e & 63, 64),
+                             __shfl(cut.lane_held.len, e & 63, 64)};
+            else if (e < a.n)
+                lane_held = held_by(c, a, e, nullptr);
+            const uint32_t own = e < a.n ? span_of(a, lane_held.len).tiles : 0;
+            uint32_t past = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(past, d, 64);
+                if (lane >= d) past += up;
+            }
+            const uint64_t stop = __ballot(e >= a.n || own > kAlone || past > u_end - u);
+            const int run = stop ? __builtin_ctzll(stop) : 64;
+            const uint64_t items = __ballot(lane < run && own != 0);
+            alone = __popcll(items) >= kManyAlone;
+            if (alone) {
+                const int rank = __popcll(items & ((1ull << lane) - 1));
+                mine = __ballot((items >> lane & 1) && rank % W == wave);
+                u_next = u + lane_value(past, run - 1);
+            }
+        }
+        const int entry0 = entry;
+        for (; mine; mine &= mine - 1) {
+        uint32_t t_first = t0 + wave, stride = W;
+        if (alone) {
+            const int l = __builtin_ctzll(mine);
+            entry = entry0 + l;
+            held = {lane_value(lane_held.seq, l), lane_value(lane_held.len, l)};
+            sp = span_of(a, held.len);
+            t0 = 0, t1 = sp.tiles, t_first = 0, stride = 1;
+        }
         const uint32_t seq = held.seq;
-        const Span sp = span_of(a, held.len);
-        const uint32_t t0 = u - item;
-        const uint32_t t1 = sp.tiles - t0 <= u_end - u ? sp.tiles : t0 + (u_end - u);
         const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
 
         // queries: the B operand, column = query head
@@ -508,22 +555,22 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
             }
         };
 
-        uint32_t t = t0 + wave;
+        uint32_t t = t_first;
         uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
         if (t < t1) {
             pos = tile_pos(t);
             k_page = page_of(pos + k_block * 8);
             v_page = page_of(pos + quad * 8);
-            if (t + W < t1) {
-                k_next = page_of(tile_pos(t + W) + k_block * 8);
-                v_next = page_of(tile_pos(t + W) + quad * 8);
+            if (t + stride < t1) {
+                k_next = page_of(tile_pos(t + stride) + k_block * 8);
+                v_next = page_of(tile_pos(t + stride) + quad * 8);
             }
             load_k(k_page, pos);
             load_v(v_page, pos);
         }
-        for (; t < t1; t += W) {
-            const bool more = t + W < t1;
-            const uint32_t pos_next = more ? tile_pos(t + W) : 0;
+        for (; t < t1; t += stride) {
+            const bool more = t + stride < t1;
+            const uint32_t pos_next = more ? tile_pos(t + stride) : 0;
             // scores
             f32x4 s[2];
 #pragma unroll
@@ -603,8 +650,8 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                 load_v(v_next, pos_next);
                 v_page = v_next;
                 pos = pos_next;
-                if (t + 2 * W < t1) {
-                    const uint32_t after = tile_pos(t + 2 * W);
+                if (t + 2 * stride < t1) {
+                    const uint32_t after = tile_pos(t + 2 * stride);
                     k_next = page_of(after + k_block * 8);
                     v_next = page_of(after + quad * 8);
                 }
@@ -612,6 +659,19 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
         }
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
+        if (alone) {
+            const float out = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < VD; e++) {
+                    const int d = (quad * 4 + i) * VD + e;
+                    if (col < cols && (FULL || d < dim))
+                        store_result(c, a, qrow + (size_t)col * dim + d,
+                                     sum == 0 ? 0.0f : o[e][i] * out);
+                }
+            continue;
+        }
 
         // the waves' parts of this pair
         __syncthreads();
@@ -673,7 +733,8 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
-        u += t1 - t0;
+        }
+        u = u_next;
     }
 }
 
@@ -1274,26 +1335,26 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         }
 }
 
-template <bool BF16, int QT, int PT, int DIM, bool FULL>
+template <bool BF16, int QT, int PT, int DIM, bool FULL, bool MANY>
 void decode(Device* d, hipStream_t st, const KvCache& c, const Attention& a, const uint32_t* sums,
             uint32_t heads, uint32_t stretches, uint32_t* tickets, float* parts) {
     const uint32_t grid = heads * stretches;
-    hipLaunchKernelGGL((paged_decode_kernel<BF16, QT, PT, DIM, FULL>), dim3(grid),
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, QT, PT, DIM, FULL, MANY>), dim3(grid),
                        dim3(64 * kWaves<DIM>), 0, st, c, a, sums, stretches, tickets,
                        (uint32_t)(kWorkspaceCounterBytes / 4) / grid, parts, d->fault_dev);
 }
 
-template <bool BF16, int QT, int PT>
+template <bool BF16, int QT, int PT, bool MANY>
 void decode_dims(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
                  const uint32_t* sums, uint32_t heads, uint32_t stretches, uint32_t* tickets,
                  float* parts) {
     const auto go = [&](auto f) { f(d, st, c, a, sums, heads, stretches, tickets, parts); };
-    if (c.dim == 64) go(decode<BF16, QT, PT, 64, true>);
-    else if (c.dim < 64) go(decode<BF16, QT, PT, 64, false>);
-    else if (c.dim == 128) go(decode<BF16, QT, PT, 128, true>);
-    else if (c.dim < 128) go(decode<BF16, QT, PT, 128, false>);
-    else if (c.dim == 256) go(decode<BF16, QT, PT, 256, true>);
-    else go(decode<BF16, QT, PT, 256, false>);
+    if (c.dim == 64) go(decode<BF16, QT, PT, 64, true, MANY>);
+    else if (c.dim < 64) go(decode<BF16, QT, PT, 64, false, MANY>);
+    else if (c.dim == 128) go(decode<BF16, QT, PT, 128, true, MANY>);
+    else if (c.dim < 128) go(decode<BF16, QT, PT, 128, false, MANY>);
+    else if (c.dim == 256) go(decode<BF16, QT, PT, 256, true, MANY>);
+    else go(decode<BF16, QT, PT, 256, false, MANY>);
 }
 
 }  // namespace
@@ -1328,12 +1389,16 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
         f(d, st, c, a, summed ? sums : nullptr, heads, stretches,
           reinterpret_cast<uint32_t*>(ws), parts);
     };
+    // Runs of short sequences need more than one a stretch, on average two; with
+    // fewer the search for them costs 0.3 us and finds nothing (one of 200 tokens
+    // 8.1 against 8.5 us).
+    const bool many = (uint64_t)a.n * heads >= 2 * (uint64_t)d->cu_count;
     if (a.q_f32) {
-        if (c.bf16) go(decode_dims<true, 3, 3>);
-        else go(decode_dims<false, 2, 2>);
+        if (c.bf16) many ? go(decode_dims<true, 3, 3, true>) : go(decode_dims<true, 3, 3, false>);
+        else many ? go(decode_dims<false, 2, 2, true>) : go(decode_dims<false, 2, 2, false>);
     } else {
-        if (c.bf16) go(decode_dims<true, 1, 2>);
-        else go(decode_dims<false, 1, 2>);
+        if (c.bf16) many ? go(decode_dims<true, 1, 2, true>) : go(decode_dims<true, 1, 2, false>);
+        else many ? go(decode_dims<false, 1, 2, true>) : go(decode_dims<false, 1, 2, false>);
     }
     return hipGetLastError();
 }

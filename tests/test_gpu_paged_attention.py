@@ -189,6 +189,27 @@ def test_decode_ragged_batch(dev, q, kv):
 
 
 @types
+@pytest.mark.parametrize("dim", [40, 64, 128, 200])
+@pytest.mark.parametrize("n", [61, 150])
+def test_decode_many_short_sequences(dev, q, kv, dim, n):
+    """Enough sequences that runs of short ones go to a wave each, long and
+    empty ones between them; a lane's or a table's lookup of them."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 200, n)]
+    for i in (5, 17, 18, 40):
+        lens[i] = 0
+    lens[11], lens[30], lens[-1] = 900, 390, 1
+    seqs = [int(x) for x in rng.permutation(n)]
+    seqs[7] = KV_NONE
+    # heads of one group each: 512 pairs or more
+    heads = -(-512 // n)
+    Case(dev, lens, heads=heads, kv_heads=heads, dim=dim, page=8, q=q, kv=kv, seqs=seqs,
+         seed=n).check()
+    Case(dev, lens, heads=heads, kv_heads=heads, dim=dim, page=8, q=q, kv=kv, seqs=seqs,
+         seed=n).check(window=70, sinks=5)
+
+
+@types
 @pytest.mark.parametrize("n", [4000, 20001])
 def test_decode_split_over_a_long_cache(dev, q, kv, n):
     Case(dev, [n, 5, n // 3], heads=2, kv_heads=1, q=q, kv=kv, seed=n).check()
