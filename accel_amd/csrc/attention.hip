@@ -832,7 +832,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 
     // this workgroup's tile of rows: the longest (last) ones first; where all
     // tiles run at once, two a CU, the second half of them shortest first, so
-    // that a long one shares its CU with a short one
+    // that a long one shares its CU with a short one (two prompts of 1024, 64
+    // dims: 32 -> 28 us)
     Cut cut;
     cut.n = a.n;
     cut.sums = sums;

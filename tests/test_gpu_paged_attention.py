@@ -488,6 +488,32 @@ def test_a_long_prompt_in_blocks(dev):
     c.free()
 
 
+def test_keys_far_apart_in_a_large_cache(dev):
+    """Offsets past 32 bits: the last pages of layer 1 of 2.3e9 elements a plane
+    give what the first pages of a small cache give, bit for bit."""
+    rng = np.random.default_rng(2)
+    KV, P, D, H, n = 8, 256, 256, 16, 700
+    k, v = (rng.standard_normal((n, KV, D)).astype(np.float32) for _ in range(2))
+    q = narrow(rng.standard_normal((40, H, D)) * 2, BF16)
+    u = lambda x: dev.upload(np.asarray(x, np.uint32), U32)  # noqa: E731
+    res = []
+    for layers, pages, before in ((2, 2200, 2197), (1, 3, 0)):
+        c = dev.kv_cache(layers, pages, KV, P, D, 2, 2200)
+        if before:
+            dev.KVReserve(c, u([before * P]), u([1]))
+        dev.KVReserve(c, u([n]), u([0]))
+        dev.KVAppend(c, layers - 1, dev.upload(k), dev.upload(v), u([0]), u([0, n]))
+        one, many = dev.alloc((1, H, D), BF16), dev.alloc((40, H, D), BF16)
+        dev.PagedAttention(dev.upload(q[:1], BF16), c, one, layer=layers - 1, seqs=u([0]))
+        dev.PagedPrefill(dev.upload(q, BF16), u([0, 40]), c, many, layer=layers - 1, seqs=u([0]))
+        dev.sync()
+        assert c.tables.numpy()[0, 0] == before
+        res.append((one.numpy(), many.numpy()))
+        c.free()
+    for a, b in zip(*res):
+        assert np.array_equal(a, b) and np.isfinite(widen(a, BF16)).all()
+
+
 # ---- together ---------------------------------------------------------------------
 
 @types
