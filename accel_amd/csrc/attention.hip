@@ -777,8 +777,13 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 
 constexpr int kRows = 128;            // rows a workgroup
 
-// s_waitcnt vmcnt(0), as an instruction that the compiler counts itself.
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// s_waitcnt vmcnt(0), as an instruction that the compiler counts itself; reads of
+// what the loads brought to LDS stay behind it.
+__device__ __forceinline__ void wait_loads() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
 
 // Four keys of one dim: see the kernel's v_from.
 __device__ __forceinline__ u32x2 read_turned(const char* p) {
