@@ -242,15 +242,15 @@ __device__ __forceinline__ uint32_t cut_at(const Cut& k, const KvCache& c, const
 }
 
 // The join of a sequence's parts (of workgroups w0, w0 + 1 .. of the head) by the
-// whole workgroup: sum and values scaled to
-// the largest maximum and added in the parts' order.  A part is (maximum, sum)
-// of each column, then the columns' values.  The maxima of all parts are read
-// at once and the parts' factors kept in LDS (`room` floats), then a lane takes
-// two dims of a column, BATCH parts' loads in flight.
+// whole workgroup: sum and values scaled to the largest maximum and added in the
+// parts' order.  A part is (maximum, sum) of each column, then the columns'
+// values.  The maxima of all parts are read at once and the parts' factors kept
+// in LDS (`room` floats), then a lane takes two dims of a column, BATCH parts'
+// loads in flight.
 template <int WAVES, int BATCH>
 __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, size_t slot_size,
-                           uint32_t w0, uint32_t heads, uint32_t head, int count, int cols, int dim, size_t qrow, float* sh,
-                           int room) {
+                           uint32_t w0, uint32_t heads, uint32_t head, int count, int cols,
+                           int dim, size_t qrow, float* sh, int room) {
     const auto slot = [&](int p) {
         return parts + (2 * ((w0 + p) * (size_t)heads + head) + (p == 0 ? 1 : 0)) * slot_size;
     };
@@ -297,7 +297,8 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, s
             for (int p0 = 0; p0 < count; p0 += BATCH) {
                 f32x2 v[BATCH];
 #pragma unroll
-                for (int x = 0; x < BATCH; x++) v[x] = load2(slot(p0 + x < count ? p0 + x : p0) + at);
+                for (int x = 0; x < BATCH; x++)
+                    v[x] = load2(slot(p0 + x < count ? p0 + x : p0) + at);
 #pragma unroll
                 for (int x = 0; x < BATCH; x++) {
                     const float f = p0 + x < count ? factor[g * count + p0 + x] : 0.0f;
@@ -422,317 +423,321 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
         }
         const int entry0 = entry;
         for (; mine; mine &= mine - 1) {
-        uint32_t t_first = t0 + wave, stride = W;
-        if (alone) {
-            const int l = __builtin_ctzll(mine);
-            entry = entry0 + l;
-            held = {lane_value(lane_held.seq, l), lane_value(lane_held.len, l)};
-            sp = span_of(a, held.len);
-            t0 = 0, t1 = sp.tiles, t_first = 0, stride = 1;
-        }
-        const uint32_t seq = held.seq;
-        const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
-
-        // queries: the B operand, column = query head
-        u32x4 q[QT][NJ];
-        float factor = a.scale * 1.44269504088896340736f;
-        if constexpr (F32) {
-            const float* src = static_cast<const float*>(a.q) + qrow + (size_t)col * dim;
-            float v[NJ][8];
-            float top = 0;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                const int d = j * 32 + quad * 8;
-                const bool in = col < cols && d < dim;
-                f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-                if (in) {
-                    lo = *reinterpret_cast<const f32x4*>(src + d);
-                    hi = *reinterpret_cast<const f32x4*>(src + d + 4);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[j][e] = e < 4 ? lo[e] : hi[e - 4];
-                    top = fmaxf(top, fabsf(v[j][e]));
-                }
+            uint32_t t_first = t0 + wave, stride = W;
+            if (alone) {
+                const int l = __builtin_ctzll(mine);
+                entry = entry0 + l;
+                held = {lane_value(lane_held.seq, l), lane_value(lane_held.len, l)};
+                sp = span_of(a, held.len);
+                t0 = 0, t1 = sp.tiles, t_first = 0, stride = 1;
             }
-            if constexpr (!BF16) {
-                // f16 terms: the row's largest value goes to [2^14, 2^15)
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const int ex = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-                factor *= ldexpf(1.0f, -ex);
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[j][e] = ldexpf(v[j][e], ex);
-            }
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t t[QT];
-                    terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
-#pragma unroll
-                    for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
-                }
-        } else {
-            const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow + (size_t)col * dim;
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                const int d = j * 32 + quad * 8;
-                q[0][j] = col < cols && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
-                                                : (u32x4){0, 0, 0, 0};
-            }
-        }
+            const uint32_t seq = held.seq;
+            const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
 
-        f32x4 o[VD];
-#pragma unroll
-        for (int e = 0; e < VD; e++) o[e] = (f32x4){0, 0, 0, 0};
-        float m = kLowest, sum = 0;
-
-        const uint32_t* table = c.tables + (size_t)seq * c.slots;
-        const uint32_t row_mask = (1u << c.shift) - 1;
-        const uint32_t kv_row = head << c.shift;      // rows before this head's in a page
-        const int k_block = col >> 2;
-        // first position of tile t
-        const auto tile_pos = [&](uint32_t t) {
-            return (t < sp.sink_tiles ? t : sp.start + (t - sp.sink_tiles)) * kTile;
-        };
-        // the page of eight positions from pos (a multiple of 8) on, where a
-        // key among them is seen; ~0 where it names none
-        const auto seen8 = [&](uint32_t pos) {
-            return pos < sp.n && (pos + 8 > sp.lo || pos < sp.first);
-        };
-        const auto page_of = [&](uint32_t pos) {
-            uint32_t p = 0;
-            if (seen8(pos)) p = table[pos >> c.shift];
-            return p;
-        };
-        const auto k_rows = [&](uint32_t page, uint32_t pos) {
-            const uint32_t p = page < c.pages ? page : 0;
-            return c.keys + layer +
-                   ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
-                    ((pos + k_block * 8 + (col & 3)) & row_mask)) * dim + quad * 8;
-        };
-        const auto v_rows = [&](uint32_t page, uint32_t pos) {
-            const uint32_t p = page < c.pages ? page : 0;
-            const int d = FULL || col * VD < dim ? col * VD : 0;
-            return c.values + layer +
-                   ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
-                    ((pos + quad * 8) & row_mask)) * dim + d;
-        };
-        u32x4 k[2][NJ];
-        uint32_t v[8][VW];
-        const auto load_k = [&](uint32_t page, uint32_t pos) {
-            const uint16_t* p = k_rows(page, pos);
-#pragma unroll
-            for (int t = 0; t < 2; t++)
+            // queries: the B operand, column = query head
+            u32x4 q[QT][NJ];
+            float factor = a.scale * 1.44269504088896340736f;
+            if constexpr (F32) {
+                const float* src = static_cast<const float*>(a.q) + qrow + (size_t)col * dim;
+                float v[NJ][8];
+                float top = 0;
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    if (FULL || j * 32 + quad * 8 < dim)
-                        k[t][j] = *reinterpret_cast<const u32x4*>(p + t * 4 * dim + j * 32);
-                    else
-                        k[t][j] = (u32x4){0, 0, 0, 0};
-                }
-        };
-        const auto load_v = [&](uint32_t page, uint32_t pos) {
-            const uint16_t* p = v_rows(page, pos);
+                    const int d = j * 32 + quad * 8;
+                    const bool in = col < cols && d < dim;
+                    f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+                    if (in) {
+                        lo = *reinterpret_cast<const f32x4*>(src + d);
+                        hi = *reinterpret_cast<const f32x4*>(src + d + 4);
+                    }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (VW == 2) {
-                    const u32x2 w = *reinterpret_cast<const u32x2*>(p + i * dim);
-                    v[i][0] = w[0], v[i][1] = w[1];
-                } else {
-#pragma unroll
-                    for (int h = 0; h < VW / 4; h++) {
-                        // a head may end inside a lane's sixteen dims
-                        const int d = FULL || h == 0 || col * VD + h * 8 < dim ? h * 8 : 0;
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(p + i * dim + d);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v[i][4 * h + e] = w[e];
+                    for (int e = 0; e < 8; e++) {
+                        v[j][e] = e < 4 ? lo[e] : hi[e - 4];
+                        top = fmaxf(top, fabsf(v[j][e]));
                     }
                 }
-            }
-        };
-
-        uint32_t t = t_first;
-        uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
-        if (t < t1) {
-            pos = tile_pos(t);
-            k_page = page_of(pos + k_block * 8);
-            v_page = page_of(pos + quad * 8);
-            if (t + stride < t1) {
-                k_next = page_of(tile_pos(t + stride) + k_block * 8);
-                v_next = page_of(tile_pos(t + stride) + quad * 8);
-            }
-            load_k(k_page, pos);
-            load_v(v_page, pos);
-        }
-        for (; t < t1; t += stride) {
-            const bool more = t + stride < t1;
-            const uint32_t pos_next = more ? tile_pos(t + stride) : 0;
-            // scores
-            f32x4 s[2];
+                if constexpr (!BF16) {
+                    // f16 terms: the row's largest value goes to [2^14, 2^15)
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const int ex =
+                        top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+                    factor *= ldexpf(1.0f, -ex);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                s[i] = (f32x4){0, 0, 0, 0};
+                    for (int j = 0; j < NJ; j++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[j][e] = ldexpf(v[j][e], ex);
+                }
 #pragma unroll
                 for (int j = 0; j < NJ; j++)
 #pragma unroll
-                    for (int x = QT - 1; x >= 0; x--) s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
-            }
-            const uint32_t page_now = v_page;
-            if (more) load_k(k_next, pos_next);
-            // which of them are seen
-            const bool all = pos + kTile <= sp.n && (pos >= sp.lo || pos + kTile <= sp.first) &&
-                             !__any(page_now >= c.pages);
-            float y[8];
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t t[QT];
+                        terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
-            uint32_t hidden = 0;
-            if (!all) {
-                const uint32_t p0 = pos + quad * 8;
-                if (page_now >= c.pages) report(fault, kFaultKvPage);
-                // selects without a branch: written with && and ||, this
-                // compiler left y[0] of a key behind the window as it was
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const bool ok = (p0 + e < sp.n) & ((p0 + e >= sp.lo) | (p0 + e < sp.first)) &
-                                    (page_now < c.pages);
-                    hidden |= ok ? 0u : 1u << e;
-                    y[e] = ok ? y[e] : -INFINITY;
-                }
-            }
-            float top = y[0];
-#pragma unroll
-            for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-            if (__any(top > m + kLift)) {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float up = fmaxf(m, top);
-                const float keep = __builtin_amdgcn_exp2f(m - up);
-                m = up;
-                sum *= keep;
-#pragma unroll
-                for (int e = 0; e < VD; e++) o[e] *= keep;
-            }
-            u32x4 w[PT];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
-                const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
-                sum += a0 + a1;
-                uint32_t x[PT];
-                terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
-#pragma unroll
-                for (int i = 0; i < PT; i++) w[i][e] = x[i];
-            }
-            // values of keys that are not seen count as 0, whatever they hold
-            if (!all) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (hidden >> i & 1) {
-#pragma unroll
-                        for (int e = 0; e < VW; e++) v[i][e] = 0;
+                        for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
                     }
-            }
+            } else {
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow + (size_t)col * dim;
 #pragma unroll
-            for (int e = 0; e < VD; e++) {
-                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                u32x4 f;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    f[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], sel);
-#pragma unroll
-                for (int i = PT - 1; i >= 0; i--) o[e] = mfma16<BF16>(f, w[i], o[e]);
-            }
-            if (more) {
-                load_v(v_next, pos_next);
-                v_page = v_next;
-                pos = pos_next;
-                if (t + 2 * stride < t1) {
-                    const uint32_t after = tile_pos(t + 2 * stride);
-                    k_next = page_of(after + k_block * 8);
-                    v_next = page_of(after + quad * 8);
+                for (int j = 0; j < NJ; j++) {
+                    const int d = j * 32 + quad * 8;
+                    q[0][j] = col < cols && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
+                                                    : (u32x4){0, 0, 0, 0};
                 }
             }
-        }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (alone) {
-            const float out = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
+
+            f32x4 o[VD];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int e = 0; e < VD; e++) o[e] = (f32x4){0, 0, 0, 0};
+            float m = kLowest, sum = 0;
+
+            const uint32_t* table = c.tables + (size_t)seq * c.slots;
+            const uint32_t row_mask = (1u << c.shift) - 1;
+            const uint32_t kv_row = head << c.shift;      // rows before this head's in a page
+            const int k_block = col >> 2;
+            // first position of tile t
+            const auto tile_pos = [&](uint32_t t) {
+                return (t < sp.sink_tiles ? t : sp.start + (t - sp.sink_tiles)) * kTile;
+            };
+            // the page of eight positions from pos (a multiple of 8) on, where a
+            // key among them is seen; ~0 where it names none
+            const auto seen8 = [&](uint32_t pos) {
+                return pos < sp.n && (pos + 8 > sp.lo || pos < sp.first);
+            };
+            const auto page_of = [&](uint32_t pos) {
+                uint32_t p = 0;
+                if (seen8(pos)) p = table[pos >> c.shift];
+                return p;
+            };
+            const auto k_rows = [&](uint32_t page, uint32_t pos) {
+                const uint32_t p = page < c.pages ? page : 0;
+                return c.keys + layer +
+                       ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                        ((pos + k_block * 8 + (col & 3)) & row_mask)) * dim + quad * 8;
+            };
+            const auto v_rows = [&](uint32_t page, uint32_t pos) {
+                const uint32_t p = page < c.pages ? page : 0;
+                const int d = FULL || col * VD < dim ? col * VD : 0;
+                return c.values + layer +
+                       ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                        ((pos + quad * 8) & row_mask)) * dim + d;
+            };
+            u32x4 k[2][NJ];
+            uint32_t v[8][VW];
+            const auto load_k = [&](uint32_t page, uint32_t pos) {
+                const uint16_t* p = k_rows(page, pos);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        if (FULL || j * 32 + quad * 8 < dim)
+                            k[t][j] = *reinterpret_cast<const u32x4*>(p + t * 4 * dim + j * 32);
+                        else
+                            k[t][j] = (u32x4){0, 0, 0, 0};
+                    }
+            };
+            const auto load_v = [&](uint32_t page, uint32_t pos) {
+                const uint16_t* p = v_rows(page, pos);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if constexpr (VW == 2) {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(p + i * dim);
+                        v[i][0] = w[0], v[i][1] = w[1];
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < VW / 4; h++) {
+                            // a head may end inside a lane's sixteen dims
+                            const int d = FULL || h == 0 || col * VD + h * 8 < dim ? h * 8 : 0;
+                            const u32x4 w = *reinterpret_cast<const u32x4*>(p + i * dim + d);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[i][4 * h + e] = w[e];
+                        }
+                    }
+                }
+            };
+
+            uint32_t t = t_first;
+            uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
+            if (t < t1) {
+                pos = tile_pos(t);
+                k_page = page_of(pos + k_block * 8);
+                v_page = page_of(pos + quad * 8);
+                if (t + stride < t1) {
+                    k_next = page_of(tile_pos(t + stride) + k_block * 8);
+                    v_next = page_of(tile_pos(t + stride) + quad * 8);
+                }
+                load_k(k_page, pos);
+                load_v(v_page, pos);
+            }
+            for (; t < t1; t += stride) {
+                const bool more = t + stride < t1;
+                const uint32_t pos_next = more ? tile_pos(t + stride) : 0;
+                // scores
+                f32x4 s[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    s[i] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < NJ; j++)
+#pragma unroll
+                        for (int x = QT - 1; x >= 0; x--)
+                            s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
+                }
+                const uint32_t page_now = v_page;
+                if (more) load_k(k_next, pos_next);
+                // which of them are seen
+                const bool all = pos + kTile <= sp.n && (pos >= sp.lo || pos + kTile <= sp.first) &&
+                                 !__any(page_now >= c.pages);
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
+                uint32_t hidden = 0;
+                if (!all) {
+                    const uint32_t p0 = pos + quad * 8;
+                    if (page_now >= c.pages) report(fault, kFaultKvPage);
+                    // selects without a branch: written with && and ||, this
+                    // compiler left y[0] of a key behind the window as it was
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const bool ok = (p0 + e < sp.n) &
+                                        ((p0 + e >= sp.lo) | (p0 + e < sp.first)) &
+                                        (page_now < c.pages);
+                        hidden |= ok ? 0u : 1u << e;
+                        y[e] = ok ? y[e] : -INFINITY;
+                    }
+                }
+                float top = y[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
+                if (__any(top > m + kLift)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float up = fmaxf(m, top);
+                    const float keep = __builtin_amdgcn_exp2f(m - up);
+                    m = up;
+                    sum *= keep;
+#pragma unroll
+                    for (int e = 0; e < VD; e++) o[e] *= keep;
+                }
+                u32x4 w[PT];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
+                    const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
+                    sum += a0 + a1;
+                    uint32_t x[PT];
+                    terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
+#pragma unroll
+                    for (int i = 0; i < PT; i++) w[i][e] = x[i];
+                }
+                // values of keys that are not seen count as 0, whatever they hold
+                if (!all) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (hidden >> i & 1) {
+#pragma unroll
+                            for (int e = 0; e < VW; e++) v[i][e] = 0;
+                        }
+                }
 #pragma unroll
                 for (int e = 0; e < VD; e++) {
-                    const int d = (quad * 4 + i) * VD + e;
-                    if (col < cols && (FULL || d < dim))
-                        store_result(c, a, qrow + (size_t)col * dim + d,
-                                     sum == 0 ? 0.0f : o[e][i] * out);
-                }
-            continue;
-        }
-
-        // the waves' parts of this pair
-        __syncthreads();
-        if (col < cols) {
-            if (quad == 0) max_sh[wave][col] = m, sum_sh[wave][col] = sum;
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                    u32x4 f;
 #pragma unroll
-            for (int e = 0; e < VD; e++)
+                    for (int i = 0; i < 4; i++)
+                        f[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], sel);
+#pragma unroll
+                    for (int i = PT - 1; i >= 0; i--) o[e] = mfma16<BF16>(f, w[i], o[e]);
+                }
+                if (more) {
+                    load_v(v_next, pos_next);
+                    v_page = v_next;
+                    pos = pos_next;
+                    if (t + 2 * stride < t1) {
+                        const uint32_t after = tile_pos(t + 2 * stride);
+                        k_next = page_of(after + k_block * 8);
+                        v_next = page_of(after + quad * 8);
+                    }
+                }
+            }
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (alone) {
+                const float out = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    acc_sh[wave][col][(quad * 4 + i) * VD + e] = o[e][i] * (1.0f / kWeightGain);
-        }
-        __syncthreads();
-        const bool whole = t0 == 0 && t1 == sp.tiles;
-        const uint32_t per = (uint32_t)(cols * dim);
-        const size_t slot_size = (size_t)(group < 16 ? group : 16) * (dim + 2);
-        float* part = parts + (2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * slot_size;
-        for (uint32_t i = threadIdx.x; i < per; i += 64 * W) {
-            const int g = (int)(i / dim), d = (int)(i - g * dim);
-            float top = max_sh[0][g];
 #pragma unroll
-            for (int x = 1; x < W; x++) top = fmaxf(top, max_sh[x][g]);
-            float den = 0, num = 0;
-#pragma unroll
-            for (int x = 0; x < W; x++) {
-                const float f = __builtin_amdgcn_exp2f(max_sh[x][g] - top);
-                den += f * sum_sh[x][g];
-                num += f * acc_sh[x][g][d];
+                    for (int e = 0; e < VD; e++) {
+                        const int d = (quad * 4 + i) * VD + e;
+                        if (col < cols && (FULL || d < dim))
+                            store_result(c, a, qrow + (size_t)col * dim + d,
+                                         sum == 0 ? 0.0f : o[e][i] * out);
+                    }
+                continue;
             }
-            if (whole) {
-                store_result(c, a, qrow + (size_t)g * dim + d, den == 0 ? 0.0f : num / den);
-            } else {
-                store_device(part + 2 * cols + i, num);
-                if (d == 0) {
-                    store_device(part + 2 * g, top);
-                    store_device(part + 2 * g + 1, den);
+
+            // the waves' parts of this pair
+            __syncthreads();
+            if (col < cols) {
+                if (quad == 0) max_sh[wave][col] = m, sum_sh[wave][col] = sum;
+#pragma unroll
+                for (int e = 0; e < VD; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        acc_sh[wave][col][(quad * 4 + i) * VD + e] = o[e][i] * (1.0f / kWeightGain);
+            }
+            __syncthreads();
+            const bool whole = t0 == 0 && t1 == sp.tiles;
+            const uint32_t per = (uint32_t)(cols * dim);
+            const size_t slot_size = (size_t)(group < 16 ? group : 16) * (dim + 2);
+            float* part = parts + (2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * slot_size;
+            for (uint32_t i = threadIdx.x; i < per; i += 64 * W) {
+                const int g = (int)(i / dim), d = (int)(i - g * dim);
+                float top = max_sh[0][g];
+#pragma unroll
+                for (int x = 1; x < W; x++) top = fmaxf(top, max_sh[x][g]);
+                float den = 0, num = 0;
+#pragma unroll
+                for (int x = 0; x < W; x++) {
+                    const float f = __builtin_amdgcn_exp2f(max_sh[x][g] - top);
+                    den += f * sum_sh[x][g];
+                    num += f * acc_sh[x][g][d];
+                }
+                if (whole) {
+                    store_result(c, a, qrow + (size_t)g * dim + d, den == 0 ? 0.0f : num / den);
+                } else {
+                    store_device(part + 2 * cols + i, num);
+                    if (d == 0) {
+                        store_device(part + 2 * g, top);
+                        store_device(part + 2 * g + 1, den);
+                    }
                 }
             }
-        }
-        if (!whole) {
-            // the stretches that hold a part: w0, whose end is the first cut
-            // farther than kNear from the sequence's ends, to w1, whose start
-            // is the last; the one to arrive last joins them all
-            const uint64_t end = (uint64_t)item + sp.tiles;
-            const uint32_t w0 = (uint32_t)(((uint64_t)item + kNear) / cut.chunk);
-            const uint32_t w1 = (uint32_t)((end - kNear + cut.chunk - 1) / cut.chunk) - 1;
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __builtin_amdgcn_s_waitcnt(0);
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __syncthreads();
-            uint32_t* ticket = tickets + ((size_t)w0 * heads + head_tile) * ticket_stride;
-            if (threadIdx.x == 0)
-                last_sh = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
-                                                 __HIP_MEMORY_SCOPE_AGENT) == w1 - w0;
-            __syncthreads();
-            if (last_sh) {
-                join_parts<W, 16>(c, a, parts, slot_size, w0, heads, head_tile, (int)(w1 - w0) + 1,
-                                  cols, dim, qrow, &acc_sh[0][0][0], W * 16 * (DIM + 4));
+            if (!whole) {
+                // the stretches that hold a part: w0, whose end is the first cut
+                // farther than kNear from the sequence's ends, to w1, whose start
+                // is the last; the one to arrive last joins them all
+                const uint64_t end = (uint64_t)item + sp.tiles;
+                const uint32_t w0 = (uint32_t)(((uint64_t)item + kNear) / cut.chunk);
+                const uint32_t w1 = (uint32_t)((end - kNear + cut.chunk - 1) / cut.chunk) - 1;
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                __builtin_amdgcn_s_waitcnt(0);
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                __syncthreads();
+                uint32_t* ticket = tickets + ((size_t)w0 * heads + head_tile) * ticket_stride;
                 if (threadIdx.x == 0)
-                    __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    last_sh = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT) == w1 - w0;
+                __syncthreads();
+                if (last_sh) {
+                    join_parts<W, 16>(c, a, parts, slot_size, w0, heads, head_tile,
+                                      (int)(w1 - w0) + 1, cols, dim, qrow, &acc_sh[0][0][0],
+                                      W * 16 * (DIM + 4));
+                    if (threadIdx.x == 0)
+                        __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
             }
-        }
         }
         u = u_next;
     }
@@ -1188,7 +1193,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             for (int i = 0; i < SUB; i++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
+                    const float w0 =
+                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
                     const float w1 =
                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
                     part[e & 3] += w0 + w1;

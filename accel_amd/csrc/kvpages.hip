@@ -119,7 +119,9 @@ struct Marks {
     PlanScratch* sh;
     uint32_t* far;
     bool near;
-    __device__ uint32_t first(uint32_t s) const { return near ? sh->marks[s] : load_fresh(far + s); }
+    __device__ uint32_t first(uint32_t s) const {
+        return near ? sh->marks[s] : load_fresh(far + s);
+    }
 };
 __device__ Marks mark_first(const KvCache& c, const uint32_t* seqs, int n, PlanScratch* sh,
                             uint32_t* far) {
@@ -439,8 +441,9 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache c, const uint32_t*
 
 // A block a sequence.  An entry is claimed by exchanging it for ACCEL_KV_NONE,
 // so a sequence named twice gives each page back once.
-__global__ __launch_bounds__(256) void kv_free_kernel(KvCache c, const uint32_t* seqs, int64_t window,
-                                                      int64_t sinks, uint32_t* fault) {
+__global__ __launch_bounds__(256) void kv_free_kernel(KvCache c, const uint32_t* seqs,
+                                                      int64_t window, int64_t sinks,
+                                                      uint32_t* fault) {
     const uint32_t s = sequence_of(c, seqs, (int)blockIdx.x, fault);
     if (s == kNoSequence) return;
     uint32_t lo = 0, hi = c.slots;
