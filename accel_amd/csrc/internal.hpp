@@ -425,7 +425,8 @@ hipError_t launch_kv_append(Device* d, hipStream_t st, const KvCache& c, int64_t
                             const uint32_t* offsets, int n, int rows);
 hipError_t launch_kv_fork(Device* d, hipStream_t st, const KvCache& c, const uint32_t* parents,
                           const uint32_t* children, int n, int* status);
-// Empties the sequences (window 0), or gives back the pages behind the window.
+// Empties the sequences (window 0), or gives back the pages behind the window
+// (window and sinks up to INT32_MAX).
 hipError_t launch_kv_free(Device* d, hipStream_t st, const KvCache& c, const uint32_t* seqs,
                           int n, int64_t window, int64_t sinks);
 hipError_t launch_kv_compact(Device* d, hipStream_t st, const KvCache& c, uint32_t* live,

@@ -273,6 +273,9 @@ ACCEL_API int accel_kv_trim(int dev, void* stream, const accel_kv_cache_t* cache
                  (long long)window, (long long)sinks);
         return refuse(op, buf);
     }
+    // no table holds as many positions; the kernel adds a page to the sinks
+    if (window > INT32_MAX) window = INT32_MAX;
+    if (sinks > INT32_MAX) sinks = INT32_MAX;
     int64_t n = -1;
     const uint32_t* list;
     if ((rc = check_seqs(op, seqs, c, &n, &list)) != ACCEL_OK) return rc;
