@@ -158,10 +158,15 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
                                                            uint32_t* list, uint32_t* first,
                                                            uint32_t* mark, uint32_t* fault) {
     __shared__ PlanScratch sh;
+    __shared__ uint32_t short_sh[2];
     const uint32_t cap = c.slots << c.shift, up = (1u << c.shift) - 1;
     const Counts ahead = read_ahead(c);
     Marks marks = {};
     if (seqs) marks = mark_first(c, seqs, n, &sh, mark);
+    const auto need_of = [&](uint32_t s, int i) {
+        const uint32_t len = c.lens[s];
+        return ((len + grow[i] + up) >> c.shift) - ((len + up) >> c.shift);
+    };
     // what each entry needs, and where its pages begin in the list; an entry
     // that cannot be served is marked and needs none
     constexpr uint32_t kLeftOut = 0xffffffffu;
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
                     if (len > cap || g > cap - len) {
                         report(fault, kFaultKvRoom);
                     } else {
-                        need = ((len + g + up) >> c.shift) - ((len + up) >> c.shift);
+                        need = need_of(s, i);
                         ok = true;
                     }
                 }
@@ -198,6 +203,46 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
     const uint32_t found =
         want ? list_pages<true>(c.refs, 0, c.pages, list, want, sh.sums, &ahead) : 0;
     __syncthreads();
+    if (found < needed) {
+        // The pool is short: the entries are gone through in order, each served
+        // that fits into what those before it left.  A pass over the entries at
+        // hand serves those before the first that does not fit, and leaves out
+        // that one and whatever needs more than is left then; so a pass that
+        // serves few leaves out much, and few passes are usual (600 entries
+        // made to need one each: 0.5 ms).
+        uint32_t left = found;
+        for (int base = 0; base < n; base += kPlan) {
+            const int i = base + threadIdx.x;
+            bool open = i < n && first[i] != kLeftOut;
+            const uint32_t need = open ? need_of(seqs ? seqs[i] : (uint32_t)i, i) : 0;
+            for (;;) {
+                if (open && need > left) {
+                    open = false;
+                    first[i] = kLeftOut;
+                    report(fault, kFaultKvRoom);
+                }
+                // the scan's barriers stand between the last pass's reads of
+                // short_sh and this one's reset
+                uint32_t total;
+                const uint32_t at = block_scan(open ? need : 0u, sh.sums, &total);
+                if (threadIdx.x == 0) short_sh[0] = kPlan, short_sh[1] = 0;
+                __syncthreads();
+                const bool over = open && (at > left || need > left - at);
+                if (over) atomicMin(&short_sh[0], (uint32_t)threadIdx.x);
+                __syncthreads();
+                const uint32_t stop = short_sh[0];
+                if (open && threadIdx.x < stop) {
+                    first[i] = found - left + at;
+                    open = false;
+                    atomicMax(&short_sh[1], at + need);
+                }
+                __syncthreads();
+                left -= short_sh[1];
+                if (stop == kPlan) break;
+            }
+        }
+        __syncthreads();
+    }
     // a wave an entry: the slots of a long prompt are filled side by side
     const int lane = threadIdx.x & 63;
     for (int i = threadIdx.x >> 6; i < n; i += kPlanWaves) {
@@ -205,12 +250,7 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
         if (at == kLeftOut) continue;
         const uint32_t s = seqs ? seqs[i] : (uint32_t)i;
         const uint32_t len = c.lens[s], g = grow[i];
-        const uint32_t have = (len + up) >> c.shift;
-        const uint32_t need = ((len + g + up) >> c.shift) - have;
-        if (need && (at > found || need > found - at)) {
-            if (lane == 0) report(fault, kFaultKvRoom);
-            continue;
-        }
+        const uint32_t have = (len + up) >> c.shift, need = need_of(s, i);
         for (uint32_t j = lane; j < need; j += 64) {
             const uint32_t page = list[at + j];
             c.tables[(size_t)s * c.slots + have + j] = page;

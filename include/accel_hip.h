@@ -635,8 +635,9 @@ int accel_kv_clear(int dev, void* stream, const accel_kv_cache_t* cache);
  * [n]) positions: its length, and a page for each slot of its table that they
  * reach, the lowest free pages first, entry by entry in the list's order.  An
  * entry for which the pool or the table has no room is left unchanged and
- * reported, and so are the second of two entries with one sequence and a
- * sequence index outside the cache; ACCEL_KV_NONE is skipped. */
+ * reported, and those after it are served as if it were not there; unchanged
+ * and reported are also the second of two entries with one sequence and a
+ * sequence index outside the cache.  ACCEL_KV_NONE is skipped. */
 int accel_kv_reserve(int dev, void* stream, const accel_kv_cache_t* cache,
                      const accel_tensor_t* seqs, const accel_tensor_t* grow);
 

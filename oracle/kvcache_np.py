@@ -28,8 +28,6 @@ class Pages:
         seqs = range(len(self.lens)) if seqs is None else seqs
         free, seen, slots = self._free(), set(), self.tables.shape[1]
         take = []
-        # every entry's place in the list of free pages comes from the needs of
-        # all before it, those that find none left among them
         for i, (s, g) in enumerate(zip(seqs, grow)):
             if s == NONE:
                 continue
@@ -53,7 +51,7 @@ class Pages:
                     self.tables[s, have + j] = free[at + j]
                     self.refs[free[at + j]] = 1
                 self.lens[s] += g
-            at += need
+                at += need
 
     def append(self, layer, k, v, seqs=None, offsets=None):
         offsets = range(len(k) + 1) if offsets is None else offsets
