@@ -809,7 +809,7 @@ __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_
 
 template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT>
 __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
-    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t splits,
+    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
     uint32_t* tickets, uint32_t ticket_stride, float* parts, uint32_t* fault) {
     constexpr int NS = DIM / 16;            // MFMA steps of a score
     constexpr int NC = DIM / 8;             // 16-byte chunks of a key
@@ -834,7 +834,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const uint32_t heads = (uint32_t)(c.heads * group_tiles);
     // shares are the slow index: those that have nothing to do come last
     const uint32_t places = gridDim.x / splits;
-    const uint32_t split = blockIdx.x / places, place = blockIdx.x - split * places;
+    const uint32_t split = blockIdx.x / places, place = place0 + blockIdx.x - split * places;
     const uint32_t order = place / heads, head_tile = place - order * heads;
     const uint32_t head = head_tile / group_tiles;
     const int g0 = (int)(head_tile - head * group_tiles) * per;
@@ -1455,11 +1455,17 @@ hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, con
         hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
                            sums, d->fault_dev);
     const uint32_t fold = slots > (uint32_t)d->cu_count ? (uint32_t)d->cu_count / heads : 0;
-    const dim3 grid((unsigned)(bound * splits));
     const uint32_t stride = (uint32_t)(kWorkspaceCounterBytes / 4) / slots;
+    // a launch of 256 lanes a workgroup holds fewer than 2^24 of them, as a
+    // grid's lanes are counted in 32 bits; that many places are not split
+    constexpr uint64_t kPlaces = 1 << 22;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, c, a, sums, fold, splits, tickets,
-                           stride, parts, d->fault_dev);
+        for (uint64_t place = 0; place < bound; place += kPlaces) {
+            const uint64_t places = bound - place < kPlaces ? bound - place : kPlaces;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(places * splits)), dim3(256), 0, st, c, a,
+                               sums, fold, splits, (uint32_t)place, tickets, stride, parts,
+                               d->fault_dev);
+        }
     };
     const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
     const auto dims = [&](auto bf16, auto qt, auto pt) {

@@ -145,7 +145,7 @@ bool same_rows(const accel_tensor_t* a, const accel_tensor_t* b) {
            a->shape[2] == b->shape[2];
 }
 
-// A launch of so many blocks an entry, or a refusal.
+// So many pieces of work an entry, below 2^31 in all, or a refusal.
 int check_blocks(const char* op, int64_t n, int64_t each) {
     char buf[128];
     if (n <= INT32_MAX / each) return ACCEL_OK;

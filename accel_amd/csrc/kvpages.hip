@@ -19,6 +19,12 @@ constexpr int kPlan = 1024;            // lanes of a planning workgroup
 constexpr int kPlanWaves = kPlan / 64;
 constexpr int kScan = 16;              // pages a lane tests at once
 
+// Workgroups of a launch, at most: one of 256 lanes holds fewer than 2^24, as a
+// grid's lanes are counted in 32 bits.  The kernels below walk over more work
+// than that.
+constexpr int64_t kGrid = 1 << 22;
+dim3 grid_of(size_t blocks) { return dim3((unsigned)(blocks < (size_t)kGrid ? blocks : kGrid)); }
+
 // A word another lane of the workgroup changed with an atomic: read past the
 // vector cache, which may hold the line as it was.
 __device__ __forceinline__ uint32_t load_fresh(const uint32_t* p) {
@@ -276,16 +282,10 @@ __device__ __forceinline__ uint16_t narrow(float f, bool bf16) {
 // each.  HBM-bound; a row's [kv_heads, dim] goes to kv_heads places of dim
 // elements, and rows of one sequence follow each other within a head's part of
 // the page, so stores fill whole lines.
-__global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, size_t layer_elems,
-                                                        const void* k, const void* v,
-                                                        int32_t dtype, const uint32_t* seqs,
-                                                        const uint32_t* offsets, int n, int rows,
-                                                        uint32_t* fault) {
-    const uint32_t per = (uint32_t)c.heads * (c.dim >> 3);
-    const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t row = (uint32_t)(item / per);
-    if (row >= (uint32_t)rows) return;
-    const uint32_t part = (uint32_t)(item - (size_t)row * per);
+__device__ __forceinline__ void append_item(const KvCache& c, size_t layer_elems, const void* k,
+                                            const void* v, int32_t dtype, const uint32_t* seqs,
+                                            const uint32_t* offsets, int n, uint32_t row,
+                                            uint32_t part, uint32_t* fault) {
     int e = row;
     uint32_t left = 1;                  // rows of the entry from this one on
     if (offsets) {
@@ -336,6 +336,20 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, size_t layer_
             }
         }
         *reinterpret_cast<u32x4*>(dst) = o;
+    }
+}
+__global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, size_t layer_elems,
+                                                        const void* k, const void* v,
+                                                        int32_t dtype, const uint32_t* seqs,
+                                                        const uint32_t* offsets, int n, int rows,
+                                                        uint32_t* fault) {
+    const uint32_t per = (uint32_t)c.heads * (c.dim >> 3);
+    const size_t items = (size_t)rows * per;
+    for (size_t item = (size_t)blockIdx.x * 256 + threadIdx.x; item < items;
+         item += (size_t)gridDim.x * 256) {
+        const uint32_t row = (uint32_t)(item / per);
+        append_item(c, layer_elems, k, v, dtype, seqs, offsets, n, row,
+                    (uint32_t)(item - (size_t)row * per), fault);
     }
 }
 
@@ -442,68 +456,77 @@ __device__ __forceinline__ void copy_part(const KvCache& c, uint32_t from, uint3
 }
 
 // Blocks 2 * layers a branch: its last page's copy; and one more a branch for
-// its row of the table and the shared pages' counts.
+// its row of the table and the shared pages' counts.  (Blocks in all: below 2^31.)
 __global__ __launch_bounds__(256) void kv_fork_kernel(KvCache c, const uint32_t* parents,
                                                       const uint32_t* children,
-                                                      const Branch* plan) {
-    const uint32_t parts = 2 * (uint32_t)c.layers + 1;
-    const uint32_t i = blockIdx.x / parts, part = blockIdx.x - i * parts;
-    const Branch b = plan[i];
-    if (!b.ok) return;
-    if (part + 1 < parts) {
-        if (b.to != ACCEL_KV_NONE) copy_part(c, b.from, b.to, part);
-        return;
+                                                      const Branch* plan, int n) {
+    const uint32_t parts = 2 * (uint32_t)c.layers + 1, work = (uint32_t)n * parts;
+    for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const uint32_t i = w / parts, part = w - i * parts;
+        const Branch b = plan[i];
+        if (!b.ok) continue;
+        if (part + 1 < parts) {
+            if (b.to != ACCEL_KV_NONE) copy_part(c, b.from, b.to, part);
+            continue;
+        }
+        const uint32_t* from = c.tables + (size_t)parents[i] * c.slots;
+        uint32_t* to = c.tables + (size_t)children[i] * c.slots;
+        for (uint32_t j = threadIdx.x; j < b.whole; j += 256) {
+            const uint32_t page = from[j];
+            to[j] = page < c.pages ? page : ACCEL_KV_NONE;
+            if (page < c.pages)
+                __hip_atomic_fetch_add(c.refs + page, 1u, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (threadIdx.x == 0 && b.to != ACCEL_KV_NONE) to[b.whole] = b.to;
     }
-    const uint32_t* from = c.tables + (size_t)parents[i] * c.slots;
-    uint32_t* to = c.tables + (size_t)children[i] * c.slots;
-    for (uint32_t j = threadIdx.x; j < b.whole; j += 256) {
-        const uint32_t page = from[j];
-        to[j] = page < c.pages ? page : ACCEL_KV_NONE;
-        if (page < c.pages)
-            __hip_atomic_fetch_add(c.refs + page, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (threadIdx.x == 0 && b.to != ACCEL_KV_NONE) to[b.whole] = b.to;
 }
 
-// Blocks 2 * layers a pair.
+// Blocks 2 * layers a pair, below 2^31 in all.
 __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache c, const uint32_t* src,
-                                                      const uint32_t* dst, uint32_t* fault) {
-    const uint32_t parts = 2 * (uint32_t)c.layers;
-    const uint32_t i = blockIdx.x / parts, part = blockIdx.x - i * parts;
-    const uint32_t from = src[i], to = dst[i];
-    if (from >= c.pages || to >= c.pages) {
-        if (from != ACCEL_KV_NONE && to != ACCEL_KV_NONE && threadIdx.x == 0)
-            report(fault, kFaultKvSequence);
-        return;
+                                                      const uint32_t* dst, int n,
+                                                      uint32_t* fault) {
+    const uint32_t parts = 2 * (uint32_t)c.layers, work = (uint32_t)n * parts;
+    for (uint32_t w = blockIdx.x; w < work; w += gridDim.x) {
+        const uint32_t i = w / parts, part = w - i * parts;
+        const uint32_t from = src[i], to = dst[i];
+        if (from >= c.pages || to >= c.pages) {
+            if (from != ACCEL_KV_NONE && to != ACCEL_KV_NONE && threadIdx.x == 0)
+                report(fault, kFaultKvSequence);
+            continue;
+        }
+        if (from != to) copy_part(c, from, to, part);
     }
-    if (from != to) copy_part(c, from, to, part);
 }
 
 // A block a sequence.  An entry is claimed by exchanging it for ACCEL_KV_NONE,
 // so a sequence named twice gives each page back once.
-__global__ __launch_bounds__(256) void kv_free_kernel(KvCache c, const uint32_t* seqs,
+__global__ __launch_bounds__(256) void kv_free_kernel(KvCache c, const uint32_t* seqs, int n,
                                                       int64_t window, int64_t sinks,
                                                       uint32_t* fault) {
-    const uint32_t s = sequence_of(c, seqs, (int)blockIdx.x, fault);
-    if (s == kNoSequence) return;
-    uint32_t lo = 0, hi = c.slots;
-    if (window) {
-        // slots wholly past the sinks and wholly before the window of the
-        // query at the last position
-        const int64_t len = length_of(c, s);
-        const int64_t first = (sinks + (1 << c.shift) - 1) >> c.shift;
-        lo = (uint32_t)(first < (int64_t)c.slots ? first : (int64_t)c.slots);
-        hi = len > window ? (uint32_t)((len - window) >> c.shift) : 0;
+    for (uint32_t i = blockIdx.x; i < (uint32_t)n; i += gridDim.x) {
+        const uint32_t s = sequence_of(c, seqs, (int)i, fault);
+        if (s == kNoSequence) continue;
+        uint32_t lo = 0, hi = c.slots;
+        if (window) {
+            // slots wholly past the sinks and wholly before the window of the
+            // query at the last position
+            const int64_t len = length_of(c, s);
+            const int64_t first = (sinks + (1 << c.shift) - 1) >> c.shift;
+            lo = (uint32_t)(first < (int64_t)c.slots ? first : (int64_t)c.slots);
+            hi = len > window ? (uint32_t)((len - window) >> c.shift) : 0;
+        }
+        uint32_t* row = c.tables + (size_t)s * c.slots;
+        for (uint32_t j = lo + threadIdx.x; j < hi; j += 256) {
+            if (row[j] == ACCEL_KV_NONE) continue;
+            const uint32_t page = __hip_atomic_exchange(row + j, ACCEL_KV_NONE, __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT);
+            if (page < c.pages)
+                __hip_atomic_fetch_sub(c.refs + page, 1u, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (!window && threadIdx.x == 0) c.lens[s] = 0;
     }
-    uint32_t* row = c.tables + (size_t)s * c.slots;
-    for (uint32_t j = lo + threadIdx.x; j < hi; j += 256) {
-        if (row[j] == ACCEL_KV_NONE) continue;
-        const uint32_t page = __hip_atomic_exchange(row + j, ACCEL_KV_NONE, __ATOMIC_RELAXED,
-                                                    __HIP_MEMORY_SCOPE_AGENT);
-        if (page < c.pages)
-            __hip_atomic_fetch_sub(c.refs + page, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (!window && threadIdx.x == 0) c.lens[s] = 0;
 }
 
 // The moves of a compaction.  Scratch: head[0] = how many, head[1] = pages in
@@ -598,7 +621,7 @@ hipError_t launch_kv_append(Device* d, hipStream_t st, const KvCache& c, int64_t
                             const void* k, const void* v, int32_t dtype, const uint32_t* seqs,
                             const uint32_t* offsets, int n, int rows) {
     const size_t items = (size_t)rows * c.heads * (c.dim >> 3);
-    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, c,
+    hipLaunchKernelGGL(kv_append_kernel, grid_of((items + 255) / 256), dim3(256), 0, st, c,
                        (size_t)layer * c.pages * c.page_elems(), k, v, dtype, seqs, offsets, n,
                        rows, d->fault_dev);
     return hipGetLastError();
@@ -612,15 +635,15 @@ hipError_t launch_kv_fork(Device* d, hipStream_t st, const KvCache& c, const uin
     uint32_t* list = w + (size_t)n * 4;
     hipLaunchKernelGGL(kv_fork_plan_kernel, dim3(1), dim3(kPlan), 0, st, c, parents, children, n,
                        list, plan, list + n, d->fault_dev);
-    hipLaunchKernelGGL(kv_fork_kernel, dim3((unsigned)(n * (2 * c.layers + 1))), dim3(256), 0, st,
-                       c, parents, children, plan);
+    hipLaunchKernelGGL(kv_fork_kernel, grid_of((size_t)n * (2 * c.layers + 1)), dim3(256), 0, st, c,
+                       parents, children, plan, n);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_free(Device* d, hipStream_t st, const KvCache& c, const uint32_t* seqs,
                           int n, int64_t window, int64_t sinks) {
-    hipLaunchKernelGGL(kv_free_kernel, dim3((unsigned)n), dim3(256), 0, st, c, seqs, window, sinks,
-                       d->fault_dev);
+    hipLaunchKernelGGL(kv_free_kernel, grid_of((size_t)n), dim3(256), 0, st, c, seqs, n, window,
+                       sinks, d->fault_dev);
     return hipGetLastError();
 }
 
@@ -638,8 +661,8 @@ hipError_t launch_kv_compact(Device* d, hipStream_t st, const KvCache& c, uint32
 
 hipError_t launch_kv_copy(Device* d, hipStream_t st, const KvCache& c, const uint32_t* src,
                           const uint32_t* dst, int n) {
-    hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)(n * (2 * c.layers))), dim3(256), 0, st, c,
-                       src, dst, d->fault_dev);
+    hipLaunchKernelGGL(kv_copy_kernel, grid_of((size_t)n * (2 * c.layers)), dim3(256), 0, st, c,
+                       src, dst, n, d->fault_dev);
     return hipGetLastError();
 }
 

@@ -5,8 +5,10 @@ runs short.  Bounds are those of test_gpu_paged_attention.py unless said."""
 import numpy as np
 import pytest
 
-from accel_amd import KV_NONE
+import accel_amd
+from accel_amd import BF16, U32, KV_NONE
 from test_gpu_kv_pages import Both
+from test_gpu_paged_attention import Case
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +20,92 @@ def test_trim_with_windows_and_sinks_past_any_table(dev, window, sinks):
     b.reserve([0, 1, 8, 64, 95])
     b.trim(window, sinks)
     assert (b.m.tables != KV_NONE).sum() == 22       # nothing is given back
+
+
+# ---- more work than one launch's lanes, which are counted in 32 bits ------------
+
+MANY = (1 << 24) + 9
+
+
+def test_more_sequences_than_a_launch_has_blocks(dev):
+    """Pages given back by lists, and by all sequences, past 2^24 of them."""
+    c = dev.kv_cache(1, 8, 1, 8, 8, MANY, 2)
+    u = lambda x: dev.upload(np.asarray(x, np.uint32), U32)  # noqa: E731
+    some = [0, MANY // 2, MANY - 1]
+    order = dev.upload(np.arange(MANY, dtype=np.uint32)[::-1].copy(), U32)
+    dev.KVReserve(c, u([16, 16, 16]), u(some))
+    dev.KVTrim(c, 8)
+    dev.sync()
+    t = c.tables.numpy()
+    assert (t[some, 0] == KV_NONE).all() and (t[some, 1] != KV_NONE).all()
+    assert c.refs.numpy().sum() == 3
+    dev.KVFree(c, order)
+    dev.KVReserve(c, u([16, 16, 16]), u(some))
+    dev.sync()
+    assert (c.tables.numpy()[some] == np.arange(6).reshape(3, 2)).all()
+    dev.KVFree(c)
+    dev.sync()
+    assert not c.refs.numpy().any() and not c.lens.numpy().any()
+    assert (c.tables.numpy() == KV_NONE).all()
+    c.free()
+
+
+def test_more_copies_and_branches_than_a_launch_has_blocks(dev):
+    """2 blocks a pair and 3 a branch, all but the first and last are padding."""
+    b = Both(dev, layers=1, pages=12, sequences=5, slots=4)
+    b.reserve([11, 20], [0, 1])
+    n = MANY // 2 + 1
+
+    def padded(first, last):
+        x = np.full(n, KV_NONE, np.uint32)
+        x[0], x[-1] = first, last
+        return dev.upload(x, U32)
+
+    b.m.copy([0, 1], [9, 11])
+    dev.KVCopy(b.c, padded(0, 1), padded(9, 11))
+    b.settle()
+    b.m.fork([0, 1], [2, 3])
+    dev.KVFork(b.c, padded(0, 1), padded(2, 3))
+    b.settle()
+
+
+def test_more_rows_than_a_launch_has_lanes(dev):
+    """2^32 and some pieces of rows of which the last row alone has a sequence
+    (64 GB of rows, not read)."""
+    T, KV, D = 32769, 4096, 256
+    c = dev.kv_cache(1, 2, KV, 8, D, 1, 2)
+    u = lambda x: dev.upload(np.asarray(x, np.uint32), U32)  # noqa: E731
+    rows = dev.alloc((T, KV, D), BF16)
+    last = np.random.default_rng(4).integers(0, 1 << 16, (KV, D)).astype(np.uint16)
+    accel_amd._check(accel_amd.lib().accel_hip_write(
+        dev.index, rows.ptr, (T - 1) * KV * D * 2, last.ctypes.data, last.nbytes))
+    dev.KVReserve(c, u([11]))
+    dev.KVAppend(c, 0, rows, rows, u([KV_NONE, 0]), u([0, T - 1, T]))
+    dev.sync()
+    for plane in (c.keys, c.values):
+        assert np.array_equal(plane.numpy()[0, 1, :, 2], last)
+    rows.free()
+    c.free()
+
+
+def test_more_prompt_tiles_than_a_launch_has_blocks(dev):
+    """Entries of a token each, 2^24 tiles of rows and some: each of them as in
+    a short list."""
+    n, period = 2_100_000, 5
+    c = Case(dev, [40, 7, 100, 0, 63], new=[1] * period, heads=8, kv_heads=8, dim=8, page=8)
+    c.upload()
+    c.call()
+    dev.sync()
+    c.compare()
+    want = c.out.numpy()
+    q = dev.upload(np.tile(c.qh, (n // period, 1, 1)), BF16)
+    out = dev.alloc((n, 8, 8), BF16)
+    dev.PagedPrefill(q, dev.upload(np.arange(n + 1, dtype=np.uint32), U32), c.cache, out,
+                     seqs=dev.upload(np.arange(n, dtype=np.uint32) % period, U32))
+    dev.sync()
+    got = out.numpy().reshape(n // period, *want.shape)
+    assert (got == want).all()
+    c.free()
 
 
 def test_a_short_pool_serves_who_fits(dev):
