@@ -80,6 +80,9 @@ int check_cache(const char* op, const accel_kv_cache_t* c, KvCache* out) {
     return ACCEL_OK;
 }
 
+// Entries of a list, at most: the kernels step over them by up to 1024 in 31 bits.
+constexpr int64_t kMostEntries = INT32_MAX - 1024;
+
 // A u32 vector of n entries (n < 0: any number); *len its length.
 int check_list(const char* op, const char* what, const accel_tensor_t* t, int64_t n,
                int64_t* len) {
@@ -92,7 +95,12 @@ int check_list(const char* op, const char* what, const accel_tensor_t* t, int64_
         snprintf(buf, sizeof buf, "%s is missing", what);
         return refuse(op, buf);
     }
-    if (t->shape[0] > INT32_MAX - 1 || (n >= 0 && t->shape[0] != n)) {
+    if (t->shape[0] > kMostEntries) {
+        snprintf(buf, sizeof buf, "%s has %lld entries; up to %lld are served", what,
+                 (long long)t->shape[0], (long long)kMostEntries);
+        return refuse(op, buf);
+    }
+    if (n >= 0 && t->shape[0] != n) {
         snprintf(buf, sizeof buf, "%s has %lld entries and the call has %lld", what,
                  (long long)t->shape[0], (long long)n);
         return refuse(op, buf);

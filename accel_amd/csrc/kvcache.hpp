@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t length_of(const KvCache& c, uint32_t seq) {
 __device__ __forceinline__ int entry_of(const uint32_t* offsets, int n, uint32_t row) {
     int lo = 0, hi = n + 1;            // the first offset past row is in [lo, hi]
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
+        const int mid = lo + ((hi - lo) >> 1);      // lo + hi may pass 31 bits
         if (offsets[mid] <= row) lo = mid + 1;
         else hi = mid;
     }

@@ -108,6 +108,34 @@ def test_more_prompt_tiles_than_a_launch_has_blocks(dev):
     c.free()
 
 
+def test_rows_of_an_entry_past_half_of_31_bits(dev):
+    """2^30 empty entries before the one that has a row: places in the offsets
+    whose sum passes 31 bits."""
+    n = (1 << 30) + 5
+    c = dev.kv_cache(1, 2, 1, 8, 8, n, 1)
+    lib = accel_amd.lib()
+
+    def put(buffer, at, x):
+        x = np.asarray(x, np.uint32)
+        accel_amd._check(lib.accel_hip_write(dev.index, buffer.ptr, 4 * at, x.ctypes.data,
+                                             x.nbytes))
+
+    put(c.lens, n - 1, [1])
+    put(c.tables, n - 1, [1])
+    off = dev.alloc((n + 1,), U32)
+    zeros = np.zeros(1 << 26, np.uint32)
+    for at in range(0, n, len(zeros)):
+        put(off, at, zeros[:n - at])
+    put(off, n, [1])
+    x = np.arange(8, dtype=np.uint16).reshape(1, 1, 8)
+    row = dev.upload(x, BF16)
+    dev.KVAppend(c, 0, row, row, None, off)
+    dev.sync()
+    assert np.array_equal(c.keys.numpy()[0, 1, 0, 0], x[0, 0])
+    off.free()
+    c.free()
+
+
 def test_a_short_pool_serves_who_fits(dev):
     """An entry that the pool cannot serve takes nothing from those after it."""
     b = Both(dev, pages=50, sequences=8, slots=100)

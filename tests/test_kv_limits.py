@@ -1,0 +1,35 @@
+"""Sizes at the ends of what the paged cache's calls count in (CPU: every check
+runs before a device is touched)."""
+import pytest
+
+import accel_amd
+from accel_amd import BF16
+from test_kv_refusals import L, R, cache, refused, tensor
+
+MOST = 2 ** 31 - 1 - 1024
+
+
+@pytest.mark.parametrize("n", [MOST + 1, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 40])
+def test_lists_longer_than_the_kernels_step_over(n):
+    c, u = cache(), tensor((n,))
+    q = tensor((4, 2, 64), BF16)
+    refused(L.accel_kv_reserve(0, None, R(c), R(u), R(u)), f"grow has {n}", f"up to {MOST}")
+    refused(L.accel_kv_free(0, None, R(c), R(u)), f"sequences has {n}")
+    refused(L.accel_kv_trim(0, None, R(c), R(u), 5, 0), f"sequences has {n}")
+    refused(L.accel_kv_fork(0, None, R(c), R(u), R(u)), f"parents has {n}")
+    refused(L.accel_kv_copy(0, None, R(c), R(u), R(u)), f"pages has {n}")
+    refused(L.accel_kv_append(0, None, R(c), 0, R(q), R(q), None, R(u)), f"offsets has {n}")
+    refused(L.accel_paged_prefill(0, None, R(q), R(u), R(c), 0, None, None, R(q)),
+            f"offsets has {n}")
+
+
+def test_the_longest_lists_pass_the_checks():
+    # a device that is not open is the first thing found wrong
+    c, u = cache(), tensor((MOST,))
+    q = tensor((4, 2, 64), BF16)
+    s = tensor((MOST - 1,))
+    for rc in (L.accel_kv_reserve(63, None, R(c), R(u), R(u)),
+               L.accel_kv_free(63, None, R(c), R(u)),
+               L.accel_kv_append(63, None, R(c), 0, R(q), R(q), R(s), R(u)),
+               L.accel_paged_prefill(63, None, R(q), R(u), R(c), 0, R(s), None, R(q))):
+        assert rc == accel_amd.E_NO_DEVICE, accel_amd.last_error()
