@@ -86,6 +86,15 @@ __device__ __forceinline__ float widen(uint16_t h, bool bf16) {
     return half_bits_to_float(h);
 }
 
+// f16 terms of f32 queries: the power of two that takes a row's largest magnitude
+// to [2^14, 2^15), less where the scores' factor, which takes it back, would leave
+// the normal range: scores hidden as -infinity are multiplied by it.
+__device__ __forceinline__ int query_shift(float top, float factor) {
+    const int ex = top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+    const int most = 125 + __builtin_amdgcn_frexp_expf(factor);
+    return ex < most ? ex : most;
+}
+
 __device__ __forceinline__ void store_result(const KvCache& c, const Attention& a, size_t i,
                                              float v) {
     if (a.q_f32) static_cast<float*>(a.out)[i] = v;
@@ -457,12 +466,10 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     }
                 }
                 if constexpr (!BF16) {
-                    // f16 terms: the row's largest value goes to [2^14, 2^15)
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const int ex =
-                        top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-                    factor *= ldexpf(1.0f, -ex);
+                    const int ex = query_shift(top, factor);
+                    factor = ldexpf(factor, -ex);
 #pragma unroll
                     for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -900,7 +907,6 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         const float* src = static_cast<const float*>(a.q) + qrow;
         float top = 0;
         if constexpr (!BF16) {
-            // f16 terms: the row's largest value goes to [2^14, 2^15)
 #pragma unroll
             for (int j = 0; j < NS; j++) {
                 const int d = j * 16 + half * 8;
@@ -910,9 +916,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             }
             top = fmaxf(top, __shfl_xor(top, 32, 64));
         }
-        const int ex = !BF16 && top > 0 && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top)
-                                                          : 0;
-        if constexpr (!BF16) factor *= ldexpf(1.0f, -ex);
+        const int ex = BF16 ? 0 : query_shift(top, factor);
+        if constexpr (!BF16) factor = ldexpf(factor, -ex);
 #pragma unroll
         for (int j = 0; j < NS; j++) {
             const int d = j * 16 + half * 8;

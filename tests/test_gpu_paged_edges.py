@@ -6,9 +6,9 @@ import numpy as np
 import pytest
 
 import accel_amd
-from accel_amd import BF16, U32, KV_NONE
+from accel_amd import BF16, F16, F32, U32, KV_NONE
 from test_gpu_kv_pages import Both
-from test_gpu_paged_attention import Case
+from test_gpu_paged_attention import Case, types
 
 pytestmark = pytest.mark.gpu
 
@@ -134,6 +134,35 @@ def test_rows_of_an_entry_past_half_of_31_bits(dev):
     assert np.array_equal(c.keys.numpy()[0, 1, 0, 0], x[0, 0])
     off.free()
     c.free()
+
+
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("scale", [1e-45, 1e-41, 2e-38])
+def test_scales_below_the_normal_range(dev, q, kv, prompt, scale):
+    """All scores are nearly 0 and all weights nearly equal; keys that a row
+    does not see stay out of it."""
+    Case(dev, [140, 70], new=[140, 9] if prompt else None, q=q, kv=kv).check(scale=scale)
+    Case(dev, [140, 70], new=[140, 9] if prompt else None, q=q, kv=kv).check(
+        scale=scale, window=20, sinks=3)
+
+
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_f32_queries_below_the_normal_range(dev, kv, prompt):
+    """Rows whose largest element is anything down to the smallest subnormal,
+    beside ordinary rows; under the usual scale, and one that lifts them."""
+    rng = np.random.default_rng(5)
+    for scale in (0.0, 1e30):
+        c = Case(dev, [140, 70], new=[140, 9] if prompt else None, q=F32, kv=kv, kv_gain=0.01)
+        size = 2.0 ** rng.integers(-149, -100, c.q.shape[:2])
+        size[::3] = 2.0 ** -149
+        if not scale:
+            size[1::3] = 1
+        x = (rng.standard_normal(c.q.shape) * size[..., None]).astype(np.float32)
+        c.q[:], c.qh[:] = x, x
+        c.check(scale=scale)
+        c.check(scale=scale, window=20, sinks=3)
 
 
 def test_a_short_pool_serves_who_fits(dev):
