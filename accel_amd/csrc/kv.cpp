@@ -383,10 +383,11 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
         return refuse(op, "queries and output must start at 16-byte aligned addresses");
     Attention a{};
     if (opt) {
-        if (!std::isfinite(opt->scale) || opt->scale < 0 || opt->window < 0 || opt->sinks < 0) {
+        // scores are in units of log 2: the scale times log2 e is finite too
+        if (!(opt->scale >= 0 && opt->scale <= 0x1p127f) || opt->window < 0 || opt->sinks < 0) {
             snprintf(buf, sizeof buf,
                      "scale %g, window %lld and sinks %lld; none is negative and the scale is "
-                     "finite",
+                     "finite, 2^127 at most",
                      (double)opt->scale, (long long)opt->window, (long long)opt->sinks);
             return refuse(op, buf);
         }

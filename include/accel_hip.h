@@ -695,7 +695,7 @@ int accel_kv_copy(int dev, void* stream, const accel_kv_cache_t* cache,
 /* What a query sees.  The query at position p of a sequence sees the keys at
  * positions j <= p with, where window is not 0, p - j < window or j < sinks. */
 typedef struct accel_attention {
-    float scale;      /* of a query's product with a key; 0: 1 / sqrt(head_dim) */
+    float scale;      /* of a query's product with a key, up to 2^127; 0: 1 / sqrt(head_dim) */
     int64_t window;   /* positions seen, its own among them; 0: all */
     int64_t sinks;    /* first positions that stay visible past the window */
 } accel_attention_t;

@@ -3,7 +3,7 @@ runs before a device is touched)."""
 import pytest
 
 import accel_amd
-from accel_amd import BF16
+from accel_amd import BF16, AttentionDesc
 from test_kv_refusals import L, R, cache, refused, tensor
 
 MOST = 2 ** 31 - 1 - 1024
@@ -33,3 +33,14 @@ def test_the_longest_lists_pass_the_checks():
                L.accel_kv_append(63, None, R(c), 0, R(q), R(q), R(s), R(u)),
                L.accel_paged_prefill(63, None, R(q), R(u), R(c), 0, R(s), None, R(q))):
         assert rc == accel_amd.E_NO_DEVICE, accel_amd.last_error()
+
+
+def test_scales_that_pass_the_range_in_units_of_log_2():
+    c, q, off = cache(), tensor((4, 4, 64), BF16), tensor((5,))
+    for scale in (3.4e38, 2.4e38, 1.8e38):
+        o = AttentionDesc(scale, 0, 0)
+        refused(L.accel_paged_attention(63, None, R(q), R(c), 0, None, R(o), R(q)), "2^127")
+        refused(L.accel_paged_prefill(63, None, R(q), R(off), R(c), 0, None, R(o), R(q)), "2^127")
+    o = AttentionDesc(2.0 ** 127, 0, 0)
+    rc = L.accel_paged_attention(63, None, R(q), R(c), 0, None, R(o), R(q))
+    assert rc == accel_amd.E_NO_DEVICE
