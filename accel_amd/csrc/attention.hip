@@ -86,6 +86,44 @@ __device__ __forceinline__ float widen(uint16_t h, bool bf16) {
     return half_bits_to_float(h);
 }
 
+// Values that are not finite.  What the definition gives for one that is seen, as
+// every weight is more than 0, is itself; a weight's terms of either sign, and
+// weights that are 0 in 32 bits or fewer, make it NaN in a product.  So a pass over
+// the keys whose result is not finite is made again with such values apart: taken
+// out of the products and added as they are.
+
+// A factor of sums: with INF they may hold an infinity, which 0 would make NaN; the
+// smallest number instead leaves what is finite as it was.
+template <bool INF>
+__device__ __forceinline__ float kept(float f) {
+    return INF ? fmaxf(f, 0x1p-149f) : f;
+}
+
+// Takes the values that are not finite out of eight.  One whose exponent is all
+// ones carries into the sign's place.
+template <bool BF16>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+    constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
+    return ((w & kExp) + kOne) & 0x80008000u;
+}
+template <bool BF16>
+__device__ __forceinline__ u32x4 take_odd(u32x4& f) {
+    u32x4 odd;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t mask = (odd_bits<BF16>(f[i]) >> 15) * 0xffffu;
+        odd[i] = f[i] & mask;
+        f[i] &= ~mask;
+    }
+    return odd;
+}
+template <bool BF16>
+__device__ __forceinline__ u32x4 ones() {
+    constexpr uint32_t k = BF16 ? 0x3f803f80u : 0x3c003c00u;
+    return (u32x4){k, k, k, k};
+}
+
 // f16 terms of f32 queries: the power of two that takes a row's largest magnitude
 // to [2^14, 2^15), less where the scores' factor, which takes it back, would leave
 // the normal range: scores hidden as -infinity are multiplied by it.
@@ -289,7 +327,7 @@ __device__ void join_parts(const KvCache& c, const Attention& a, float* parts, s
                 float term = 0;
                 if (p < count) {
                     const f32x2 ml = load2(slot(p) + 2 * (g0 + g));
-                    const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+                    const float f = kept<true>(__builtin_amdgcn_exp2f(ml[0] - top));
                     factor[g * count + p] = f;
                     term = f * ml[1];
                 }
@@ -443,231 +481,248 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
             const uint32_t seq = held.seq;
             const size_t qrow = ((size_t)entry * a.heads + head * group + g0) * dim;
 
-            // queries: the B operand, column = query head
-            u32x4 q[QT][NJ];
-            float factor = a.scale * 1.44269504088896340736f;
-            if constexpr (F32) {
-                const float* src = static_cast<const float*>(a.q) + qrow + (size_t)col * dim;
-                float v[NJ][8];
-                float top = 0;
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    const int d = j * 32 + quad * 8;
-                    const bool in = col < cols && d < dim;
-                    f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-                    if (in) {
-                        lo = *reinterpret_cast<const f32x4*>(src + d);
-                        hi = *reinterpret_cast<const f32x4*>(src + d + 4);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        v[j][e] = e < 4 ? lo[e] : hi[e - 4];
-                        top = fmaxf(top, fabsf(v[j][e]));
-                    }
-                }
-                if constexpr (!BF16) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const int ex = query_shift(top, factor);
-                    factor = ldexpf(factor, -ex);
-#pragma unroll
-                    for (int j = 0; j < NJ; j++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) v[j][e] = ldexpf(v[j][e], ex);
-                }
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        uint32_t t[QT];
-                        terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
-#pragma unroll
-                        for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
-                    }
-            } else {
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow + (size_t)col * dim;
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    const int d = j * 32 + quad * 8;
-                    q[0][j] = col < cols && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
-                                                    : (u32x4){0, 0, 0, 0};
-                }
-            }
-
+            // A first pass takes the values as they are; where something in it is
+            // not finite the wave goes over its keys again, carefully.
             f32x4 o[VD];
-#pragma unroll
-            for (int e = 0; e < VD; e++) o[e] = (f32x4){0, 0, 0, 0};
-            float m = kLowest, sum = 0;
-
-            const uint32_t* table = c.tables + (size_t)seq * c.slots;
-            const uint32_t row_mask = (1u << c.shift) - 1;
-            const uint32_t kv_row = head << c.shift;      // rows before this head's in a page
-            const int k_block = col >> 2;
-            // first position of tile t
-            const auto tile_pos = [&](uint32_t t) {
-                return (t < sp.sink_tiles ? t : sp.start + (t - sp.sink_tiles)) * kTile;
-            };
-            // the page of eight positions from pos (a multiple of 8) on, where a
-            // key among them is seen; ~0 where it names none
-            const auto seen8 = [&](uint32_t pos) {
-                return pos < sp.n && (pos + 8 > sp.lo || pos < sp.first);
-            };
-            const auto page_of = [&](uint32_t pos) {
-                uint32_t p = 0;
-                if (seen8(pos)) p = table[pos >> c.shift];
-                return p;
-            };
-            const auto k_rows = [&](uint32_t page, uint32_t pos) {
-                const uint32_t p = page < c.pages ? page : 0;
-                return c.keys + layer +
-                       ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
-                        ((pos + k_block * 8 + (col & 3)) & row_mask)) * dim + quad * 8;
-            };
-            const auto v_rows = [&](uint32_t page, uint32_t pos) {
-                const uint32_t p = page < c.pages ? page : 0;
-                const int d = FULL || col * VD < dim ? col * VD : 0;
-                return c.values + layer +
-                       ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
-                        ((pos + quad * 8) & row_mask)) * dim + d;
-            };
-            u32x4 k[2][NJ];
-            uint32_t v[8][VW];
-            const auto load_k = [&](uint32_t page, uint32_t pos) {
-                const uint16_t* p = k_rows(page, pos);
-#pragma unroll
-                for (int t = 0; t < 2; t++)
+            float m, sum;
+            const auto pass = [&](auto careful) {
+                constexpr bool CAREFUL = decltype(careful)::value;
+                // queries: the B operand, column = query head
+                u32x4 q[QT][NJ];
+                float factor = a.scale * 1.44269504088896340736f;
+                if constexpr (F32) {
+                    const float* src = static_cast<const float*>(a.q) + qrow + (size_t)col * dim;
+                    float v[NJ][8];
+                    float top = 0;
 #pragma unroll
                     for (int j = 0; j < NJ; j++) {
-                        if (FULL || j * 32 + quad * 8 < dim)
-                            k[t][j] = *reinterpret_cast<const u32x4*>(p + t * 4 * dim + j * 32);
-                        else
-                            k[t][j] = (u32x4){0, 0, 0, 0};
-                    }
-            };
-            const auto load_v = [&](uint32_t page, uint32_t pos) {
-                const uint16_t* p = v_rows(page, pos);
+                        const int d = j * 32 + quad * 8;
+                        const bool in = col < cols && d < dim;
+                        f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+                        if (in) {
+                            lo = *reinterpret_cast<const f32x4*>(src + d);
+                            hi = *reinterpret_cast<const f32x4*>(src + d + 4);
+                        }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if constexpr (VW == 2) {
-                        const u32x2 w = *reinterpret_cast<const u32x2*>(p + i * dim);
-                        v[i][0] = w[0], v[i][1] = w[1];
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < VW / 4; h++) {
-                            // a head may end inside a lane's sixteen dims
-                            const int d = FULL || h == 0 || col * VD + h * 8 < dim ? h * 8 : 0;
-                            const u32x4 w = *reinterpret_cast<const u32x4*>(p + i * dim + d);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) v[i][4 * h + e] = w[e];
+                        for (int e = 0; e < 8; e++) {
+                            v[j][e] = e < 4 ? lo[e] : hi[e - 4];
+                            top = fmaxf(top, fabsf(v[j][e]));
                         }
                     }
-                }
-            };
-
-            uint32_t t = t_first;
-            uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
-            if (t < t1) {
-                pos = tile_pos(t);
-                k_page = page_of(pos + k_block * 8);
-                v_page = page_of(pos + quad * 8);
-                if (t + stride < t1) {
-                    k_next = page_of(tile_pos(t + stride) + k_block * 8);
-                    v_next = page_of(tile_pos(t + stride) + quad * 8);
-                }
-                load_k(k_page, pos);
-                load_v(v_page, pos);
-            }
-            for (; t < t1; t += stride) {
-                const bool more = t + stride < t1;
-                const uint32_t pos_next = more ? tile_pos(t + stride) : 0;
-                // scores
-                f32x4 s[2];
+                    if constexpr (!BF16) {
+                        top = fmaxf(top, __shfl_xor(top, 16, 64));
+                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        const int ex = query_shift(top, factor);
+                        factor = ldexpf(factor, -ex);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    s[i] = (f32x4){0, 0, 0, 0};
+                        for (int j = 0; j < NJ; j++)
+#pragma unroll
+                            for (int e = 0; e < 8; e++) v[j][e] = ldexpf(v[j][e], ex);
+                    }
 #pragma unroll
                     for (int j = 0; j < NJ; j++)
 #pragma unroll
-                        for (int x = QT - 1; x >= 0; x--)
-                            s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
-                }
-                const uint32_t page_now = v_page;
-                if (more) load_k(k_next, pos_next);
-                // which of them are seen
-                const bool all = pos + kTile <= sp.n && (pos >= sp.lo || pos + kTile <= sp.first) &&
-                                 !__any(page_now >= c.pages);
-                float y[8];
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t t[QT];
+                            terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
-                uint32_t hidden = 0;
-                if (!all) {
-                    const uint32_t p0 = pos + quad * 8;
-                    if (page_now >= c.pages) report(fault, kFaultKvPage);
-                    // selects without a branch: written with && and ||, this
-                    // compiler left y[0] of a key behind the window as it was
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const bool ok = (p0 + e < sp.n) &
-                                        ((p0 + e >= sp.lo) | (p0 + e < sp.first)) &
-                                        (page_now < c.pages);
-                        hidden |= ok ? 0u : 1u << e;
-                        y[e] = ok ? y[e] : -INFINITY;
-                    }
-                }
-                float top = y[0];
-#pragma unroll
-                for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-                if (__any(top > m + kLift)) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float up = fmaxf(m, top);
-                    const float keep = __builtin_amdgcn_exp2f(m - up);
-                    m = up;
-                    sum *= keep;
-#pragma unroll
-                    for (int e = 0; e < VD; e++) o[e] *= keep;
-                }
-                u32x4 w[PT];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
-                    const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
-                    sum += a0 + a1;
-                    uint32_t x[PT];
-                    terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
-#pragma unroll
-                    for (int i = 0; i < PT; i++) w[i][e] = x[i];
-                }
-                // values of keys that are not seen count as 0, whatever they hold
-                if (!all) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (hidden >> i & 1) {
-#pragma unroll
-                            for (int e = 0; e < VW; e++) v[i][e] = 0;
+                            for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
                         }
-                }
+                } else {
+                    const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow + (size_t)col * dim;
 #pragma unroll
-                for (int e = 0; e < VD; e++) {
-                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                    u32x4 f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        f[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], sel);
-#pragma unroll
-                    for (int i = PT - 1; i >= 0; i--) o[e] = mfma16<BF16>(f, w[i], o[e]);
-                }
-                if (more) {
-                    load_v(v_next, pos_next);
-                    v_page = v_next;
-                    pos = pos_next;
-                    if (t + 2 * stride < t1) {
-                        const uint32_t after = tile_pos(t + 2 * stride);
-                        k_next = page_of(after + k_block * 8);
-                        v_next = page_of(after + quad * 8);
+                    for (int j = 0; j < NJ; j++) {
+                        const int d = j * 32 + quad * 8;
+                        q[0][j] = col < cols && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
+                                                        : (u32x4){0, 0, 0, 0};
                     }
                 }
-            }
+
+#pragma unroll
+                for (int e = 0; e < VD; e++) o[e] = (f32x4){0, 0, 0, 0};
+                m = kLowest, sum = 0;
+
+                const uint32_t* table = c.tables + (size_t)seq * c.slots;
+                const uint32_t row_mask = (1u << c.shift) - 1;
+                const uint32_t kv_row = head << c.shift;      // rows before this head's in a page
+                const int k_block = col >> 2;
+                // first position of tile t
+                const auto tile_pos = [&](uint32_t t) {
+                    return (t < sp.sink_tiles ? t : sp.start + (t - sp.sink_tiles)) * kTile;
+                };
+                // the page of eight positions from pos (a multiple of 8) on, where a
+                // key among them is seen; ~0 where it names none
+                const auto seen8 = [&](uint32_t pos) {
+                    return pos < sp.n && (pos + 8 > sp.lo || pos < sp.first);
+                };
+                const auto page_of = [&](uint32_t pos) {
+                    uint32_t p = 0;
+                    if (seen8(pos)) p = table[pos >> c.shift];
+                    return p;
+                };
+                const auto k_rows = [&](uint32_t page, uint32_t pos) {
+                    const uint32_t p = page < c.pages ? page : 0;
+                    return c.keys + layer +
+                           ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                            ((pos + k_block * 8 + (col & 3)) & row_mask)) * dim + quad * 8;
+                };
+                const auto v_rows = [&](uint32_t page, uint32_t pos) {
+                    const uint32_t p = page < c.pages ? page : 0;
+                    const int d = FULL || col * VD < dim ? col * VD : 0;
+                    return c.values + layer +
+                           ((size_t)p * ((size_t)c.heads << c.shift) + kv_row +
+                            ((pos + quad * 8) & row_mask)) * dim + d;
+                };
+                u32x4 k[2][NJ];
+                uint32_t v[8][VW];
+                const auto load_k = [&](uint32_t page, uint32_t pos) {
+                    const uint16_t* p = k_rows(page, pos);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) {
+                            if (FULL || j * 32 + quad * 8 < dim)
+                                k[t][j] = *reinterpret_cast<const u32x4*>(p + t * 4 * dim + j * 32);
+                            else
+                                k[t][j] = (u32x4){0, 0, 0, 0};
+                        }
+                };
+                const auto load_v = [&](uint32_t page, uint32_t pos) {
+                    const uint16_t* p = v_rows(page, pos);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if constexpr (VW == 2) {
+                            const u32x2 w = *reinterpret_cast<const u32x2*>(p + i * dim);
+                            v[i][0] = w[0], v[i][1] = w[1];
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < VW / 4; h++) {
+                                // a head may end inside a lane's sixteen dims
+                                const int d = FULL || h == 0 || col * VD + h * 8 < dim ? h * 8 : 0;
+                                const u32x4 w = *reinterpret_cast<const u32x4*>(p + i * dim + d);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) v[i][4 * h + e] = w[e];
+                            }
+                        }
+                    }
+                };
+
+                uint32_t t = t_first;
+                uint32_t pos = 0, k_page = 0, v_page = 0, k_next = 0, v_next = 0;
+                if (t < t1) {
+                    pos = tile_pos(t);
+                    k_page = page_of(pos + k_block * 8);
+                    v_page = page_of(pos + quad * 8);
+                    if (t + stride < t1) {
+                        k_next = page_of(tile_pos(t + stride) + k_block * 8);
+                        v_next = page_of(tile_pos(t + stride) + quad * 8);
+                    }
+                    load_k(k_page, pos);
+                    load_v(v_page, pos);
+                }
+                for (; t < t1; t += stride) {
+                    const bool more = t + stride < t1;
+                    const uint32_t pos_next = more ? tile_pos(t + stride) : 0;
+                    // scores
+                    f32x4 s[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        s[i] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < NJ; j++)
+#pragma unroll
+                            for (int x = QT - 1; x >= 0; x--)
+                                s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
+                    }
+                    const uint32_t page_now = v_page;
+                    if (more) load_k(k_next, pos_next);
+                    // which of them are seen
+                    const bool all = pos + kTile <= sp.n && (pos >= sp.lo || pos + kTile <= sp.first) &&
+                                     !__any(page_now >= c.pages);
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
+                    uint32_t hidden = 0;
+                    if (!all) {
+                        const uint32_t p0 = pos + quad * 8;
+                        if (page_now >= c.pages) report(fault, kFaultKvPage);
+                        // selects without a branch: written with && and ||, this
+                        // compiler left y[0] of a key behind the window as it was
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const bool ok = (p0 + e < sp.n) &
+                                            ((p0 + e >= sp.lo) | (p0 + e < sp.first)) &
+                                            (page_now < c.pages);
+                            hidden |= ok ? 0u : 1u << e;
+                            y[e] = ok ? y[e] : -INFINITY;
+                        }
+                    }
+                    float top = y[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
+                    if (__any(top > m + kLift)) {
+                        top = fmaxf(top, __shfl_xor(top, 16, 64));
+                        top = fmaxf(top, __shfl_xor(top, 32, 64));
+                        const float up = fmaxf(m, top);
+                        const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
+                        m = up;
+                        sum *= keep;
+#pragma unroll
+                        for (int e = 0; e < VD; e++) o[e] *= keep;
+                    }
+                    u32x4 w[PT];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
+                        const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
+                        sum += a0 + a1;
+                        uint32_t x[PT];
+                        terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
+#pragma unroll
+                        for (int i = 0; i < PT; i++) w[i][e] = x[i];
+                    }
+                    // values of keys that are not seen count as 0, whatever they hold
+                    if (!all) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (hidden >> i & 1) {
+#pragma unroll
+                                for (int e = 0; e < VW; e++) v[i][e] = 0;
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < VD; e++) {
+                        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                        u32x4 f;
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            f[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1], sel);
+                        if constexpr (CAREFUL) {
+                            const u32x4 odd = take_odd<BF16>(f);
+                            o[e] = mfma16<BF16>(odd, ones<BF16>(), o[e]);
+                        }
+#pragma unroll
+                        for (int i = PT - 1; i >= 0; i--) o[e] = mfma16<BF16>(f, w[i], o[e]);
+                    }
+                    if (more) {
+                        load_v(v_next, pos_next);
+                        v_page = v_next;
+                        pos = pos_next;
+                        if (t + 2 * stride < t1) {
+                            const uint32_t after = tile_pos(t + 2 * stride);
+                            k_next = page_of(after + k_block * 8);
+                            v_next = page_of(after + quad * 8);
+                        }
+                    }
+                }
+            };
+            pass(std::false_type());
+            float odd = sum * 0.0f;
+#pragma unroll
+            for (int e = 0; e < VD; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) odd = __builtin_fmaf(o[e][i], 0.0f, odd);
+            if (__any(odd != 0.0f)) pass(std::true_type());
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (alone) {
@@ -707,7 +762,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                 float den = 0, num = 0;
 #pragma unroll
                 for (int x = 0; x < W; x++) {
-                    const float f = __builtin_amdgcn_exp2f(max_sh[x][g] - top);
+                    const float f = kept<true>(__builtin_amdgcn_exp2f(max_sh[x][g] - top));
                     den += f * sum_sh[x][g];
                     num += f * acc_sh[x][g][d];
                 }
@@ -831,6 +886,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     // keys of a tile with values that are not finite: tile t's in place t % 3,
     // which is cleared two steps before it is read, a barrier before it is set
     __shared__ uint32_t odd_sh[3][2];
+    __shared__ uint32_t again_sh;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -899,59 +955,6 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int p_last = base + (tok_b < (int)toks ? tok_b : (int)toks - 1);
     const int p_b = p_last > -1 ? p_last : -1;
     const int p_end = base + (int)toks;           // past the workgroup's last
-
-    // queries: the B operand, column = row
-    u32x4 q[QT][NS];
-    float factor = a.scale * 1.44269504088896340736f;
-    if constexpr (F32) {
-        const float* src = static_cast<const float*>(a.q) + qrow;
-        float top = 0;
-        if constexpr (!BF16) {
-#pragma unroll
-            for (int j = 0; j < NS; j++) {
-                const int d = j * 16 + half * 8;
-                if (real && d < dim)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(src[d + e]));
-            }
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-        }
-        const int ex = BF16 ? 0 : query_shift(top, factor);
-        if constexpr (!BF16) factor = ldexpf(factor, -ex);
-#pragma unroll
-        for (int j = 0; j < NS; j++) {
-            const int d = j * 16 + half * 8;
-            f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if (real && d < dim) {
-                x[0] = *reinterpret_cast<const f32x4*>(src + d);
-                x[1] = *reinterpret_cast<const f32x4*>(src + d + 4);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float y0 = x[e >> 1][2 * (e & 1)], y1 = x[e >> 1][2 * (e & 1) + 1];
-                if constexpr (!BF16) y0 = ldexpf(y0, ex), y1 = ldexpf(y1, ex);
-                uint32_t t[QT];
-                terms16<BF16, QT>(y0, y1, t);
-#pragma unroll
-                for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
-            }
-        }
-    } else {
-        const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow;
-#pragma unroll
-        for (int j = 0; j < NS; j++) {
-            const int d = j * 16 + half * 8;
-            q[0][j] = real && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
-                                      : (u32x4){0, 0, 0, 0};
-        }
-    }
-
-    f32x16 o[DT];
-#pragma unroll
-    for (int e = 0; e < DT; e++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[e][i] = 0;
-    float m = kLowest, sum = 0;
 
     // tiles of keys: those of the sinks, then those from the first window's
     // start to the last position
@@ -1042,17 +1045,15 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const auto plain = [&](int pos) {
         return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
     };
-    const auto arrive = [&](uint32_t pages, int pos, int odd, auto buf) {
+    const auto arrive = [&](uint32_t pages, int pos, int odd, auto buf, auto careful) {
         constexpr int B = decltype(buf)::value;
+        constexpr bool CAREFUL = decltype(careful)::value;
         // what this wave staged is in LDS before the barrier that follows
         wait_loads();
-        if (plain(pos) && !__any(pages >= c.pages)) return;
+        if (!CAREFUL && plain(pos) && !__any(pages >= c.pages)) return;
         // values no row sees count as 0, whatever they hold; those that are not
         // finite are left out of the product, where a row that does not see them
-        // would meet them, and added apart.  A 16-bit value whose exponent is
-        // all ones carries into the sign's place.
-        constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
-        constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u;
+        // would meet them, and added apart
 #pragma unroll
         for (int i = 0; i < KL; i++) {
             const int at = (wave * KL + i) * 64 + lane, key = at / NC;
@@ -1066,7 +1067,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 w = *chunk;
                 u32x4 over;
 #pragma unroll
-                for (int e = 0; e < 4; e++) over[e] = ((w[e] & kExp) + kOne) & 0x80008000u;
+                for (int e = 0; e < 4; e++) over[e] = odd_bits<BF16>(w[e]);
                 if ((over[0] | over[1] | over[2] | over[3]) == 0) continue;
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] &= ~((over[e] >> 15) * 0xffffu);
@@ -1081,184 +1082,252 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
             reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
     }
-    uint32_t pages = 0, pages_next = 0;
-    if (threadIdx.x < 6) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
-    __syncthreads();
-    if (t_begin < t_end) {
-        pages = page_of(tile_pos(t_begin));
-        if (t_begin + 1 < t_end) pages_next = page_of(tile_pos(t_begin + 1));
-        load(pages, tile_pos(t_begin), std::integral_constant<int, 0>());
-        arrive(pages, tile_pos(t_begin), 0, std::integral_constant<int, 0>());
-    }
-    // the lane's part of what it reads: row 8 x + 4 h + b of K's operand holds
-    // key 16 (x / 2) + 8 h + 4 (x % 2) + b
-    const int k_from = k_byte(16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3),
-                              half);
-    // values through the transposing read: of sixteen lanes four take 32 bytes
-    // of one key's dims, and each receives one dim of the four keys
-    const int v_from = v_byte(half * 8 + (col >> 2 & 3), (col >> 4) * 2 + (col >> 1 & 1)) +
-                       (col & 1) * 8;
-    // the queries have arrived: without this the loop's first product waits for
-    // every load in flight, each time
-    wait_loads();
-    int odd_at = 0;
+    // A first pass takes the values of tiles that all rows see as they are; where
+    // something in it is not finite the workgroup goes over its keys again.
+    f32x16 o[DT];
+    float m, sum;
     bool unnamed = false;       // a page some row sees and the table does not name
-    const auto step = [&](int t, auto buf) {
-        constexpr int B = decltype(buf)::value;
-        const std::integral_constant<int, B ^ 1> other;
-        const int pos = tile_pos(t);
-        const bool more = t + 1 < t_end;
-        unnamed |= pages >= c.pages;
-        __syncthreads();
-        const uint32_t odd0 = odd_sh[odd_at][0], odd1 = odd_sh[odd_at][1];
-        const int odd_next = odd_at == 2 ? 0 : odd_at + 1;
-        if (threadIdx.x < 2) odd_sh[odd_next == 2 ? 0 : odd_next + 1][threadIdx.x] = 0;
-        odd_at = odd_next;
-        if (more) load(pages_next, tile_pos(t + 1), other);
-        // a whole step ahead of its use
-        const uint32_t pages_after = t + 2 < t_end ? page_of(tile_pos(t + 2)) : 0;
-        // a wave none of whose rows sees the tile only stages
-        if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
-            f32x16 s[SUB];
+    const auto pass = [&](auto careful) {
+        constexpr bool CAREFUL = decltype(careful)::value;
+        // queries: the B operand, column = row
+        u32x4 q[QT][NS];
+        float factor = a.scale * 1.44269504088896340736f;
+        if constexpr (F32) {
+            const float* src = static_cast<const float*>(a.q) + qrow;
+            float top = 0;
+            if constexpr (!BF16) {
 #pragma unroll
-            for (int i = 0; i < SUB; i++)
+                for (int j = 0; j < NS; j++) {
+                    const int d = j * 16 + half * 8;
+                    if (real && d < dim)
 #pragma unroll
-                for (int e = 0; e < 16; e++) s[i][e] = 0;
+                        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(src[d + e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+            }
+            const int ex = BF16 ? 0 : query_shift(top, factor);
+            if constexpr (!BF16) factor = ldexpf(factor, -ex);
 #pragma unroll
             for (int j = 0; j < NS; j++) {
-                u32x4 kf[SUB];
-#pragma unroll
-                for (int i = 0; i < SUB; i++)
-                    kf[i] = *reinterpret_cast<const u32x4*>(
-                        k_sh[B] + (k_from ^ k_byte(0, 2 * j)) + k_byte(i * 32, 0));
-#pragma unroll
-                for (int x = QT - 1; x >= 0; x--)
-#pragma unroll
-                    for (int i = 0; i < SUB; i++) s[i] = mfma32<BF16>(kf[i], q[x][j], s[i]);
-            }
-            // reads three products ahead of their use
-            if constexpr (QT == 1) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 3 * SUB, 0);
-#pragma unroll
-                for (int j = 0; j < NS - 3; j++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, SUB, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, SUB, 0);
+                const int d = j * 16 + half * 8;
+                f32x4 x[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                if (real && d < dim) {
+                    x[0] = *reinterpret_cast<const f32x4*>(src + d);
+                    x[1] = *reinterpret_cast<const f32x4*>(src + d + 4);
                 }
-                __builtin_amdgcn_sched_group_barrier(0x008, 3 * SUB, 0);
-            }
-            // keys a row does not see, by a key's place x in the tile: past the
-            // row's position, behind its window, on a page without a number
-            const int here = pos + half * 8;
-            const int until = p - here;
-            const auto hide = [&](auto seen) {
 #pragma unroll
-                for (int i = 0; i < SUB; i++)
+                for (int e = 0; e < 4; e++) {
+                    float y0 = x[e >> 1][2 * (e & 1)], y1 = x[e >> 1][2 * (e & 1) + 1];
+                    if constexpr (!BF16) y0 = ldexpf(y0, ex), y1 = ldexpf(y1, ex);
+                    uint32_t t[QT];
+                    terms16<BF16, QT>(y0, y1, t);
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        s[i][e] = seen(i * 32 + (e >> 3) * 16 + (e & 7)) ? s[i][e] : -INFINITY;
-            };
-            if (pos + KT > p_a + 1) hide([&](int x) { return x <= until; });
-            if (!(pos > p_b - window || pos + KT <= sinks)) {
-                // the first place the row's window holds; none where it is all past
-                const int from = until < window ? -KT : until - window + 1;
-                if (pos >= sinks) {
-                    hide([&](int x) { return x >= from; });
-                } else {
-                    const int kept = sinks - here;
-                    hide([&](int x) { return (x >= from) | (x < kept); });
+                    for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
                 }
             }
-            const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
-            if (~named & ((1ull << BLOCKS) - 1)) {
-                const uint32_t mine = (uint32_t)named >> half;
-                hide([&](int x) { return (mine >> (x >> 3) & 1) != 0; });
-            }
-            // two chains of three-way maxima
-            float top = s[0][0], top1 = s[0][1];
+        } else {
+            const uint16_t* src = static_cast<const uint16_t*>(a.q) + qrow;
 #pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    top = fmaxf(fmaxf(top, s[i][e]), s[i][e + 1]);
-                    top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
-                }
-            top = fmaxf(top, top1) * factor;
-            if (__any(top > m + kLift)) {
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float up = fmaxf(m, top);
-                const float keep = __builtin_amdgcn_exp2f(m - up);
-                m = up;
-                sum *= keep;
-#pragma unroll
-                for (int e = 0; e < DT; e++) o[e] *= keep;
-            }
-            u32x4 w[PT][SUB][2];
-            float part[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float w0 =
-                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
-                    const float w1 =
-                        __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
-                    part[e & 3] += w0 + w1;
-                    uint32_t x[PT];
-                    terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
-#pragma unroll
-                    for (int k = 0; k < PT; k++) w[k][i][e >> 2][e & 3] = x[k];
-                }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int e = 0; e < DT; e++) {
-                        u32x2 part[2];
-#pragma unroll
-                        for (int x = 0; x < 2; x++)
-                            part[x] = read_turned(v_sh[B] + (v_from ^ v_byte(0, e * 4)) +
-                                                  (i * 32 + j * 16 + x * 4) * NC * 16);
-                        const u32x4 vf = {part[0][0], part[0][1], part[1][0], part[1][1]};
-#pragma unroll
-                        for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
-                    }
-            // the values that are not finite, for the rows that see them: whatever
-            // the weight, the sum is what they are
-            for (uint64_t odd = odd0 | (uint64_t)odd1 << 32; odd; odd &= odd - 1) {
-                const int x = pos + (int)__builtin_ctzll(odd);
-                const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
-                const uint32_t page = table[(uint32_t)x >> c.shift];
-                const uint16_t* src = reinterpret_cast<const uint16_t*>(
-                    values + (page < c.pages ? page : 0) * page_bytes +
-                    (uint64_t)(head_row + ((uint32_t)x & row_mask)) * row_bytes);
-#pragma unroll
-                for (int y = 0; y < DT; y++)
-#pragma unroll
-                    for (int z = 0; z < 4; z++) {
-                        const int d = y * 32 + 8 * z + 4 * half;
-                        u32x2 f = {0, 0};
-                        if (FULL || d < dim) f = *reinterpret_cast<const u32x2*>(src + d);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float v = widen((uint16_t)(f[e >> 1] >> 16 * (e & 1)), BF16);
-                            o[y][4 * z + e] += ok && !(fabsf(v) < INFINITY) ? v : 0.0f;
-                        }
-                    }
+            for (int j = 0; j < NS; j++) {
+                const int d = j * 16 + half * 8;
+                q[0][j] = real && d < dim ? *reinterpret_cast<const u32x4*>(src + d)
+                                          : (u32x4){0, 0, 0, 0};
             }
         }
-        if (more) {
-            // every wave has passed the barrier above, so none reads this buffer
-            pages = pages_next;
-            arrive(pages, tile_pos(t + 1), odd_next, other);
-            pages_next = pages_after;
+
+#pragma unroll
+        for (int e = 0; e < DT; e++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[e][i] = 0;
+        m = kLowest, sum = 0;
+        uint32_t pages = 0, pages_next = 0;
+        if (threadIdx.x < 6) odd_sh[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+        __syncthreads();
+        if (t_begin < t_end) {
+            pages = page_of(tile_pos(t_begin));
+            if (t_begin + 1 < t_end) pages_next = page_of(tile_pos(t_begin + 1));
+            load(pages, tile_pos(t_begin), std::integral_constant<int, 0>());
+            arrive(pages, tile_pos(t_begin), 0, std::integral_constant<int, 0>(), careful);
+        }
+        // the lane's part of what it reads: row 8 x + 4 h + b of K's operand holds
+        // key 16 (x / 2) + 8 h + 4 (x % 2) + b
+        const int k_from = k_byte(16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3),
+                                  half);
+        // values through the transposing read: of sixteen lanes four take 32 bytes
+        // of one key's dims, and each receives one dim of the four keys
+        const int v_from = v_byte(half * 8 + (col >> 2 & 3), (col >> 4) * 2 + (col >> 1 & 1)) +
+                           (col & 1) * 8;
+        // the queries have arrived: without this the loop's first product waits for
+        // every load in flight, each time
+        wait_loads();
+        int odd_at = 0;
+        const auto step = [&](int t, auto buf) {
+            constexpr int B = decltype(buf)::value;
+            const std::integral_constant<int, B ^ 1> other;
+            const int pos = tile_pos(t);
+            const bool more = t + 1 < t_end;
+            unnamed |= pages >= c.pages;
+            __syncthreads();
+            const uint32_t odd0 = odd_sh[odd_at][0], odd1 = odd_sh[odd_at][1];
+            const int odd_next = odd_at == 2 ? 0 : odd_at + 1;
+            if (threadIdx.x < 2) odd_sh[odd_next == 2 ? 0 : odd_next + 1][threadIdx.x] = 0;
+            odd_at = odd_next;
+            if (more) load(pages_next, tile_pos(t + 1), other);
+            // a whole step ahead of its use
+            const uint32_t pages_after = t + 2 < t_end ? page_of(tile_pos(t + 2)) : 0;
+            // a wave none of whose rows sees the tile only stages
+            if (busy && pos <= p_b && (pos + KT > p_a + 1 - window || pos < sinks)) {
+                f32x16 s[SUB];
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[i][e] = 0;
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    u32x4 kf[SUB];
+#pragma unroll
+                    for (int i = 0; i < SUB; i++)
+                        kf[i] = *reinterpret_cast<const u32x4*>(
+                            k_sh[B] + (k_from ^ k_byte(0, 2 * j)) + k_byte(i * 32, 0));
+#pragma unroll
+                    for (int x = QT - 1; x >= 0; x--)
+#pragma unroll
+                        for (int i = 0; i < SUB; i++) s[i] = mfma32<BF16>(kf[i], q[x][j], s[i]);
+                }
+                // reads three products ahead of their use
+                if constexpr (QT == 1) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 3 * SUB, 0);
+#pragma unroll
+                    for (int j = 0; j < NS - 3; j++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, SUB, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, SUB, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, 3 * SUB, 0);
+                }
+                // keys a row does not see, by a key's place x in the tile: past the
+                // row's position, behind its window, on a page without a number
+                const int here = pos + half * 8;
+                const int until = p - here;
+                const auto hide = [&](auto seen) {
+#pragma unroll
+                    for (int i = 0; i < SUB; i++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            s[i][e] = seen(i * 32 + (e >> 3) * 16 + (e & 7)) ? s[i][e] : -INFINITY;
+                };
+                if (pos + KT > p_a + 1) hide([&](int x) { return x <= until; });
+                if (!(pos > p_b - window || pos + KT <= sinks)) {
+                    // the first place the row's window holds; none where it is all past
+                    const int from = until < window ? -KT : until - window + 1;
+                    if (pos >= sinks) {
+                        hide([&](int x) { return x >= from; });
+                    } else {
+                        const int kept = sinks - here;
+                        hide([&](int x) { return (x >= from) | (x < kept); });
+                    }
+                }
+                const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
+                if (~named & ((1ull << BLOCKS) - 1)) {
+                    const uint32_t mine = (uint32_t)named >> half;
+                    hide([&](int x) { return (mine >> (x >> 3) & 1) != 0; });
+                }
+                // two chains of three-way maxima
+                float top = s[0][0], top1 = s[0][1];
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        top = fmaxf(fmaxf(top, s[i][e]), s[i][e + 1]);
+                        top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
+                    }
+                top = fmaxf(top, top1) * factor;
+                if (__any(top > m + kLift)) {
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float up = fmaxf(m, top);
+                    const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
+                    m = up;
+                    sum *= keep;
+#pragma unroll
+                    for (int e = 0; e < DT; e++) o[e] *= keep;
+                }
+                u32x4 w[PT][SUB][2];
+                float part[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float w0 =
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
+                        const float w1 =
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
+                        part[e & 3] += w0 + w1;
+                        uint32_t x[PT];
+                        terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
+#pragma unroll
+                        for (int k = 0; k < PT; k++) w[k][i][e >> 2][e & 3] = x[k];
+                    }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int e = 0; e < DT; e++) {
+                            u32x2 part[2];
+#pragma unroll
+                            for (int x = 0; x < 2; x++)
+                                part[x] = read_turned(v_sh[B] + (v_from ^ v_byte(0, e * 4)) +
+                                                      (i * 32 + j * 16 + x * 4) * NC * 16);
+                            const u32x4 vf = {part[0][0], part[0][1], part[1][0], part[1][1]};
+#pragma unroll
+                            for (int x = PT - 1; x >= 0; x--) o[e] = mfma32<BF16>(vf, w[x][i][j], o[e]);
+                        }
+                // the values that are not finite, for the rows that see them: whatever
+                // the weight, the sum is what they are
+                for (uint64_t odd = odd0 | (uint64_t)odd1 << 32; odd; odd &= odd - 1) {
+                    const int x = pos + (int)__builtin_ctzll(odd);
+                    const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                    const uint32_t page = table[(uint32_t)x >> c.shift];
+                    const uint16_t* src = reinterpret_cast<const uint16_t*>(
+                        values + (page < c.pages ? page : 0) * page_bytes +
+                        (uint64_t)(head_row + ((uint32_t)x & row_mask)) * row_bytes);
+#pragma unroll
+                    for (int y = 0; y < DT; y++)
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const int d = y * 32 + 8 * z + 4 * half;
+                            u32x2 f = {0, 0};
+                            if (FULL || d < dim) f = *reinterpret_cast<const u32x2*>(src + d);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float v = widen((uint16_t)(f[e >> 1] >> 16 * (e & 1)), BF16);
+                                o[y][4 * z + e] += ok && !(fabsf(v) < INFINITY) ? v : 0.0f;
+                            }
+                        }
+                }
+            }
+            if (more) {
+                // every wave has passed the barrier above, so none reads this buffer
+                pages = pages_next;
+                arrive(pages, tile_pos(t + 1), odd_next, other, careful);
+                pages_next = pages_after;
+            }
+        };
+        for (int t = t_begin; t < t_end; t += 2) {
+            step(t, std::integral_constant<int, 0>());
+            if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>());
         }
     };
-    for (int t = t_begin; t < t_end; t += 2) {
-        step(t, std::integral_constant<int, 0>());
-        if (t + 1 < t_end) step(t + 1, std::integral_constant<int, 1>());
-    }
+    if (threadIdx.x == 0) again_sh = 0;
+    pass(std::false_type());
+    float odd = sum * 0.0f;
+#pragma unroll
+    for (int e = 0; e < DT; e++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) odd = __builtin_fmaf(o[e][i], 0.0f, odd);
+    if (__any(real && odd != 0.0f)) again_sh = 1;
+    __syncthreads();
+    if (again_sh) pass(std::true_type());
     if (unnamed && wave == 0) report(fault, kFaultKvPage);
     if (held_shares > 1) {
         // a share's maximum, sum and values as the lanes hold them; the share to
@@ -1318,7 +1387,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 if (x + y >= held_shares) break;
-                const float f = __builtin_amdgcn_exp2f(ml[y][0] - m);
+                const float f = kept<true>(__builtin_amdgcn_exp2f(ml[y][0] - m));
                 sum += f * ml[y][1];
 #pragma unroll
                 for (int z = 0; z < DT * 8; z++) {

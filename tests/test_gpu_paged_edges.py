@@ -7,8 +7,8 @@ import pytest
 
 import accel_amd
 from accel_amd import BF16, F16, F32, U32, KV_NONE
-from test_gpu_kv_pages import Both
-from test_gpu_paged_attention import Case, types
+from test_gpu_kv_pages import Both, narrow
+from test_gpu_paged_attention import Case, bound, types
 
 pytestmark = pytest.mark.gpu
 
@@ -163,6 +163,87 @@ def test_f32_queries_below_the_normal_range(dev, kv, prompt):
         c.q[:], c.qh[:] = x, x
         c.check(scale=scale)
         c.check(scale=scale, window=20, sinks=3)
+
+
+def seen_not_finite(dev, q, kv, new, lens, put_k=(), put_v=(), tiny=(), **kw):
+    """A case with keys' or values' elements set to what is not finite, run and
+    compared: (sequence, position, head, dim, value) each.  The result has to be
+    what 64 bits give, infinities and NaN where they are; elsewhere within the
+    bounds, the scores' part of them from the keys without those elements."""
+    c = Case(dev, lens, new=new, heads=4, kv_heads=2, dim=64, q=q, kv=kv, seed=17, **kw)
+    for row, dim, x in tiny:
+        c.q[row, :, dim] = c.qh[row, :, dim] = x
+    _, _, size = c.want()
+    for bits, held, puts in ((c.kh, c.k, put_k), (c.vh, c.v, put_v)):
+        for s, pos, h, d, x in puts:
+            at = 0, c.tables[s, pos // 16], h, pos % 16, d
+            held[at] = x
+            bits[at] = narrow(np.array([x], np.float32), kv)[0]
+    with np.errstate(invalid="ignore"):
+        want, _, _ = c.want()
+        c.v = np.nan_to_num(c.v, nan=0.0, posinf=0.0, neginf=0.0)
+        _, mass, _ = c.want()
+    c.upload()
+    c.call()
+    dev.sync()
+    got = c.got()
+    c.free()
+    tol = bound(np.where(np.isfinite(want), want, 0), np.nan_to_num(mass), size, q, kv, 64,
+                max(lens), new is not None)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    off = np.isinf(want)
+    assert np.array_equal(np.isinf(got), off) and np.array_equal(got[off], want[off])
+    ok = np.isfinite(want)
+    assert (np.abs(got[ok] - want[ok]) <= tol[ok]).all()
+    return want
+
+
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("gain", [2.0, 30.0])
+def test_infinite_values_that_are_seen(dev, q, kv, prompt, gain):
+    """One infinity in a column gives it, two of one sign too, two of both NaN,
+    whatever their keys' weights (with a gain of 30 most are below what f32
+    holds), in tiles that all rows see and in those that some see."""
+    inf, nan = np.inf, np.nan
+    put = [(0, 20, 0, 5, inf), (0, 250, 0, 6, -inf), (0, 21, 1, 7, inf), (0, 299, 1, 7, -inf),
+           (0, 40, 1, 8, inf), (0, 260, 1, 8, inf), (1, 2, 0, 63, -inf), (1, 30, 1, 0, nan),
+           (0, 290, 0, 40, inf)]
+    want = seen_not_finite(dev, q, kv, [60, 33] if prompt else None, [300, 40], put_v=put,
+                           gain=gain)
+    assert np.isinf(want).any() and np.isnan(want).any()
+
+
+@types
+def test_infinite_values_of_a_cache_that_is_cut(dev, q, kv):
+    """The parts that workgroups hand to a join."""
+    put = [(0, 20, 0, 5, np.inf), (0, 2500, 0, 6, -np.inf), (0, 1500, 1, 7, np.inf),
+           (0, 2990, 1, 7, np.inf), (0, 700, 1, 9, np.inf), (0, 2700, 1, 9, -np.inf)]
+    for new in (None, [5]):
+        for gain in (2.0, 40.0):
+            seen_not_finite(dev, q, kv, new, [3000], put_v=put, gain=gain)
+
+
+@types
+def test_infinite_values_of_many_short_sequences(dev, q, kv):
+    """Sequences that a wave has to itself, and one after them on the same wave."""
+    n = 200
+    lens = [20 + i % 90 for i in range(n)]
+    c = Case(dev, lens, heads=4, kv_heads=4, dim=64, q=q, kv=kv, seed=3)
+    want, mass, size = c.want()
+    for s in range(0, n, 7):
+        at = 0, c.tables[s, 0], 1, 3, 9
+        c.vh[at] = narrow(np.array([-np.inf], np.float32), kv)[0]
+        want[s, 1, 9] = -np.inf
+    c.upload()
+    c.call()
+    dev.sync()
+    got = c.got()
+    c.free()
+    tol = bound(np.where(np.isfinite(want), want, 0), mass, size, q, kv, 64, max(lens), False)
+    off = np.isinf(want)
+    assert off.sum() == 29 and np.array_equal(got[off], want[off])
+    assert (np.abs(got[~off] - want[~off]) <= tol[~off]).all()
 
 
 def test_a_short_pool_serves_who_fits(dev):
