@@ -124,6 +124,16 @@ __device__ __forceinline__ u32x4 ones() {
     return (u32x4){k, k, k, k};
 }
 
+// Keys that are not finite, under f32 queries: the first of the query's terms, the
+// largest, gives the score there; those of either sign together give NaN.  It has
+// the query's sign, however small the query: what would round to 0 is the term's
+// smallest number instead (2^-38 of the row's largest magnitude).
+template <bool BF16, bool CAREFUL>
+__device__ __forceinline__ float signed_first(float v) {
+    constexpr float kLeast = BF16 ? 0x1p-126f : 0x1p-24f;
+    return CAREFUL && v != 0 && fabsf(v) < kLeast ? copysignf(kLeast, v) : v;
+}
+
 // f16 terms of f32 queries: the power of two that takes a row's largest magnitude
 // to [2^14, 2^15), less where the scores' factor, which takes it back, would leave
 // the normal range: scores hidden as -infinity are multiplied by it.
@@ -524,7 +534,8 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             uint32_t t[QT];
-                            terms16<BF16, QT>(v[j][2 * e], v[j][2 * e + 1], t);
+                            terms16<BF16, QT>(signed_first<BF16, CAREFUL>(v[j][2 * e]),
+                                              signed_first<BF16, CAREFUL>(v[j][2 * e + 1]), t);
 #pragma unroll
                             for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
                         }
@@ -628,11 +639,18 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         s[i] = (f32x4){0, 0, 0, 0};
+                        f32x4 low = {0, 0, 0, 0};
 #pragma unroll
                         for (int j = 0; j < NJ; j++)
 #pragma unroll
-                            for (int x = QT - 1; x >= 0; x--)
-                                s[i] = mfma16<BF16>(k[i][j], q[x][j], s[i]);
+                            for (int x = QT - 1; x >= 0; x--) {
+                                f32x4& to = CAREFUL && x ? low : s[i];
+                                to = mfma16<BF16>(k[i][j], q[x][j], to);
+                            }
+                        if constexpr (CAREFUL)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                s[i][e] += fabsf(s[i][e]) < INFINITY ? low[e] : 0.0f;
                     }
                     const uint32_t page_now = v_page;
                     if (more) load_k(k_next, pos_next);
@@ -1120,7 +1138,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     float y0 = x[e >> 1][2 * (e & 1)], y1 = x[e >> 1][2 * (e & 1) + 1];
                     if constexpr (!BF16) y0 = ldexpf(y0, ex), y1 = ldexpf(y1, ex);
                     uint32_t t[QT];
-                    terms16<BF16, QT>(y0, y1, t);
+                    terms16<BF16, QT>(signed_first<BF16, CAREFUL>(y0),
+                                      signed_first<BF16, CAREFUL>(y1), t);
 #pragma unroll
                     for (int k = 0; k < QT; k++) q[k][j][e] = t[k];
                 }
@@ -1193,6 +1212,24 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     for (int x = QT - 1; x >= 0; x--)
 #pragma unroll
                         for (int i = 0; i < SUB; i++) s[i] = mfma32<BF16>(kf[i], q[x][j], s[i]);
+                }
+                if constexpr (CAREFUL && F32) {
+                    // first terms alone where the score is not finite
+#pragma unroll
+                    for (int i = 0; i < SUB; i++) {
+                        f32x16 first;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) first[e] = 0;
+#pragma unroll
+                        for (int j = 0; j < NS; j++)
+                            first = mfma32<BF16>(
+                                *reinterpret_cast<const u32x4*>(
+                                    k_sh[B] + (k_from ^ k_byte(0, 2 * j)) + k_byte(i * 32, 0)),
+                                q[0][j], first);
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            s[i][e] = fabsf(first[e]) < INFINITY ? s[i][e] : first[e];
+                    }
                 }
                 // reads three products ahead of their use
                 if constexpr (QT == 1) {

@@ -246,6 +246,47 @@ def test_infinite_values_of_many_short_sequences(dev, q, kv):
     assert (np.abs(got[~off] - want[~off]) <= tol[~off]).all()
 
 
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+def test_infinite_keys_that_are_seen(dev, q, kv, prompt):
+    """A score of -inf has no weight, and the result is finite; one of +inf
+    makes it NaN.  Both come of the same key, as the queries' signs are."""
+    put = [(0, 20, 0, 9, np.inf), (0, 270, 0, 9, np.inf), (0, 100, 1, 33, -np.inf),
+           (1, 20, 0, 3, np.inf)]
+    want = seen_not_finite(dev, q, kv, [60, 33] if prompt else None, [300, 40], put_k=put)
+    assert np.isnan(want).any() and np.isfinite(want[:1 if not prompt else 60]).any()
+
+
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_infinite_keys_under_small_f32_queries(dev, kv, prompt):
+    """The sign of a query's element decides, however small it is beside the
+    row's others; the -inf it gives leaves the key out."""
+    rows = 60 if prompt else 1
+    tiny = [(r, 9, -1e-20 if r % 2 == 0 else -1e-9) for r in range(rows)]
+    want = seen_not_finite(dev, F32, kv, [60] if prompt else None, [300], tiny=tiny,
+                           put_k=[(0, 20, 0, 9, np.inf), (0, 230, 1, 9, np.inf)])
+    assert np.isfinite(want).all()
+
+
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+def test_scores_that_are_all_minus_infinity(dev, q, kv, prompt):
+    """No key has a weight then: zeros, as for a query that sees none."""
+    c = Case(dev, [70, 5], new=[3, 5] if prompt else None, heads=4, kv_heads=2, dim=64, q=q,
+             kv=kv)
+    c.q[:, :, 9] = -1
+    c.qh[:, :, 9] = -1 if q == F32 else narrow(np.array([-1.0]), q)[0]
+    for s, n in enumerate([70, 5]):
+        for p in range(n):
+            c.kh[0, c.tables[s, p // 16], :, p % 16, 9] = narrow(np.array([np.inf]), kv)[0]
+    c.upload()
+    c.call()
+    dev.sync()
+    assert not c.got().any()
+    c.free()
+
+
 def test_a_short_pool_serves_who_fits(dev):
     """An entry that the pool cannot serve takes nothing from those after it."""
     b = Both(dev, pages=50, sequences=8, slots=100)
