@@ -99,6 +99,23 @@ __device__ __forceinline__ float kept(float f) {
     return INF ? fmaxf(f, 0x1p-149f) : f;
 }
 
+// Whether a sum of weights or of values is: products with 0, by fours of an
+// operand's rows that count.
+template <int N, typename V, typename F>
+__device__ __forceinline__ bool not_finite(float sum, const V (&o)[N], F counts) {
+    float odd = sum * 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / 16); i++) {
+            float x = o[e][4 * i] * 0.0f;
+#pragma unroll
+            for (int k = 1; k < 4; k++) x = __builtin_fmaf(o[e][4 * i + k], 0.0f, x);
+            odd += counts(e, i) ? x : 0.0f;
+        }
+    return odd != 0.0f;
+}
+
 // Takes the values that are not finite out of eight.  One whose exponent is all
 // ones carries into the sign's place.
 template <bool BF16>
@@ -735,12 +752,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                 }
             };
             pass(std::false_type());
-            float odd = sum * 0.0f;
-#pragma unroll
-            for (int e = 0; e < VD; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) odd = __builtin_fmaf(o[e][i], 0.0f, odd);
-            if (__any(odd != 0.0f)) pass(std::true_type());
+            if (__any(not_finite(sum, o, [](int, int) { return true; }))) pass(std::true_type());
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (alone) {
@@ -1357,12 +1369,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     };
     if (threadIdx.x == 0) again_sh = 0;
     pass(std::false_type());
-    float odd = sum * 0.0f;
-#pragma unroll
-    for (int e = 0; e < DT; e++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) odd = __builtin_fmaf(o[e][i], 0.0f, odd);
-    if (__any(real && odd != 0.0f)) again_sh = 1;
+    // past the head's dims there is whatever LDS held
+    const auto counts = [&](int e, int i) { return FULL || e * 32 + 8 * i + 4 * half < dim; };
+    if (__any(real && not_finite(sum, o, counts))) again_sh = 1;
     __syncthreads();
     if (again_sh) pass(std::true_type());
     if (unnamed && wave == 0) report(fault, kFaultKvPage);

@@ -707,7 +707,7 @@ typedef struct accel_attention {
  * query head h reads key-value head h / (heads / kv_heads).  q is f32, or the
  * cache's type; products, softmax and sums are f32 (f32 queries and weights
  * are not rounded to the cache's type).  A query that sees no key (an empty
- * sequence, ACCEL_KV_NONE) gives zeros.  A value that is seen and is not finite
+ * sequence, ACCEL_KV_NONE), or none with a score past -infinity, gives zeros.  A value that is seen and is not finite
  * enters its sum as it is, however small its key's weight.  A page missing where
  * the query would see it is left out of the softmax and reported.  q and out
  * 16-byte aligned.  opt may be NULL (all zero). */
