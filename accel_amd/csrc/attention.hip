@@ -171,7 +171,7 @@ __device__ __forceinline__ void store_result(const KvCache& c, const Attention& 
 
 constexpr int kTile = 32;             // keys a wave step
 constexpr float kLift = 8.0f;         // how far scores may exceed the running maximum
-constexpr float kLowest = -3.0e38f;   // the maximum before any key
+constexpr float kLowest = -__FLT_MAX__;   // the maximum before any key
 // A cut this near to a sequence's first or last tile moves there: a join costs
 // about two steps of eight waves.  One sequence of 4096, eight heads of 128: 20.6
 // us with 24, 15.5 with 12 or 8; 33 sequences seen through a window of 1000, 33

@@ -287,6 +287,26 @@ def test_scores_that_are_all_minus_infinity(dev, q, kv, prompt):
     c.free()
 
 
+@pytest.mark.parametrize("prompt", [False, True])
+def test_scores_at_the_lowest_end_of_f32(dev, prompt):
+    """All scores between -3.4e38 and -3e38 in units of log 2: one key's value."""
+    for n in (1, 90):
+        c = Case(dev, [n], new=[1] if prompt else None, heads=2, kv_heads=1, dim=64, q=F32)
+        c.q[:], c.qh[:] = 0, 0
+        c.q[..., 3] = c.qh[..., 3] = -2.2e19
+        # the first key's score is the largest by 2^120 and more
+        k = np.full((n, 64), 1.02e19, np.float32)
+        k[0] = 1e19
+        for p in range(n):
+            c.kh[0, c.tables[0, p // 16], 0, p % 16] = narrow(k[p], BF16)
+        c.upload()
+        c.call(scale=1.0)
+        dev.sync()
+        v = c.v[0, c.tables[0, 0], 0, 0]
+        assert np.abs(c.got()[0] - v).max() <= 2.0 ** -20 * np.abs(v).max()
+        c.free()
+
+
 def test_a_short_pool_serves_who_fits(dev):
     """An entry that the pool cannot serve takes nothing from those after it."""
     b = Both(dev, pages=50, sequences=8, slots=100)
