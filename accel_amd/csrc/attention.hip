@@ -116,6 +116,17 @@ __device__ __forceinline__ bool not_finite(float sum, const V (&o)[N], F counts)
     return odd != 0.0f;
 }
 
+// A score in units of log 2 and its weight, each rounded by itself: the largest
+// score's weight is what it is to be, however large they are.
+__device__ __forceinline__ float scaled(float s, float factor) {
+#pragma clang fp contract(off)
+    return s * factor;
+}
+__device__ __forceinline__ float weight_of(float y, float m) {
+#pragma clang fp contract(off)
+    return __builtin_amdgcn_exp2f(y - m);
+}
+
 // Takes the values that are not finite out of eight.  One whose exponent is all
 // ones carries into the sign's place.
 template <bool BF16>
@@ -676,7 +687,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                                      !__any(page_now >= c.pages);
                     float y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = s[e >> 2][e & 3] * factor;
+                    for (int e = 0; e < 8; e++) y[e] = scaled(s[e >> 2][e & 3], factor);
                     uint32_t hidden = 0;
                     if (!all) {
                         const uint32_t p0 = pos + quad * 8;
@@ -695,7 +706,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     float top = y[0];
 #pragma unroll
                     for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-                    if (__any(top > m + kLift)) {
+                    if (__any(top - m > kLift)) {
                         top = fmaxf(top, __shfl_xor(top, 16, 64));
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
                         const float up = fmaxf(m, top);
@@ -708,8 +719,8 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     u32x4 w[PT];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float a0 = __builtin_amdgcn_exp2f(y[2 * e] - m);
-                        const float a1 = __builtin_amdgcn_exp2f(y[2 * e + 1] - m);
+                        const float a0 = weight_of(y[2 * e], m);
+                        const float a1 = weight_of(y[2 * e + 1], m);
                         sum += a0 + a1;
                         uint32_t x[PT];
                         terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
@@ -1113,7 +1124,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
     }
     // A first pass takes the values of tiles that all rows see as they are; where
-    // something in it is not finite the workgroup goes over its keys again.
+    // something in it is not finite, or scores are large, the workgroup goes over
+    // its keys again.
     f32x16 o[DT];
     float m, sum;
     bool unnamed = false;       // a page some row sees and the table does not name
@@ -1289,8 +1301,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                         top = fmaxf(fmaxf(top, s[i][e]), s[i][e + 1]);
                         top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
                     }
-                top = fmaxf(top, top1) * factor;
-                if (__any(top > m + kLift)) {
+                top = scaled(fmaxf(top, top1), factor);
+                if (__any(top - m > kLift)) {
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
                     const float up = fmaxf(m, top);
                     const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
@@ -1305,10 +1317,15 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 for (int i = 0; i < SUB; i++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float w0 =
-                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
-                        const float w1 =
-                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e + 1], factor, -m));
+                        float w0, w1;
+                        if constexpr (CAREFUL) {
+                            w0 = weight_of(scaled(s[i][2 * e], factor), m);
+                            w1 = weight_of(scaled(s[i][2 * e + 1], factor), m);
+                        } else {
+                            w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][2 * e], factor, -m));
+                            w1 = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(s[i][2 * e + 1], factor, -m));
+                        }
                         part[e & 3] += w0 + w1;
                         uint32_t x[PT];
                         terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
@@ -1371,7 +1388,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     pass(std::false_type());
     // past the head's dims there is whatever LDS held
     const auto counts = [&](int e, int i) { return FULL || e * 32 + 8 * i + 4 * half < dim; };
-    if (__any(real && not_finite(sum, o, counts))) again_sh = 1;
+    // nor do scores from 2^20 on stand in one fused step with their maximum, which
+    // is rounded: what that leaves out is 2^-4 there and soon past any weight
+    const bool large = fabsf(m) >= 0x1p20f && m > kLowest;
+    if (__any(real && (large || not_finite(sum, o, counts)))) again_sh = 1;
     __syncthreads();
     if (again_sh) pass(std::true_type());
     if (unnamed && wave == 0) report(fault, kFaultKvPage);

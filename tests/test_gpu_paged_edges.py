@@ -307,6 +307,43 @@ def test_scores_at_the_lowest_end_of_f32(dev, prompt):
         c.free()
 
 
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_past_what_f32_tells_apart(dev, q, kv, prompt, sign):
+    """Scores of sizes up to f32's last, all equal (the mean of the values) or
+    one above all others by a part of itself (its value): a score's rounding is
+    then more than the exponential's whole range."""
+    n, dim = 150, 64
+    for same in (True, False):
+        c = Case(dev, [n], new=[20] if prompt else None, heads=2, kv_heads=1, dim=dim, q=q, kv=kv)
+        x = np.zeros(dim, np.float32)
+        x[3] = 1.375
+        c.qh[:] = x if q == F32 else narrow(x, q)
+        for p in range(n):
+            k = np.zeros(dim, np.float32)
+            k[3] = sign * (0.75 if same or (p == 40) == (sign > 0) else 0.625)
+            c.kh[0, c.tables[0, p // 16], 0, p % 16] = narrow(k, kv)
+        v = np.stack([c.v[0, c.tables[0, p // 16], 0, p % 16] for p in range(n)])
+        rows = range(n - 20, n) if prompt else [n - 1]
+        c.upload()
+        for e in (10, 18, 19, 20, 21, 22, 23, 24, 25, 26, 27, 28, 29, 30, 31, 40, 80, 125.6):
+            for f in (1.0, 1.2345678):
+                c.call(scale=f * 2.0 ** e)
+                dev.sync()
+                got = c.got()
+                if same:
+                    want = np.stack([v[:p + 1].mean(0, dtype=np.float64) for p in rows])
+                    mass = np.stack([np.abs(v[:p + 1]).mean(0, dtype=np.float64) for p in rows])
+                else:
+                    want = np.broadcast_to(v[40].astype(np.float64), (len(rows), dim))
+                    mass = np.abs(want)
+                tol = bound(want, mass, np.zeros(len(rows)), q, kv, dim, n, prompt)
+                bad = np.abs(got - want[:, None]) > tol[:, None]
+                assert np.isfinite(got).all() and not bad.any(), (e, f, same)
+        c.free()
+
+
 def test_a_short_pool_serves_who_fits(dev):
     """An entry that the pool cannot serve takes nothing from those after it."""
     b = Both(dev, pages=50, sequences=8, slots=100)
