@@ -17,13 +17,14 @@
 // - A lane loads V for those eight keys, DIM / 16 consecutive dims of each, and
 //   turns the block by byte permutes (half an instruction an element) into A
 //   operands with the eight keys along k; which dim is which row is free too.
-// - The running maximum is only moved when some score exceeds it by 2^8 (sums
-//   and weights stay far inside f32 and the 16-bit types' ranges), so most
-//   steps have no exchange between lanes.  A lane sums its own weights.
+// - The running maximum is only moved when some weight would pass 2^8 of it (over
+//   an f16 cache 2^6: kOver, kLift), so most steps have no exchange between
+//   lanes.  A lane sums its own weights.
 //
 // Weights are split into two 16-bit terms (f32 queries: three bf16 or two f16
 // terms, queries too), so a 16-bit call rounds only its result and an f32 call
-// keeps 2^-22 of each; the matrix cores have the time.
+// keeps 2^-22 of each (over an f16 cache, where the last term's steps end, 2^-34 of
+// the row's largest weight); the matrix cores have the time.
 //
 // The work is cut evenly over the workgroups whatever the lengths: the tiles of
 // 32 keys of all sequences in one line a key-value head, a workgroup an equal
@@ -181,8 +182,17 @@ __device__ __forceinline__ void store_result(const KvCache& c, const Attention& 
 // ---- one new token a sequence ---------------------------------------------------
 
 constexpr int kTile = 32;             // keys a wave step
-constexpr float kLift = 8.0f;         // how far scores may exceed the running maximum
-constexpr float kLowest = -__FLT_MAX__;   // the maximum before any key
+// A weight is 2^(score - m), where m is the running maximum less kOver, and m moves
+// when some score exceeds it by more than kOver + kLift.  f16 holds 2^-14 to 2^16 in
+// full and steps of 2^-24 below: weights of 2^9 to 2^15 for the largest leave those
+// down to 2^-23 of it all their bits, and half a step is 2^-34 of it.  (f16 prompt of
+// 2048 with 7 + 8, 9 + 6 and 11 + 4: 60.0, 60.4 and 61.3 us, 59.0 with the largest at
+// 1; f32 of 1000: 49.0, 49.8 and 51.1.)
+template <bool BF16>
+constexpr float kOver = BF16 ? 0.0f : 9.0f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 8.0f : 6.0f;
+constexpr float kLowest = -__FLT_MAX__;   // m before any key
 // A cut this near to a sequence's first or last tile moves there: a join costs
 // about two steps of eight waves.  One sequence of 4096, eight heads of 128: 20.6
 // us with 24, 15.5 with 12 or 8; 33 sequences seen through a window of 1000, 33
@@ -194,6 +204,13 @@ constexpr uint32_t kNear = 12;
 // 56 -> 45 with up to 8 tiles, 40 with 12 or 16).
 constexpr uint32_t kAlone = 12;
 constexpr int kManyAlone = 3;
+
+// m for a maximum.  Where f32's steps are 16, kOver less is 16 less.
+template <bool BF16>
+__device__ __forceinline__ float below(float top) {
+    const float m = top - kOver<BF16>;
+    return top - m > kOver<BF16> + kLift<BF16> ? top : m;
+}
 
 // The keys a query at position n - 1 sees: [0, first) and [lo, n); the tiles
 // that hold them, in order.
@@ -414,8 +431,6 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
     constexpr int VD = DIM / 16;       // dims of a value a lane holds
     constexpr int VW = VD / 2;         // and words
     constexpr bool F32 = QT > 1;
-    // f16 terms of f32 weights: 2^7 keeps the last one's steps below 2^-30
-    constexpr float kWeightGain = !BF16 ? 128.0f : 1.0f;
     __shared__ float acc_sh[W][16][DIM + 4];
     __shared__ float max_sh[W][16], sum_sh[W][16];
     __shared__ int last_sh;
@@ -706,10 +721,10 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     float top = y[0];
 #pragma unroll
                     for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-                    if (__any(top - m > kLift)) {
+                    if (__any(top - m > kOver<BF16> + kLift<BF16>)) {
                         top = fmaxf(top, __shfl_xor(top, 16, 64));
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const float up = fmaxf(m, top);
+                        const float up = fmaxf(m, below<BF16>(top));
                         const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
                         m = up;
                         sum *= keep;
@@ -723,7 +738,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                         const float a1 = weight_of(y[2 * e + 1], m);
                         sum += a0 + a1;
                         uint32_t x[PT];
-                        terms16<BF16, PT>(a0 * kWeightGain, a1 * kWeightGain, x);
+                        terms16<BF16, PT>(a0, a1, x);
 #pragma unroll
                         for (int i = 0; i < PT; i++) w[i][e] = x[i];
                     }
@@ -767,7 +782,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (alone) {
-                const float out = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
+                const float out = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -788,7 +803,7 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                 for (int e = 0; e < VD; e++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        acc_sh[wave][col][(quad * 4 + i) * VD + e] = o[e][i] * (1.0f / kWeightGain);
+                        acc_sh[wave][col][(quad * 4 + i) * VD + e] = o[e][i];
             }
             __syncthreads();
             const bool whole = t0 == 0 && t1 == sp.tiles;
@@ -856,11 +871,12 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
 // scores and sums (its column), half of the keys, and the other half is 32
 // lanes on.  As in the decode kernel the keys' order in K's rows is chosen so that
 // a lane's scores are its part of P^T's operand, and the running maximum moves
-// only when scores exceed it by 2^8.
+// as rarely.
 //
 // Weights of a 16-bit call are rounded to its type once (the sum of them is not):
-// half a step of each, as the product's operands have to be 16 bits; f32 calls
-// split queries and weights as the decode kernel does.
+// half a step of each, in f16 no less than 2^-34 of the row's largest, as the
+// product's operands have to be 16 bits; f32 calls split queries and weights as the
+// decode kernel does.
 //
 // What bounds it is issue: with two waves a SIMD the MFMAs take 38% of a step's
 // cycles and some 280 VALU instructions a wave most of the rest; 2048 tokens
@@ -921,7 +937,6 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
     constexpr int KL = KT * NC / 256;       // chunks of K, and of V, a lane stages
     constexpr bool F32 = QT > 1;
-    constexpr float kWeightGain = F32 && !BF16 ? 128.0f : 1.0f;
     __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
     __shared__ __attribute__((aligned(256))) char v_sh[2][KT * NC * 16];
     // keys of a tile with values that are not finite: tile t's in place t % 3,
@@ -1302,9 +1317,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                         top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
                     }
                 top = scaled(fmaxf(top, top1), factor);
-                if (__any(top - m > kLift)) {
+                if (__any(top - m > kOver<BF16> + kLift<BF16>)) {
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float up = fmaxf(m, top);
+                    const float up = fmaxf(m, below<BF16>(top));
                     const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
                     m = up;
                     sum *= keep;
@@ -1328,7 +1343,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                         }
                         part[e & 3] += w0 + w1;
                         uint32_t x[PT];
-                        terms16<BF16, PT>(w0 * kWeightGain, w1 * kWeightGain, x);
+                        terms16<BF16, PT>(w0, w1, x);
 #pragma unroll
                         for (int k = 0; k < PT; k++) w[k][i][e >> 2][e & 3] = x[k];
                     }
@@ -1465,7 +1480,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     }
     if (!real) return;
     sum += __shfl_xor(sum, 32, 64);
-    const float scale = sum == 0 ? 0.0f : (1.0f / kWeightGain) / sum;
+    const float scale = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int e = 0; e < DT; e++)
 #pragma unroll

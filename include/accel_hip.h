@@ -722,7 +722,8 @@ int accel_paged_attention(int dev, void* stream, const accel_tensor_t* q,
  * values are in the cache already).  offsets u32 [n+1], ascending from 0.  Rows
  * past the last offset are left as they were.  For a 16-bit q the softmax
  * weights are rounded to the cache's type before the product with the values
- * (their sum is not). */
+ * (their sum is not).  Here and in accel_paged_attention weights over an f16
+ * cache are rounded by up to 2^-34 of the row's largest where that is more. */
 int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q,
                         const accel_tensor_t* offsets, const accel_kv_cache_t* cache,
                         int64_t layer, const accel_tensor_t* seqs,

@@ -287,6 +287,49 @@ def test_scores_that_are_all_minus_infinity(dev, q, kv, prompt):
     c.free()
 
 
+@types
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("gap", [14, 18, 21, 23])
+@pytest.mark.parametrize("n", [190, 4000])
+def test_a_first_key_of_value_zero_that_dominates(dev, q, kv, prompt, n, gap):
+    """A first key `gap` nats above all others, its value 0: the result is
+    theirs alone.  Over an f16 cache weights, or their last terms, are f16
+    numbers, 2^9 or more for the row's largest; their steps below the normal
+    range are 2^-24, half of one 2^-25 / 2^9 = 2^-34 of the largest, which is 1
+    at most.  That times the value, for each key, comes to the bound."""
+    dim = 64
+    c = Case(dev, [n], new=[40] if prompt else None, heads=2, kv_heads=1, dim=dim, q=q, kv=kv,
+             seed=gap, gain=0.05)
+    first = 0, c.tables[0, 0], 0, 0
+    rng = np.random.default_rng(gap)
+    x = (1000 * (1 + rng.standard_normal(c.v.shape) / 4)).astype(np.float32)
+    held = ((c.vh & 0x7fff) != (0x7fc0 if kv == BF16 else 0x7e00))
+    bits = narrow(x, kv)
+    c.vh[held] = bits[held]
+    c.v = (bits.astype(np.uint32) << 16).view(np.float32) if kv == BF16 else \
+        bits.view(np.float16).astype(np.float32)
+    c.k[..., 0] = 0
+    c.kh[..., 0][held[..., 0]] = 0
+    c.q[..., 0] = 4
+    c.qh[..., 0] = 4 if q == F32 else narrow(np.array([4.0]), q)[0]
+    c.v[first], c.vh[first] = 0, 0
+    c.k[first] = 0
+    c.k[first + (0,)] = gap / 4
+    c.kh[first] = narrow(c.k[first], kv)
+    want, mass, size = c.want(scale=1.0)
+    c.upload()
+    c.call(scale=1.0)
+    dev.sync()
+    got = c.got()
+    c.free()
+    tol = bound(want, mass, size, q, kv, dim, n, prompt)
+    if kv == F16:
+        total = sum(np.abs(c.v[0, c.tables[0, p // 16], 0, p % 16]) for p in range(n))
+        tol = tol + 2.0 ** -34 * total
+    assert want.min() > 0
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got / want - 1)).max()
+
+
 @pytest.mark.parametrize("prompt", [False, True])
 def test_scores_at_the_lowest_end_of_f32(dev, prompt):
     """All scores between -3.4e38 and -3e38 in units of log 2: one key's value."""
