@@ -889,10 +889,18 @@ class Device:
                  sequences: int, slots: int, dtype: int = BF16, stream=None) -> KVCache:
         """Allocates a cache and clears it (accel_kv_clear)."""
         shape = (layers, pages, kv_heads, page_size, head_dim)
-        c = KVCache(self, self.alloc(shape, dtype), self.alloc(shape, dtype),
-                    self.alloc((pages,), U32), self.alloc((sequences, slots), U32),
-                    self.alloc((sequences,), U32))
-        self.KVClear(c, stream)
+        held = []
+        try:
+            for s, t in ((shape, dtype), (shape, dtype), ((pages,), U32),
+                         ((sequences, slots), U32), ((sequences,), U32)):
+                held.append(self.alloc(s, t))
+            c = KVCache(self, *held)
+            self.KVClear(c, stream)
+        except Exception:
+            # memory that ran out, or a cache that is refused, keeps none
+            for b in held:
+                b.free()
+            raise
         return c
 
     def KVClear(self, cache: KVCache, stream=None) -> None:

@@ -3,8 +3,8 @@ runs before a device is touched)."""
 import pytest
 
 import accel_amd
-from accel_amd import BF16, AttentionDesc
-from test_kv_refusals import L, R, cache, refused, tensor
+from accel_amd import BF16, AccelError, AttentionDesc
+from test_kv_refusals import A, L, R, cache, refused, tensor
 
 MOST = 2 ** 31 - 1 - 1024
 
@@ -44,3 +44,31 @@ def test_scales_that_pass_the_range_in_units_of_log_2():
     o = AttentionDesc(2.0 ** 127, 0, 0)
     rc = L.accel_paged_attention(63, None, R(q), R(c), 0, None, R(o), R(q))
     assert rc == accel_amd.E_NO_DEVICE
+
+
+def test_a_cache_that_is_refused_keeps_no_memory():
+    class Held:
+        def __init__(self, shape, dtype):
+            self.shape, self.dtype, self.ptr = shape, dtype, A
+            held.append(self)
+
+        def free(self):
+            self.ptr = 0
+
+    held = []
+    dev = accel_amd.Device.__new__(accel_amd.Device)
+    dev.index, dev.alloc = 63, Held
+    with pytest.raises(AccelError, match="pages of 24"):
+        dev.kv_cache(1, 4, 2, 24, 64, 3, 2)
+    assert len(held) == 5 and not any(b.ptr for b in held)
+
+    def short(shape, dtype):
+        if len(held) == 3:
+            raise AccelError(accel_amd.E_NO_DEVICE, "out of memory")
+        return Held(shape, dtype)
+
+    held.clear()
+    dev.alloc = short
+    with pytest.raises(AccelError, match="out of memory"):
+        dev.kv_cache(1, 4, 2, 16, 64, 3, 2)
+    assert len(held) == 3 and not any(b.ptr for b in held)
