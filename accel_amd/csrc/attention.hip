@@ -6,8 +6,8 @@
 // (all j <= p without a window).
 //
 // One new token a sequence (paged_decode_kernel).  The bytes of the keys and
-// values bound it: each is read once, for all the query heads of its group.
-// A wave takes 32 keys at a time against up to 16 query heads as
+// values bound it: each is read once for up to 16 query heads of its group, once
+// more for every further 16.  A wave takes 32 keys at a time against those heads as
 // S^T = K Q^T and O^T += V^T P^T on the matrix cores, everything in registers:
 //
 // - K goes from memory to the A operand as it is (a lane 16 bytes of one key a
@@ -80,11 +80,6 @@ __device__ __forceinline__ void terms16(float a, float b, uint32_t (&t)[TERMS]) 
             b -= (float)h[1];
         }
     }
-}
-
-__device__ __forceinline__ float widen(uint16_t h, bool bf16) {
-    if (bf16) return __uint_as_float((uint32_t)h << 16);
-    return half_bits_to_float(h);
 }
 
 // Values that are not finite.  What the definition gives for one that is seen, as
@@ -707,8 +702,9 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     if (!all) {
                         const uint32_t p0 = pos + quad * 8;
                         if (page_now >= c.pages) report(fault, kFaultKvPage);
-                        // selects without a branch: written with && and ||, this
-                        // compiler left y[0] of a key behind the window as it was
+                        // conditions without branches, a select each: joined with &&
+                        // and || an earlier form did not hide y[0] of a key behind the
+                        // window (why was not found; the window tests hold this one)
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             const bool ok = (p0 + e < sp.n) &

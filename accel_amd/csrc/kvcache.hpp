@@ -31,6 +31,14 @@ __device__ __forceinline__ uint32_t length_of(const KvCache& c, uint32_t seq) {
     return n < cap ? n : cap;
 }
 
+// A value of the cache's type.
+__device__ __forceinline__ float widen(uint16_t h, bool bf16) {
+    if (bf16) return __uint_as_float((uint32_t)h << 16);
+    _Float16 v;
+    __builtin_memcpy(&v, &h, 2);
+    return (float)v;
+}
+
 // The entry of ascending offsets [n + 1] that row belongs to, or -1.
 __device__ __forceinline__ int entry_of(const uint32_t* offsets, int n, uint32_t row) {
     int lo = 0, hi = n + 1;            // the first offset past row is in [lo, hi]

@@ -267,12 +267,6 @@ __global__ __launch_bounds__(kPlan) void kv_reserve_kernel(KvCache c, const uint
 }
 
 // f32 or 16-bit values, eight of them, as the cache's 16-bit type.
-__device__ __forceinline__ float widen(uint16_t h, bool bf16) {
-    if (bf16) return __uint_as_float((uint32_t)h << 16);
-    _Float16 v;
-    __builtin_memcpy(&v, &h, 2);
-    return (float)v;
-}
 __device__ __forceinline__ uint16_t narrow(float f, bool bf16) {
     if (bf16) return __builtin_bit_cast(uint16_t, (__bf16)f);
     return __builtin_bit_cast(uint16_t, (_Float16)f);

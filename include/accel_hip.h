@@ -662,7 +662,9 @@ int accel_kv_append(int dev, void* stream, const accel_kv_cache_t* cache, int64_
  * this, that names a sequence outside the cache or that finds no free page
  * leaves its child empty and is reported; an entry with an ACCEL_KV_NONE is
  * skipped.  Parents are read as they were before the call.  A parent's slot
- * without a page (accel_kv_trim) has none in the branch. */
+ * without a page (accel_kv_trim) has none in the branch.  Rows of positions that
+ * a parent has reserved are appended before it branches: a later row of either
+ * would be in a page that both have. */
 int accel_kv_fork(int dev, void* stream, const accel_kv_cache_t* cache,
                   const accel_tensor_t* parents, const accel_tensor_t* children);
 

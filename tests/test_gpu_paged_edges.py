@@ -421,3 +421,25 @@ def test_a_short_pool_of_many_entries(dev, seed):
         grow = rng.integers(0, [60, 500, 20, 300][seed % 4], n)
         b.reserve([int(x) for x in grow], [int(s) for s in seqs])
         b.free([int(s) for s in rng.permutation(n)[:n // 3]])
+
+
+@types
+@pytest.mark.parametrize("dim", [40, 128, 200])
+def test_prompts_of_more_entries_than_a_wave_has_lanes(dev, q, kv, dim):
+    """Entries summed up by a launch before: ragged, empty and padded ones,
+    chunks after prefixes, a window over some of them."""
+    rng = np.random.default_rng(dim)
+    n = 150
+    new = [int(x) for x in rng.integers(0, 9, n)]
+    new[3], new[90] = 70, 41
+    lens = [x + int(y) for x, y in zip(new, rng.integers(0, 30, n))]
+    lens[90] += 200
+    seqs = [int(x) for x in rng.permutation(n)]
+    seqs[5] = KV_NONE
+    of = {s: new[i] for i, s in enumerate(seqs) if s != KV_NONE}
+    for s, x in of.items():
+        lens[s] = max(lens[s], x)
+    Case(dev, lens, new=new, heads=6, kv_heads=2, dim=dim, page=8, q=q, kv=kv, seqs=seqs,
+         extra_rows=3, seed=dim).check(window=60, sinks=5)
+    Case(dev, lens, new=new, heads=2, kv_heads=2, dim=dim, page=8, q=q, kv=kv, seqs=seqs,
+         seed=dim + 1).check()
