@@ -85,8 +85,8 @@ __device__ __forceinline__ void terms16(float a, float b, uint32_t (&t)[TERMS]) 
 // Values that are not finite.  What the definition gives for one that is seen, as
 // every weight is more than 0, is itself; a weight's terms of either sign, and
 // weights that are 0 in 32 bits or fewer, make it NaN in a product.  So a pass over
-// the keys whose result is not finite is made again with such values apart: taken
-// out of the products and added as they are.  Where all is finite that costs the
+// the keys whose result is not finite, or near that, is made again with such values
+// apart: taken out of the products and added as they are.  Where all is finite that costs the
 // look at the result and a barrier: 0.4 us of a window over 33 sequences' 14.4, 0.7 of
 // a prompt; f32 prompts of 136 to 256 dims, whose registers spill, 4 to 5%.
 
@@ -97,21 +97,22 @@ __device__ __forceinline__ float kept(float f) {
     return INF ? fmaxf(f, 0x1p-149f) : f;
 }
 
-// Whether a sum of weights or of values is: products with 0, by fours of an
-// operand's rows that count.
+// Whether a sum of weights or of values is, or of values so large (2^110) that sums
+// of them may not be: products that leave the range then, by fours of an operand's
+// rows that count.
 template <int N, typename V, typename F>
 __device__ __forceinline__ bool not_finite(float sum, const V (&o)[N], F counts) {
-    float odd = sum * 0.0f;
+    float odd = sum * 0x1p18f;
 #pragma unroll
     for (int e = 0; e < N; e++)
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(V) / 16); i++) {
-            float x = o[e][4 * i] * 0.0f;
+            float x = o[e][4 * i] * 0x1p18f;
 #pragma unroll
-            for (int k = 1; k < 4; k++) x = __builtin_fmaf(o[e][4 * i + k], 0.0f, x);
+            for (int k = 1; k < 4; k++) x = __builtin_fmaf(o[e][4 * i + k], 0x1p18f, x);
             odd += counts(e, i) ? x : 0.0f;
         }
-    return odd != 0.0f;
+    return !(fabsf(odd) < INFINITY);
 }
 
 // A score in units of log 2 and its weight, each rounded by itself: the largest
@@ -184,9 +185,10 @@ constexpr int kTile = 32;             // keys a wave step
 // full and steps of 2^-24 below: weights of 2^9 to 2^15 for the largest leave those
 // down to 2^-23 of it all their bits, and half a step is 2^-34 of it.  (f16 prompt of
 // 2048 with 7 + 8, 9 + 6 and 11 + 4: 60.0, 60.4 and 61.3 us, 59.0 with the largest at
-// 1; f32 of 1000: 49.0, 49.8 and 51.1.)
-template <bool BF16>
-constexpr float kOver = BF16 ? 0.0f : 9.0f;
+// 1; f32 of 1000: 49.0, 49.8 and 51.1.)  A second pass over a bf16 cache takes 2^-40
+// for the largest: 2^31 values of up to 2^128 stay in f32's range.
+template <bool BF16, bool CAREFUL>
+constexpr float kOver = !BF16 ? 9.0f : CAREFUL ? -40.0f : 0.0f;
 template <bool BF16>
 constexpr float kLift = BF16 ? 8.0f : 6.0f;
 constexpr float kLowest = -__FLT_MAX__;   // m before any key
@@ -202,11 +204,12 @@ constexpr uint32_t kNear = 12;
 constexpr uint32_t kAlone = 12;
 constexpr int kManyAlone = 3;
 
-// m for a maximum.  Where f32's steps are 16, kOver less is 16 less.
-template <bool BF16>
+// m for a maximum.  Where f32's steps are 16, 9 less is 16 less.
+template <bool BF16, bool CAREFUL>
 __device__ __forceinline__ float below(float top) {
-    const float m = top - kOver<BF16>;
-    return top - m > kOver<BF16> + kLift<BF16> ? top : m;
+    constexpr float over = kOver<BF16, CAREFUL>;
+    const float m = top - over;
+    return top - m > over + kLift<BF16> ? top : m;
 }
 
 // The keys a query at position n - 1 sees: [0, first) and [lo, n); the tiles
@@ -719,10 +722,10 @@ __global__ __launch_bounds__(64 * kWaves<DIM>) void paged_decode_kernel(
                     float top = y[0];
 #pragma unroll
                     for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-                    if (__any(top - m > kOver<BF16> + kLift<BF16>)) {
+                    if (__any(top - m > kOver<BF16, CAREFUL> + kLift<BF16>)) {
                         top = fmaxf(top, __shfl_xor(top, 16, 64));
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const float up = fmaxf(m, below<BF16>(top));
+                        const float up = fmaxf(m, below<BF16, CAREFUL>(top));
                         const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
                         m = up;
                         sum *= keep;
@@ -1315,9 +1318,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                         top1 = fmaxf(fmaxf(top1, s[i][e + 2]), s[i][e + 3]);
                     }
                 top = scaled(fmaxf(top, top1), factor);
-                if (__any(top - m > kOver<BF16> + kLift<BF16>)) {
+                if (__any(top - m > kOver<BF16, CAREFUL> + kLift<BF16>)) {
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float up = fmaxf(m, below<BF16>(top));
+                    const float up = fmaxf(m, below<BF16, CAREFUL>(top));
                     const float keep = kept<CAREFUL>(__builtin_amdgcn_exp2f(m - up));
                     m = up;
                     sum *= keep;

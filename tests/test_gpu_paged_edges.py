@@ -387,6 +387,27 @@ def test_scores_far_past_what_f32_tells_apart(dev, q, kv, prompt, sign):
         c.free()
 
 
+@pytest.mark.parametrize("q", [F32, BF16])
+@pytest.mark.parametrize("new", [None, [60], [5]])
+def test_values_at_the_end_of_bf16(dev, q, new):
+    """Sums of weights times values pass f32's range where weights are more than
+    1, or keys many; the mean they stand for does not."""
+    for n in (300, 3000):
+        if new == [60] and n == 3000:
+            continue
+        for gain in (2.0, 12.0):
+            c = Case(dev, [n], new=new, heads=4, kv_heads=2, dim=64, q=q, kv=BF16, seed=n,
+                     gain=gain)
+            held = c.vh != 0x7fc0
+            # magnitudes up to 2^128 (1 - 2^-8), a column of one sign and size
+            x = (c.v * np.float32(2.0 ** 125)).clip(-3.38e38, 3.38e38)
+            x[..., 7] = 3.38e38
+            bits = narrow(x, BF16)
+            c.vh[held] = bits[held]
+            c.v = (bits.astype(np.uint32) << 16).view(np.float32)
+            c.check()
+
+
 def test_a_short_pool_serves_who_fits(dev):
     """An entry that the pool cannot serve takes nothing from those after it."""
     b = Both(dev, pages=50, sequences=8, slots=100)
