@@ -129,6 +129,15 @@ class AttentionDesc(ctypes.Structure):
                 ("sinks", ctypes.c_int64)]
 
 
+class SamplingDesc(ctypes.Structure):
+    """accel_sampling_t."""
+    _fields_ = [("temperature", ctypes.POINTER(Tensor)), ("top_k", ctypes.POINTER(Tensor)),
+                ("top_p", ctypes.POINTER(Tensor)), ("min_p", ctypes.POINTER(Tensor))]
+
+
+NO_TOKEN = 0xffffffff
+DRAFT_NODES = 256
+
 QFMT_AWQ, QFMT_GPTQ, QFMT_GPTQ_V2 = 1, 2, 3
 
 
@@ -233,6 +242,13 @@ SIGNATURES = {
                                _P(AttentionDesc), _P(Tensor)], _i),
     "accel_paged_prefill": ([_i, _vp, _P(Tensor), _P(Tensor), _P(KVCacheDesc), ctypes.c_int64,
                              _P(Tensor), _P(AttentionDesc), _P(Tensor)], _i),
+    "accel_paged_tree_attention": ([_i, _vp, _P(Tensor), _P(Tensor), _P(Tensor),
+                                    _P(KVCacheDesc), ctypes.c_int64, _P(Tensor),
+                                    _P(AttentionDesc), _P(Tensor)], _i),
+    "accel_sample": ([_i, _vp, _P(Tensor), _P(Tensor), _P(SamplingDesc), _P(Tensor),
+                      _P(Tensor)], _i),
+    "accel_tree_accept": ([_i, _vp] + [_P(Tensor)] * 7, _i),
+    "accel_kv_keep": ([_i, _vp, _P(KVCacheDesc)] + [_P(Tensor)] * 4, _i),
     "accel_quant_matmul": ([_i, _vp, _P(Tensor), _P(Tensor), _P(Tensor), _P(Tensor)], _i),
     "accel_int8_quantize": ([_vp, ctypes.c_int64, _vp, _vp], _i),
     "accel_int8_dequantize": ([_vp, _vp, ctypes.c_int64, _vp], _i),
@@ -959,6 +975,38 @@ class Device:
         _check(_lib.accel_paged_prefill(self.index, stream, _opt(q), _opt(offsets),
                                         ctypes.byref(cache.desc()), layer, _opt(seqs),
                                         ctypes.byref(opt), _opt(out)))
+
+    def PagedTreeAttention(self, q: Buffer, offsets: Buffer, parents: Buffer, cache: KVCache,
+                           out: Buffer, layer: int = 0, seqs: Buffer = None, scale: float = 0.0,
+                           window: int = 0, sinks: int = 0, stream=None) -> None:
+        """Attention of drafts' nodes over their contexts and paths
+        (accel_paged_tree_attention)."""
+        opt = AttentionDesc(scale, window, sinks)
+        _check(_lib.accel_paged_tree_attention(self.index, stream, _opt(q), _opt(offsets),
+                                               _opt(parents), ctypes.byref(cache.desc()), layer,
+                                               _opt(seqs), ctypes.byref(opt), _opt(out)))
+
+    def Sample(self, logits: Buffer, u: Buffer, tokens: Buffer, logprobs: Buffer = None,
+               temperature: Buffer = None, top_k: Buffer = None, top_p: Buffer = None,
+               min_p: Buffer = None, stream=None) -> None:
+        """A token of each row of logits from given random numbers (accel_sample)."""
+        held = [None if b is None else b.tensor() for b in (temperature, top_k, top_p, min_p)]
+        opt = SamplingDesc(*(None if t is None else ctypes.pointer(t) for t in held))
+        _check(_lib.accel_sample(self.index, stream, _opt(logits), _opt(u), ctypes.byref(opt),
+                                 _opt(tokens), _opt(logprobs)))
+
+    def TreeAccept(self, tokens: Buffer, parents: Buffer, offsets: Buffer, sampled: Buffer,
+                   path: Buffer, counts: Buffer, next_tokens: Buffer, stream=None) -> None:
+        """The walk down each draft along sampled tokens (accel_tree_accept)."""
+        _check(_lib.accel_tree_accept(self.index, stream, _opt(tokens), _opt(parents),
+                                      _opt(offsets), _opt(sampled), _opt(path), _opt(counts),
+                                      _opt(next_tokens)))
+
+    def KVKeep(self, cache: KVCache, path: Buffer, counts: Buffer, offsets: Buffer,
+               seqs: Buffer = None, stream=None) -> None:
+        """What sequences keep of their last positions (accel_kv_keep)."""
+        _check(_lib.accel_kv_keep(self.index, stream, ctypes.byref(cache.desc()), _opt(seqs),
+                                  _opt(offsets), _opt(path), _opt(counts)))
 
     def QuantMatMul(self, x: Buffer, quants: Buffer, scales: Buffer, out: Buffer,
                     stream=None) -> None:

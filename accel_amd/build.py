@@ -22,7 +22,8 @@ ARCH = "gfx950"
 
 SOURCES = ["runtime.cpp", "quant.cpp", "ops.cpp", "decode.hip", "gemm.hip",
            "grouped.hip", "quantize.hip", "step.hip", "int8.hip", "repack.cpp", "panel.hip", "split.hip", "ragged.hip",
-           "kv.cpp", "kvpages.hip", "attention.hip"]
+           "kv.cpp", "kvpages.hip", "attention.hip", "tree.hip",
+           "draft.hip", "sampling.cpp", "sample.hip"]
 
 COMMON = [
     f"--offload-arch={ARCH}",

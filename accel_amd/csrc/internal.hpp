@@ -26,7 +26,8 @@ constexpr uint32_t kFaultWaitGaveUp = 1u;     // a split-K hand-off's bounded wa
 constexpr uint32_t kFaultKvRoom = 2u;         // no free page, or no slot left in a table
 constexpr uint32_t kFaultKvPage = 4u;         // no page where a position is read or written
 constexpr uint32_t kFaultKvSequence = 8u;     // a sequence or page index that cannot be served
-constexpr uint32_t kFaultKv = kFaultKvRoom | kFaultKvPage | kFaultKvSequence;
+constexpr uint32_t kFaultDraft = 16u;         // a draft whose parents or sizes cannot be served
+constexpr uint32_t kFaultKv = kFaultKvRoom | kFaultKvPage | kFaultKvSequence | kFaultDraft;
 
 // Per-device state: the open flag, sticky loss, fault injection, the
 // library-owned workspace and the fault word.
@@ -447,12 +448,41 @@ struct Attention {
     float scale;
     uint32_t window, sinks;    // window 0: all
 };
+// The same of drafts: the rows of an entry are a tree's nodes.
+struct Drafts : Attention {
+    const uint32_t* parents;   // [rows] of each node, in its entry; ACCEL_KV_NONE: none
+};
 // n entries' tiles of 32 keys have to be counted in 32 bits.
 bool paged_attention_counts(const KvCache& c, const Attention& a);
 hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
                                   const Attention& a, int* status);
 hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
                                 int* status);
+hipError_t launch_paged_tree(Device* d, hipStream_t st, const KvCache& c, const Drafts& a,
+                             int* status);
+
+// Drafts' nodes that were accepted (draft.hip): the walk down each tree, and what a
+// cache keeps of them.
+hipError_t launch_tree_accept(Device* d, hipStream_t st, const uint32_t* tokens,
+                              const uint32_t* parents, const uint32_t* offsets,
+                              const uint32_t* sampled, int64_t rows, int64_t n, int64_t width,
+                              uint32_t* path, uint32_t* counts, uint32_t* next);
+hipError_t launch_kv_keep(Device* d, hipStream_t st, const KvCache& c, const uint32_t* seqs,
+                          const uint32_t* offsets, const uint32_t* path, int64_t width,
+                          const uint32_t* counts, int64_t n, int* status);
+
+// Sampling (sample.hip): rows of logits [rows, width] and each row's settings, null
+// where all rows have none; logprobs may be null.
+struct Sampling {
+    const void* logits;
+    int32_t dtype;             // ACCEL_F32, ACCEL_F16 or ACCEL_BF16
+    uint32_t rows, width;
+    const float *u, *temperature, *top_p, *min_p;
+    const uint32_t* top_k;
+    uint32_t* tokens;
+    float* logprobs;
+};
+hipError_t launch_sample(Device* d, hipStream_t st, const Sampling& s, int* status);
 
 // Device quantizer.
 hipError_t launch_int4_quantize(hipStream_t st, const float* w, int64_t n,

@@ -351,7 +351,7 @@ namespace {
 int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
           const accel_tensor_t* offsets, bool ragged, const accel_kv_cache_t* cache,
           int64_t layer, const accel_tensor_t* seqs, const accel_attention_t* opt,
-          accel_tensor_t* out) {
+          accel_tensor_t* out, const accel_tensor_t* parents = nullptr, bool tree = false) {
     char buf[256];
     KvCache c;
     int rc = check_cache(op, cache, &c);
@@ -381,7 +381,12 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
     if (T && (!q->data || !out->data)) return refuse(op, "an operand is missing");
     if (!aligned16(q->data) || !aligned16(out->data))
         return refuse(op, "queries and output must start at 16-byte aligned addresses");
-    Attention a{};
+    Drafts a{};
+    if (tree) {
+        int64_t rows;
+        if ((rc = check_list(op, "the list of parents", parents, T, &rows)) != ACCEL_OK) return rc;
+        a.parents = static_cast<const uint32_t*>(parents->data);
+    }
     if (opt) {
         // scores are in units of log 2: the scale times log2 e is finite too
         if (!(opt->scale >= 0 && opt->scale <= 0x1p127f) || opt->window < 0 || opt->sinks < 0) {
@@ -415,8 +420,9 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
     a.layer = layer;
     a.q_f32 = q->dtype == ACCEL_F32;
     int status = ACCEL_OK;
-    const hipError_t e = ragged ? launch_paged_prefill(d, (hipStream_t)stream, c, a, &status)
-                                : launch_paged_attention(d, (hipStream_t)stream, c, a, &status);
+    const hipError_t e = tree     ? launch_paged_tree(d, (hipStream_t)stream, c, a, &status)
+                         : ragged ? launch_paged_prefill(d, (hipStream_t)stream, c, a, &status)
+                                  : launch_paged_attention(d, (hipStream_t)stream, c, a, &status);
     return done(d, e, status, op);
 }
 
@@ -436,4 +442,83 @@ ACCEL_API int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q
                                   const accel_attention_t* opt, accel_tensor_t* out) {
     clear_error();
     return paged("PagedPrefill", dev, stream, q, offsets, true, cache, layer, seqs, opt, out);
+}
+
+ACCEL_API int accel_paged_tree_attention(int dev, void* stream, const accel_tensor_t* q,
+                                         const accel_tensor_t* offsets,
+                                         const accel_tensor_t* parents,
+                                         const accel_kv_cache_t* cache, int64_t layer,
+                                         const accel_tensor_t* seqs,
+                                         const accel_attention_t* opt, accel_tensor_t* out) {
+    clear_error();
+    return paged("PagedTreeAttention", dev, stream, q, offsets, true, cache, layer, seqs, opt, out,
+                 parents, true);
+}
+
+namespace {
+
+// A u32 matrix of one row an entry, up to 4096 wide.
+int check_path(const char* op, const accel_tensor_t* t, int64_t n, int64_t* width) {
+    char buf[256];
+    if (!valid_tensor(t) || t->rank != 2 || t->dtype != ACCEL_U32 || t->shape[0] != n ||
+        t->shape[1] < 1 || t->shape[1] > 4096) {
+        snprintf(buf, sizeof buf,
+                 "the paths must be u32 [%lld, width], a row an entry of 1 to 4096", (long long)n);
+        return refuse(op, buf);
+    }
+    if (n && !t->data) return refuse(op, "the paths are missing");
+    *width = t->shape[1];
+    return check_blocks(op, n, *width);
+}
+
+}  // namespace
+
+ACCEL_API int accel_tree_accept(int dev, void* stream, const accel_tensor_t* tokens,
+                                const accel_tensor_t* parents, const accel_tensor_t* offsets,
+                                const accel_tensor_t* sampled, accel_tensor_t* path,
+                                accel_tensor_t* counts, accel_tensor_t* next) {
+    clear_error();
+    const char* op = "TreeAccept";
+    int rc;
+    int64_t T, n, len, width;
+    if ((rc = check_list(op, "the list of tokens", tokens, -1, &T)) != ACCEL_OK ||
+        (rc = check_list(op, "the list of parents", parents, T, &len)) != ACCEL_OK ||
+        (rc = check_list(op, "the list of sampled tokens", sampled, T, &len)) != ACCEL_OK ||
+        (rc = check_offsets(op, offsets, &n)) != ACCEL_OK ||
+        (rc = check_path(op, path, n, &width)) != ACCEL_OK ||
+        (rc = check_list(op, "the list of counts", counts, n, &len)) != ACCEL_OK ||
+        (rc = check_list(op, "the list of next tokens", next, n, &len)) != ACCEL_OK)
+        return rc;
+    Device* d;
+    if ((rc = begin(dev, &d)) != ACCEL_OK || n == 0) return rc;
+    const auto u32 = [](const accel_tensor_t* t) { return static_cast<uint32_t*>(t->data); };
+    return classify(d, launch_tree_accept(d, (hipStream_t)stream, u32(tokens), u32(parents),
+                                          u32(offsets), u32(sampled), T, n, width, u32(path),
+                                          u32(counts), u32(next)),
+                    "TreeAccept launch");
+}
+
+ACCEL_API int accel_kv_keep(int dev, void* stream, const accel_kv_cache_t* cache,
+                            const accel_tensor_t* seqs, const accel_tensor_t* offsets,
+                            const accel_tensor_t* path, const accel_tensor_t* counts) {
+    clear_error();
+    const char* op = "KVKeep";
+    KvCache c;
+    int rc = check_cache(op, cache, &c);
+    if (rc != ACCEL_OK) return rc;
+    int64_t n, len, width;
+    const uint32_t* list;
+    if ((rc = check_offsets(op, offsets, &n)) != ACCEL_OK ||
+        (rc = check_path(op, path, n, &width)) != ACCEL_OK ||
+        (rc = check_list(op, "the list of counts", counts, n, &len)) != ACCEL_OK ||
+        (rc = check_seqs(op, seqs, c, &n, &list)) != ACCEL_OK)
+        return rc;
+    Device* d;
+    if ((rc = begin(dev, &d)) != ACCEL_OK || n == 0) return rc;
+    int status = ACCEL_OK;
+    const hipError_t e = launch_kv_keep(d, (hipStream_t)stream, c, list,
+                                        static_cast<const uint32_t*>(offsets->data),
+                                        static_cast<const uint32_t*>(path->data), width,
+                                        static_cast<const uint32_t*>(counts->data), n, &status);
+    return done(d, e, status, "KVKeep launch");
 }

@@ -74,9 +74,24 @@ constexpr int kTilesAShare = F32 ? 2 : 4;
 __host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
 __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
 
-template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT>
+// Drafts: an entry's rows are the nodes of a tree behind its sequence's context.  A
+// node sees the context and, of the nodes, those on its path to its root; it stands
+// for the position of its depth behind the context.  All rows see the same keys up
+// to the context's end, so only the tiles past it look at the paths: a bit for each
+// of up to kDraft nodes, made by a lane a node that walks up its parents in LDS.
+constexpr int kDraft = ACCEL_DRAFT_NODES;
+struct Paths {
+    // words of a node's bits, and as many past them as a tile reads; an odd stride,
+    // for a wave's rows to meet in different banks
+    uint32_t bits[kRows][kDraft / 32 + 3];
+    int depth[kRows];                 // -1: a parent on the path is not before its child
+    uint32_t parent[kDraft];
+};
+struct NoPaths {};
+
+template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call>
 __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
-    KvCache c, Attention a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
+    KvCache c, Call a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
     uint32_t* tickets, uint32_t ticket_stride, float* parts, uint32_t* fault) {
     constexpr int NS = DIM / 16;            // MFMA steps of a score
     constexpr int NC = DIM / 8;             // 16-byte chunks of a key
@@ -85,6 +100,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
     constexpr int KL = KT * NC / 256;       // chunks of K, and of V, a lane stages
     constexpr bool F32 = QT > 1;
+    constexpr bool TREE = std::is_same<Call, Drafts>::value;
+    __shared__ typename std::conditional<TREE, Paths, NoPaths>::type paths;
     __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
     __shared__ __attribute__((aligned(256))) char v_sh[2][KT * NC * 16];
     // keys of a tile with values that are not finite: tile t's in place t % 3,
@@ -140,8 +157,16 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const uint32_t toks = rows.count - tok0 < (uint32_t)tokens ? rows.count - tok0 : tokens;
     const Held held = sums ? held_by(c, a, entry, threadIdx.x ? nullptr : fault)
                            : entry_held(cut, c, a, entry);
-    // the position of the tile's first token; below 0 it sees nothing
-    const int base = (int)held.len - (int)rows.count + (int)tok0;
+    // the position of the tile's first token, or of a draft's roots; below 0 it sees
+    // nothing
+    const int base = (int)held.len - (int)rows.count + (TREE ? 0 : (int)tok0);
+    // the tile's first place past base
+    const int at0 = TREE ? (int)tok0 : 0;
+    const bool drafted = !TREE || (base > -1 && rows.count <= (uint32_t)kDraft);
+    if constexpr (TREE) {
+        if (!drafted && held.seq != kNoSequence && threadIdx.x == 0)
+            report(fault, base > -1 ? kFaultDraft : kFaultKvPage);
+    }
     const int window = a.window ? (int)a.window : 0x7fffffff;
     const int sinks = a.window ? (int)a.sinks : 0;
 
@@ -149,16 +174,17 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int r = wave * 32 + col;
     const int tok = r / per, g = r - tok * per;
     const bool real = tok < (int)toks && g < gs;
-    const int p = real && base + tok > -1 ? base + tok : -1;
     const size_t qrow = ((size_t)(rows.first + tok0 + (real ? tok : 0)) * a.heads + head * group +
                          g0 + (real ? g : 0)) * dim;
     // the wave's first and last position, and the workgroup's
     const int tok_a = wave * 32 / per, tok_b = (wave * 32 + 31) / per;
     const bool busy = tok_a < (int)toks;
-    const int p_a = base + tok_a > -1 ? base + tok_a : -1;
-    const int p_last = base + (tok_b < (int)toks ? tok_b : (int)toks - 1);
+    const int p_first = base + (TREE ? 0 : tok_a);
+    const int p_a = p_first > -1 ? p_first : -1;
+    const int p_last = base + at0 + (tok_b < (int)toks ? tok_b : (int)toks - 1);
     const int p_b = p_last > -1 ? p_last : -1;
-    const int p_end = base + (int)toks;           // past the workgroup's last
+    // past the workgroup's last
+    const int p_end = drafted ? base + at0 + (int)toks : 0;
 
     // tiles of keys: those of the sinks, then those from the first window's
     // start to the last position
@@ -176,6 +202,39 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int share = (count + shares - 1) / shares;
     const int held_shares = count > 0 ? (count + share - 1) / share : 1;
     if ((int)split >= held_shares) return;
+
+    // this lane's row's position, or -1 where it sees nothing
+    int p = real && base + tok > -1 ? base + tok : -1;
+    bool lost = false;      // some row of the wave's is such a draft
+    if constexpr (TREE) {
+        const int nodes = drafted ? at0 + (int)toks : 0;
+        for (int i = threadIdx.x; i < nodes; i += 256)
+            paths.parent[i] = a.parents[rows.first + i];
+        for (int i = threadIdx.x; i < kRows * (int)(sizeof paths.bits[0] / 4); i += 256)
+            (&paths.bits[0][0])[i] = 0;
+        __syncthreads();
+        if ((int)threadIdx.x < kRows) {
+            const int x = threadIdx.x;
+            int depth = -1;
+            if (drafted && x < (int)toks) {
+                const auto up = [&](uint32_t t) { return paths.parent[t]; };
+                uint32_t t = at0 + x;
+                for (depth = 0; up(t) < t; depth++) t = up(t);
+                if (up(t) != ACCEL_KV_NONE) depth = -1;
+                // the node k steps up stands k positions before this one
+                t = at0 + x;
+                for (int k = 0; k <= depth; k++, t = up(t))
+                    if (k < window || base + depth - k < sinks)
+                        paths.bits[x][t >> 5] |= 1u << (t & 31);
+                if (depth < 0) report(fault, kFaultDraft);
+            }
+            paths.depth[x] = depth;
+        }
+        __syncthreads();
+        const int depth = paths.depth[tok];
+        p = real && depth > -1 ? base + depth : -1;
+        lost = __any(real && depth < 0);
+    }
     const int t_begin = (int)split * share;
     const int t_end = t_begin + share < count ? t_begin + share : count;
     const auto tile_pos = [&](int t) {
@@ -247,7 +306,8 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     };
     // whether every row of the workgroup sees all of the tile
     const auto plain = [&](int pos) {
-        return pos + KT <= base + 1 && (pos > p_end - 1 - window || pos + KT <= sinks);
+        return pos + KT <= base + (TREE ? 0 : 1) &&
+               (pos > p_end - 1 - window || pos + KT <= sinks);
     };
     const auto arrive = [&](uint32_t pages, int pos, int odd, auto buf, auto careful) {
         constexpr int B = decltype(buf)::value;
@@ -439,15 +499,38 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                         for (int e = 0; e < 16; e++)
                             s[i][e] = seen(i * 32 + (e >> 3) * 16 + (e & 7)) ? s[i][e] : -INFINITY;
                 };
-                if (pos + KT > p_a + 1) hide([&](int x) { return x <= until; });
+                if constexpr (TREE) {
+                    if (pos + KT > base || lost) {
+                        // a bit a key: those before the context's end, then the path's
+                        const int past = pos - base;
+                        uint64_t seen = past >= 0 ? 0 : past > -64 ? (1ull << -past) - 1 : ~0ull;
+                        if (p < 0) seen = 0;
+                        if (past > -64) {
+                            const uint32_t* w = paths.bits[tok] + (past > 0 ? past >> 5 : 0);
+                            const uint64_t low = w[0] | (uint64_t)w[1] << 32;
+                            const int by = past & 31;
+                            seen |= past <= 0 ? low << -past
+                                    : by      ? low >> by | (uint64_t)w[2] << (64 - by)
+                                              : low;
+                        }
+                        seen >>= half * 8;
+                        hide([&](int x) { return (seen >> x & 1) != 0; });
+                    }
+                } else {
+                    if (pos + KT > p_a + 1) hide([&](int x) { return x <= until; });
+                }
                 if (!(pos > p_b - window || pos + KT <= sinks)) {
                     // the first place the row's window holds; none where it is all past
                     const int from = until < window ? -KT : until - window + 1;
+                    // a draft's nodes have been looked at by their depths
+                    const int nodes = TREE ? base - here : KT;
                     if (pos >= sinks) {
-                        hide([&](int x) { return x >= from; });
+                        hide([&](int x) { return (x >= from) | (TREE && x >= nodes); });
                     } else {
                         const int kept = sinks - here;
-                        hide([&](int x) { return (x >= from) | (x < kept); });
+                        hide([&](int x) {
+                            return (x >= from) | (x < kept) | (TREE && x >= nodes);
+                        });
                     }
                 }
                 const uint64_t named = __ballot(pages < c.pages);   // bit b: block b's page
@@ -515,7 +598,11 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 // the weight, the sum is what they are
                 for (uint64_t odd = odd0 | (uint64_t)odd1 << 32; odd; odd &= odd - 1) {
                     const int x = pos + (int)__builtin_ctzll(odd);
-                    const bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                    bool ok = (x <= p) & ((x > p - window) | (x < sinks));
+                    if constexpr (TREE) {
+                        const int t = x - base;
+                        if (t >= 0) ok = (paths.bits[tok][t >> 5] >> (t & 31) & 1) != 0;
+                    }
                     const uint32_t page = table[(uint32_t)x >> c.shift];
                     const uint16_t* src = reinterpret_cast<const uint16_t*>(
                         values + (page < c.pages ? page : 0) * page_bytes +
@@ -648,6 +735,87 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     (u32x2){x[0][0], x[1][0]};
             }
         }
+}
+
+template <typename Call>
+hipError_t launch_prompts(Device* d, hipStream_t st, const KvCache& c, const Call& a,
+                          int* status) {
+    constexpr bool TREE = std::is_same<Call, Drafts>::value;
+    *status = ACCEL_OK;
+    const int group = a.heads / c.heads;
+    const int per = prompt_heads(group), tokens = prompt_tokens(group);
+    const uint32_t heads = (uint32_t)(c.heads * ((group + per - 1) / per));
+    // an entry's last tile may be partly filled
+    const uint64_t tiles = (uint64_t)a.rows / tokens + (a.n < a.rows ? a.n : a.rows);
+    const uint64_t bound = tiles * heads;
+    // two workgroups a CU of a 16-bit type up to 128 dims, else one; with fewer
+    // tiles of rows than that, several workgroups share one
+    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 ? 2 : 1);
+    uint32_t splits = bound < slots ? (uint32_t)(slots / bound) : 1;
+    // as many as the longest sequence's keys can be worth
+    const int64_t kt = c.dim <= 128 ? 64 : 32;
+    int64_t most = ((int64_t)c.slots << c.shift) / kt + 1;
+    if (a.window) {
+        const int64_t near = ((int64_t)a.window + (TREE ? kDraft : tokens)) / kt + a.sinks / kt + 3;
+        most = near < most ? near : most;
+    }
+    const int64_t worth = most / (a.q_f32 ? kTilesAShare<true> : kTilesAShare<false>);
+    splits = worth < (int64_t)splits ? (uint32_t)(worth > 1 ? worth : 1) : splits;
+    const int wide = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    const size_t part_words =
+        splits > 1 ? (size_t)(bound * splits) * 256 * (wide / 32 * 16 + 2) : 0;
+    const bool summed = a.n > 64;
+    const size_t sums_words = summed ? ((size_t)a.n + 1) & ~(size_t)1 : 0;
+    uint32_t *tickets = nullptr, *sums = nullptr;
+    float* parts = nullptr;
+    if (part_words + sums_words) {
+        char* ws = static_cast<char*>(workspace(d, st, (part_words + sums_words) * 4, status));
+        if (!ws) return hipSuccess;
+        tickets = reinterpret_cast<uint32_t*>(ws);
+        parts = reinterpret_cast<float*>(ws + kWorkspaceCounterBytes);
+        if (summed) sums = reinterpret_cast<uint32_t*>(parts + part_words);
+    }
+    if (summed)
+        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
+                           sums, d->fault_dev);
+    const uint32_t fold = slots > (uint32_t)d->cu_count ? (uint32_t)d->cu_count / heads : 0;
+    const uint32_t stride = (uint32_t)(kWorkspaceCounterBytes / 4) / slots;
+    // a launch of 256 lanes a workgroup holds fewer than 2^24 of them, as a
+    // grid's lanes are counted in 32 bits; that many places are not split
+    constexpr uint64_t kPlaces = 1 << 22;
+    const auto go = [&](auto kernel) {
+        for (uint64_t place = 0; place < bound; place += kPlaces) {
+            const uint64_t places = bound - place < kPlaces ? bound - place : kPlaces;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(places * splits)), dim3(256), 0, st, c, a,
+                               sums, fold, splits, (uint32_t)place, tickets, stride, parts,
+                               d->fault_dev);
+        }
+    };
+    const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
+    const auto dims = [&](auto bf16, auto qt, auto pt) {
+        constexpr bool B = decltype(bf16)::value;
+        constexpr int Q = decltype(qt)::value, P = decltype(pt)::value;
+        if (c.dim <= 64)
+            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64, Call>)
+                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64, Call>);
+        else if (c.dim <= 128)
+            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64, Call>)
+                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64, Call>);
+        else
+            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32, Call>)
+                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32, Call>);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 3> three;
+    if (a.q_f32) {
+        if (c.bf16) dims(std::true_type(), three, three);
+        else dims(std::false_type(), two, two);
+    } else {
+        if (c.bf16) dims(std::true_type(), one, one);
+        else dims(std::false_type(), one, one);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace

@@ -191,6 +191,7 @@ int take_fault(Device* d) {
         {kFaultKvRoom, "a key-value pool had no free page, or a table no slot left"},
         {kFaultKvPage, "a key-value table names no page for a position read or written"},
         {kFaultKvSequence, "a sequence or page index cannot be served"},
+        {kFaultDraft, "a draft's parents, its path or its size cannot be served"},
     };
     char what[320] = "";
     uint32_t rest = f;

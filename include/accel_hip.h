@@ -731,6 +731,92 @@ int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q,
                         int64_t layer, const accel_tensor_t* seqs,
                         const accel_attention_t* opt, accel_tensor_t* out);
 
+/* ---- drafts: several tokens checked in one step ------------------------- */
+
+/* A draft of a sequence is a tree of up to ACCEL_DRAFT_NODES tokens after its
+ * context: node 0 is the newest token, each other node a guess for the token
+ * that follows its parent.  The nodes of all drafts of a call are rows, entry
+ * i's nodes 0 .. m-1 the rows [offsets[i], offsets[i+1]) (u32 [n+1], ascending
+ * from 0); parents (u32 [T]) gives each row's parent as a number in its entry,
+ * below its own, or ACCEL_KV_NONE.  Their keys and values lie in the cache in
+ * the rows' order, at the sequence's last m positions (accel_kv_reserve and
+ * accel_kv_append put them there). */
+#define ACCEL_DRAFT_NODES 256
+
+/* Attention of drafts' nodes: node t of a sequence with L positions before its
+ * nodes stands at position L + d, d the number of its ancestors, and sees the
+ * positions j < L, its ancestors and itself, at the positions that they stand
+ * for, as accel_attention_t says.  q, out, layer, seqs, opt, rounding and what is
+ * not finite are as in accel_paged_prefill.  A node without a parent starts a
+ * tree of its own.  Rows of a node on whose path a parent is not below its
+ * child, of an entry of more than ACCEL_DRAFT_NODES nodes and of one with more
+ * nodes than its sequence has positions are zeros, and reported. */
+int accel_paged_tree_attention(int dev, void* stream, const accel_tensor_t* q,
+                               const accel_tensor_t* offsets, const accel_tensor_t* parents,
+                               const accel_kv_cache_t* cache, int64_t layer,
+                               const accel_tensor_t* seqs, const accel_attention_t* opt,
+                               accel_tensor_t* out);
+
+/* A row's settings, each a vector of one value a row, or NULL where no row has
+ * one. */
+typedef struct accel_sampling {
+    const accel_tensor_t* temperature; /* f32; 0 (and what is no number above it): the first
+                                          of the order.  NULL: 1 */
+    const accel_tensor_t* top_k;       /* u32; 0: all */
+    const accel_tensor_t* top_p;       /* f32; 1 and more, and no number: all */
+    const accel_tensor_t* min_p;       /* f32; 0 and less, and no number: all */
+} accel_sampling_t;
+
+/* Logits a row, at most. */
+#define ACCEL_SAMPLE_WIDTH (1 << 24)
+/* What a row without a logit past -infinity gives. */
+#define ACCEL_NO_TOKEN 0xffffffffu
+
+/* A token of each row of logits [rows, width] (or [width]), f32, f16 or bf16.  A
+ * row's logits are put in order, the larger first, of equal ones the lower index
+ * first; logit x has the weight exp((x - the largest) / temperature).  top_k keeps
+ * the first k; top_p of those the fewest first ones whose weights reach top_p of
+ * theirs; min_p those whose weight is min_p or more (1 and more: those of weight 1).
+ * The first is always kept.  The token (u32) is the index of the first kept logit
+ * at which the weights' running sum passes u (f32 [rows], in [0, 1): what is outside,
+ * or no number, counts as the nearest, 0) times the sum of all that are kept;
+ * logprobs (f32 [rows], or NULL) is the logarithm of its weight's share of that sum.
+ * Weights and sums are of 64 bits and do not depend on an order, so a call gives the
+ * same tokens whatever runs beside it; a weight below 2^-46 of a row's largest may
+ * count as 0 (rows of up to 2^17; a bit less a doubling past that).  A NaN counts
+ * as -infinity, which is never kept; of infinite logits each has the weight 1 and all
+ * others 0.  Rows are independent of each other. */
+int accel_sample(int dev, void* stream, const accel_tensor_t* logits, const accel_tensor_t* u,
+                 const accel_sampling_t* opt, accel_tensor_t* tokens, accel_tensor_t* logprobs);
+
+/* The walk down each draft along sampled tokens: from node 0, to the lowest node
+ * past it whose parent it is and whose token (u32 [T]) is the one sampled (u32 [T])
+ * at it, and so on.  path (u32 [n, width], 1 to 4096 wide) receives the nodes'
+ * numbers in their entry, node 0 first and no more than the width, then
+ * ACCEL_KV_NONE; counts (u32 [n]) how many; next (u32 [n]) the token sampled at
+ * the last, the sequence's new token, whose key and value the next step appends.
+ * ACCEL_NO_TOKEN ends a walk.  An entry without nodes has count 0 and next
+ * ACCEL_NO_TOKEN, and so has one of more than ACCEL_DRAFT_NODES, which is reported. */
+int accel_tree_accept(int dev, void* stream, const accel_tensor_t* tokens,
+                      const accel_tensor_t* parents, const accel_tensor_t* offsets,
+                      const accel_tensor_t* sampled, accel_tensor_t* path,
+                      accel_tensor_t* counts, accel_tensor_t* next);
+
+/* What sequences keep of their last positions: entry i's sequence seqs[i] (u32 [n];
+ * NULL: i) keeps of its last offsets[i+1] - offsets[i] positions the counts[i] ones
+ * that path[i] (u32 [n, width]) names, ascending from 0 at the first of them.  In
+ * every layer their keys and values move up to follow each other, the length becomes
+ * that of what is left, and pages past it are given back.  A count of 0 takes all of
+ * those positions back.  Left as it is and reported is an entry whose path does not
+ * ascend, names a position past the last or is shorter than its count; one of more
+ * positions than its sequence has, or with no page where a row moves; one that would
+ * move a row into a page that another sequence has too; a sequence index outside the
+ * cache; and one of two entries with one sequence (not specified which).
+ * ACCEL_KV_NONE is skipped. */
+int accel_kv_keep(int dev, void* stream, const accel_kv_cache_t* cache,
+                  const accel_tensor_t* seqs, const accel_tensor_t* offsets,
+                  const accel_tensor_t* path, const accel_tensor_t* counts);
+
 /* ---- int8 weights ------------------------------------------------------ */
 
 /* tensor.QuantMatMul (tensor/quantized.go:72-163): x f32 or f16 [M,K] times
