@@ -40,6 +40,17 @@ __device__ __forceinline__ float logit(const void* p, size_t i) {
     else return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
 }
 
+// A number that all lanes have, for a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+__device__ __forceinline__ double uniform(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(
+        double, (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32 |
+                    (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b));
+}
+
 // A row's settings, in range.
 struct Rules {
     double temperature, top_p, min_p, u;
@@ -50,13 +61,13 @@ __device__ __forceinline__ Rules rules_of(const Sampling& s, uint32_t row) {
     Rules r;
     const float t = s.temperature ? s.temperature[row] : 1.0f;
     r.greedy = !(t > 0);
-    r.temperature = t;
+    r.temperature = uniform((double)t);
     const float p = s.top_p ? s.top_p[row] : 1.0f;
-    r.top_p = p < 1 ? fmaxf(p, 0.0f) : 1.0f;
+    r.top_p = uniform((double)(p < 1 ? fmaxf(p, 0.0f) : 1.0f));
     const float m = s.min_p ? s.min_p[row] : 0.0f;
-    r.min_p = m > 0 ? fminf(m, 1.0f) : 0.0f;
+    r.min_p = uniform((double)(m > 0 ? fminf(m, 1.0f) : 0.0f));
     const float u = s.u[row];
-    r.u = u > 0 ? fminf(u, 1.0f - 0x1p-24f) : 0.0f;
+    r.u = uniform((double)(u > 0 ? fminf(u, 1.0f - 0x1p-24f) : 0.0f));
     const uint32_t k = s.top_k ? s.top_k[row] : 0u;
     r.top_k = k ? k : 0xffffffffu;
     return r;
@@ -275,16 +286,6 @@ __device__ __forceinline__ Binned binned(float x, double per) {
             __builtin_bit_cast(uint64_t, q) -
                 (__builtin_bit_cast(uint64_t, kBase) - (1ull << kCount))};
 }
-// A number that all lanes have, for a scalar register.
-__device__ __forceinline__ float uniform(float x) {
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
-}
-__device__ __forceinline__ double uniform(double x) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    return __builtin_bit_cast(
-        double, (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32 |
-                    (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b));
-}
 // Logits per bin's width: 16 log2(e) / T.
 __device__ __forceinline__ double bins_per(const Rules& r) {
     return uniform(16 * 1.44269504088896340736 / r.temperature);
@@ -406,7 +407,7 @@ __device__ __forceinline__ float top_of(Scratch& sh, float m) {
 #pragma unroll
     for (int w = 1; w < kWaves; w++) m = fmaxf(m, sh.wave_top[w]);
     __syncthreads();
-    return m;
+    return uniform(m);
 }
 
 // Bins below a window's top that its ring holds, whatever the edges' roundings.
@@ -586,6 +587,18 @@ __device__ __forceinline__ int last_needed(const Plan& p) {
 // Place in the order, ascending.
 __device__ __forceinline__ uint64_t placed(float x, uint32_t index) {
     return (uint64_t)~key_of(x) << 32 | index;
+}
+
+// Lists a lane's logits of the plan's bins, none of which holds one below low.
+template <typename F>
+__device__ __forceinline__ void list_near(Scratch& sh, const Plan& plan, int top, float low,
+                                          double per, const float (&x)[kTile], F index) {
+#pragma unroll
+    for (int e = 0; e < kTile; e++)
+        if (x[e] >= low && needed(plan, top - binned(x[e], per).bin)) {
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            if (at < kList) sh.list[at] = placed(x[e], index(e));
+        }
 }
 
 // Sorts sh.list[0 .. n) up; n <= kList.  A lane an element up to kLanes, exchanged
@@ -881,115 +894,104 @@ static_assert(kTiles * kTile * kLanes / kCopies <= kMostEach, "a word's count an
 static_assert(kTile * kLanes <= kMostEach, "the same, of a part's copies together");
 
 template <int DT>
-__global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s) {
+__global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uint32_t first_row) {
     __shared__ Scratch sh;
     __shared__ uint8_t far[kTiles][kLanes];
     constexpr uint32_t kStep = kTile / Blocks<DT>::kEach * kLanes;
-    for (uint32_t r = blockIdx.x; r < s.rows; r += gridDim.x) {
-        const Rules rules = rules_of(s, r);
-        const Blocks<DT> row(s, r);
-        if (rules.greedy) {
-            give_first(s, r, least_of(sh, least_in<DT>(row, 0, row.count)));
-            continue;
-        }
-        const double per = bins_per(rules);
-        float x[kTile];
-        read_tile<DT>(row, 0, row.count, 0, x);
-        float top = largest(x);
-        clear_ring(sh);
-        // the window is set by the first tile, with room for the rest to pass it by a
-        // factor of four; what passes it further is added afterwards
-        const float first = top_of(sh, top);
-        const bool bins = has_bins(first, per);
-        Window w = {0, INFINITY, -INFINITY};
-        if (bins) w.set(binned(first, per).bin + 32, per);
-#pragma clang loop unroll(disable)
-        for (uint32_t t = 0;;) {
-            const float m = largest(x);
-            top = fmaxf(top, m);
-            // how far the lane's largest is from the window's top
-            int code = kFar;
-            if (m > w.high) code = 0;
-            else if (m >= w.low) code = 1 + ((w.top - binned(m, per).bin) >> 2);
-            far[t][threadIdx.x] = (uint8_t)code;
-            add_to_ring(sh, x, per, [&](float v) { return v >= w.low && v <= w.high; });
-            if (++t * kStep >= row.count) break;
-            read_tile<DT>(row, 0, row.count, t, x);
-        }
-        top = top_of(sh, top);
-        if (top == -INFINITY) {
-            give_first(s, r, ~0ull);
-            continue;
-        }
-        bool listed = has_bins(top, per);
-        if (listed) {
-            const int bin = binned(top, per).bin;
-            if (top > w.high) {
-                const int past = bins ? bin - w.top : kRing;
-                if (past >= kRing) {
-                    clear_ring(sh);
-                } else if ((int)threadIdx.x < past) {
-                    uint64_t* p = &sh.ring[((bin - (int)threadIdx.x) & (kRing - 1)) * kCopies];
-#pragma unroll
-                    for (int i = 0; i < kCopies; i++) p[i] = 0;
-                }
-                __syncthreads();
-                const float low = (float)((bin - (kLow - 1)) / per);
-#pragma clang loop unroll(disable)
-                for (uint32_t t = 0; t * kStep < row.count; t++) {
-                    if (far[t][threadIdx.x]) continue;
-                    read_tile<DT>(row, 0, row.count, t, x);
-                    add_to_ring(sh, x, per, [&](float v) { return v > w.high && v >= low; });
-                }
-                __syncthreads();
-            }
-            uint32_t count;
-            uint64_t rest;
-            read_ring(sh, bin, &count, &rest);
-            make_plan(sh, rules, top, per, count, rest);
-            const Plan plan = sh.plan;
-            listed = plan.listed && plan.listed <= kList;
-            if (listed) {
-                if (threadIdx.x == 0) sh.listed = 0;
-                __syncthreads();
-                const float low = (float)((bin - last_needed(plan) - 1) / per);
-                const int most = bins ? 1 + ((w.top - bin + last_needed(plan)) >> 2) : 0;
-#pragma clang loop unroll(disable)
-                for (uint32_t t = 0; t * kStep < row.count; t++) {
-                    const int code = far[t][threadIdx.x];
-                    if (code && code > most) continue;
-                    read_tile<DT>(row, 0, row.count, t, x);
-#pragma unroll
-                    for (int e = 0; e < kTile; e++)
-                        if (x[e] >= low && needed(plan, bin - binned(x[e], per).bin)) {
-                            const uint32_t at = atomicAdd(&sh.listed, 1u);
-                            if (at < kList) sh.list[at] = placed(x[e], index_in<DT>(row, 0, t, e));
-                        }
-                }
-                __syncthreads();
-                draw(sh, s, r, rules, per, sh.listed < kList ? sh.listed : kList);
-            }
-        }
-        if (!listed) draw_slowly<DT>(sh.slow, s, r, rules, top);
+    const uint32_t r = first_row + blockIdx.x;
+    const Rules rules = rules_of(s, r);
+    const Blocks<DT> row(s, r);
+    if (rules.greedy) {
+        give_first(s, r, least_of(sh, least_in<DT>(row, 0, row.count)));
+        return;
     }
+    const double per = bins_per(rules);
+    float x[kTile];
+    read_tile<DT>(row, 0, row.count, 0, x);
+    float top = largest(x);
+    clear_ring(sh);
+    // the window is set by the first tile, with room for the rest to pass it by a
+    // factor of four; what passes it further is added afterwards
+    const float first = top_of(sh, top);
+    const bool bins = has_bins(first, per);
+    Window w = {0, INFINITY, -INFINITY};
+    if (bins) w.set(binned(first, per).bin + 32, per);
+#pragma clang loop unroll(disable)
+    for (uint32_t t = 0;;) {
+        const float m = largest(x);
+        top = fmaxf(top, m);
+        // how far the lane's largest is from the window's top
+        int code = kFar;
+        if (m > w.high) code = 0;
+        else if (m >= w.low) code = 1 + ((w.top - binned(m, per).bin) >> 2);
+        far[t][threadIdx.x] = (uint8_t)code;
+        add_to_ring(sh, x, per, [&](float v) { return v >= w.low && v <= w.high; });
+        if (++t * kStep >= row.count) break;
+        read_tile<DT>(row, 0, row.count, t, x);
+    }
+    top = top_of(sh, top);
+    if (top == -INFINITY) {
+        give_first(s, r, ~0ull);
+        return;
+    }
+    bool listed = has_bins(top, per);
+    if (listed) {
+        const int bin = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
+        if (top > w.high) {
+            const int past = bins ? bin - w.top : kRing;
+            if (past >= kRing) {
+                clear_ring(sh);
+            } else if ((int)threadIdx.x < past) {
+                uint64_t* p = &sh.ring[((bin - (int)threadIdx.x) & (kRing - 1)) * kCopies];
+#pragma unroll
+                for (int i = 0; i < kCopies; i++) p[i] = 0;
+            }
+            __syncthreads();
+            const float low = (float)((bin - (kLow - 1)) / per);
+#pragma clang loop unroll(disable)
+            for (uint32_t t = 0; t * kStep < row.count; t++) {
+                if (far[t][threadIdx.x]) continue;
+                read_tile<DT>(row, 0, row.count, t, x);
+                add_to_ring(sh, x, per, [&](float v) { return v > w.high && v >= low; });
+            }
+            __syncthreads();
+        }
+        uint32_t count;
+        uint64_t rest;
+        read_ring(sh, bin, &count, &rest);
+        make_plan(sh, rules, top, per, count, rest);
+        const Plan plan = sh.plan;
+        listed = plan.listed && plan.listed <= kList;
+        if (listed) {
+            if (threadIdx.x == 0) sh.listed = 0;
+            __syncthreads();
+            const float low = (float)((bin - last_needed(plan) - 1) / per);
+            const int most = bins ? 1 + ((w.top - bin + last_needed(plan)) >> 2) : 0;
+#pragma clang loop unroll(disable)
+            for (uint32_t t = 0; t * kStep < row.count; t++) {
+                const int code = far[t][threadIdx.x];
+                if (code && code > most) continue;
+                read_tile<DT>(row, 0, row.count, t, x);
+                list_near(sh, plan, bin, low, per, x,
+                          [&](int e) { return index_in<DT>(row, 0, t, e); });
+            }
+            __syncthreads();
+            draw(sh, s, r, rules, per, sh.listed < kList ? sh.listed : kList);
+        }
+    }
+    if (!listed) draw_slowly<DT>(sh.slow, s, r, rules, top);
 }
 
 // Longer rows, and too few rows to fill the chip: a workgroup a part of up to one tile.
-// The last of a row's parts adds up their bins and plans; a second launch gathers the
-// logits of the plan's bins, and its last part draws.
-enum : uint32_t { kDone, kListed, kSlow };
-struct Row {
-    Plan plan;
-    Sums sums;
-    uint32_t state;
-    uint64_t list[kList];
-};
+// The last of a row's parts to end adds up their bins and goes on as above.
+constexpr int kBatch = 8;              // parts whose words are asked for at once
+constexpr int kMostParts = ACCEL_SAMPLE_WIDTH / (kTile * kLanes) + kBatch;
 struct Parts {
     uint64_t* rings;                   // [rows, parts, kRing]
-    float* tops;                       // [rows, parts]
     uint64_t* least;                   // [rows, parts]
-    Row* rows;
-    uint32_t* counters;                // [rows, 4]: zero between calls
+    float* tops;                       // [rows, parts]
+    uint8_t* far;                      // [rows, parts, kLanes]
+    uint32_t* tickets;                 // [rows]: zero between calls
     uint32_t first, parts, blocks;     // the launch's first row; a part's blocks
 };
 
@@ -1008,6 +1010,7 @@ __device__ __forceinline__ bool is_last(Scratch& sh, uint32_t* ticket, uint32_t 
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __syncthreads();
     if (threadIdx.x == 0) {
+        sh.listed = 0;
         sh.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
                                          __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
         if (sh.last) put(ticket, 0u);
@@ -1017,28 +1020,35 @@ __device__ __forceinline__ bool is_last(Scratch& sh, uint32_t* ticket, uint32_t 
 }
 
 template <int DT>
-__global__ __launch_bounds__(kLanes, 8) void sample_scan_kernel(Sampling s, Parts p) {
+__global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Parts p) {
     __shared__ Scratch sh;
+    __shared__ int bins[kMostParts];
     const uint32_t local = blockIdx.x / p.parts, part = blockIdx.x - local * p.parts;
     const uint32_t r = p.first + local;
     const Rules rules = rules_of(s, r);
     const Blocks<DT> row(s, r);
-    const uint32_t begin = part * p.blocks < row.count ? part * p.blocks : row.count;
-    const uint32_t end = row.count - begin < p.blocks ? row.count : begin + p.blocks;
-    const size_t slot = (size_t)local * p.parts + part;
+    const auto begin_of = [&](uint32_t i) {
+        return i * p.blocks < row.count ? i * p.blocks : row.count;
+    };
+    const uint32_t begin = begin_of(part), end = begin_of(part + 1);
+    const size_t slot0 = (size_t)local * p.parts, slot = slot0 + part;
     const double per = bins_per(rules);
+    float x[kTile];
     if (rules.greedy) {
         const uint64_t least = least_of(sh, least_in<DT>(row, begin, end));
         if (threadIdx.x == 0) put(p.least + slot, least);
     } else {
-        float x[kTile];
         read_tile<DT>(row, begin, end, 0, x);
         clear_ring(sh);
-        const float top = top_of(sh, largest(x));
+        const float most = largest(x);
+        const float top = top_of(sh, most);
         if (threadIdx.x == 0) put(p.tops + slot, top);
         if (top > -INFINITY && has_bins(top, per)) {
             Window w;
             w.set(binned(top, per).bin, per);
+            int code = kFar;
+            if (most >= w.low) code = (w.top - binned(most, per).bin) >> 2;
+            put(p.far + slot * kLanes + threadIdx.x, (uint8_t)code);
             add_to_ring(sh, x, per, [&](float v) { return v >= w.low; });
             __syncthreads();
             uint32_t count;
@@ -1048,9 +1058,7 @@ __global__ __launch_bounds__(kLanes, 8) void sample_scan_kernel(Sampling s, Part
                 (uint64_t)count << kCount | rest);
         }
     }
-    if (!is_last(sh, p.counters + 4 * local, p.parts)) return;
-    Row& out = p.rows[local];
-    const size_t slot0 = (size_t)local * p.parts;
+    if (!is_last(sh, p.tickets + local, p.parts)) return;
     if (rules.greedy) {
         uint64_t least = ~0ull;
         for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
@@ -1058,89 +1066,78 @@ __global__ __launch_bounds__(kLanes, 8) void sample_scan_kernel(Sampling s, Part
             least = v < least ? v : least;
         }
         give_first(s, r, least_of(sh, least));
-        if (threadIdx.x == 0) out.state = kDone;
         return;
     }
+    constexpr int kNone = 1 << 30;
     float top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) top = fmaxf(top, get(p.tops + slot0 + i));
+    for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
+        const float t = get(p.tops + slot0 + i);
+        top = fmaxf(top, t);
+        bins[i] = !(t > -INFINITY) ? -kNone : has_bins(t, per) ? binned(t, per).bin : kNone;
+    }
     top = top_of(sh, top);
+    for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
+        if (bins[i] != kNone) continue;
+        // far from zero: far from the row's largest too, or the row has no bins
+        bins[i] = -kNone;
+        if (!(((double)top - (double)get(p.tops + slot0 + i)) * per > 2 * kRing)) sh.listed = 1;
+    }
+    __syncthreads();
     if (top == -INFINITY) {
         give_first(s, r, ~0ull);
-        if (threadIdx.x == 0) out.state = kDone;
         return;
     }
-    if (!has_bins(top, per)) {
-        if (threadIdx.x == 0) out.state = kSlow, out.plan.top = top;
-        return;
-    }
-    const int bin = binned(top, per).bin - (int)threadIdx.x;
-    uint32_t count = 0;
-    uint64_t rest = 0;
-    bool odd = false;
-    for (uint32_t i = 0; i < p.parts; i++) {
-        const float t = get(p.tops + slot0 + i);
-        if (!(t > -INFINITY)) continue;
-        if (!has_bins(t, per)) {
-            // far from zero, and perhaps near the row's largest all the same
-            odd |= ((double)top - (double)t) * per < 2 * kRing;
-            continue;
-        }
-        const int d = binned(t, per).bin - bin;
-        if (d < 0 || d >= kRing) continue;
-        const uint64_t v = get(p.rings + (slot0 + i) * kRing + (bin & (kRing - 1)));
-        count += (uint32_t)(v >> kCount);
-        rest += v & ((1ull << kCount) - 1);
-    }
-    make_plan(sh, rules, top, per, count, rest);
-    const uint32_t listed = sh.plan.listed;
-    out.sums.mass[threadIdx.x] = sh.sums.mass[threadIdx.x];
-    out.sums.count[threadIdx.x] = sh.sums.count[threadIdx.x];
-    if (threadIdx.x == 0) {
-        out.plan = sh.plan;
-        out.state = !odd && listed && listed <= kList ? kListed : kSlow;
-    }
-}
-
-template <int DT>
-__global__ __launch_bounds__(kLanes, 8) void sample_pick_kernel(Sampling s, Parts p) {
-    __shared__ Scratch sh;
-    const uint32_t local = blockIdx.x / p.parts, part = blockIdx.x - local * p.parts;
-    const uint32_t r = p.first + local;
-    Row& in = p.rows[local];
-    const uint32_t state = in.state;
-    if (state == kDone) return;
-    const Rules rules = rules_of(s, r);
-    if (state == kSlow) {
-        if (part == 0) draw_slowly<DT>(sh.slow, s, r, rules, in.plan.top);
-        return;
-    }
-    const Plan plan = in.plan;
-    const Blocks<DT> row(s, r);
-    const uint32_t begin = part * p.blocks < row.count ? part * p.blocks : row.count;
-    const uint32_t end = row.count - begin < p.blocks ? row.count : begin + p.blocks;
-    const double per = bins_per(rules);
-    const int bin = binned(plan.top, per).bin;
-    const float low = (float)((bin - last_needed(plan) - 1) / per);
-    uint32_t* counters = p.counters + 4 * local;
-    float x[kTile];
-    read_tile<DT>(row, begin, end, 0, x);
+    bool listed = has_bins(top, per) && !sh.listed;
+    if (listed) {
+        const int big = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
+        const int bin = big - (int)threadIdx.x;
+        uint32_t count = 0;
+        uint64_t rest = 0;
+#pragma clang loop unroll(disable)
+        for (uint32_t i = 0; i < p.parts; i += kBatch) {
+            uint64_t v[kBatch];
+            const uint64_t* ring = p.rings + (slot0 + i) * kRing + (bin & (kRing - 1));
 #pragma unroll
-    for (int e = 0; e < kTile; e++)
-        if (x[e] >= low && needed(plan, bin - binned(x[e], per).bin)) {
-            const uint32_t at = __hip_atomic_fetch_add(counters + 1, 1u, __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT);
-            if (at < kList) put(in.list + at, placed(x[e], index_in<DT>(row, begin, 0, e)));
+            for (int j = 0; j < kBatch; j++) {
+                const bool has = i + j < p.parts && bins[i + j] - bin >= 0 &&
+                                 bins[i + j] - bin < kRing;
+                v[j] = has ? get(const_cast<uint64_t*>(ring) + (size_t)j * kRing) : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; j++) {
+                count += (uint32_t)(v[j] >> kCount);
+                rest += v[j] & ((1ull << kCount) - 1);
+            }
         }
-    if (!is_last(sh, counters + 2, p.parts)) return;
-    uint32_t n = get(counters + 1);
-    n = n < kList ? n : kList;
-    for (uint32_t i = threadIdx.x; i < n; i += kLanes) sh.list[i] = get(in.list + i);
-    sh.sums.mass[threadIdx.x] = in.sums.mass[threadIdx.x];
-    sh.sums.count[threadIdx.x] = in.sums.count[threadIdx.x];
-    if (threadIdx.x == 0) sh.plan = plan;
-    __syncthreads();
-    if (threadIdx.x == 0) put(counters + 1, 0u);
-    draw(sh, s, r, rules, per, n);
+        make_plan(sh, rules, top, per, count, rest);
+        const Plan plan = sh.plan;
+        listed = plan.listed && plan.listed <= kList;
+        if (listed) {
+            const float low = (float)((big - last_needed(plan) - 1) / per);
+            const int below = big - last_needed(plan);
+#pragma clang loop unroll(disable)
+            for (uint32_t i = 0; i < p.parts; i += kBatch) {
+                uint32_t look = 0;
+#pragma unroll
+                for (int j = 0; j < kBatch; j++) {
+                    if (i + j >= p.parts || bins[i + j] < below) continue;
+                    const int code = get(p.far + (slot0 + i + j) * kLanes + threadIdx.x);
+                    look |= bins[i + j] - 4 * code >= below ? 1u << j : 0u;
+                }
+                while (look) {
+                    const uint32_t at = i + __builtin_ctz(look);
+                    look &= look - 1;
+                    read_tile<DT>(row, begin_of(at), begin_of(at + 1), 0, x);
+                    list_near(sh, plan, big, low, per, x, [&](int e) {
+                        return index_in<DT>(row, begin_of(at), 0, e);
+                    });
+                }
+            }
+            __syncthreads();
+            draw(sh, s, r, rules, per, sh.listed < kList ? sh.listed : kList);
+        }
+    }
+    if (!listed) draw_slowly<DT>(sh.slow, s, r, rules, top);
 }
 
 template <int DT>
@@ -1151,35 +1148,39 @@ hipError_t launch(Device* d, hipStream_t st, const Sampling& s, int* status) {
     constexpr uint32_t kMost = kTile / E * kLanes;
     const uint32_t least = (blocks + kMost - 1) / kMost;
     if (least <= 1 || (least <= kTiles && s.rows >= (uint32_t)d->cu_count)) {
-        const dim3 grid(s.rows < (1u << 21) ? s.rows : 1u << 21);
-        hipLaunchKernelGGL(sample_whole_kernel<DT>, grid, dim3(kLanes), 0, st, s);
+        // a grid's lanes are counted in 32 bits
+        constexpr uint32_t kRows = 1u << 21;
+        for (uint32_t first = 0; first < s.rows; first += kRows) {
+            const uint32_t n = s.rows - first < kRows ? s.rows - first : kRows;
+            hipLaunchKernelGGL(sample_whole_kernel<DT>, dim3(n), dim3(kLanes), 0, st, s, first);
+        }
         return hipGetLastError();
     }
     uint32_t parts = 2 * (uint32_t)d->cu_count / s.rows;
-    const uint32_t most = (blocks + kMost / 4 - 1) / (kMost / 4);
+    const uint32_t most = (blocks + kMost / 2 - 1) / (kMost / 2);
     parts = parts < most ? parts : most;
     parts = parts > least ? parts : least;
     Parts p{};
     p.blocks = (blocks + parts - 1) / parts;
     p.parts = (blocks + p.blocks - 1) / p.blocks;
-    // launches of up to 64 MiB of rings and 4096 rows' counters
+    // launches of up to 64 MiB of rings, and of as many rows as there are tickets
     uint32_t rows = (64u << 20) / (p.parts * kRing * 8);
-    rows = rows < 4096 ? (rows ? rows : 1) : 4096;
+    constexpr uint32_t kTickets = kWorkspaceCounterBytes / 4;
+    rows = rows < kTickets ? (rows ? rows : 1) : kTickets;
     rows = rows < s.rows ? rows : s.rows;
     const size_t slots = (size_t)rows * p.parts;
-    char* ws = static_cast<char*>(workspace(
-        d, st, slots * (kRing * 8 + 8 + 8) + rows * sizeof(Row), status));
+    char* ws = static_cast<char*>(
+        workspace(d, st, slots * (kRing * 8 + 8 + 4 + kLanes), status));
     if (!ws) return hipSuccess;
-    p.counters = reinterpret_cast<uint32_t*>(ws);
+    p.tickets = reinterpret_cast<uint32_t*>(ws);
     p.rings = reinterpret_cast<uint64_t*>(ws + kWorkspaceCounterBytes);
     p.least = p.rings + slots * kRing;
-    p.rows = reinterpret_cast<Row*>(p.least + slots);
-    p.tops = reinterpret_cast<float*>(p.rows + rows);
+    p.tops = reinterpret_cast<float*>(p.least + slots);
+    p.far = reinterpret_cast<uint8_t*>(p.tops + slots);
     for (uint32_t first = 0; first < s.rows; first += rows) {
         const uint32_t n = s.rows - first < rows ? s.rows - first : rows;
         p.first = first;
-        hipLaunchKernelGGL(sample_scan_kernel<DT>, dim3(n * p.parts), dim3(kLanes), 0, st, s, p);
-        hipLaunchKernelGGL(sample_pick_kernel<DT>, dim3(n * p.parts), dim3(kLanes), 0, st, s, p);
+        hipLaunchKernelGGL(sample_parts_kernel<DT>, dim3(n * p.parts), dim3(kLanes), 0, st, s, p);
     }
     return hipGetLastError();
 }
