@@ -8,12 +8,14 @@
 // logit is 16 e rounded, i, and its weight 2^(i / 16) 2^(r / 16), |r| <= 1/2 the
 // rest.  A pass over the logits adds up each bin's count and its 2^(r / 16), both in
 // one 64-bit word, as whole numbers: the sums are exact and the same in any order.
-// Sums over bins then say in which bins the borders of k, p, m and u lie; the logits
-// of those few are gathered, sorted and weighed one by one.
+// Sums over bins then say in which bins the borders of k, p, m and u lie.  Where those
+// hold up to 64 logits together, one more look gathers them, and a wave puts them in
+// order and finds the borders.  Otherwise the borders are found one by one, each bin
+// cut into 1024 by another histogram first if it holds more than 64.
 //
 // Bins are absolute, not relative to the row's largest, so one pass is enough: a ring
-// of 1024 bins (64 factors of two) whose top follows the largest seen.  Weights below
-// 2^-60 of the largest are left out.
+// of 1024 bins (64 factors of two), set by the first logits seen.  Weights below 2^-46
+// of the largest are left out.
 #include <hip/hip_runtime.h>
 
 #include "internal.hpp"
@@ -249,53 +251,65 @@ __device__ uint32_t index_of(const void* row, uint32_t width, uint32_t key, uint
 
 constexpr int kRing = 1024;            // bins of the ring: a lane each
 constexpr int kCopies = 8;             // of each bin's word, for lanes that meet in it
-constexpr int kReach = 960;            // bins below the largest's that count
-constexpr int kList = 2048;            // logits near the borders, at most
+constexpr int kReach = 736;            // bins below the largest's that count
+constexpr int kFew = 64;               // logits that a wave puts in order
 
 // A bin's word: 2^49 for each logit, and 2^39 (2^(r / 16) - kLeast).  Up to 2^14 of
 // them: the lower sum stays below 2^39 0.0434 2^14 < 2^49.
 constexpr int kUnit = 39, kCount = 49;
 constexpr double kLeast = 1002.0 / 1024;               // below 2^(-1 / 32)
 constexpr uint64_t kLeastUnits = 1002ull << (kUnit - 10);
+constexpr uint64_t kRest = (1ull << kCount) - 1;
 constexpr uint32_t kMostEach = 1u << 14;
 
-// A logit's bin and its part of the bin's word.  2^(r / 16) to the fifth power of its
-// series: off by (ln 2 / 32)^6 / 720 = 2^-42.7 of it, and rounded by 2^-40.  Bins have
-// to be the same wherever they are asked for, so no sum is fused here that is not
-// written so.
+// 2^(r / 16), by the fifth power of its series: off by (ln 2 / 32)^6 / 720 = 2^-42.7 of
+// it for |r| <= 1/2.  `one` is the series' first number.
+__device__ __forceinline__ double sixteenth_of(double r, double one) {
+    constexpr double z = 0.69314718055994530942 / 16;
+    constexpr double c1 = z, c2 = z * z / 2, c3 = z * z * z / 6, c4 = z * z * z * z / 24,
+                     c5 = z * z * z * z * z / 120;
+    double q = __builtin_fma(c5, r, c4);
+    q = __builtin_fma(q, r, c3);
+    q = __builtin_fma(q, r, c2);
+    q = __builtin_fma(q, r, c1);
+    return __builtin_fma(q, r, one);
+}
+// A logit's bin, its place r in it and its part of the bin's word, rounded by 2^-40.
+// Bins have to be the same wherever they are asked for, so no sum is fused here that is
+// not written so.
 struct Binned {
     int bin;
+    double r;
     uint64_t word;
 };
 __device__ __forceinline__ Binned binned(float x, double per) {
 #pragma clang fp contract(off)
     constexpr double kMagic = 6755399441055744.0;      // 3 * 2^51: the sum's low word is whole
-    constexpr double z = 0.69314718055994530942 / 16;
-    constexpr double c1 = z, c2 = z * z / 2, c3 = z * z * z / 6, c4 = z * z * z * z / 24,
-                     c5 = z * z * z * z * z / 120;
     constexpr double kBase = 8192.0;                   // its last place is 2^-39
     const double e = (double)x * per;
     const double t = e + kMagic;
     const double r = e - (t - kMagic);
-    double q = __builtin_fma(c5, r, c4);
-    q = __builtin_fma(q, r, c3);
-    q = __builtin_fma(q, r, c2);
-    q = __builtin_fma(q, r, c1);
-    q = __builtin_fma(q, r, kBase + (1 - kLeast));
-    return {(int)(uint32_t)__builtin_bit_cast(uint64_t, t),
+    const double q = sixteenth_of(r, kBase + (1 - kLeast));
+    return {(int)(uint32_t)__builtin_bit_cast(uint64_t, t), r,
             __builtin_bit_cast(uint64_t, q) -
                 (__builtin_bit_cast(uint64_t, kBase) - (1ull << kCount))};
 }
-// Logits per bin's width: 16 log2(e) / T.
+// Bins a logit's unit: 16 log2(e) / T.
 __device__ __forceinline__ double bins_per(const Rules& r) {
     return uniform(16 * 1.44269504088896340736 / r.temperature);
 }
-// A weight in units of 2^-39 of 2^(bin / 16), exact.
+// A weight, or a sum of them, in units of 2^-39 of 2^(bin / 16), exact.
 __device__ __forceinline__ uint64_t units(uint64_t count, uint64_t rest) {
     return count * kLeastUnits + rest;
 }
-__device__ __forceinline__ uint64_t units_of(const Binned& b) {
-    return units(1, b.word & ((1ull << kCount) - 1));
+__device__ __forceinline__ uint64_t units_of(const Binned& b) { return units(1, b.word & kRest); }
+// 2^(-d / 16), to a few of its last places.
+__device__ __forceinline__ double two_to(int d) {
+    double t = d & 1 ? 0.9576032806985737 : 1.0;
+    t *= d & 2 ? 0.9170040432046712 : 1.0;
+    t *= d & 4 ? 0.8408964152537145 : 1.0;
+    t *= d & 8 ? 0.7071067811865476 : 1.0;
+    return __builtin_amdgcn_ldexp(t, -(d >> 4));
 }
 
 // A row as aligned blocks of 16 bytes; what its ends leave of the first and the last
@@ -335,16 +349,19 @@ struct Blocks {
         else return (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e >> 1] >> 16 * (e & 1)));
     }
 };
-constexpr int kTile = 16;              // logits a lane reads at once
-
-// Tile t's logits of this lane, of the blocks [first, last).
+// Logits a lane reads at once; a tile is two such strips of all lanes.
+constexpr int kStrip = 8;
 template <int DT>
-__device__ __forceinline__ void read_tile(const Blocks<DT>& row, uint32_t first, uint32_t last,
-                                          uint32_t t, float (&x)[kTile]) {
+constexpr uint32_t kStripBlocks = kStrip / Blocks<DT>::kEach * kLanes;
+
+// This lane's logits of strip t of the blocks [first, last).
+template <int DT>
+__device__ __forceinline__ void read_strip(const Blocks<DT>& row, uint32_t first, uint32_t last,
+                                           uint32_t t, float (&x)[kStrip]) {
     constexpr int E = Blocks<DT>::kEach;
 #pragma unroll
-    for (int q = 0; q < kTile / E; q++) {
-        const uint32_t b = first + (t * (kTile / E) + q) * kLanes + threadIdx.x;
+    for (int q = 0; q < kStrip / E; q++) {
+        const uint32_t b = first + t * kStripBlocks<DT> + q * kLanes + threadIdx.x;
         if (b < last) row.read(b, x + q * E);
         else
 #pragma unroll
@@ -355,48 +372,44 @@ template <int DT>
 __device__ __forceinline__ uint32_t index_in(const Blocks<DT>& row, uint32_t first, uint32_t t,
                                              int e) {
     constexpr int E = Blocks<DT>::kEach;
-    return (first + (t * (kTile / E) + e / E) * kLanes + threadIdx.x) * E + e % E - row.before;
+    return (first + t * kStripBlocks<DT> + e / E * kLanes + threadIdx.x) * E + e % E - row.before;
 }
-__device__ __forceinline__ float largest(const float (&x)[kTile]) {
+__device__ __forceinline__ float largest(const float (&x)[kStrip]) {
     float m = fmaxf(x[0], x[1]);
 #pragma unroll
-    for (int e = 2; e < kTile; e++) m = fmaxf(m, x[e]);
+    for (int e = 2; e < kStrip; e++) m = fmaxf(m, x[e]);
     return m;
 }
 
-// Sums of a row's bins, from the largest's down, and where its borders lie.
-struct Span {
-    int lo, hi;                        // bins below the largest's
-};
-struct Plan {
-    float top;                         // the row's largest logit
-    uint32_t listed;                   // logits of the bins below
-    double all;                        // the row's sum
-    Span k, p, m, s;                   // an empty one: hi < lo
-};
-struct Sums {
-    double mass[kRing];                // up to the bin's end
-    uint32_t count[kRing];
-};
+constexpr int kFirsts = 24;
 struct Scratch {
     union {
         uint64_t ring[kRing * kCopies + kCopies];      // the last: logits of no bin
         struct {
-            Sums sums;
-            uint64_t list[kList];
-            double upto[kList];         // the row's sum up to a listed logit's end
-            uint32_t rank[kList];       // its place in the order
-            int bin[kList];
+            double mass[kRing];        // the row's sum up to a bin's end, from the largest's
+            uint32_t count[kRing];
+            uint64_t fine[kRing];      // a bin's words, cut into 1024
+            uint64_t list[kFew];
+            uint8_t near[kRing];       // bins that a border may lie in
         };
         RowScratch slow;
     };
-    Plan plan;
     double wave_mass[kWaves];
     uint32_t wave_count[kWaves];
     float wave_top[kWaves];
-    int first[4];
-    uint32_t listed, last;
+    int first[kFirsts];                // a search's each, none found yet
+    uint32_t listed, planned, least, most, last;
+    double kept, weight;               // what a wave found
+    uint32_t kept_count, token;
 };
+__device__ __forceinline__ void clear_scratch(Scratch& sh) {
+    uint4* p = reinterpret_cast<uint4*>(sh.ring);
+#pragma unroll
+    for (int i = 0; i < kRing * kCopies / 2 / kLanes; i++)
+        p[i * kLanes + threadIdx.x] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < kFirsts) sh.first[threadIdx.x] = 0x7fffffff;
+    if (threadIdx.x == 0) sh.planned = 0;
+}
 
 __device__ __forceinline__ float top_of(Scratch& sh, float m) {
 #pragma unroll
@@ -428,20 +441,14 @@ __device__ __forceinline__ bool has_bins(float top, double per) {
     return fabs((double)top * per) < 0x1p17 && per > 0x1p-60;
 }
 
-__device__ __forceinline__ void clear_ring(Scratch& sh) {
-    uint4* p = reinterpret_cast<uint4*>(sh.ring);
-#pragma unroll
-    for (int i = 0; i < kRing * kCopies / 2 / kLanes; i++)
-        p[i * kLanes + threadIdx.x] = make_uint4(0, 0, 0, 0);
-}
 // Adds a lane's logits that are in; the others' words go where nobody reads, without a
 // branch a logit.
 template <typename F>
-__device__ __forceinline__ void add_to_ring(Scratch& sh, const float (&x)[kTile], double per,
+__device__ __forceinline__ void add_to_ring(Scratch& sh, const float (&x)[kStrip], double per,
                                             F in) {
     uint64_t* mine = sh.ring + (threadIdx.x & (kCopies - 1));
 #pragma unroll
-    for (int e = 0; e < kTile; e++) {
+    for (int e = 0; e < kStrip; e++) {
         const Binned b = binned(x[e], per);
         const int slot = in(x[e]) ? b.bin & (kRing - 1) : kRing;
         atomicAdd((unsigned long long*)(mine + slot * kCopies), (unsigned long long)b.word);
@@ -457,131 +464,48 @@ __device__ __forceinline__ void read_ring(const Scratch& sh, int top, uint32_t* 
 #pragma unroll
     for (int i = 0; i < kCopies; i++) {
         *count += (uint32_t)(p[i] >> kCount);
-        *rest += p[i] & ((1ull << kCount) - 1);
+        *rest += p[i] & kRest;
     }
 }
 
-// The first lane for which it holds, or `none`; all lanes call it.
+// ---- the borders ----------------------------------------------------------------
+
+// The first lane for which it holds, or `none`, N questions at once; all lanes call it.
 template <int N>
-__device__ __forceinline__ void first_lanes(Scratch& sh, const bool (&is)[N], int none,
+__device__ __forceinline__ void first_lanes(Scratch& sh, int& next, const bool (&is)[N], int none,
                                             int (&at)[N]) {
-    if (threadIdx.x < N) sh.first[threadIdx.x] = none;
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const uint64_t b = __ballot(is[i]);
         if (b && (threadIdx.x & 63) == 0)
-            atomicMin(&sh.first[i], (int)(threadIdx.x & ~63u) + (int)__builtin_ctzll(b));
+            atomicMin(&sh.first[next + i], (int)threadIdx.x + (int)__builtin_ctzll(b));
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; i++) at[i] = sh.first[i];
-    __syncthreads();
+    for (int i = 0; i < N; i++) {
+        const int x = __builtin_amdgcn_readfirstlane(sh.first[next + i]);
+        at[i] = x < none ? x : none;
+    }
+    next += N;
 }
 
-// Where the borders lie, from each lane's bin (so many below the largest's).  What a
-// border leaves or cuts off of its bin is not known yet, so a sum behind it lies
-// between two, and the bins where the next border may be with it.
-__device__ void make_plan(Scratch& sh, const Rules& rules, float top, double per, uint32_t count,
-                          uint64_t rest) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = threadIdx.x;
-    const Binned big = binned(top, per);
-    const uint64_t one = units_of(big);
-    double mass = 0;
-    if (d >= kReach) count = 0, rest = 0;
-    if (count) {
-        const uint64_t all = units(count, rest);
-        // the largest's own bin in whole weights and their rest, so that equal logits'
-        // sums are whole
-        if (d == 0) mass = (double)(all / one) + (double)(all % one) / (double)one;
-        else mass = (double)all / (double)one * exp2(-d / 16.0);
-    }
-    double up = mass;
-    uint32_t up_count = count;
+// Sums over the workgroup's lanes up to and with this one.
+__device__ __forceinline__ void sums_upto(Scratch& sh, double& mass, uint32_t& count) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) {
-        const double m = __shfl_up(up, x, 64);
-        const uint32_t c = __shfl_up(up_count, x, 64);
-        if (lane >= x) up += m, up_count += c;
+        const double m = __shfl_up(mass, x, 64);
+        const uint32_t c = __shfl_up(count, x, 64);
+        if (lane >= x) mass += m, count += c;
     }
-    if (lane == 63) sh.wave_mass[wave] = up, sh.wave_count[wave] = up_count;
-    __syncthreads();                    // every lane has read the ring, too
+    if (lane == 63) sh.wave_mass[wave] = mass, sh.wave_count[wave] = count;
+    __syncthreads();
     double before = 0;
     uint32_t before_count = 0;
+#pragma unroll 1
     for (int w = 0; w < wave; w++) before += sh.wave_mass[w], before_count += sh.wave_count[w];
-    const double inc = before + up;
-    const uint32_t inc_count = before_count + up_count;
-    sh.sums.mass[d] = inc;
-    sh.sums.count[d] = inc_count;
-    __syncthreads();
-    const double all = sh.sums.mass[kRing - 1];
-    const uint32_t all_count = sh.sums.count[kRing - 1];
-    const auto mass_before = [&](int b) { return b > 0 ? sh.sums.mass[b - 1] : 0.0; };
-    Plan plan;
-    plan.top = top;
-    plan.k = plan.p = plan.m = plan.s = {0, -1};
-    double lo = all, hi = all;          // what is kept
-    int end = kRing - 1;
-    {
-        const bool is[2] = {inc_count >= rules.top_k, inc_count >= all_count};
-        int at[2];
-        first_lanes<2>(sh, is, kRing - 1, at);
-        end = at[1];                    // the last that holds any
-        if (rules.top_k < all_count) {
-            end = at[0];
-            plan.k = {at[0], at[0]};
-            lo = mass_before(at[0]), hi = sh.sums.mass[at[0]];
-        }
-    }
-    if (rules.top_p < 1) {
-        const bool is[2] = {inc >= rules.top_p * lo, inc >= rules.top_p * hi};
-        int at[2];
-        first_lanes<2>(sh, is, end, at);
-        // an empty bin has its predecessor's sum, so a border is in one that holds any
-        plan.p = {at[0] < end ? at[0] : end, at[1] < end ? at[1] : end};
-        lo = mass_before(plan.p.lo);
-        hi = sh.sums.mass[plan.p.hi];
-        end = plan.p.hi;
-    }
-    if (rules.min_p > 0) {
-        const double e = (double)top * per;
-        const double r = e - rint(e);
-        // bins before this one are kept whole, those past it not at all
-        const double at = rint(-16 * log2(rules.min_p) - r);
-        if (at <= end) {
-            end = at > 0 ? (int)at : 0;
-            plan.m = {end, end};
-            lo = fmin(lo, mass_before(end));
-            hi = fmin(hi, sh.sums.mass[end]);
-        }
-    }
-    {
-        const bool is[2] = {inc > rules.u * lo, inc > rules.u * hi};
-        int at[2];
-        first_lanes<2>(sh, is, end, at);
-        plan.s = {at[0] < end ? at[0] : end, at[1] < end ? at[1] : end};
-    }
-    plan.all = all;
-    const auto in = [](const Span& s, int b) { return b >= s.lo && b <= s.hi; };
-    const bool need = in(plan.k, d) || in(plan.p, d) || in(plan.m, d) || in(plan.s, d);
-    uint32_t listed = need ? count : 0;
-#pragma unroll
-    for (int x = 32; x; x >>= 1) listed += __shfl_xor(listed, x, 64);
-    if (lane == 0) sh.wave_count[wave] = listed;
-    __syncthreads();
-    listed = 0;
-    for (int w = 0; w < kWaves; w++) listed += sh.wave_count[w];
-    plan.listed = listed;
-    if (threadIdx.x == 0) sh.plan = plan;
-    __syncthreads();
-}
-__device__ __forceinline__ bool needed(const Plan& p, int d) {
-    return (d >= p.k.lo && d <= p.k.hi) || (d >= p.p.lo && d <= p.p.hi) ||
-           (d >= p.m.lo && d <= p.m.hi) || (d >= p.s.lo && d <= p.s.hi);
-}
-__device__ __forceinline__ int last_needed(const Plan& p) {
-    const int a = p.k.hi > p.p.hi ? p.k.hi : p.p.hi, b = p.m.hi > p.s.hi ? p.m.hi : p.s.hi;
-    return a > b ? a : b;
+    mass += before;
+    count += before_count;
 }
 
 // Place in the order, ascending.
@@ -589,188 +513,357 @@ __device__ __forceinline__ uint64_t placed(float x, uint32_t index) {
     return (uint64_t)~key_of(x) << 32 | index;
 }
 
-// Lists a lane's logits of the plan's bins, none of which holds one below low.
-template <typename F>
-__device__ __forceinline__ void list_near(Scratch& sh, const Plan& plan, int top, float low,
-                                          double per, const float (&x)[kTile], F index) {
-#pragma unroll
-    for (int e = 0; e < kTile; e++)
-        if (x[e] >= low && needed(plan, top - binned(x[e], per).bin)) {
-            const uint32_t at = atomicAdd(&sh.listed, 1u);
-            if (at < kList) sh.list[at] = placed(x[e], index(e));
-        }
+// What a look over the row is for: bins lo .. hi below the largest's, of them (joint)
+// those that are near a border; to cut them into 1024 (fine), or to list their logits,
+// those of one of the 1024 where part is not -1.
+struct Ask {
+    int lo, hi, part;
+    bool joint, fine;
+};
+__device__ __forceinline__ int part_of(double r) {
+    const int p = (int)((0.5 - r) * kRing);
+    return p < 0 ? 0 : p < kRing ? p : kRing - 1;
+}
+__device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, double per, float x,
+                                       uint32_t index) {
+    const Binned b = binned(x, per);
+    const int d = top - b.bin;
+    if (d < ask.lo || d > ask.hi || (ask.joint && !sh.near[d])) return;
+    if (ask.fine) {
+        atomicAdd((unsigned long long*)&sh.fine[part_of(b.r)], (unsigned long long)b.word);
+    } else if (ask.part < 0 || part_of(b.r) == ask.part) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kFew) sh.list[at] = placed(x, index);
+        const uint32_t key = key_of(x);
+        atomicMin(&sh.least, key);
+        atomicMax(&sh.most, key);
+    }
 }
 
-// Sorts sh.list[0 .. n) up; n <= kList.  A lane an element up to kLanes, exchanged
-// within a wave without LDS.
-__device__ void sort_list(Scratch& sh, uint32_t n) {
-    constexpr int kPer = kList / kLanes;
-    const uint32_t size = n <= 64 ? 64 : 1u << (32 - __builtin_clz(n - 1));
-    const int per = size > kLanes ? (int)(size / kLanes) : 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kLanes) sh.list[i] = ~0ull;
+// A wave's list in order, a lane a logit: its weight, its bin, and the sums up to it.
+struct Listed {
+    double weight, upto;
+    uint32_t token, rank;              // rank: how many that is, itself among them
+    int bin;
+};
+template <typename B>
+__device__ __forceinline__ Listed in_order(Scratch& sh, uint32_t n, int top, double per,
+                                           double one, B before) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t at = lane < n ? sh.list[lane] : ~0ull;
+    uint32_t place = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < n; i++) {
+        const uint64_t o =
+            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), i) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((uint32_t)at, i);
+        place += o < at;
+    }
+    if (lane < n) sh.list[place] = at;
+    // a lane reads what another has written
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (lane < n) at = sh.list[lane];
+    const Binned b = binned(value_of(~(uint32_t)(at >> 32)), per);
+    Listed l;
+    l.token = (uint32_t)at;
+    l.bin = lane < n ? top - b.bin : kRing;
+    l.weight = lane < n ? (double)units_of(b) / one * two_to(l.bin) : 0.0;
+    l.upto = l.weight;
+    l.rank = 1;
+#pragma unroll 1
+    for (int x = 1; x < 64; x <<= 1) {
+        const double m = __shfl_up(l.upto, x, 64);
+        const uint32_t c = __shfl_up(l.rank, x, 64);
+        const int o = __shfl_up(l.bin, x, 64);
+        if ((int)lane >= x && o == l.bin) l.upto += m, l.rank += c;
+    }
+    before(l);
+    return l;
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(
+        double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(b >> 32), lane) << 32 |
+                    (uint32_t)__builtin_amdgcn_readlane((uint32_t)b, lane));
+}
+
+// What is left of a row: its sum and how many logits.
+struct Left {
+    double sum;
+    uint32_t count;
+};
+
+// The token of a row, from each lane's bin (so many below the largest's): its logits and
+// the rest of their weights.  look(ask) goes over the row's logits.  False where the
+// borders' bins hold too much.
+template <int DT, typename L>
+__device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t row,
+                                       const Rules& rules, double per, float top, uint32_t count,
+                                       uint64_t rest, L look) {
+    const int d = threadIdx.x;
+    const Binned big = binned(top, per);
+    const int top_bin = __builtin_amdgcn_readfirstlane(big.bin);
+    const uint64_t one_units = units_of(big);
+    const double one = uniform((double)one_units);
+    // units as weights, the largest's 1: whole ones and their rest, so that sums of
+    // equal logits are whole
+    const auto share = [&](uint64_t u) {
+        const int q = (int)rint((double)u / one);
+        return q + (double)((int64_t)u - (int64_t)q * (int64_t)one_units) / one;
+    };
+    const double scale = two_to(d);
+    if (d >= kReach) count = 0, rest = 0;
+    double mass = count ? share(units(count, rest)) * scale : 0.0;
+    uint32_t upto_count = count;
+    // every lane has read the ring when its place is taken
+    sums_upto(sh, mass, upto_count);
+    sh.mass[d] = mass;
+    sh.count[d] = upto_count;
     __syncthreads();
-    uint64_t v[kPer];
+    const auto mass_before = [&](int b) { return b > 0 ? sh.mass[b - 1] : 0.0; };
+    const auto count_before = [&](int b) { return b > 0 ? sh.count[b - 1] : 0u; };
+    const double all = uniform(sh.mass[kRing - 1]);
+    const uint32_t all_count = __builtin_amdgcn_readfirstlane(sh.count[kRing - 1]);
+    // the least weight that a bin of this lane's may hold
+    const double edge = uniform(sixteenth_of(-0.5, 1.0) * sixteenth_of(-big.r, 1.0));
+    const bool by_k = rules.top_k < all_count, by_p = rules.top_p < 1, by_m = rules.min_p > 0;
+    int next = 0;
+
+    // Where the borders may lie.  What one leaves of its bin is not known yet, so a sum
+    // behind it is between two, and the next border's bin with it.
+    struct Span {
+        int lo, hi;
+    };
+    Span k = {0, -1}, p = {0, -1}, m = {0, -1}, u;
+    double lo = all, hi = all;
+    int end, last;
+    {
+        const bool is[2] = {upto_count >= rules.top_k, upto_count >= all_count};
+        int at[2];
+        first_lanes<2>(sh, next, is, kRing - 1, at);
+        end = last = at[1];             // the last that holds any
+        if (by_k) {
+            end = at[0];
+            k = {end, end};
+            lo = mass_before(end), hi = sh.mass[end];
+        }
+    }
+    if (by_p) {
+        const bool is[2] = {mass >= rules.top_p * lo, mass >= rules.top_p * hi};
+        int at[2];
+        first_lanes<2>(sh, next, is, end, at);
+        p = {at[0], at[1]};
+        lo = mass_before(p.lo), hi = sh.mass[p.hi];
+        end = p.hi;
+    }
+    if (by_m) {
+        const bool is[1] = {scale * edge < rules.min_p};
+        int at[1];
+        first_lanes<1>(sh, next, is, kRing, at);
+        if (at[0] <= end) {
+            end = at[0];
+            m = {end, end};
+            lo = fmin(lo, mass_before(end)), hi = fmin(hi, sh.mass[end]);
+        }
+    }
+    {
+        const bool is[2] = {mass > rules.u * lo, mass > rules.u * hi};
+        int at[2];
+        first_lanes<2>(sh, next, is, end, at);
+        u = {at[0], at[1]};
+    }
+    const auto in = [&](const Span& x) { return d >= x.lo && d <= x.hi; };
+    const bool near = in(k) || in(p) || in(m) || in(u);
+    sh.near[d] = near;
+    uint32_t planned = near ? count : 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++)
-        v[i] = i < per && i * kLanes + threadIdx.x < size ? sh.list[i * kLanes + threadIdx.x] : ~0ull;
-    for (uint32_t k = 2; k <= size; k <<= 1)
-        for (uint32_t j = k >> 1; j; j >>= 1) {
-            if (j >= 64) {
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < kPer; i++)
-                    if (i < per && i * kLanes + threadIdx.x < size)
-                        sh.list[i * kLanes + threadIdx.x] = v[i];
-                __syncthreads();
+    for (int x = 32; x; x >>= 1) planned += __shfl_xor(planned, x, 64);
+    if ((d & 63) == 0 && planned) atomicAdd(&sh.planned, planned);
+    if (d == 0) sh.listed = 0, sh.least = ~0u, sh.most = 0;
+    __syncthreads();
+    Ask ask;
+    ask.joint = sh.planned <= kFew;
+    ask.fine = false;
+    ask.part = -1;
+    ask.lo = 0;
+    ask.hi = max(max(k.hi, p.hi), max(m.hi, u.hi));
+
+    enum { kByK, kByP, kByM, kByU };
+    Left left = {all, all_count};
+    int stage = kByK;
+    end = last;
+    double base = 0;
+    uint32_t base_count = 0;
+    for (;;) {
+        if (!ask.joint && ask.part < 0) {
+            // the next border's bin
+            while ((stage == kByK && !by_k) || (stage == kByP && !by_p) || (stage == kByM && !by_m))
+                stage++;
+            const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
+            const bool is[1] = {stage == kByK   ? upto_count >= rules.top_k
+                                : stage == kByP ? mass >= border
+                                : stage == kByM ? scale * edge < rules.min_p
+                                                : mass > border};
+            int at[1];
+            first_lanes<1>(sh, next, is, stage == kByM ? kRing : end, at);
+            if (stage == kByM && at[0] > end) {
+                stage++;
+                continue;
             }
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const uint32_t x = i * kLanes + threadIdx.x;
-                if (j < 64 || (i < per && x < size)) {
-                    const uint64_t o = j < 64 ? __shfl_xor(v[i], (int)j, 64) : sh.list[x ^ j];
-                    const bool up = (x & k) == 0, low = (x & j) == 0;
-                    if ((o < v[i]) == (up == low)) v[i] = o;
+            ask.lo = ask.hi = at[0];
+            base = uniform(mass_before(at[0]));
+            base_count = __builtin_amdgcn_readfirstlane(count_before(at[0]));
+            const uint32_t here = sh.count[at[0]] - base_count;
+            if (here > kMostEach) return false;
+            ask.fine = here > kFew;
+            if (ask.fine) sh.fine[d] = 0;
+            if (d == 0) sh.listed = 0, sh.least = ~0u, sh.most = 0;
+            __syncthreads();
+        }
+        look(ask);
+        __syncthreads();
+        if (ask.fine) {
+            // the 1024th that holds the border
+            const uint64_t word = sh.fine[d];
+            uint32_t c = (uint32_t)(word >> kCount);
+            double mm = c ? share(units(c, word & kRest)) * two_to(ask.lo) : 0.0;
+            const double own = mm;
+            const uint32_t own_count = c;
+            sums_upto(sh, mm, c);
+            mm += base, c += base_count;
+            const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
+            const double below = two_to(ask.lo) * sixteenth_of(-big.r, 1.0) *
+                                 sixteenth_of(0.5 - (d + 1) * (1.0 / kRing), 1.0);
+            const bool is[2] = {own_count && (stage == kByK   ? c >= rules.top_k
+                                              : stage == kByP ? mm >= border
+                                              : stage == kByM ? below < rules.min_p
+                                                              : mm > border),
+                                c >= sh.count[ask.lo]};
+            int at[2];
+            first_lanes<2>(sh, next, is, kRing - 1, at);
+            const int part = at[0] < at[1] ? at[0] : at[1];
+            if (d == part) {
+                sh.kept = mm - own, sh.kept_count = c - own_count;
+                sh.listed = 0, sh.least = ~0u, sh.most = 0;
+            }
+            __syncthreads();
+            base = uniform(sh.kept);
+            base_count = __builtin_amdgcn_readfirstlane(sh.kept_count);
+            ask.part = part;
+            ask.fine = false;
+            continue;
+        }
+        const uint32_t n = sh.listed;
+        if (ask.joint) {
+            if (d < 64) {
+                const Listed l = in_order(sh, n, top_bin, per, one, [&](Listed& x) {
+                    const int b = x.bin < kRing ? x.bin : 0;
+                    x.upto += mass_before(b);
+                    x.rank += count_before(b);
+                });
+                const auto of = [&](const Span& x) { return l.bin >= x.lo && l.bin <= x.hi; };
+                // the first listed logit of a span for which it holds, or the span's last
+                const auto find = [&](const Span& x, bool is) {
+                    const uint64_t some = __ballot(of(x)), hit = __ballot(of(x) && is);
+                    return hit ? (int)__builtin_ctzll(hit)
+                               : some ? 63 - (int)__builtin_clzll(some) : 0;
+                };
+                const auto cut = [&](int at) {
+                    const uint32_t c = __builtin_amdgcn_readlane(l.rank, at);
+                    if (c < left.count) left = {lane_of(l.upto, at), c};
+                };
+                if (by_k) cut(find(k, l.rank >= rules.top_k));
+                if (by_p) cut(find(p, l.upto >= rules.top_p * left.sum));
+                if (m.lo <= m.hi) {
+                    // all of its bin that weigh as much, and all before it
+                    const uint64_t ok = __ballot(of(m) && l.weight >= rules.min_p);
+                    if (ok) cut(63 - (int)__builtin_clzll(ok));
+                    else if (count_before(m.lo) < left.count)
+                        left = {mass_before(m.lo), count_before(m.lo)};
+                }
+                int at = find(u, l.upto > rules.u * left.sum);
+                // sums of bins and of their logits are rounded apart
+                while (at && (uint32_t)__builtin_amdgcn_readlane(l.rank, at) > left.count) at--;
+                if (d == 0) {
+                    sh.token = __builtin_amdgcn_readlane(l.token, at);
+                    sh.weight = lane_of(l.weight, at);
+                    sh.kept = left.sum;
                 }
             }
+            break;
         }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-        if (i < per && i * kLanes + threadIdx.x < size) sh.list[i * kLanes + threadIdx.x] = v[i];
-    __syncthreads();
-}
-
-// The first of the list's n elements, one past the other, for which it holds, or n.
-template <typename F>
-__device__ uint32_t first_listed(Scratch& sh, uint32_t n, F is) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.first[0] = (int)n;
-    __syncthreads();
-    for (uint32_t base = 0; base < n; base += kLanes) {
-        const uint32_t i = base + threadIdx.x;
-        const uint64_t b = __ballot(i < n && is(i));
-        if (b && (threadIdx.x & 63) == 0)
-            atomicMin(&sh.first[0], (int)(i + __builtin_ctzll(b)));
-    }
-    __syncthreads();
-    return (uint32_t)sh.first[0];
-}
-
-// The token, from the sums over bins and the n logits of the plan's bins.
-__device__ void draw(Scratch& sh, const Sampling& s, uint32_t row, const Rules& rules, double per,
-                     uint32_t n) {
-    sort_list(sh, n);
-    const Plan plan = sh.plan;
-    const Binned big = binned(plan.top, per);
-    const double one = (double)units_of(big);
-    const auto binned_at = [&](uint32_t i) {
-        return binned(value_of(~(uint32_t)(sh.list[i] >> 32)), per);
-    };
-    const auto weight_of = [&](const Binned& b) {
-        const int d = big.bin - b.bin;
-        const double w = (double)units_of(b) / one;
-        return d ? w * exp2(-d / 16.0) : w;
-    };
-    const auto mass_before = [&](int d) { return d ? sh.sums.mass[d - 1] : 0.0; };
-    const auto count_before = [&](int d) { return d ? sh.sums.count[d - 1] : 0u; };
-    // the first listed logit of bin d or one past it
-    const auto start_of = [&](int d) {
-        uint32_t lo = 0, hi = n;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (sh.bin[mid] < d) lo = mid + 1;
-            else hi = mid;
+        const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
+        const uint32_t most = sh.most;
+        if (n <= kFew) {
+            if (d < 64) {
+                const Listed l = in_order(sh, n, top_bin, per, one, [&](Listed& x) {
+                    x.upto += base;
+                    x.rank += base_count;
+                });
+                const uint64_t hit = __ballot(
+                    d < (int)n && (stage == kByK   ? l.rank >= rules.top_k
+                                   : stage == kByP ? l.upto >= border
+                                   : stage == kByM ? !(l.weight >= rules.min_p)
+                                                   : l.upto > border || l.rank == left.count));
+                int at = hit ? (int)__builtin_ctzll(hit) : (int)n - 1;
+                double upto = base;
+                uint32_t rank = base_count;
+                // the first that is too light goes with those behind it
+                if (stage == kByM && hit) at--;
+                if (at >= 0) upto = lane_of(l.upto, at), rank = __builtin_amdgcn_readlane(l.rank, at);
+                if (d == 0) {
+                    sh.kept = upto, sh.kept_count = rank;
+                    sh.token = __builtin_amdgcn_readlane(l.token, at < 0 ? 0 : at);
+                    sh.weight = lane_of(l.weight, at < 0 ? 0 : at);
+                }
+            }
+        } else {
+            // equal logits: so many of them
+            if (sh.least != most) return false;
+            const Binned b = binned(value_of(most), per);
+            const double w = (double)units_of(b) / one * two_to(top_bin - b.bin);
+            uint32_t take = stage == kByK ? rules.top_k - base_count : 0;
+            if (stage == kByP) take = (uint32_t)fmax(ceil((border - base) / w), 1.0);
+            if (stage == kByM) take = w >= rules.min_p ? n : 0;
+            if (stage == kByU) take = (uint32_t)fmax(floor((border - base) / w), 0.0) + 1;
+            if (stage == kByU && base_count + take > left.count) take = left.count - base_count;
+            if (take > n) take = n;
+            __syncthreads();
+            if (stage == kByU) {
+                const void* at = static_cast<const char*>(s.logits) +
+                                 (size_t)row * s.width * (DT == ACCEL_F32 ? 4 : 2);
+                const uint32_t token = index_of<DT>(at, s.width, most, take ? take - 1 : 0, sh.slow);
+                if (d == 0) sh.token = token;
+            }
+            if (d == 0) sh.kept = base + take * w, sh.kept_count = base_count + take, sh.weight = w;
         }
-        return lo;
-    };
-    // running sums of the list, kLanes at a time, then of the row
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double carry = 0;
-    for (uint32_t base = 0; base < n; base += kLanes) {
-        const uint32_t i = base + threadIdx.x;
-        double up = 0;
-        if (i < n) {
-            const Binned b = binned_at(i);
-            sh.bin[i] = big.bin - b.bin;
-            up = weight_of(b);
+        if (stage == kByU) {
+            if (d == 0) sh.kept = left.sum;
+            break;
         }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-            const double m = __shfl_up(up, x, 64);
-            if (lane >= x) up += m;
-        }
-        if (lane == 63) sh.wave_mass[wave] = up;
         __syncthreads();
-        double before = carry;
-        for (int w = 0; w < kWaves; w++) {
-            if (w < wave) before += sh.wave_mass[w];
-            carry += sh.wave_mass[w];
+        const uint32_t c = __builtin_amdgcn_readfirstlane(sh.kept_count);
+        if (c < left.count) {
+            left = {uniform(sh.kept), c};
+            end = ask.lo;
         }
-        if (i < n) sh.upto[i] = before + up;
+        stage++;
+        ask.part = -1;
         __syncthreads();
     }
-    double upto[kList / kLanes];
-#pragma unroll
-    for (int x = 0; x < kList / kLanes; x++) {
-        const uint32_t i = x * kLanes + threadIdx.x;
-        if (i >= n) continue;
-        const int d = sh.bin[i];
-        const uint32_t at = start_of(d);
-        upto[x] = mass_before(d) + (sh.upto[i] - (at ? sh.upto[at - 1] : 0.0));
-        sh.rank[i] = count_before(d) + (i - at);
+    if (d == 0) {
+        s.tokens[row] = sh.token;
+        if (s.logprobs) s.logprobs[row] = (float)log(sh.weight / sh.kept);
     }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < kList / kLanes; x++) {
-        const uint32_t i = x * kLanes + threadIdx.x;
-        if (i < n) sh.upto[i] = upto[x];
-    }
-    __syncthreads();
-    double kept = plan.all;
-    uint32_t count = sh.sums.count[kRing - 1];
-    const auto cut = [&](double mass, uint32_t upto_count) {
-        if (upto_count < count) kept = mass, count = upto_count;
-    };
-    if (plan.k.lo <= plan.k.hi) {
-        const uint32_t i = start_of(plan.k.lo) + (rules.top_k - 1 - count_before(plan.k.lo));
-        kept = sh.upto[i < n ? i : n - 1];
-        count = rules.top_k;
-    }
-    // the first in a span of bins whose sum is past a border, or the span's last
-    const auto crossing = [&](const Span& span, auto past) {
-        const uint32_t lo = start_of(span.lo), hi = start_of(span.hi + 1);
-        const uint32_t i =
-            first_listed(sh, hi, [&](uint32_t x) { return x >= lo && past(sh.upto[x]); });
-        return i < hi ? i : hi - 1;
-    };
-    if (plan.p.lo <= plan.p.hi) {
-        const double border = rules.top_p * kept;
-        const uint32_t i = crossing(plan.p, [&](double m) { return m >= border; });
-        cut(sh.upto[i], sh.rank[i] + 1);
-    }
-    if (plan.m.lo <= plan.m.hi) {
-        const int d = plan.m.lo;
-        const uint32_t lo = start_of(d), hi = start_of(d + 1);
-        const uint32_t i = first_listed(sh, hi, [&](uint32_t x) {
-            return x >= lo && !(weight_of(binned_at(x)) >= rules.min_p);
-        });
-        if (i > lo) cut(sh.upto[i - 1], sh.rank[i - 1] + 1);
-        else cut(mass_before(d), count_before(d));
-    }
-    const double border = rules.u * kept;
-    uint32_t i = crossing(plan.s, [&](double m) { return m > border; });
-    // sums of bins and of their logits are rounded apart
-    while (i && sh.rank[i] >= count) i--;
-    if (threadIdx.x == 0) {
-        s.tokens[row] = (uint32_t)sh.list[i];
-        if (s.logprobs) s.logprobs[row] = (float)log(weight_of(binned_at(i)) / kept);
-    }
-    __syncthreads();
+    return true;
 }
 
 // ---- the kernels ----------------------------------------------------------------
 
-// A row that has no bins, or too many logits near its borders: place by place.
+// A row that has no bins, or more than 64 logits of several values in a 1024th of one:
+// borders digit by digit of the keys.
 template <int DT>
 __device__ __attribute__((noinline)) void draw_slowly(RowScratch& sh, const Sampling& s, uint32_t r, const Rules& rules,
                             float top) {
@@ -858,22 +951,21 @@ __device__ __forceinline__ uint64_t least_of(Scratch& sh, uint64_t v) {
     if ((threadIdx.x & 63) == 0) sh.list[threadIdx.x >> 6] = v;
     __syncthreads();
     v = sh.list[0];
-#pragma unroll
+#pragma unroll 1
     for (int w = 1; w < kWaves; w++) v = sh.list[w] < v ? sh.list[w] : v;
     __syncthreads();
     return v;
 }
 template <int DT>
 __device__ __forceinline__ uint64_t least_in(const Blocks<DT>& row, uint32_t first, uint32_t last) {
-    constexpr uint32_t kStep = kTile / Blocks<DT>::kEach * kLanes;
     float best = -INFINITY;
     uint32_t at = 0;
-    for (uint32_t t = 0; t * kStep < last - first; t++) {
-        float x[kTile];
-        read_tile<DT>(row, first, last, t, x);
-        // a lane's logits are read in their order, but for the blocks of a tile
+    for (uint32_t t = 0; t * kStripBlocks<DT> < last - first; t++) {
+        float x[kStrip];
+        read_strip<DT>(row, first, last, t, x);
+        // a lane's logits are read in their order
 #pragma unroll
-        for (int e = 0; e < kTile; e++)
+        for (int e = 0; e < kStrip; e++)
             if (x[e] > best) best = x[e], at = index_in<DT>(row, first, t, e);
     }
     return best > -INFINITY ? placed(best, at) : ~0ull;
@@ -886,9 +978,10 @@ __device__ __forceinline__ void give_first(const Sampling& s, uint32_t row, uint
 }
 
 // Rows of up to kTiles tiles, a workgroup each, two workgroups a CU.  Of each tile of a
-// lane it is kept how far its largest logit is from the top, so the second look goes
-// only to what may hold something near a border.
+// lane it is kept how far its largest logit is from the window's top, so a second look
+// goes only to what may hold something near a border.
 constexpr int kTiles = 8;
+constexpr int kTile = 2 * kStrip;
 constexpr int kFar = 255;              // below the window; nearer ones are 253 at most
 static_assert(kTiles * kTile * kLanes / kCopies <= kMostEach, "a word's count and sum");
 static_assert(kTile * kLanes <= kMostEach, "the same, of a part's copies together");
@@ -897,7 +990,6 @@ template <int DT>
 __global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uint32_t first_row) {
     __shared__ Scratch sh;
     __shared__ uint8_t far[kTiles][kLanes];
-    constexpr uint32_t kStep = kTile / Blocks<DT>::kEach * kLanes;
     const uint32_t r = first_row + blockIdx.x;
     const Rules rules = rules_of(s, r);
     const Blocks<DT> row(s, r);
@@ -906,52 +998,56 @@ __global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uin
         return;
     }
     const double per = bins_per(rules);
-    float x[kTile];
-    read_tile<DT>(row, 0, row.count, 0, x);
-    float top = largest(x);
-    clear_ring(sh);
-    // the window is set by the first tile, with room for the rest to pass it by a
-    // factor of four; what passes it further is added afterwards
+    float x[kStrip];
+    read_strip<DT>(row, 0, row.count, 0, x);
+    clear_scratch(sh);
+    float most = largest(x), top = most;
+    // the window is set by the first strip, with room for the rest to pass it by 2^16;
+    // what passes it further is added afterwards
     const float first = top_of(sh, top);
     const bool bins = has_bins(first, per);
     Window w = {0, INFINITY, -INFINITY};
-    if (bins) w.set(binned(first, per).bin + 32, per);
+    if (bins) w.set(binned(first, per).bin + 256, per);
+    const uint32_t strips = (row.count + kStripBlocks<DT> - 1) / kStripBlocks<DT>;
 #pragma clang loop unroll(disable)
-    for (uint32_t t = 0;;) {
-        const float m = largest(x);
-        top = fmaxf(top, m);
-        // how far the lane's largest is from the window's top
-        int code = kFar;
-        if (m > w.high) code = 0;
-        else if (m >= w.low) code = 1 + ((w.top - binned(m, per).bin) >> 2);
-        far[t][threadIdx.x] = (uint8_t)code;
+    for (uint32_t t = 0; t < strips; t++) {
+        float ahead[kStrip];
+        read_strip<DT>(row, 0, row.count, t + 1, ahead);
+        if ((t & 1) || t + 1 == strips) {
+            int code = kFar;
+            if (most > w.high) code = 0;
+            else if (most >= w.low) code = 1 + ((w.top - binned(most, per).bin) >> 2);
+            far[t >> 1][threadIdx.x] = (uint8_t)code;
+            most = -INFINITY;
+        }
         add_to_ring(sh, x, per, [&](float v) { return v >= w.low && v <= w.high; });
-        if (++t * kStep >= row.count) break;
-        read_tile<DT>(row, 0, row.count, t, x);
+#pragma unroll
+        for (int e = 0; e < kStrip; e++) x[e] = ahead[e];
+        const float m = largest(x);
+        most = fmaxf(most, m);
+        top = fmaxf(top, m);
     }
     top = top_of(sh, top);
     if (top == -INFINITY) {
         give_first(s, r, ~0ull);
         return;
     }
-    bool listed = has_bins(top, per);
-    if (listed) {
+    bool done = has_bins(top, per);
+    if (done) {
         const int bin = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
         if (top > w.high) {
             const int past = bins ? bin - w.top : kRing;
-            if (past >= kRing) {
-                clear_ring(sh);
-            } else if ((int)threadIdx.x < past) {
-                uint64_t* p = &sh.ring[((bin - (int)threadIdx.x) & (kRing - 1)) * kCopies];
-#pragma unroll
-                for (int i = 0; i < kCopies; i++) p[i] = 0;
+            for (int i = threadIdx.x; i < past && i < kRing; i += kLanes) {
+                uint64_t* p = &sh.ring[((bin - i) & (kRing - 1)) * kCopies];
+#pragma unroll 1
+                for (int c = 0; c < kCopies; c++) p[c] = 0;
             }
             __syncthreads();
-            const float low = (float)((bin - (kLow - 1)) / per);
+            const float low = uniform((float)((bin - (kLow - 1)) / per));
 #pragma clang loop unroll(disable)
-            for (uint32_t t = 0; t * kStep < row.count; t++) {
-                if (far[t][threadIdx.x]) continue;
-                read_tile<DT>(row, 0, row.count, t, x);
+            for (uint32_t t = 0; t < strips; t++) {
+                if (far[t >> 1][threadIdx.x]) continue;
+                read_strip<DT>(row, 0, row.count, t, x);
                 add_to_ring(sh, x, per, [&](float v) { return v > w.high && v >= low; });
             }
             __syncthreads();
@@ -959,27 +1055,24 @@ __global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uin
         uint32_t count;
         uint64_t rest;
         read_ring(sh, bin, &count, &rest);
-        make_plan(sh, rules, top, per, count, rest);
-        const Plan plan = sh.plan;
-        listed = plan.listed && plan.listed <= kList;
-        if (listed) {
-            if (threadIdx.x == 0) sh.listed = 0;
-            __syncthreads();
-            const float low = (float)((bin - last_needed(plan) - 1) / per);
-            const int most = bins ? 1 + ((w.top - bin + last_needed(plan)) >> 2) : 0;
+        done = finish<DT>(sh, s, r, rules, per, top, count, rest, [&](const Ask& ask) {
+            const float low = uniform((float)((bin - ask.hi - 1) / per));
+            const int near = bins ? 1 + ((w.top - bin + ask.hi) >> 2) : 0;
 #pragma clang loop unroll(disable)
-            for (uint32_t t = 0; t * kStep < row.count; t++) {
-                const int code = far[t][threadIdx.x];
-                if (code && code > most) continue;
-                read_tile<DT>(row, 0, row.count, t, x);
-                list_near(sh, plan, bin, low, per, x,
-                          [&](int e) { return index_in<DT>(row, 0, t, e); });
+            for (uint32_t t = 0; t < strips; t++) {
+                const int code = far[t >> 1][threadIdx.x];
+                if (code && code > near) continue;
+                float v[kStrip];
+                read_strip<DT>(row, 0, row.count, t, v);
+#pragma unroll
+                for (int e = 0; e < kStrip; e++)
+                    if (v[e] >= low)
+                        answer(sh, ask, bin, per, v[e], index_in<DT>(row, 0, t, e));
             }
-            __syncthreads();
-            draw(sh, s, r, rules, per, sh.listed < kList ? sh.listed : kList);
-        }
+        });
     }
-    if (!listed) draw_slowly<DT>(sh.slow, s, r, rules, top);
+    __syncthreads();
+    if (!done) draw_slowly<DT>(sh.slow, s, r, rules, top);
 }
 
 // Longer rows, and too few rows to fill the chip: a workgroup a part of up to one tile.
@@ -1033,14 +1126,15 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
     const uint32_t begin = begin_of(part), end = begin_of(part + 1);
     const size_t slot0 = (size_t)local * p.parts, slot = slot0 + part;
     const double per = bins_per(rules);
-    float x[kTile];
     if (rules.greedy) {
         const uint64_t least = least_of(sh, least_in<DT>(row, begin, end));
         if (threadIdx.x == 0) put(p.least + slot, least);
     } else {
-        read_tile<DT>(row, begin, end, 0, x);
-        clear_ring(sh);
-        const float most = largest(x);
+        float x[kStrip], y[kStrip];
+        read_strip<DT>(row, begin, end, 0, x);
+        read_strip<DT>(row, begin, end, 1, y);
+        clear_scratch(sh);
+        const float most = fmaxf(largest(x), largest(y));
         const float top = top_of(sh, most);
         if (threadIdx.x == 0) put(p.tops + slot, top);
         if (top > -INFINITY && has_bins(top, per)) {
@@ -1049,7 +1143,13 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
             int code = kFar;
             if (most >= w.low) code = (w.top - binned(most, per).bin) >> 2;
             put(p.far + slot * kLanes + threadIdx.x, (uint8_t)code);
-            add_to_ring(sh, x, per, [&](float v) { return v >= w.low; });
+            const int strips = end - begin > kStripBlocks<DT> ? 2 : 1;
+#pragma clang loop unroll(disable)
+            for (int t = 0; t < strips; t++) {
+                add_to_ring(sh, x, per, [&](float v) { return v >= w.low; });
+#pragma unroll
+                for (int e = 0; e < kStrip; e++) x[e] = y[e];
+            }
             __syncthreads();
             uint32_t count;
             uint64_t rest;
@@ -1087,8 +1187,8 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
         give_first(s, r, ~0ull);
         return;
     }
-    bool listed = has_bins(top, per) && !sh.listed;
-    if (listed) {
+    bool done = has_bins(top, per) && !sh.listed;
+    if (done) {
         const int big = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
         const int bin = big - (int)threadIdx.x;
         uint32_t count = 0;
@@ -1096,48 +1196,46 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
 #pragma clang loop unroll(disable)
         for (uint32_t i = 0; i < p.parts; i += kBatch) {
             uint64_t v[kBatch];
-            const uint64_t* ring = p.rings + (slot0 + i) * kRing + (bin & (kRing - 1));
+            uint64_t* ring = p.rings + (slot0 + i) * kRing + (bin & (kRing - 1));
 #pragma unroll
             for (int j = 0; j < kBatch; j++) {
-                const bool has = i + j < p.parts && bins[i + j] - bin >= 0 &&
-                                 bins[i + j] - bin < kRing;
-                v[j] = has ? get(const_cast<uint64_t*>(ring) + (size_t)j * kRing) : 0;
+                const int below = i + j < p.parts ? bins[i + j] - bin : -1;
+                v[j] = below >= 0 && below < kRing ? get(ring + (size_t)j * kRing) : 0;
             }
 #pragma unroll
             for (int j = 0; j < kBatch; j++) {
                 count += (uint32_t)(v[j] >> kCount);
-                rest += v[j] & ((1ull << kCount) - 1);
+                rest += v[j] & kRest;
             }
         }
-        make_plan(sh, rules, top, per, count, rest);
-        const Plan plan = sh.plan;
-        listed = plan.listed && plan.listed <= kList;
-        if (listed) {
-            const float low = (float)((big - last_needed(plan) - 1) / per);
-            const int below = big - last_needed(plan);
+        done = finish<DT>(sh, s, r, rules, per, top, count, rest, [&](const Ask& ask) {
+            const float low = uniform((float)((big - ask.hi - 1) / per));
+            const int below = big - ask.hi;
 #pragma clang loop unroll(disable)
             for (uint32_t i = 0; i < p.parts; i += kBatch) {
-                uint32_t look = 0;
+                uint32_t near = 0;
 #pragma unroll
                 for (int j = 0; j < kBatch; j++) {
-                    if (i + j >= p.parts || bins[i + j] < below) continue;
+                    const int b = i + j < p.parts ? bins[i + j] : -kNone;
+                    if (b < below) continue;
                     const int code = get(p.far + (slot0 + i + j) * kLanes + threadIdx.x);
-                    look |= bins[i + j] - 4 * code >= below ? 1u << j : 0u;
+                    near |= b - 4 * code >= below ? 3u << 2 * j : 0u;
                 }
-                while (look) {
-                    const uint32_t at = i + __builtin_ctz(look);
-                    look &= look - 1;
-                    read_tile<DT>(row, begin_of(at), begin_of(at + 1), 0, x);
-                    list_near(sh, plan, big, low, per, x, [&](int e) {
-                        return index_in<DT>(row, begin_of(at), 0, e);
-                    });
+                while (near) {
+                    const uint32_t at = __builtin_ctz(near), first = begin_of(i + (at >> 1));
+                    near &= near - 1;
+                    float v[kStrip];
+                    read_strip<DT>(row, first, begin_of(i + (at >> 1) + 1), at & 1, v);
+#pragma unroll
+                    for (int e = 0; e < kStrip; e++)
+                        if (v[e] >= low)
+                            answer(sh, ask, big, per, v[e], index_in<DT>(row, first, at & 1, e));
                 }
             }
-            __syncthreads();
-            draw(sh, s, r, rules, per, sh.listed < kList ? sh.listed : kList);
-        }
+        });
     }
-    if (!listed) draw_slowly<DT>(sh.slow, s, r, rules, top);
+    __syncthreads();
+    if (!done) draw_slowly<DT>(sh.slow, s, r, rules, top);
 }
 
 template <int DT>
