@@ -75,7 +75,7 @@ __device__ __forceinline__ Rules rules_of(const Sampling& s, uint32_t row) {
     return r;
 }
 
-constexpr int kLanes = 1024, kWaves = kLanes / 64;
+constexpr int kLanes = 512, kWaves = kLanes / 64;
 constexpr int kDigit = 11, kBins = 1 << kDigit;
 
 struct RowScratch {
@@ -109,7 +109,7 @@ struct Weigher {
 template <typename F>
 __device__ __forceinline__ uint32_t find_bin(RowScratch& sh, uint64_t mass0, uint32_t count0,
                                              F crosses) {
-    constexpr int kPer = kBins / kLanes;
+    constexpr int kPer = kBins / kLanes;      // digits a lane
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) sh.first = 0xffffffffu, sh.last = 0;
     uint64_t mass = 0;
@@ -249,7 +249,8 @@ __device__ uint32_t index_of(const void* row, uint32_t width, uint32_t key, uint
 
 // ---- the histogram ------------------------------------------------------------
 
-constexpr int kRing = 1024;            // bins of the ring: a lane each
+constexpr int kRing = 1024;            // bins of the ring
+constexpr int kPer = kRing / kLanes;   // consecutive ones a lane
 constexpr int kCopies = 8;             // of each bin's word, for lanes that meet in it
 constexpr int kReach = 736;            // bins below the largest's that count
 constexpr int kFew = 64;               // logits that a wave puts in order
@@ -368,6 +369,20 @@ __device__ __forceinline__ void read_strip(const Blocks<DT>& row, uint32_t first
             for (int e = 0; e < E; e++) x[q * E + e] = -INFINITY;
     }
 }
+// Those of strips t and t + 1.
+template <int DT>
+__device__ __forceinline__ void read_tile(const Blocks<DT>& row, uint32_t first, uint32_t last,
+                                          uint32_t t, float (&x)[2 * kStrip]) {
+    constexpr int E = Blocks<DT>::kEach;
+#pragma unroll
+    for (int q = 0; q < 2 * kStrip / E; q++) {
+        const uint32_t b = first + t * kStripBlocks<DT> + q * kLanes + threadIdx.x;
+        if (b < last) row.read(b, x + q * E);
+        else
+#pragma unroll
+            for (int e = 0; e < E; e++) x[q * E + e] = -INFINITY;
+    }
+}
 template <int DT>
 __device__ __forceinline__ uint32_t index_in(const Blocks<DT>& row, uint32_t first, uint32_t t,
                                              int e) {
@@ -381,7 +396,7 @@ __device__ __forceinline__ float largest(const float (&x)[kStrip]) {
     return m;
 }
 
-constexpr int kFirsts = 24;
+constexpr int kFirsts = 24;            // searches of a row: 7, and up to 4 a border
 struct Scratch {
     union {
         uint64_t ring[kRing * kCopies + kCopies];      // the last: logits of no bin
@@ -397,8 +412,8 @@ struct Scratch {
     double wave_mass[kWaves];
     uint32_t wave_count[kWaves];
     float wave_top[kWaves];
-    int first[kFirsts];                // a search's each, none found yet
-    uint32_t listed, planned, least, most, last;
+    int first[kFirsts][kWaves];        // a search's each
+    uint32_t listed, least, most, last;
     double kept, weight;               // what a wave found
     uint32_t kept_count, token;
 };
@@ -407,8 +422,6 @@ __device__ __forceinline__ void clear_scratch(Scratch& sh) {
 #pragma unroll
     for (int i = 0; i < kRing * kCopies / 2 / kLanes; i++)
         p[i * kLanes + threadIdx.x] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x < kFirsts) sh.first[threadIdx.x] = 0x7fffffff;
-    if (threadIdx.x == 0) sh.planned = 0;
 }
 
 __device__ __forceinline__ float top_of(Scratch& sh, float m) {
@@ -456,56 +469,93 @@ __device__ __forceinline__ void add_to_ring(Scratch& sh, const float (&x)[kStrip
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 }
-// This lane's bin, so many below top: its copies' sum.
-__device__ __forceinline__ void read_ring(const Scratch& sh, int top, uint32_t* count,
-                                          uint64_t* rest) {
-    const uint64_t* p = &sh.ring[((top - (int)threadIdx.x) & (kRing - 1)) * kCopies];
-    *count = 0, *rest = 0;
+// A lane's bins: how many logits, and the rest of their weights.
+struct Bins {
+    uint32_t count[kPer];
+    uint64_t rest[kPer];
+};
+// Those so many below top, from the ring: the copies' sums.
+__device__ __forceinline__ Bins read_ring(const Scratch& sh, int top) {
+    Bins b;
 #pragma unroll
-    for (int i = 0; i < kCopies; i++) {
-        *count += (uint32_t)(p[i] >> kCount);
-        *rest += p[i] & kRest;
+    for (int j = 0; j < kPer; j++) {
+        const int bin = top - (int)(threadIdx.x * kPer) - j;
+        const uint64_t* p = &sh.ring[(bin & (kRing - 1)) * kCopies];
+        b.count[j] = 0, b.rest[j] = 0;
+#pragma unroll
+        for (int i = 0; i < kCopies; i++) {
+            b.count[j] += (uint32_t)(p[i] >> kCount);
+            b.rest[j] += p[i] & kRest;
+        }
     }
+    return b;
 }
 
 // ---- the borders ----------------------------------------------------------------
 
-// The first lane for which it holds, or `none`, N questions at once; all lanes call it.
+// The first bin for which it holds, or `none`, N questions at once; all lanes call it,
+// each time for another place of sh.first.  (A word a wave: an atomic minimum would be a
+// loop over the lanes.)
 template <int N>
-__device__ __forceinline__ void first_lanes(Scratch& sh, int& next, const bool (&is)[N], int none,
-                                            int (&at)[N]) {
+__device__ __forceinline__ void first_bins(Scratch& sh, int& next, const bool (&is)[N][kPer],
+                                           int none, int (&at)[N]) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const uint64_t b = __ballot(is[i]);
-        if (b && (threadIdx.x & 63) == 0)
-            atomicMin(&sh.first[next + i], (int)threadIdx.x + (int)__builtin_ctzll(b));
+        int mine = kRing;
+#pragma unroll
+        for (int j = kPer - 1; j >= 0; j--) mine = is[i][j] ? (int)threadIdx.x * kPer + j : mine;
+        const uint64_t b = __ballot(mine < kRing);
+        const int first = __builtin_amdgcn_readlane(mine, b ? (int)__builtin_ctzll(b) : 0);
+        if (lane == 0) sh.first[next + i][threadIdx.x >> 6] = first;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int x = __builtin_amdgcn_readfirstlane(sh.first[next + i]);
+        int x = sh.first[next + i][lane & (kWaves - 1)];
+#pragma unroll
+        for (int d = kWaves / 2; d; d >>= 1) {
+            const int o = __shfl_xor(x, d, 64);
+            x = o < x ? o : x;
+        }
+        x = __builtin_amdgcn_readfirstlane(x);
         at[i] = x < none ? x : none;
     }
     next += N;
 }
 
-// Sums over the workgroup's lanes up to and with this one.
-__device__ __forceinline__ void sums_upto(Scratch& sh, double& mass, uint32_t& count) {
+// Sums over bins up to and with each of this lane's.
+struct Sums {
+    double mass[kPer];
+    uint32_t count[kPer];
+};
+__device__ __forceinline__ void sums_upto(Scratch& sh, Sums& x) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const double m = __shfl_up(mass, x, 64);
-        const uint32_t c = __shfl_up(count, x, 64);
-        if (lane >= x) mass += m, count += c;
+    for (int j = 1; j < kPer; j++) x.mass[j] += x.mass[j - 1], x.count[j] += x.count[j - 1];
+    const double own = x.mass[kPer - 1];
+    const uint32_t own_count = x.count[kPer - 1];
+    double mass = own;
+    uint32_t count = own_count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double m = __shfl_up(mass, d, 64);
+        const uint32_t c = __shfl_up(count, d, 64);
+        if (lane >= d) mass += m, count += c;
     }
     if (lane == 63) sh.wave_mass[wave] = mass, sh.wave_count[wave] = count;
+    // the lanes before this one, not this sum less the lane's own: that would be rounded
+    double before = __shfl_up(mass, 1, 64);
+    uint32_t before_count = __shfl_up(count, 1, 64);
+    if (lane == 0) before = 0, before_count = 0;
     __syncthreads();
-    double before = 0;
-    uint32_t before_count = 0;
+    double waves = 0;
+    uint32_t waves_count = 0;
 #pragma unroll 1
-    for (int w = 0; w < wave; w++) before += sh.wave_mass[w], before_count += sh.wave_count[w];
-    mass += before;
-    count += before_count;
+    for (int w = 0; w < wave; w++) waves += sh.wave_mass[w], waves_count += sh.wave_count[w];
+    before += waves, before_count += waves_count;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) x.mass[j] += before, x.count[j] += before_count;
 }
 
 // Place in the order, ascending.
@@ -524,19 +574,36 @@ __device__ __forceinline__ int part_of(double r) {
     const int p = (int)((0.5 - r) * kRing);
     return p < 0 ? 0 : p < kRing ? p : kRing - 1;
 }
-__device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, double per, float x,
-                                       uint32_t index) {
-    const Binned b = binned(x, per);
-    const int d = top - b.bin;
-    if (d < ask.lo || d > ask.hi || (ask.joint && !sh.near[d])) return;
-    if (ask.fine) {
-        atomicAdd((unsigned long long*)&sh.fine[part_of(b.r)], (unsigned long long)b.word);
-    } else if (ask.part < 0 || part_of(b.r) == ask.part) {
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kFew) sh.list[at] = placed(x, index);
-        const uint32_t key = key_of(x);
-        atomicMin(&sh.least, key);
-        atomicMax(&sh.most, key);
+// A lane's logits x, none of a near bin below low: those that are asked for.
+template <typename F>
+__device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, double per, float low,
+                                       const float (&x)[2 * kStrip], F index) {
+    uint32_t some = 0;
+#pragma unroll
+    for (int e = 0; e < 2 * kStrip; e++) some |= x[e] >= low ? 1u << e : 0u;
+    // one at a time, so that the code is there once
+#pragma unroll 1
+    while (some) {
+        const int e = __builtin_ctz(some);
+        some &= some - 1;
+        float v = x[0];
+#pragma unroll
+        for (int i = 1; i < 2 * kStrip; i++) v = e == i ? x[i] : v;
+        const Binned b = binned(v, per);
+        const int d = top - b.bin;
+        if (d < ask.lo || d > ask.hi || (ask.joint && !sh.near[d])) continue;
+        const int part = part_of(b.r);
+        if (ask.fine) {
+            atomicAdd((unsigned long long*)&sh.fine[part], (unsigned long long)b.word);
+        } else if (ask.part < 0 || part == ask.part) {
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            if (at < kFew) {
+                sh.list[at] = placed(v, index(e));
+            } else {
+                atomicMin(&sh.least, key_of(v));
+                atomicMax(&sh.most, key_of(v));
+            }
+        }
     }
 }
 
@@ -595,14 +662,14 @@ struct Left {
     uint32_t count;
 };
 
-// The token of a row, from each lane's bin (so many below the largest's): its logits and
-// the rest of their weights.  look(ask) goes over the row's logits.  False where the
-// borders' bins hold too much.
+// The token of a row, from each lane's bins, so many below the largest's.  look(ask) goes
+// over the row's logits.  False where a border's bin holds too much.
 template <int DT, typename L>
 __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t row,
-                                       const Rules& rules, double per, float top, uint32_t count,
-                                       uint64_t rest, L look) {
-    const int d = threadIdx.x;
+                                       const Rules& rules, double per, float top, const Bins& own,
+                                       L look) {
+    const int first = threadIdx.x * kPer;
+    const bool leads = threadIdx.x == 0;
     const Binned big = binned(top, per);
     const int top_bin = __builtin_amdgcn_readfirstlane(big.bin);
     const uint64_t one_units = units_of(big);
@@ -613,78 +680,98 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
         const int q = (int)rint((double)u / one);
         return q + (double)((int64_t)u - (int64_t)q * (int64_t)one_units) / one;
     };
-    const double scale = two_to(d);
-    if (d >= kReach) count = 0, rest = 0;
-    double mass = count ? share(units(count, rest)) * scale : 0.0;
-    uint32_t upto_count = count;
+    Sums upto;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        const bool some = first + j < kReach && own.count[j];
+        upto.count[j] = some ? own.count[j] : 0u;
+        upto.mass[j] = some ? share(units(own.count[j], own.rest[j])) * two_to(first + j) : 0.0;
+    }
     // every lane has read the ring when its place is taken
-    sums_upto(sh, mass, upto_count);
-    sh.mass[d] = mass;
-    sh.count[d] = upto_count;
+    sums_upto(sh, upto);
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        sh.mass[first + j] = upto.mass[j];
+        sh.count[first + j] = upto.count[j];
+    }
     __syncthreads();
     const auto mass_before = [&](int b) { return b > 0 ? sh.mass[b - 1] : 0.0; };
     const auto count_before = [&](int b) { return b > 0 ? sh.count[b - 1] : 0u; };
     const double all = uniform(sh.mass[kRing - 1]);
     const uint32_t all_count = __builtin_amdgcn_readfirstlane(sh.count[kRing - 1]);
-    // the least weight that a bin of this lane's may hold
+    // the least weight that a bin may hold, as a share of two_to
     const double edge = uniform(sixteenth_of(-0.5, 1.0) * sixteenth_of(-big.r, 1.0));
     const bool by_k = rules.top_k < all_count, by_p = rules.top_p < 1, by_m = rules.min_p > 0;
     int next = 0;
-
-    // Where the borders may lie.  What one leaves of its bin is not known yet, so a sum
-    // behind it is between two, and the next border's bin with it.
+    const auto first_one = [&](auto holds, int none) {
+        bool is[1][kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) is[0][j] = holds(j);
+        int at[1];
+        first_bins<1>(sh, next, is, none, at);
+        return at[0];
+    };
     struct Span {
         int lo, hi;
     };
+    const auto first_two = [&](auto lo_holds, auto hi_holds, int none) {
+        bool is[2][kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; j++) is[0][j] = lo_holds(j), is[1][j] = hi_holds(j);
+        int at[2];
+        first_bins<2>(sh, next, is, none, at);
+        return Span{at[0], at[1]};
+    };
+
+    // Where the borders may lie.  What one leaves of its bin is not known yet, so a sum
+    // behind it is between two, and the next border's bin with it.
     Span k = {0, -1}, p = {0, -1}, m = {0, -1}, u;
     double lo = all, hi = all;
-    int end, last;
-    {
-        const bool is[2] = {upto_count >= rules.top_k, upto_count >= all_count};
-        int at[2];
-        first_lanes<2>(sh, next, is, kRing - 1, at);
-        end = last = at[1];             // the last that holds any
-        if (by_k) {
-            end = at[0];
-            k = {end, end};
-            lo = mass_before(end), hi = sh.mass[end];
-        }
+    u = first_two([&](int j) { return upto.count[j] >= rules.top_k; },
+                  [&](int j) { return upto.count[j] >= all_count; }, kRing - 1);
+    const int last = u.hi;              // the last that holds any
+    int end = last;
+    if (by_k) {
+        end = u.lo;
+        k = {end, end};
+        lo = uniform(mass_before(end)), hi = uniform(sh.mass[end]);
     }
     if (by_p) {
-        const bool is[2] = {mass >= rules.top_p * lo, mass >= rules.top_p * hi};
-        int at[2];
-        first_lanes<2>(sh, next, is, end, at);
-        p = {at[0], at[1]};
-        lo = mass_before(p.lo), hi = sh.mass[p.hi];
+        p = first_two([&](int j) { return upto.mass[j] >= rules.top_p * lo; },
+                      [&](int j) { return upto.mass[j] >= rules.top_p * hi; }, end);
+        lo = uniform(mass_before(p.lo)), hi = uniform(sh.mass[p.hi]);
         end = p.hi;
     }
     if (by_m) {
-        const bool is[1] = {scale * edge < rules.min_p};
-        int at[1];
-        first_lanes<1>(sh, next, is, kRing, at);
-        if (at[0] <= end) {
-            end = at[0];
+        const int at = first_one(
+            [&](int j) { return two_to(first + j) * edge < rules.min_p; }, kRing);
+        if (at <= end) {
+            end = at;
             m = {end, end};
-            lo = fmin(lo, mass_before(end)), hi = fmin(hi, sh.mass[end]);
+            lo = uniform(fmin(lo, mass_before(end))), hi = uniform(fmin(hi, sh.mass[end]));
         }
     }
-    {
-        const bool is[2] = {mass > rules.u * lo, mass > rules.u * hi};
-        int at[2];
-        first_lanes<2>(sh, next, is, end, at);
-        u = {at[0], at[1]};
+    u = first_two([&](int j) { return upto.mass[j] > rules.u * lo; },
+                  [&](int j) { return upto.mass[j] > rules.u * hi; }, end);
+    const auto in = [](const Span& x, int b) { return b >= x.lo && b <= x.hi; };
+    uint32_t planned = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+        const int b = first + j;
+        const bool near = in(k, b) || in(p, b) || in(m, b) || in(u, b);
+        sh.near[b] = near;
+        planned += near ? sh.count[b] - count_before(b) : 0u;
     }
-    const auto in = [&](const Span& x) { return d >= x.lo && d <= x.hi; };
-    const bool near = in(k) || in(p) || in(m) || in(u);
-    sh.near[d] = near;
-    uint32_t planned = near ? count : 0;
 #pragma unroll
     for (int x = 32; x; x >>= 1) planned += __shfl_xor(planned, x, 64);
-    if ((d & 63) == 0 && planned) atomicAdd(&sh.planned, planned);
-    if (d == 0) sh.listed = 0, sh.least = ~0u, sh.most = 0;
+    if ((threadIdx.x & 63) == 0) sh.wave_count[threadIdx.x >> 6] = planned;
+    if (leads) sh.listed = 0, sh.least = ~0u, sh.most = 0;
     __syncthreads();
+    planned = sh.wave_count[threadIdx.x & (kWaves - 1)];
+#pragma unroll
+    for (int x = kWaves / 2; x; x >>= 1) planned += __shfl_xor(planned, x, 64);
     Ask ask;
-    ask.joint = sh.planned <= kFew;
+    ask.joint = (uint32_t)__builtin_amdgcn_readfirstlane(planned) <= kFew;
     ask.fine = false;
     ask.part = -1;
     ask.lo = 0;
@@ -697,67 +784,79 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
     double base = 0;
     uint32_t base_count = 0;
     for (;;) {
+        const double border = uniform((stage == kByP ? rules.top_p : rules.u) * left.sum);
+        // whether a sum, or the least weight there, is past the stage's border
+        const auto past = [&](double mass, uint32_t count, double least) {
+            return stage == kByK   ? count >= rules.top_k
+                   : stage == kByP ? mass >= border
+                   : stage == kByM ? least < rules.min_p
+                                   : mass > border;
+        };
         if (!ask.joint && ask.part < 0) {
             // the next border's bin
-            while ((stage == kByK && !by_k) || (stage == kByP && !by_p) || (stage == kByM && !by_m))
-                stage++;
-            const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
-            const bool is[1] = {stage == kByK   ? upto_count >= rules.top_k
-                                : stage == kByP ? mass >= border
-                                : stage == kByM ? scale * edge < rules.min_p
-                                                : mass > border};
-            int at[1];
-            first_lanes<1>(sh, next, is, stage == kByM ? kRing : end, at);
-            if (stage == kByM && at[0] > end) {
+            if ((stage == kByK && !by_k) || (stage == kByP && !by_p) || (stage == kByM && !by_m)) {
                 stage++;
                 continue;
             }
-            ask.lo = ask.hi = at[0];
-            base = uniform(mass_before(at[0]));
-            base_count = __builtin_amdgcn_readfirstlane(count_before(at[0]));
-            const uint32_t here = sh.count[at[0]] - base_count;
+            const int at = first_one(
+                [&](int j) {
+                    return past(sh.mass[first + j], sh.count[first + j], two_to(first + j) * edge);
+                },
+                stage == kByM ? kRing : end);
+            if (stage == kByM && at > end) {
+                stage++;
+                continue;
+            }
+            ask.lo = ask.hi = at;
+            base = uniform(mass_before(at));
+            base_count = __builtin_amdgcn_readfirstlane(count_before(at));
+            const uint32_t here = __builtin_amdgcn_readfirstlane(sh.count[at]) - base_count;
             if (here > kMostEach) return false;
             ask.fine = here > kFew;
-            if (ask.fine) sh.fine[d] = 0;
-            if (d == 0) sh.listed = 0, sh.least = ~0u, sh.most = 0;
+#pragma unroll
+            for (int j = 0; j < kPer; j++) sh.fine[first + j] = 0;
+            if (leads) sh.listed = 0, sh.least = ~0u, sh.most = 0;
             __syncthreads();
         }
         look(ask);
         __syncthreads();
         if (ask.fine) {
             // the 1024th that holds the border
-            const uint64_t word = sh.fine[d];
-            uint32_t c = (uint32_t)(word >> kCount);
-            double mm = c ? share(units(c, word & kRest)) * two_to(ask.lo) : 0.0;
-            const double own = mm;
-            const uint32_t own_count = c;
-            sums_upto(sh, mm, c);
-            mm += base, c += base_count;
-            const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
-            const double below = two_to(ask.lo) * sixteenth_of(-big.r, 1.0) *
-                                 sixteenth_of(0.5 - (d + 1) * (1.0 / kRing), 1.0);
-            const bool is[2] = {own_count && (stage == kByK   ? c >= rules.top_k
-                                              : stage == kByP ? mm >= border
-                                              : stage == kByM ? below < rules.min_p
-                                                              : mm > border),
-                                c >= sh.count[ask.lo]};
-            int at[2];
-            first_lanes<2>(sh, next, is, kRing - 1, at);
-            const int part = at[0] < at[1] ? at[0] : at[1];
-            if (d == part) {
-                sh.kept = mm - own, sh.kept_count = c - own_count;
-                sh.listed = 0, sh.least = ~0u, sh.most = 0;
+            Sums x;
+            uint32_t c[kPer];
+            double w[kPer], least[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                const uint64_t word = sh.fine[first + j];
+                c[j] = x.count[j] = (uint32_t)(word >> kCount);
+                w[j] = x.mass[j] =
+                    c[j] ? share(units(c[j], word & kRest)) * two_to(ask.lo) : 0.0;
+                least[j] = two_to(ask.lo) * sixteenth_of(-big.r, 1.0) *
+                           sixteenth_of(0.5 - (first + j + 1) * (1.0 / kRing), 1.0);
             }
+            sums_upto(sh, x);
+#pragma unroll
+            for (int j = 0; j < kPer; j++) x.mass[j] += base, x.count[j] += base_count;
+            const uint32_t whole = __builtin_amdgcn_readfirstlane(sh.count[ask.lo]);
+            const Span at = first_two(
+                [&](int j) { return c[j] && past(x.mass[j], x.count[j], least[j]); },
+                [&](int j) { return x.count[j] >= whole; }, kRing - 1);
+            ask.part = at.lo < at.hi ? at.lo : at.hi;
+#pragma unroll
+            for (int j = 0; j < kPer; j++)
+                if (first + j == ask.part) {
+                    sh.kept = x.mass[j] - w[j], sh.kept_count = x.count[j] - c[j];
+                    sh.listed = 0, sh.least = ~0u, sh.most = 0;
+                }
             __syncthreads();
             base = uniform(sh.kept);
             base_count = __builtin_amdgcn_readfirstlane(sh.kept_count);
-            ask.part = part;
             ask.fine = false;
             continue;
         }
-        const uint32_t n = sh.listed;
+        const uint32_t n = __builtin_amdgcn_readfirstlane(sh.listed);
         if (ask.joint) {
-            if (d < 64) {
+            if (threadIdx.x < 64) {
                 const Listed l = in_order(sh, n, top_bin, per, one, [&](Listed& x) {
                     const int b = x.bin < kRing ? x.bin : 0;
                     x.upto += mass_before(b);
@@ -786,7 +885,7 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
                 int at = find(u, l.upto > rules.u * left.sum);
                 // sums of bins and of their logits are rounded apart
                 while (at && (uint32_t)__builtin_amdgcn_readlane(l.rank, at) > left.count) at--;
-                if (d == 0) {
+                if (leads) {
                     sh.token = __builtin_amdgcn_readlane(l.token, at);
                     sh.weight = lane_of(l.weight, at);
                     sh.kept = left.sum;
@@ -794,26 +893,22 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
             }
             break;
         }
-        const double border = (stage == kByP ? rules.top_p : rules.u) * left.sum;
-        const uint32_t most = sh.most;
         if (n <= kFew) {
-            if (d < 64) {
+            if (threadIdx.x < 64) {
                 const Listed l = in_order(sh, n, top_bin, per, one, [&](Listed& x) {
                     x.upto += base;
                     x.rank += base_count;
                 });
                 const uint64_t hit = __ballot(
-                    d < (int)n && (stage == kByK   ? l.rank >= rules.top_k
-                                   : stage == kByP ? l.upto >= border
-                                   : stage == kByM ? !(l.weight >= rules.min_p)
-                                                   : l.upto > border || l.rank == left.count));
+                    threadIdx.x < n && (past(l.upto, l.rank, l.weight) ||
+                                        (stage == kByU && l.rank == left.count)));
                 int at = hit ? (int)__builtin_ctzll(hit) : (int)n - 1;
                 double upto = base;
                 uint32_t rank = base_count;
                 // the first that is too light goes with those behind it
                 if (stage == kByM && hit) at--;
                 if (at >= 0) upto = lane_of(l.upto, at), rank = __builtin_amdgcn_readlane(l.rank, at);
-                if (d == 0) {
+                if (leads) {
                     sh.kept = upto, sh.kept_count = rank;
                     sh.token = __builtin_amdgcn_readlane(l.token, at < 0 ? 0 : at);
                     sh.weight = lane_of(l.weight, at < 0 ? 0 : at);
@@ -821,7 +916,9 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
             }
         } else {
             // equal logits: so many of them
-            if (sh.least != most) return false;
+            const uint32_t most = __builtin_amdgcn_readfirstlane(sh.most);
+            const bool odd = ~(uint32_t)(sh.list[threadIdx.x & (kFew - 1)] >> 32) != most;
+            if (sh.least != most || first_one([&](int) { return odd; }, kRing) != kRing) return false;
             const Binned b = binned(value_of(most), per);
             const double w = (double)units_of(b) / one * two_to(top_bin - b.bin);
             uint32_t take = stage == kByK ? rules.top_k - base_count : 0;
@@ -835,12 +932,12 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
                 const void* at = static_cast<const char*>(s.logits) +
                                  (size_t)row * s.width * (DT == ACCEL_F32 ? 4 : 2);
                 const uint32_t token = index_of<DT>(at, s.width, most, take ? take - 1 : 0, sh.slow);
-                if (d == 0) sh.token = token;
+                if (leads) sh.token = token;
             }
-            if (d == 0) sh.kept = base + take * w, sh.kept_count = base_count + take, sh.weight = w;
+            if (leads) sh.kept = base + take * w, sh.kept_count = base_count + take, sh.weight = w;
         }
         if (stage == kByU) {
-            if (d == 0) sh.kept = left.sum;
+            if (leads) sh.kept = left.sum;
             break;
         }
         __syncthreads();
@@ -853,7 +950,7 @@ __device__ __forceinline__ bool finish(Scratch& sh, const Sampling& s, uint32_t 
         ask.part = -1;
         __syncthreads();
     }
-    if (d == 0) {
+    if (leads) {
         s.tokens[row] = sh.token;
         if (s.logprobs) s.logprobs[row] = (float)log(sh.weight / sh.kept);
     }
@@ -980,14 +1077,14 @@ __device__ __forceinline__ void give_first(const Sampling& s, uint32_t row, uint
 // Rows of up to kTiles tiles, a workgroup each, two workgroups a CU.  Of each tile of a
 // lane it is kept how far its largest logit is from the window's top, so a second look
 // goes only to what may hold something near a border.
-constexpr int kTiles = 8;
+constexpr int kTiles = 16;
 constexpr int kTile = 2 * kStrip;
 constexpr int kFar = 255;              // below the window; nearer ones are 253 at most
 static_assert(kTiles * kTile * kLanes / kCopies <= kMostEach, "a word's count and sum");
 static_assert(kTile * kLanes <= kMostEach, "the same, of a part's copies together");
 
 template <int DT>
-__global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uint32_t first_row) {
+__global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uint32_t first_row) {
     __shared__ Scratch sh;
     __shared__ uint8_t far[kTiles][kLanes];
     const uint32_t r = first_row + blockIdx.x;
@@ -1052,22 +1149,17 @@ __global__ __launch_bounds__(kLanes, 8) void sample_whole_kernel(Sampling s, uin
             }
             __syncthreads();
         }
-        uint32_t count;
-        uint64_t rest;
-        read_ring(sh, bin, &count, &rest);
-        done = finish<DT>(sh, s, r, rules, per, top, count, rest, [&](const Ask& ask) {
+        done = finish<DT>(sh, s, r, rules, per, top, read_ring(sh, bin), [&](const Ask& ask) {
             const float low = uniform((float)((bin - ask.hi - 1) / per));
             const int near = bins ? 1 + ((w.top - bin + ask.hi) >> 2) : 0;
 #pragma clang loop unroll(disable)
-            for (uint32_t t = 0; t < strips; t++) {
+            for (uint32_t t = 0; t < strips; t += 2) {
                 const int code = far[t >> 1][threadIdx.x];
                 if (code && code > near) continue;
-                float v[kStrip];
-                read_strip<DT>(row, 0, row.count, t, v);
-#pragma unroll
-                for (int e = 0; e < kStrip; e++)
-                    if (v[e] >= low)
-                        answer(sh, ask, bin, per, v[e], index_in<DT>(row, 0, t, e));
+                float v[2 * kStrip];
+                read_tile<DT>(row, 0, row.count, t, v);
+                answer(sh, ask, bin, per, low, v,
+                       [&](int e) { return index_in<DT>(row, 0, t, e); });
             }
         });
     }
@@ -1113,7 +1205,7 @@ __device__ __forceinline__ bool is_last(Scratch& sh, uint32_t* ticket, uint32_t 
 }
 
 template <int DT>
-__global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Parts p) {
+__global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Parts p) {
     __shared__ Scratch sh;
     __shared__ int bins[kMostParts];
     const uint32_t local = blockIdx.x / p.parts, part = blockIdx.x - local * p.parts;
@@ -1151,11 +1243,12 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
                 for (int e = 0; e < kStrip; e++) x[e] = y[e];
             }
             __syncthreads();
-            uint32_t count;
-            uint64_t rest;
-            read_ring(sh, w.top, &count, &rest);
-            put(p.rings + slot * kRing + ((w.top - (int)threadIdx.x) & (kRing - 1)),
-                (uint64_t)count << kCount | rest);
+            const Bins b = read_ring(sh, w.top);
+#pragma unroll
+            for (int j = 0; j < kPer; j++)
+                put(p.rings + slot * kRing +
+                        ((w.top - (int)(threadIdx.x * kPer) - j) & (kRing - 1)),
+                    (uint64_t)b.count[j] << kCount | b.rest[j]);
         }
     }
     if (!is_last(sh, p.tickets + local, p.parts)) return;
@@ -1190,46 +1283,48 @@ __global__ __launch_bounds__(kLanes, 8) void sample_parts_kernel(Sampling s, Par
     bool done = has_bins(top, per) && !sh.listed;
     if (done) {
         const int big = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
-        const int bin = big - (int)threadIdx.x;
-        uint32_t count = 0;
-        uint64_t rest = 0;
+        Bins sum = {};
 #pragma clang loop unroll(disable)
         for (uint32_t i = 0; i < p.parts; i += kBatch) {
-            uint64_t v[kBatch];
-            uint64_t* ring = p.rings + (slot0 + i) * kRing + (bin & (kRing - 1));
+            uint64_t v[kBatch][kPer];
 #pragma unroll
-            for (int j = 0; j < kBatch; j++) {
-                const int below = i + j < p.parts ? bins[i + j] - bin : -1;
-                v[j] = below >= 0 && below < kRing ? get(ring + (size_t)j * kRing) : 0;
-            }
+            for (int x = 0; x < kBatch; x++)
 #pragma unroll
-            for (int j = 0; j < kBatch; j++) {
-                count += (uint32_t)(v[j] >> kCount);
-                rest += v[j] & kRest;
-            }
+                for (int j = 0; j < kPer; j++) {
+                    const int bin = big - (int)(threadIdx.x * kPer) - j;
+                    const int below = i + x < p.parts ? bins[i + x] - bin : -1;
+                    v[x][j] = below >= 0 && below < kRing
+                                  ? get(p.rings + (slot0 + i + x) * kRing + (bin & (kRing - 1)))
+                                  : 0;
+                }
+#pragma unroll
+            for (int x = 0; x < kBatch; x++)
+#pragma unroll
+                for (int j = 0; j < kPer; j++) {
+                    sum.count[j] += (uint32_t)(v[x][j] >> kCount);
+                    sum.rest[j] += v[x][j] & kRest;
+                }
         }
-        done = finish<DT>(sh, s, r, rules, per, top, count, rest, [&](const Ask& ask) {
+        done = finish<DT>(sh, s, r, rules, per, top, sum, [&](const Ask& ask) {
             const float low = uniform((float)((big - ask.hi - 1) / per));
             const int below = big - ask.hi;
 #pragma clang loop unroll(disable)
-            for (uint32_t i = 0; i < p.parts; i += kBatch) {
+            for (uint32_t i = 0; i < p.parts; i += 32) {
                 uint32_t near = 0;
 #pragma unroll
-                for (int j = 0; j < kBatch; j++) {
+                for (int j = 0; j < 32; j++) {
                     const int b = i + j < p.parts ? bins[i + j] : -kNone;
                     if (b < below) continue;
                     const int code = get(p.far + (slot0 + i + j) * kLanes + threadIdx.x);
-                    near |= b - 4 * code >= below ? 3u << 2 * j : 0u;
+                    near |= b - 4 * code >= below ? 1u << j : 0u;
                 }
                 while (near) {
-                    const uint32_t at = __builtin_ctz(near), first = begin_of(i + (at >> 1));
+                    const uint32_t at = i + __builtin_ctz(near), first = begin_of(at);
                     near &= near - 1;
-                    float v[kStrip];
-                    read_strip<DT>(row, first, begin_of(i + (at >> 1) + 1), at & 1, v);
-#pragma unroll
-                    for (int e = 0; e < kStrip; e++)
-                        if (v[e] >= low)
-                            answer(sh, ask, big, per, v[e], index_in<DT>(row, first, at & 1, e));
+                    float v[2 * kStrip];
+                    read_tile<DT>(row, first, begin_of(at + 1), 0, v);
+                    answer(sh, ask, big, per, low, v,
+                           [&](int e) { return index_in<DT>(row, first, 0, e); });
                 }
             }
         });
@@ -1247,7 +1342,7 @@ hipError_t launch(Device* d, hipStream_t st, const Sampling& s, int* status) {
     const uint32_t least = (blocks + kMost - 1) / kMost;
     if (least <= 1 || (least <= kTiles && s.rows >= (uint32_t)d->cu_count)) {
         // a grid's lanes are counted in 32 bits
-        constexpr uint32_t kRows = 1u << 21;
+        constexpr uint32_t kRows = 1u << 22;
         for (uint32_t first = 0; first < s.rows; first += kRows) {
             const uint32_t n = s.rows - first < kRows ? s.rows - first : kRows;
             hipLaunchKernelGGL(sample_whole_kernel<DT>, dim3(n), dim3(kLanes), 0, st, s, first);
