@@ -574,13 +574,21 @@ __device__ __forceinline__ int part_of(double r) {
     const int p = (int)((0.5 - r) * kRing);
     return p < 0 ? 0 : p < kRing ? p : kRing - 1;
 }
-// A lane's logits x, none of a near bin below low: those that are asked for.
+// The logits between which those that are asked for lie.
+struct Range {
+    float low, high;
+};
+__device__ __forceinline__ Range range_of(const Ask& ask, int top, double per) {
+    return {uniform((float)((top - ask.hi - 1) / per)), uniform((float)((top - ask.lo + 1) / per))};
+}
+// A lane's logits x: those that are asked for.
 template <typename F>
-__device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, double per, float low,
-                                       const float (&x)[2 * kStrip], F index) {
+__device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, double per,
+                                       const Range& range, const float (&x)[2 * kStrip], F index) {
     uint32_t some = 0;
 #pragma unroll
-    for (int e = 0; e < 2 * kStrip; e++) some |= x[e] >= low ? 1u << e : 0u;
+    for (int e = 0; e < 2 * kStrip; e++)
+        some |= x[e] >= range.low && x[e] <= range.high ? 1u << e : 0u;
     // one at a time, so that the code is there once
 #pragma unroll 1
     while (some) {
@@ -1150,7 +1158,7 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
             __syncthreads();
         }
         done = finish<DT>(sh, s, r, rules, per, top, read_ring(sh, bin), [&](const Ask& ask) {
-            const float low = uniform((float)((bin - ask.hi - 1) / per));
+            const Range range = range_of(ask, bin, per);
             const int near = bins ? 1 + ((w.top - bin + ask.hi) >> 2) : 0;
 #pragma clang loop unroll(disable)
             for (uint32_t t = 0; t < strips; t += 2) {
@@ -1158,7 +1166,7 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
                 if (code && code > near) continue;
                 float v[2 * kStrip];
                 read_tile<DT>(row, 0, row.count, t, v);
-                answer(sh, ask, bin, per, low, v,
+                answer(sh, ask, bin, per, range, v,
                        [&](int e) { return index_in<DT>(row, 0, t, e); });
             }
         });
@@ -1169,7 +1177,8 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
 
 // Longer rows, and too few rows to fill the chip: a workgroup a part of up to one tile.
 // The last of a row's parts to end adds up their bins and goes on as above.
-constexpr int kBatch = 8;              // parts whose words are asked for at once
+constexpr int kBatch = 8;             // parts whose words are asked for at once
+constexpr uint32_t kCodes = 16;        // and whose lanes' distances
 constexpr int kMostParts = ACCEL_SAMPLE_WIDTH / (kTile * kLanes) + kBatch;
 struct Parts {
     uint64_t* rings;                   // [rows, parts, kRing]
@@ -1207,7 +1216,11 @@ __device__ __forceinline__ bool is_last(Scratch& sh, uint32_t* ticket, uint32_t 
 template <int DT>
 __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Parts p) {
     __shared__ Scratch sh;
-    __shared__ int bins[kMostParts];
+    // a row's parts' tops and their bins
+    __shared__ union {
+        float top;
+        int bin;
+    } parts[kMostParts];
     const uint32_t local = blockIdx.x / p.parts, part = blockIdx.x - local * p.parts;
     const uint32_t r = p.first + local;
     const Rules rules = rules_of(s, r);
@@ -1261,25 +1274,27 @@ __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Par
         give_first(s, r, least_of(sh, least));
         return;
     }
+    // another workgroup's words come from far, 1.7 us, so they are asked for together
     constexpr int kNone = 1 << 30;
     float top = -INFINITY;
     for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
         const float t = get(p.tops + slot0 + i);
         top = fmaxf(top, t);
-        bins[i] = !(t > -INFINITY) ? -kNone : has_bins(t, per) ? binned(t, per).bin : kNone;
+        parts[i].top = t;
     }
     top = top_of(sh, top);
-    for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
-        if (bins[i] != kNone) continue;
-        // far from zero: far from the row's largest too, or the row has no bins
-        bins[i] = -kNone;
-        if (!(((double)top - (double)get(p.tops + slot0 + i)) * per > 2 * kRing)) sh.listed = 1;
-    }
-    __syncthreads();
     if (top == -INFINITY) {
         give_first(s, r, ~0ull);
         return;
     }
+    for (uint32_t i = threadIdx.x; i < p.parts; i += kLanes) {
+        const float t = parts[i].top;
+        const bool some = t > -INFINITY, has = some && has_bins(t, per);
+        parts[i].bin = has ? binned(t, per).bin : -kNone;
+        // far from zero: far from the row's largest too, or the row has no bins
+        if (some && !has && !(((double)top - (double)t) * per > 2 * kRing)) sh.listed = 1;
+    }
+    __syncthreads();
     bool done = has_bins(top, per) && !sh.listed;
     if (done) {
         const int big = __builtin_amdgcn_readfirstlane(binned(top, per).bin);
@@ -1291,39 +1306,44 @@ __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Par
             for (int x = 0; x < kBatch; x++)
 #pragma unroll
                 for (int j = 0; j < kPer; j++) {
+                    // whatever a part holds, so that no load waits for another
+                    const uint32_t at = i + x < p.parts ? i + x : i;
                     const int bin = big - (int)(threadIdx.x * kPer) - j;
-                    const int below = i + x < p.parts ? bins[i + x] - bin : -1;
-                    v[x][j] = below >= 0 && below < kRing
-                                  ? get(p.rings + (slot0 + i + x) * kRing + (bin & (kRing - 1)))
-                                  : 0;
+                    v[x][j] = get(p.rings + (slot0 + at) * kRing + (bin & (kRing - 1)));
                 }
 #pragma unroll
             for (int x = 0; x < kBatch; x++)
 #pragma unroll
                 for (int j = 0; j < kPer; j++) {
-                    sum.count[j] += (uint32_t)(v[x][j] >> kCount);
-                    sum.rest[j] += v[x][j] & kRest;
+                    const int bin = big - (int)(threadIdx.x * kPer) - j;
+                    const int below = i + x < p.parts ? parts[i + x].bin - bin : -1;
+                    const bool has = below >= 0 && below < kRing;
+                    sum.count[j] += has ? (uint32_t)(v[x][j] >> kCount) : 0u;
+                    sum.rest[j] += has ? v[x][j] & kRest : 0u;
                 }
         }
         done = finish<DT>(sh, s, r, rules, per, top, sum, [&](const Ask& ask) {
-            const float low = uniform((float)((big - ask.hi - 1) / per));
+            const Range range = range_of(ask, big, per);
             const int below = big - ask.hi;
 #pragma clang loop unroll(disable)
-            for (uint32_t i = 0; i < p.parts; i += 32) {
+            for (uint32_t i = 0; i < p.parts; i += kCodes) {
                 uint32_t near = 0;
+                uint8_t code[kCodes];
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const int b = i + j < p.parts ? bins[i + j] : -kNone;
-                    if (b < below) continue;
-                    const int code = get(p.far + (slot0 + i + j) * kLanes + threadIdx.x);
-                    near |= b - 4 * code >= below ? 1u << j : 0u;
+                for (uint32_t j = 0; j < kCodes; j++)
+                    code[j] = get(p.far + (slot0 + (i + j < p.parts ? i + j : i)) * kLanes +
+                                  threadIdx.x);
+#pragma unroll
+                for (uint32_t j = 0; j < kCodes; j++) {
+                    const int b = i + j < p.parts ? parts[i + j].bin : -kNone;
+                    near |= b - 4 * (int)code[j] >= below ? 1u << j : 0u;
                 }
                 while (near) {
                     const uint32_t at = i + __builtin_ctz(near), first = begin_of(at);
                     near &= near - 1;
                     float v[2 * kStrip];
                     read_tile<DT>(row, first, begin_of(at + 1), 0, v);
-                    answer(sh, ask, big, per, low, v,
+                    answer(sh, ask, big, per, range, v,
                            [&](int e) { return index_in<DT>(row, first, 0, e); });
                 }
             }
