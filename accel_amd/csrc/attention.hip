@@ -662,7 +662,81 @@ hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
 
 hipError_t launch_paged_prefill(Device* d, hipStream_t st, const KvCache& c, const Attention& a,
                                 int* status) {
-    return launch_prompts(d, st, c, a, status);
+    *status = ACCEL_OK;
+    const int group = a.heads / c.heads;
+    const int per = prompt_heads(group), tokens = prompt_tokens(group);
+    const uint32_t heads = (uint32_t)(c.heads * ((group + per - 1) / per));
+    // an entry's last tile may be partly filled
+    const uint64_t tiles = (uint64_t)a.rows / tokens + (a.n < a.rows ? a.n : a.rows);
+    const uint64_t bound = tiles * heads;
+    // two workgroups a CU of a 16-bit type up to 128 dims, else one; with fewer
+    // tiles of rows than that, several workgroups share one
+    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 ? 2 : 1);
+    uint32_t splits = bound < slots ? (uint32_t)(slots / bound) : 1;
+    // as many as the longest sequence's keys can be worth
+    const int64_t kt = c.dim <= 128 ? 64 : 32;
+    int64_t most = ((int64_t)c.slots << c.shift) / kt + 1;
+    if (a.window) {
+        const int64_t near = ((int64_t)a.window + tokens) / kt + a.sinks / kt + 3;
+        most = near < most ? near : most;
+    }
+    const int64_t worth = most / (a.q_f32 ? kTilesAShare<true> : kTilesAShare<false>);
+    splits = worth < (int64_t)splits ? (uint32_t)(worth > 1 ? worth : 1) : splits;
+    const int wide = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+    const size_t part_words =
+        splits > 1 ? (size_t)(bound * splits) * 256 * (wide / 32 * 16 + 2) : 0;
+    const bool summed = a.n > 64;
+    const size_t sums_words = summed ? ((size_t)a.n + 1) & ~(size_t)1 : 0;
+    uint32_t *tickets = nullptr, *sums = nullptr;
+    float* parts = nullptr;
+    if (part_words + sums_words) {
+        char* ws = static_cast<char*>(workspace(d, st, (part_words + sums_words) * 4, status));
+        if (!ws) return hipSuccess;
+        tickets = reinterpret_cast<uint32_t*>(ws);
+        parts = reinterpret_cast<float*>(ws + kWorkspaceCounterBytes);
+        if (summed) sums = reinterpret_cast<uint32_t*>(parts + part_words);
+    }
+    if (summed)
+        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
+                           sums, d->fault_dev);
+    const uint32_t fold = slots > (uint32_t)d->cu_count ? (uint32_t)d->cu_count / heads : 0;
+    const uint32_t stride = (uint32_t)(kWorkspaceCounterBytes / 4) / slots;
+    // a launch of 256 lanes a workgroup holds fewer than 2^24 of them, as a
+    // grid's lanes are counted in 32 bits; that many places are not split
+    constexpr uint64_t kPlaces = 1 << 22;
+    const auto go = [&](auto kernel) {
+        for (uint64_t place = 0; place < bound; place += kPlaces) {
+            const uint64_t places = bound - place < kPlaces ? bound - place : kPlaces;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(places * splits)), dim3(256), 0, st, c, a,
+                               sums, fold, splits, (uint32_t)place, tickets, stride, parts,
+                               d->fault_dev);
+        }
+    };
+    const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
+    const auto dims = [&](auto bf16, auto qt, auto pt) {
+        constexpr bool B = decltype(bf16)::value;
+        constexpr int Q = decltype(qt)::value, P = decltype(pt)::value;
+        if (c.dim <= 64)
+            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64, Attention>)
+                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64, Attention>);
+        else if (c.dim <= 128)
+            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64, Attention>)
+                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64, Attention>);
+        else
+            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32, Attention>)
+                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32, Attention>);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 3> three;
+    if (a.q_f32) {
+        if (c.bf16) dims(std::true_type(), three, three);
+        else dims(std::false_type(), two, two);
+    } else {
+        if (c.bf16) dims(std::true_type(), one, one);
+        else dims(std::false_type(), one, one);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace accel

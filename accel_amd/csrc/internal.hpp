@@ -452,7 +452,8 @@ struct Attention {
 struct Drafts : Attention {
     const uint32_t* parents;   // [rows] of each node, in its entry; ACCEL_KV_NONE: none
 };
-// n entries' tiles of 32 keys have to be counted in 32 bits.
+// n entries' tiles of 32 keys, and drafts' steps, have to be counted in 32 bits.
+bool paged_tree_counts(const KvCache& c, const Attention& a);
 bool paged_attention_counts(const KvCache& c, const Attention& a);
 hipError_t launch_paged_attention(Device* d, hipStream_t st, const KvCache& c,
                                   const Attention& a, int* status);

@@ -409,14 +409,16 @@ int paged(const char* op, int dev, void* stream, const accel_tensor_t* q,
     }
     if ((rc = check_seqs(op, seqs, c, &n, &a.seqs)) != ACCEL_OK) return rc;
     a.n = (int)n;
+    a.rows = (int)T;
+    a.heads = (int)H;
+    if (tree && !paged_tree_counts(c, a))
+        return refuse(op, "more rows over such tables than 32 bits count the tiles of");
     if (!ragged && !paged_attention_counts(c, a))
         return refuse(op, "more entries of such tables than 32 bits count the tiles of");
     Device* d;
     if ((rc = begin(dev, &d)) != ACCEL_OK || n == 0 || T == 0) return rc;
     a.q = q->data;
     a.out = out->data;
-    a.rows = (int)T;
-    a.heads = (int)H;
     a.layer = layer;
     a.q_f32 = q->dtype == ACCEL_F32;
     int status = ACCEL_OK;

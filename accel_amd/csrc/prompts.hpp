@@ -89,6 +89,67 @@ struct Paths {
 };
 struct NoPaths {};
 
+// A draft's work: its tiles of rows, and the tiles of keys of each, the sinks' and
+// those from its roots' windows' start to its last node (a tile of rows that ends
+// before has fewer).  One whose rows are zeros is a tile of keys.
+struct DraftWork {
+    uint32_t tiles, steps;
+};
+template <int KT>
+__device__ __forceinline__ DraftWork work_of(const Attention& a, uint32_t len, uint32_t nodes,
+                                             int tokens) {
+    DraftWork w = {(nodes + tokens - 1) / tokens, 1};
+    if (nodes <= len && nodes <= (uint32_t)kDraft) {
+        const uint32_t root = len - nodes;
+        const uint32_t lo = a.window && root + 1 > a.window ? root + 1 - a.window : 0;
+        const uint32_t near = a.window ? (a.sinks < lo ? a.sinks : lo) : 0;
+        const uint32_t sink_tiles = (near + KT - 1) / KT;
+        const uint32_t start = lo / KT > sink_tiles ? lo / KT : sink_tiles;
+        const uint32_t last = len ? (len - 1) / KT + 1 : 0;
+        w.steps = sink_tiles + (last > start ? last - start : 0);
+    }
+    return w;
+}
+// Of the line of all drafts' steps, a tile of rows after the other: where step x lies.
+struct DraftPlace {
+    int entry;
+    Held held;
+    uint32_t tile;                    // of the entry's rows
+    uint32_t first, past;             // its steps' places in the line
+};
+template <int KT>
+__device__ __forceinline__ DraftPlace place_of(const Cut& k, const KvCache& c, const Attention& a,
+                                               int tokens, uint32_t x) {
+    DraftPlace p;
+    uint32_t start;
+    p.entry = find_entry(k, x, &start);
+    p.held = entry_held(k, c, a, p.entry);
+    const DraftWork w = work_of<KT>(a, p.held.len, rows_of(a, p.entry).count, tokens);
+    p.tile = (x - start) / w.steps;
+    p.first = start + p.tile * w.steps;
+    p.past = p.first + w.steps;
+    return p;
+}
+// A cut this near to a tile of rows' first or last step moves there: a piece of it costs
+// its queries' way in and its part's way out, some two steps.
+constexpr uint32_t kNearDraft = 2;
+template <int KT>
+__device__ __forceinline__ uint32_t draft_cut(const Cut& k, const KvCache& c, const Attention& a,
+                                              int tokens, uint64_t w) {
+    if (w * k.chunk >= k.tiles) return k.tiles;
+    const uint32_t x = (uint32_t)(w * k.chunk);
+    const DraftPlace p = place_of<KT>(k, c, a, tokens, x);
+    return x - p.first <= kNearDraft ? p.first : p.past - x <= kNearDraft ? p.past : x;
+}
+
+// Two parts of a row, each scaled to the larger maximum.  Rounded by itself each, so
+// that it is the same whichever of the two is at hand and which comes from memory.
+__device__ __forceinline__ float joined(float x, float fx, float y, float fy) {
+#pragma clang fp contract(off)
+    const float a = x * fx, b = y * fy;
+    return a + b;
+}
+
 template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call>
 __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
     KvCache c, Call a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
@@ -108,6 +169,11 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     // which is cleared two steps before it is read, a barrier before it is set
     __shared__ uint32_t odd_sh[3][2];
     __shared__ uint32_t again_sh;
+    // dims past the head's: K's chunks there are no load's target and stay 0
+    const auto clear_keys = [&] {
+        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
+            reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
+    };
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -118,7 +184,9 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const uint32_t heads = (uint32_t)(c.heads * group_tiles);
     // shares are the slow index: those that have nothing to do come last
     const uint32_t places = gridDim.x / splits;
-    const uint32_t split = blockIdx.x / places, place = place0 + blockIdx.x - split * places;
+    const uint32_t split = TREE ? 0 : blockIdx.x / places;
+    const uint32_t place = place0 + blockIdx.x - split * places;
+    // (drafts: a stretch of the head's line of steps)
     const uint32_t order = place / heads, head_tile = place - order * heads;
     const uint32_t head = head_tile / group_tiles;
     const int g0 = (int)(head_tile - head * group_tiles) * per;
@@ -136,6 +204,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         cut.lane_held = {kNoSequence, 0};
         if (lane < a.n) cut.lane_held = held_by(c, a, lane, blockIdx.x ? nullptr : fault);
         uint32_t v = lane < a.n ? (rows_of(a, lane).count + tokens - 1) / tokens : 0;
+        if constexpr (TREE) {
+            if (lane < a.n)
+                v *= work_of<KT>(a, cut.lane_held.len, rows_of(a, lane).count, tokens).steps;
+        }
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
@@ -146,17 +218,53 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     } else {
         cut.tiles = __builtin_amdgcn_readfirstlane(sums[a.n - 1]);
     }
-    if (order >= cut.tiles) return;
-    const uint32_t tile = cut.tiles <= 2 * fold && order >= fold ? order - fold
-                                                                 : cut.tiles - 1 - order;
-    uint32_t item;
-    const int entry = find_entry(cut, tile, &item);
+    uint32_t tile = 0;
+    uint32_t u = 0, u_end = 0;           // drafts: the stretch's steps, to go and past
+    if constexpr (TREE) {
+        const uint32_t even = (uint32_t)(((uint64_t)cut.tiles + splits - 1) / splits);
+        constexpr uint32_t kLeastSteps = kTilesAShare<F32>;
+        cut.chunk = even > kLeastSteps ? even : kLeastSteps;
+        u = draft_cut<KT>(cut, c, a, tokens, order);
+        u_end = draft_cut<KT>(cut, c, a, tokens, order + 1);
+        if constexpr (!FULL) clear_keys();
+    } else {
+        if (order >= cut.tiles) return;
+        tile = cut.tiles <= 2 * fold && order >= fold ? order - fold : cut.tiles - 1 - order;
+    }
+    // a tile of rows; drafts: those of the stretch, one after the other (no lane goes on
+    // to the next before the others: there are barriers on the way)
+    do {
+    int entry;
+    Held held;
+    uint32_t tok0;
+    DraftPlace at = {};
+    uint32_t u_next = 0;
+    if constexpr (TREE) {
+        if (u >= u_end) return;
+        at = place_of<KT>(cut, c, a, tokens, u);
+        entry = at.entry;
+        held = at.held;
+        tok0 = at.tile * tokens;
+        u_next = at.past < u_end ? at.past : u_end;
+        // LDS is the last tile's until all waves are here
+        __syncthreads();
+    } else {
+        uint32_t item;
+        entry = find_entry(cut, tile, &item);
+        tok0 = (tile - item) * tokens;
+        held = sums ? held_by(c, a, entry, threadIdx.x ? nullptr : fault)
+                    : entry_held(cut, c, a, entry);
+    }
     const Rows rows = rows_of(a, entry);
-    const uint32_t tok0 = (tile - item) * tokens;
-    if (tok0 >= rows.count) return;      // offsets that do not ascend
+    if (tok0 >= rows.count) {            // offsets that do not ascend
+        if constexpr (TREE) {
+            u = u_next;
+            continue;
+        } else {
+            return;
+        }
+    }
     const uint32_t toks = rows.count - tok0 < (uint32_t)tokens ? rows.count - tok0 : tokens;
-    const Held held = sums ? held_by(c, a, entry, threadIdx.x ? nullptr : fault)
-                           : entry_held(cut, c, a, entry);
     // the position of the tile's first token, or of a draft's roots; below 0 it sees
     // nothing
     const int base = (int)held.len - (int)rows.count + (TREE ? 0 : (int)tok0);
@@ -201,7 +309,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                                                     : (int)splits;
     const int share = (count + shares - 1) / shares;
     const int held_shares = count > 0 ? (count + share - 1) / share : 1;
-    if ((int)split >= held_shares) return;
+    if (!TREE && (int)split >= held_shares) return;
 
     // this lane's row's position, or -1 where it sees nothing
     int p = real && base + tok > -1 ? base + tok : -1;
@@ -235,8 +343,12 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         p = real && depth > -1 ? base + depth : -1;
         lost = __any(real && depth < 0);
     }
-    const int t_begin = (int)split * share;
-    const int t_end = t_begin + share < count ? t_begin + share : count;
+    int t_begin = (int)split * share;
+    int t_end = t_begin + share < count ? t_begin + share : count;
+    if constexpr (TREE) {
+        t_begin = (int)(u - at.first);
+        t_end = (int)(u_next - at.first) < count ? (int)(u_next - at.first) : count;
+    }
     const auto tile_pos = [&](int t) {
         return (t < sink_tiles ? t : start + (t - sink_tiles)) * KT;
     };
@@ -341,11 +453,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         }
     };
 
-    // dims past the head's: K's chunks there are no load's target and stay 0
-    if constexpr (!FULL) {
-        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
-            reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
-    }
+    if constexpr (!FULL && !TREE) clear_keys();
     // A first pass takes the values of tiles that all rows see as they are; where
     // something in it is not finite, or scores are large, the workgroup goes over
     // its keys again.
@@ -645,7 +753,88 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     __syncthreads();
     if (again_sh) pass(std::true_type());
     if (unnamed && wave == 0) report(fault, kFaultKvPage);
-    if (held_shares > 1) {
+    if constexpr (TREE) {
+        // The pieces of a tile of rows, of stretches w0 to w1 (the first and the last cut
+        // of it that are farther than kNearDraft from its ends), join in pairs, then the
+        // pairs: of two the one to arrive last adds the other's part to its own, lane by
+        // lane, and goes on as the pair's first.  Two places a stretch: a tile's first
+        // piece, and the others'.
+        u = u_next;
+        const bool whole = t_begin == 0 && u_next == at.past;
+        if (!whole) {
+            constexpr int kWords = DT * 16 + 2;
+            const uint32_t w0 = (uint32_t)(((uint64_t)at.first + kNearDraft) / cut.chunk);
+            const uint32_t w1 =
+                (uint32_t)(((uint64_t)at.past - kNearDraft + cut.chunk - 1) / cut.chunk) - 1;
+            const uint32_t pieces = w1 - w0 + 1;
+            const auto part = [&](uint32_t i) {
+                return reinterpret_cast<uint64_t*>(parts) +
+                       (2 * ((size_t)(w0 + i) * heads + head_tile) + (i == 0 ? 1 : 0)) *
+                           (kWords / 2 * 256) + threadIdx.x;
+            };
+            uint32_t mine = order - w0;
+            bool last_one = true;
+            for (uint32_t span = 1; span < pieces; span *= 2) {
+                const uint32_t left = mine & ~(2 * span - 1), right = left + span;
+                if (right >= pieces) continue;
+                uint64_t* to = part(mine);
+                if (real) {
+                    __hip_atomic_store(to, __builtin_bit_cast(uint64_t, (f32x2){m, sum}),
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+                    for (int e = 0; e < DT; e++)
+#pragma unroll
+                        for (int x = 0; x < 8; x++)
+                            __hip_atomic_store(
+                                to + (1 + e * 8 + x) * 256,
+                                __builtin_bit_cast(uint64_t,
+                                                   (f32x2){o[e][2 * x], o[e][2 * x + 1]}),
+                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                __builtin_amdgcn_s_waitcnt(0);
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                __syncthreads();
+                uint32_t* ticket = tickets + ((size_t)(w0 + right) * heads + head_tile) *
+                                                 ticket_stride;
+                if (threadIdx.x == 0) {
+                    const uint32_t before = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED,
+                                                                   __HIP_MEMORY_SCOPE_AGENT);
+                    if (before) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_AGENT);
+                    odd_sh[0][0] = before;
+                }
+                __syncthreads();
+                last_one = __builtin_amdgcn_readfirstlane(odd_sh[0][0]) != 0;
+                if (!last_one) break;
+                uint64_t* from = part(mine == left ? right : left);
+                if (real) {
+                    const auto get = [&](int i) {
+                        return __builtin_bit_cast(
+                            f32x2, __hip_atomic_load(from + i * 256, __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT));
+                    };
+                    const f32x2 ml = get(0);
+                    f32x2 v[DT * 8];
+#pragma unroll
+                    for (int i = 0; i < DT * 8; i++) v[i] = get(1 + i);
+                    const float top = fmaxf(m, ml[0]);
+                    const float own = kept<true>(__builtin_amdgcn_exp2f(m - top));
+                    const float its = kept<true>(__builtin_amdgcn_exp2f(ml[0] - top));
+                    m = top;
+                    sum = joined(sum, own, ml[1], its);
+#pragma unroll
+                    for (int i = 0; i < DT * 8; i++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            o[i >> 3][2 * (i & 7) + x] =
+                                joined(o[i >> 3][2 * (i & 7) + x], own, v[i][x], its);
+                }
+                mine = left;
+            }
+            if (!last_one) continue;
+        }
+    } else if (held_shares > 1) {
         // a share's maximum, sum and values as the lanes hold them; the share to
         // arrive last adds them all, in the shares' order
         constexpr int kWords = DT * 16 + 2;
@@ -713,7 +902,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             }
         }
     }
-    if (!real) return;
+    if (!TREE && !real) return;
     sum += __shfl_xor(sum, 32, 64);
     const float scale = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -721,7 +910,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int d = e * 32 + 8 * i + 4 * half;
-            if (!FULL && d >= dim) continue;
+            if ((TREE && !real) || (!FULL && d >= dim)) continue;
             f32x4 v;
 #pragma unroll
             for (int x = 0; x < 4; x++) v[x] = sum == 0 ? 0.0f : o[e][4 * i + x] * scale;
@@ -735,87 +924,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                     (u32x2){x[0][0], x[1][0]};
             }
         }
-}
-
-template <typename Call>
-hipError_t launch_prompts(Device* d, hipStream_t st, const KvCache& c, const Call& a,
-                          int* status) {
-    constexpr bool TREE = std::is_same<Call, Drafts>::value;
-    *status = ACCEL_OK;
-    const int group = a.heads / c.heads;
-    const int per = prompt_heads(group), tokens = prompt_tokens(group);
-    const uint32_t heads = (uint32_t)(c.heads * ((group + per - 1) / per));
-    // an entry's last tile may be partly filled
-    const uint64_t tiles = (uint64_t)a.rows / tokens + (a.n < a.rows ? a.n : a.rows);
-    const uint64_t bound = tiles * heads;
-    // two workgroups a CU of a 16-bit type up to 128 dims, else one; with fewer
-    // tiles of rows than that, several workgroups share one
-    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 ? 2 : 1);
-    uint32_t splits = bound < slots ? (uint32_t)(slots / bound) : 1;
-    // as many as the longest sequence's keys can be worth
-    const int64_t kt = c.dim <= 128 ? 64 : 32;
-    int64_t most = ((int64_t)c.slots << c.shift) / kt + 1;
-    if (a.window) {
-        const int64_t near = ((int64_t)a.window + (TREE ? kDraft : tokens)) / kt + a.sinks / kt + 3;
-        most = near < most ? near : most;
-    }
-    const int64_t worth = most / (a.q_f32 ? kTilesAShare<true> : kTilesAShare<false>);
-    splits = worth < (int64_t)splits ? (uint32_t)(worth > 1 ? worth : 1) : splits;
-    const int wide = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
-    const size_t part_words =
-        splits > 1 ? (size_t)(bound * splits) * 256 * (wide / 32 * 16 + 2) : 0;
-    const bool summed = a.n > 64;
-    const size_t sums_words = summed ? ((size_t)a.n + 1) & ~(size_t)1 : 0;
-    uint32_t *tickets = nullptr, *sums = nullptr;
-    float* parts = nullptr;
-    if (part_words + sums_words) {
-        char* ws = static_cast<char*>(workspace(d, st, (part_words + sums_words) * 4, status));
-        if (!ws) return hipSuccess;
-        tickets = reinterpret_cast<uint32_t*>(ws);
-        parts = reinterpret_cast<float*>(ws + kWorkspaceCounterBytes);
-        if (summed) sums = reinterpret_cast<uint32_t*>(parts + part_words);
-    }
-    if (summed)
-        hipLaunchKernelGGL(paged_sums_kernel, dim3(1), dim3(1024), 0, st, c, a, (uint32_t)tokens,
-                           sums, d->fault_dev);
-    const uint32_t fold = slots > (uint32_t)d->cu_count ? (uint32_t)d->cu_count / heads : 0;
-    const uint32_t stride = (uint32_t)(kWorkspaceCounterBytes / 4) / slots;
-    // a launch of 256 lanes a workgroup holds fewer than 2^24 of them, as a
-    // grid's lanes are counted in 32 bits; that many places are not split
-    constexpr uint64_t kPlaces = 1 << 22;
-    const auto go = [&](auto kernel) {
-        for (uint64_t place = 0; place < bound; place += kPlaces) {
-            const uint64_t places = bound - place < kPlaces ? bound - place : kPlaces;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)(places * splits)), dim3(256), 0, st, c, a,
-                               sums, fold, splits, (uint32_t)place, tickets, stride, parts,
-                               d->fault_dev);
-        }
-    };
-    const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
-    const auto dims = [&](auto bf16, auto qt, auto pt) {
-        constexpr bool B = decltype(bf16)::value;
-        constexpr int Q = decltype(qt)::value, P = decltype(pt)::value;
-        if (c.dim <= 64)
-            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64, Call>)
-                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64, Call>);
-        else if (c.dim <= 128)
-            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64, Call>)
-                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64, Call>);
-        else
-            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32, Call>)
-                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32, Call>);
-    };
-    const std::integral_constant<int, 1> one;
-    const std::integral_constant<int, 2> two;
-    const std::integral_constant<int, 3> three;
-    if (a.q_f32) {
-        if (c.bf16) dims(std::true_type(), three, three);
-        else dims(std::false_type(), two, two);
-    } else {
-        if (c.bf16) dims(std::true_type(), one, one);
-        else dims(std::false_type(), one, one);
-    }
-    return hipGetLastError();
+    } while (TREE);
 }
 
 }  // namespace
