@@ -47,7 +47,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-constexpr int kRows = 128;            // rows a workgroup
+constexpr int kRows = 128;            // rows a workgroup of four waves
 
 // s_waitcnt vmcnt(0), as an instruction that the compiler counts itself; reads of
 // what the loads brought to LDS stay behind it.
@@ -71,8 +71,12 @@ template <bool F32>
 constexpr int kTilesAShare = F32 ? 2 : 4;
 
 // Tokens of a tile of rows, and the query heads of one.
-__host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
-__host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
+__host__ __device__ inline int prompt_heads(int group, int rows = kRows) {
+    return group < rows ? group : rows;
+}
+__host__ __device__ inline int prompt_tokens(int group, int rows = kRows) {
+    return rows / prompt_heads(group, rows);
+}
 
 // Drafts: an entry's rows are the nodes of a tree behind its sequence's context.  A
 // node sees the context and, of the nodes, those on its path to its root; it stands
@@ -80,11 +84,12 @@ __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_
 // to the context's end, so only the tiles past it look at the paths: a bit for each
 // of up to kDraft nodes, made by a lane a node that walks up its parents in LDS.
 constexpr int kDraft = ACCEL_DRAFT_NODES;
+template <int ROWS>
 struct Paths {
     // words of a node's bits, and as many past them as a tile reads; an odd stride,
     // for a wave's rows to meet in different banks
-    uint32_t bits[kRows][kDraft / 32 + 3];
-    int depth[kRows];                 // -1: a parent on the path is not before its child
+    uint32_t bits[ROWS][kDraft / 32 + 3];
+    int depth[ROWS];                  // -1: a parent on the path is not before its child
     uint32_t parent[kDraft];
 };
 struct NoPaths {};
@@ -133,6 +138,10 @@ __device__ __forceinline__ DraftPlace place_of(const Cut& k, const KvCache& c, c
 // A cut this near to a tile of rows' first or last step moves there: a piece of it costs
 // its queries' way in and its part's way out, some two steps.
 constexpr uint32_t kNearDraft = 2;
+// Steps that are worth a workgroup and a join (9 drafts of 1 to 100 nodes seen through a
+// window of 333, f16: 29.8 us with one, 24.4 with two, 31.0 with four).
+template <bool F32>
+constexpr uint32_t kLeastDraft = F32 ? 1 : 2;
 template <int KT>
 __device__ __forceinline__ uint32_t draft_cut(const Cut& k, const KvCache& c, const Attention& a,
                                               int tokens, uint64_t w) {
@@ -150,8 +159,8 @@ __device__ __forceinline__ float joined(float x, float fx, float y, float fy) {
     return a + b;
 }
 
-template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call>
-__global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
+template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call, int WAVES = 4>
+__global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
     KvCache c, Call a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
     uint32_t* tickets, uint32_t ticket_stride, float* parts, uint32_t* fault) {
     constexpr int NS = DIM / 16;            // MFMA steps of a score
@@ -159,10 +168,11 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     constexpr int SUB = KT / 32;            // 32-key parts of a tile
     constexpr int DT = DIM / 32;            // 32-dim parts of a row of values
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
-    constexpr int KL = KT * NC / 256;       // chunks of K, and of V, a lane stages
+    constexpr int LANES = 64 * WAVES, ROWS = 32 * WAVES;
+    constexpr int KL = KT * NC / LANES;     // chunks of K, and of V, a lane stages
     constexpr bool F32 = QT > 1;
     constexpr bool TREE = std::is_same<Call, Drafts>::value;
-    __shared__ typename std::conditional<TREE, Paths, NoPaths>::type paths;
+    __shared__ typename std::conditional<TREE, Paths<ROWS>, NoPaths>::type paths;
     __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
     __shared__ __attribute__((aligned(256))) char v_sh[2][KT * NC * 16];
     // keys of a tile with values that are not finite: tile t's in place t % 3,
@@ -171,7 +181,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     __shared__ uint32_t again_sh;
     // dims past the head's: K's chunks there are no load's target and stay 0
     const auto clear_keys = [&] {
-        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
+        for (int i = threadIdx.x; i < 2 * KT * NC; i += LANES)
             reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
     };
     const int lane = threadIdx.x & 63;
@@ -179,7 +189,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     const int col = lane & 31, half = lane >> 5;
     const int dim = FULL ? DIM : c.dim;
     const int group = a.heads / c.heads;
-    const int per = prompt_heads(group), tokens = prompt_tokens(group);
+    const int per = prompt_heads(group, ROWS), tokens = prompt_tokens(group, ROWS);
     const int group_tiles = (group + per - 1) / per;
     const uint32_t heads = (uint32_t)(c.heads * group_tiles);
     // shares are the slow index: those that have nothing to do come last
@@ -222,8 +232,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     uint32_t u = 0, u_end = 0;           // drafts: the stretch's steps, to go and past
     if constexpr (TREE) {
         const uint32_t even = (uint32_t)(((uint64_t)cut.tiles + splits - 1) / splits);
-        constexpr uint32_t kLeastSteps = kTilesAShare<F32>;
-        cut.chunk = even > kLeastSteps ? even : kLeastSteps;
+        cut.chunk = even > kLeastDraft<F32> ? even : kLeastDraft<F32>;
         u = draft_cut<KT>(cut, c, a, tokens, order);
         u_end = draft_cut<KT>(cut, c, a, tokens, order + 1);
         if constexpr (!FULL) clear_keys();
@@ -316,12 +325,12 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     bool lost = false;      // some row of the wave's is such a draft
     if constexpr (TREE) {
         const int nodes = drafted ? at0 + (int)toks : 0;
-        for (int i = threadIdx.x; i < nodes; i += 256)
+        for (int i = threadIdx.x; i < nodes; i += LANES)
             paths.parent[i] = a.parents[rows.first + i];
-        for (int i = threadIdx.x; i < kRows * (int)(sizeof paths.bits[0] / 4); i += 256)
+        for (int i = threadIdx.x; i < ROWS * (int)(sizeof paths.bits[0] / 4); i += LANES)
             (&paths.bits[0][0])[i] = 0;
         __syncthreads();
-        if ((int)threadIdx.x < kRows) {
+        if ((int)threadIdx.x < ROWS) {
             const int x = threadIdx.x;
             int depth = -1;
             if (drafted && x < (int)toks) {
@@ -770,7 +779,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             const auto part = [&](uint32_t i) {
                 return reinterpret_cast<uint64_t*>(parts) +
                        (2 * ((size_t)(w0 + i) * heads + head_tile) + (i == 0 ? 1 : 0)) *
-                           (kWords / 2 * 256) + threadIdx.x;
+                           (kWords / 2 * LANES) + threadIdx.x;
             };
             uint32_t mine = order - w0;
             bool last_one = true;
@@ -786,7 +795,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
                         for (int x = 0; x < 8; x++)
                             __hip_atomic_store(
-                                to + (1 + e * 8 + x) * 256,
+                                to + (1 + e * 8 + x) * LANES,
                                 __builtin_bit_cast(uint64_t,
                                                    (f32x2){o[e][2 * x], o[e][2 * x + 1]}),
                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -811,7 +820,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
                 if (real) {
                     const auto get = [&](int i) {
                         return __builtin_bit_cast(
-                            f32x2, __hip_atomic_load(from + i * 256, __ATOMIC_RELAXED,
+                            f32x2, __hip_atomic_load(from + i * LANES, __ATOMIC_RELAXED,
                                                      __HIP_MEMORY_SCOPE_AGENT));
                     };
                     const f32x2 ml = get(0);
@@ -840,7 +849,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
         constexpr int kWords = DT * 16 + 2;
         const auto part = [&](int x) {
             return reinterpret_cast<uint64_t*>(parts) +
-                   ((size_t)place * splits + x) * (kWords / 2 * 256) + threadIdx.x;
+                   ((size_t)place * splits + x) * (kWords / 2 * LANES) + threadIdx.x;
         };
         const auto put = [](uint64_t* p, float x, float y) {
             __hip_atomic_store(p, __builtin_bit_cast(uint64_t, (f32x2){x, y}), __ATOMIC_RELAXED,
@@ -857,7 +866,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             for (int e = 0; e < DT; e++)
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    put(mine + (1 + e * 8 + x) * 256, o[e][2 * x], o[e][2 * x + 1]);
+                    put(mine + (1 + e * 8 + x) * LANES, o[e][2 * x], o[e][2 * x + 1]);
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(0);
@@ -887,7 +896,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
             for (int y = 0; y < 2; y++) {
                 ml[y] = get(from[y]);
 #pragma unroll
-                for (int z = 0; z < DT * 8; z++) v[y][z] = get(from[y] + (1 + z) * 256);
+                for (int z = 0; z < DT * 8; z++) v[y][z] = get(from[y] + (1 + z) * LANES);
             }
 #pragma unroll
             for (int y = 0; y < 2; y++) {
