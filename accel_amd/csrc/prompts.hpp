@@ -47,7 +47,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-constexpr int kRows = 128;            // rows a workgroup of four waves
+constexpr int kRows = 128;            // rows a workgroup
 
 // s_waitcnt vmcnt(0), as an instruction that the compiler counts itself; reads of
 // what the loads brought to LDS stay behind it.
@@ -71,12 +71,8 @@ template <bool F32>
 constexpr int kTilesAShare = F32 ? 2 : 4;
 
 // Tokens of a tile of rows, and the query heads of one.
-__host__ __device__ inline int prompt_heads(int group, int rows = kRows) {
-    return group < rows ? group : rows;
-}
-__host__ __device__ inline int prompt_tokens(int group, int rows = kRows) {
-    return rows / prompt_heads(group, rows);
-}
+__host__ __device__ inline int prompt_heads(int group) { return group < kRows ? group : kRows; }
+__host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_heads(group); }
 
 // Drafts: an entry's rows are the nodes of a tree behind its sequence's context.  A
 // node sees the context and, of the nodes, those on its path to its root; it stands
@@ -84,12 +80,11 @@ __host__ __device__ inline int prompt_tokens(int group, int rows = kRows) {
 // to the context's end, so only the tiles past it look at the paths: a bit for each
 // of up to kDraft nodes, made by a lane a node that walks up its parents in LDS.
 constexpr int kDraft = ACCEL_DRAFT_NODES;
-template <int ROWS>
 struct Paths {
     // words of a node's bits, and as many past them as a tile reads; an odd stride,
     // for a wave's rows to meet in different banks
-    uint32_t bits[ROWS][kDraft / 32 + 3];
-    int depth[ROWS];                  // -1: a parent on the path is not before its child
+    uint32_t bits[kRows][kDraft / 32 + 3];
+    int depth[kRows];                 // -1: a parent on the path is not before its child
     uint32_t parent[kDraft];
 };
 struct NoPaths {};
@@ -159,8 +154,8 @@ __device__ __forceinline__ float joined(float x, float fx, float y, float fy) {
     return a + b;
 }
 
-template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call, int WAVES = 4>
-__global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
+template <bool BF16, int QT, int PT, int DIM, bool FULL, int KT, typename Call>
+__global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_prefill_kernel(
     KvCache c, Call a, const uint32_t* sums, uint32_t fold, uint32_t splits, uint32_t place0,
     uint32_t* tickets, uint32_t ticket_stride, float* parts, uint32_t* fault) {
     constexpr int NS = DIM / 16;            // MFMA steps of a score
@@ -168,11 +163,10 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
     constexpr int SUB = KT / 32;            // 32-key parts of a tile
     constexpr int DT = DIM / 32;            // 32-dim parts of a row of values
     constexpr int BLOCKS = KT / 8;          // eight keys lie in one page
-    constexpr int LANES = 64 * WAVES, ROWS = 32 * WAVES;
-    constexpr int KL = KT * NC / LANES;     // chunks of K, and of V, a lane stages
+    constexpr int KL = KT * NC / 256;       // chunks of K, and of V, a lane stages
     constexpr bool F32 = QT > 1;
     constexpr bool TREE = std::is_same<Call, Drafts>::value;
-    __shared__ typename std::conditional<TREE, Paths<ROWS>, NoPaths>::type paths;
+    __shared__ typename std::conditional<TREE, Paths, NoPaths>::type paths;
     __shared__ __attribute__((aligned(256))) char k_sh[2][KT * NC * 16];
     __shared__ __attribute__((aligned(256))) char v_sh[2][KT * NC * 16];
     // keys of a tile with values that are not finite: tile t's in place t % 3,
@@ -181,7 +175,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
     __shared__ uint32_t again_sh;
     // dims past the head's: K's chunks there are no load's target and stay 0
     const auto clear_keys = [&] {
-        for (int i = threadIdx.x; i < 2 * KT * NC; i += LANES)
+        for (int i = threadIdx.x; i < 2 * KT * NC; i += 256)
             reinterpret_cast<u32x4*>(k_sh)[i] = (u32x4){0, 0, 0, 0};
     };
     const int lane = threadIdx.x & 63;
@@ -189,7 +183,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
     const int col = lane & 31, half = lane >> 5;
     const int dim = FULL ? DIM : c.dim;
     const int group = a.heads / c.heads;
-    const int per = prompt_heads(group, ROWS), tokens = prompt_tokens(group, ROWS);
+    const int per = prompt_heads(group), tokens = prompt_tokens(group);
     const int group_tiles = (group + per - 1) / per;
     const uint32_t heads = (uint32_t)(c.heads * group_tiles);
     // shares are the slow index: those that have nothing to do come last
@@ -325,12 +319,12 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
     bool lost = false;      // some row of the wave's is such a draft
     if constexpr (TREE) {
         const int nodes = drafted ? at0 + (int)toks : 0;
-        for (int i = threadIdx.x; i < nodes; i += LANES)
+        for (int i = threadIdx.x; i < nodes; i += 256)
             paths.parent[i] = a.parents[rows.first + i];
-        for (int i = threadIdx.x; i < ROWS * (int)(sizeof paths.bits[0] / 4); i += LANES)
+        for (int i = threadIdx.x; i < kRows * (int)(sizeof paths.bits[0] / 4); i += 256)
             (&paths.bits[0][0])[i] = 0;
         __syncthreads();
-        if ((int)threadIdx.x < ROWS) {
+        if ((int)threadIdx.x < kRows) {
             const int x = threadIdx.x;
             int depth = -1;
             if (drafted && x < (int)toks) {
@@ -779,7 +773,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
             const auto part = [&](uint32_t i) {
                 return reinterpret_cast<uint64_t*>(parts) +
                        (2 * ((size_t)(w0 + i) * heads + head_tile) + (i == 0 ? 1 : 0)) *
-                           (kWords / 2 * LANES) + threadIdx.x;
+                           (kWords / 2 * 256) + threadIdx.x;
             };
             uint32_t mine = order - w0;
             bool last_one = true;
@@ -795,7 +789,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
 #pragma unroll
                         for (int x = 0; x < 8; x++)
                             __hip_atomic_store(
-                                to + (1 + e * 8 + x) * LANES,
+                                to + (1 + e * 8 + x) * 256,
                                 __builtin_bit_cast(uint64_t,
                                                    (f32x2){o[e][2 * x], o[e][2 * x + 1]}),
                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -820,7 +814,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
                 if (real) {
                     const auto get = [&](int i) {
                         return __builtin_bit_cast(
-                            f32x2, __hip_atomic_load(from + i * LANES, __ATOMIC_RELAXED,
+                            f32x2, __hip_atomic_load(from + i * 256, __ATOMIC_RELAXED,
                                                      __HIP_MEMORY_SCOPE_AGENT));
                     };
                     const f32x2 ml = get(0);
@@ -849,7 +843,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
         constexpr int kWords = DT * 16 + 2;
         const auto part = [&](int x) {
             return reinterpret_cast<uint64_t*>(parts) +
-                   ((size_t)place * splits + x) * (kWords / 2 * LANES) + threadIdx.x;
+                   ((size_t)place * splits + x) * (kWords / 2 * 256) + threadIdx.x;
         };
         const auto put = [](uint64_t* p, float x, float y) {
             __hip_atomic_store(p, __builtin_bit_cast(uint64_t, (f32x2){x, y}), __ATOMIC_RELAXED,
@@ -866,7 +860,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
             for (int e = 0; e < DT; e++)
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    put(mine + (1 + e * 8 + x) * LANES, o[e][2 * x], o[e][2 * x + 1]);
+                    put(mine + (1 + e * 8 + x) * 256, o[e][2 * x], o[e][2 * x + 1]);
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_s_waitcnt(0);
@@ -896,7 +890,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && DIM <= 128 ? 2 : 1) void pag
             for (int y = 0; y < 2; y++) {
                 ml[y] = get(from[y]);
 #pragma unroll
-                for (int z = 0; z < DT * 8; z++) v[y][z] = get(from[y] + (1 + z) * LANES);
+                for (int z = 0; z < DT * 8; z++) v[y][z] = get(from[y] + (1 + z) * 256);
             }
 #pragma unroll
             for (int y = 0; y < 2; y++) {

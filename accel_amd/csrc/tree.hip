@@ -4,9 +4,10 @@
 //
 // Here the rows are few and the contexts long and uneven, so the work is cut evenly
 // whatever the lengths: the steps (a tile of keys against a tile of rows) of all drafts
-// in one line a key-value head, a workgroup an equal stretch of a head's line.  Where
-// drafts have more rows than four waves take, workgroups have eight, and keys and values
-// are read once for up to 256 rows.
+// in one line a key-value head, a workgroup an equal stretch of a head's line.  Eight
+// waves a workgroup, keys and values read once for up to 256 rows, were tried and left:
+// 16 to 64 nodes over 32 contexts of 300 to 8000 took 217 us instead of 222, 9 drafts
+// seen through a window of 333 28.6 instead of 24.7.
 #include <hip/hip_runtime.h>
 
 #include "prompts.hpp"
@@ -46,20 +47,14 @@ __global__ __launch_bounds__(1024) void draft_sums_kernel(KvCache c, Attention a
     }
 }
 
-// Key-value heads' lines, and rows of a tile: eight waves a workgroup instead of two
-// workgroups of four where the drafts have more than 128 rows on average (16 drafts of 64
-// nodes after 4096: LINES64; of 16 nodes: LINES16).
+// Key-value heads' lines, and rows of a tile.
 struct Lines {
     int tokens;
     uint32_t heads;
-    bool wide;
 };
 Lines lines_of(const KvCache& c, const Attention& a) {
-    const int group = a.heads / c.heads;
-    const bool wide = !a.q_f32 && c.dim <= 128 &&
-                      (int64_t)a.rows * group > (int64_t)a.n * kRows;
-    const int rows = wide ? 2 * kRows : kRows, per = prompt_heads(group, rows);
-    return {prompt_tokens(group, rows), (uint32_t)(c.heads * ((group + per - 1) / per)), wide};
+    const int group = a.heads / c.heads, per = prompt_heads(group);
+    return {prompt_tokens(group), (uint32_t)(c.heads * ((group + per - 1) / per))};
 }
 constexpr int key_tile(int dim) { return dim <= 128 ? 64 : 32; }
 
@@ -75,15 +70,14 @@ hipError_t launch_paged_tree(Device* d, hipStream_t st, const KvCache& c, const 
                              int* status) {
     *status = ACCEL_OK;
     const Lines lines = lines_of(c, a);
-    // two workgroups of four waves a CU of a 16-bit type up to 128 dims, else one
-    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 && !lines.wide ? 2 : 1);
-    const int lanes = lines.wide ? 512 : 256;
+    // two workgroups a CU of a 16-bit type up to 128 dims, else one
+    const uint32_t slots = (uint32_t)d->cu_count * (!a.q_f32 && c.dim <= 128 ? 2 : 1);
     const uint32_t stretches = slots > lines.heads ? slots / lines.heads : 1;
     const uint32_t grid = lines.heads * stretches;
     const int wide = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
     // a line of one stretch is not cut, so there are no joins and no tickets
     const size_t part_words =
-        stretches > 1 ? 2 * (size_t)grid * lanes * (wide / 32 * 16 + 2) : 0;
+        stretches > 1 ? 2 * (size_t)grid * 256 * (wide / 32 * 16 + 2) : 0;
     const bool summed = a.n > 64;
     const size_t sums_words = summed ? ((size_t)a.n + 1) & ~(size_t)1 : 0;
     uint32_t *tickets = nullptr, *sums = nullptr;
@@ -105,38 +99,32 @@ hipError_t launch_paged_tree(Device* d, hipStream_t st, const KvCache& c, const 
     }
     const uint32_t stride = grid ? (uint32_t)(kWorkspaceCounterBytes / 4) / grid : 0;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(lanes), 0, st, c, a, sums, 0u, stretches, 0u,
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, c, a, sums, 0u, stretches, 0u,
                            tickets, stride, parts, d->fault_dev);
     };
     const bool full = c.dim == 64 || c.dim == 128 || c.dim == 256;
-    const auto dims = [&](auto bf16, auto qt, auto pt, auto waves) {
+    const auto dims = [&](auto bf16, auto qt, auto pt) {
         constexpr bool B = decltype(bf16)::value;
         constexpr int Q = decltype(qt)::value, P = decltype(pt)::value;
-        constexpr int W = decltype(waves)::value;
         if (c.dim <= 64)
-            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64, Drafts, W>)
-                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64, Drafts, W>);
+            full ? go(paged_prefill_kernel<B, Q, P, 64, true, 64, Drafts>)
+                 : go(paged_prefill_kernel<B, Q, P, 64, false, 64, Drafts>);
         else if (c.dim <= 128)
-            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64, Drafts, W>)
-                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64, Drafts, W>);
-        else if constexpr (W == 4)
-            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32, Drafts, W>)
-                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32, Drafts, W>);
+            full ? go(paged_prefill_kernel<B, Q, P, 128, true, 64, Drafts>)
+                 : go(paged_prefill_kernel<B, Q, P, 128, false, 64, Drafts>);
+        else
+            full ? go(paged_prefill_kernel<B, Q, P, 256, true, 32, Drafts>)
+                 : go(paged_prefill_kernel<B, Q, P, 256, false, 32, Drafts>);
     };
     const std::integral_constant<int, 1> one;
     const std::integral_constant<int, 2> two;
     const std::integral_constant<int, 3> three;
-    const std::integral_constant<int, 4> four;
-    const std::integral_constant<int, 8> eight;
     if (a.q_f32) {
-        if (c.bf16) dims(std::true_type(), three, three, four);
-        else dims(std::false_type(), two, two, four);
-    } else if (lines.wide) {
-        if (c.bf16) dims(std::true_type(), one, one, eight);
-        else dims(std::false_type(), one, one, eight);
+        if (c.bf16) dims(std::true_type(), three, three);
+        else dims(std::false_type(), two, two);
     } else {
-        if (c.bf16) dims(std::true_type(), one, one, four);
-        else dims(std::false_type(), one, one, four);
+        if (c.bf16) dims(std::true_type(), one, one);
+        else dims(std::false_type(), one, one);
     }
     return hipGetLastError();
 }
