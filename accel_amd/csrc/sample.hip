@@ -396,6 +396,7 @@ __device__ __forceinline__ float largest(const float (&x)[kStrip]) {
     return m;
 }
 
+constexpr uint32_t kHeld = 64;         // parts of a row whose distances are held
 constexpr int kFirsts = 24;            // searches of a row: 7, and up to 4 a border
 struct Scratch {
     union {
@@ -406,6 +407,7 @@ struct Scratch {
             uint64_t fine[kRing];      // a bin's words, cut into 1024
             uint64_t list[kFew];
             uint8_t near[kRing];       // bins that a border may lie in
+            uint8_t far[kHeld][kLanes];    // parts' lanes' distances
         };
         RowScratch slow;
     };
@@ -451,7 +453,7 @@ struct Window {
 // Whether a row's bins are whole numbers near which it can be weighed: places are
 // right to 2^-36 of a bin up to here, weights to 2^-40.5.
 __device__ __forceinline__ bool has_bins(float top, double per) {
-    return fabs((double)top * per) < 0x1p17 && per > 0x1p-60;
+    return fabs((double)top * per) < 0x1p17 && per > 0x1p-60 && per < 0x1p120;
 }
 
 // Adds a lane's logits that are in; the others' words go where nobody reads, without a
@@ -578,8 +580,15 @@ __device__ __forceinline__ int part_of(double r) {
 struct Range {
     float low, high;
 };
+// The edges are rounded to a logit's type, by less than 2^-6 of a bin.
 __device__ __forceinline__ Range range_of(const Ask& ask, int top, double per) {
-    return {uniform((float)((top - ask.hi - 1) / per)), uniform((float)((top - ask.lo + 1) / per))};
+    constexpr double kEdge = 1.0 / 64;
+    double low = top - ask.hi - 0.5 - kEdge, high = top - ask.lo + 0.5 + kEdge;
+    if (ask.part >= 0) {
+        low = top - ask.lo + 0.5 - (ask.part + 1) * (1.0 / kRing) - kEdge;
+        high = top - ask.lo + 0.5 - ask.part * (1.0 / kRing) + kEdge;
+    }
+    return {uniform((float)(low / per)), uniform((float)(high / per))};
 }
 // A lane's logits x: those that are asked for.
 template <typename F>
@@ -612,6 +621,22 @@ __device__ __forceinline__ void answer(Scratch& sh, const Ask& ask, int top, dou
                 atomicMax(&sh.most, key_of(v));
             }
         }
+    }
+}
+
+// The same of those of 32 tiles that a lane's bits name, whose blocks [first, last)
+// blocks_of(tile) gives.  A lane goes to the next that is its own.
+template <int DT, typename F>
+__device__ __forceinline__ void answer_tiles(Scratch& sh, const Ask& ask, int top, double per,
+                                             const Range& range, const Blocks<DT>& row,
+                                             uint32_t near, F blocks_of) {
+#pragma unroll 1
+    while (near) {
+        const uint2 b = blocks_of(__builtin_ctz(near));
+        near &= near - 1;
+        float v[2 * kStrip];
+        read_tile<DT>(row, b.x, b.y, 0, v);
+        answer(sh, ask, top, per, range, v, [&](int e) { return index_in<DT>(row, b.x, 0, e); });
     }
 }
 
@@ -1158,17 +1183,17 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
             __syncthreads();
         }
         done = finish<DT>(sh, s, r, rules, per, top, read_ring(sh, bin), [&](const Ask& ask) {
-            const Range range = range_of(ask, bin, per);
             const int near = bins ? 1 + ((w.top - bin + ask.hi) >> 2) : 0;
-#pragma clang loop unroll(disable)
-            for (uint32_t t = 0; t < strips; t += 2) {
-                const int code = far[t >> 1][threadIdx.x];
-                if (code && code > near) continue;
-                float v[2 * kStrip];
-                read_tile<DT>(row, 0, row.count, t, v);
-                answer(sh, ask, bin, per, range, v,
-                       [&](int e) { return index_in<DT>(row, 0, t, e); });
+            uint32_t tiles = 0;
+#pragma unroll
+            for (uint32_t t = 0; t < kTiles; t++) {
+                const int code = 2 * t < strips ? far[t][threadIdx.x] : kFar;
+                tiles |= !code || code <= near ? 1u << t : 0u;
             }
+            answer_tiles<DT>(sh, ask, bin, per, range_of(ask, bin, per), row, tiles,
+                             [&](uint32_t t) {
+                                 return make_uint2(t * 2 * kStripBlocks<DT>, row.count);
+                             });
         });
     }
     __syncthreads();
@@ -1178,7 +1203,6 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
 // Longer rows, and too few rows to fill the chip: a workgroup a part of up to one tile.
 // The last of a row's parts to end adds up their bins and goes on as above.
 constexpr int kBatch = 8;             // parts whose words are asked for at once
-constexpr uint32_t kCodes = 16;        // and whose lanes' distances
 constexpr int kMostParts = ACCEL_SAMPLE_WIDTH / (kTile * kLanes) + kBatch;
 struct Parts {
     uint64_t* rings;                   // [rows, parts, kRing]
@@ -1302,6 +1326,11 @@ __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Par
 #pragma clang loop unroll(disable)
         for (uint32_t i = 0; i < p.parts; i += kBatch) {
             uint64_t v[kBatch][kPer];
+            uint8_t code[kBatch];
+#pragma unroll
+            for (int x = 0; x < kBatch; x++)
+                code[x] = get(p.far + (slot0 + (i + x < p.parts ? i + x : i)) * kLanes +
+                              threadIdx.x);
 #pragma unroll
             for (int x = 0; x < kBatch; x++)
 #pragma unroll
@@ -1311,6 +1340,9 @@ __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Par
                     const int bin = big - (int)(threadIdx.x * kPer) - j;
                     v[x][j] = get(p.rings + (slot0 + at) * kRing + (bin & (kRing - 1)));
                 }
+            if (i < kHeld)
+#pragma unroll
+                for (int x = 0; x < kBatch; x++) sh.far[i + x][threadIdx.x] = code[x];
 #pragma unroll
             for (int x = 0; x < kBatch; x++)
 #pragma unroll
@@ -1323,29 +1355,28 @@ __global__ __launch_bounds__(kLanes, 4) void sample_parts_kernel(Sampling s, Par
                 }
         }
         done = finish<DT>(sh, s, r, rules, per, top, sum, [&](const Ask& ask) {
-            const Range range = range_of(ask, big, per);
             const int below = big - ask.hi;
+            const Range range = range_of(ask, big, per);
 #pragma clang loop unroll(disable)
-            for (uint32_t i = 0; i < p.parts; i += kCodes) {
+            for (uint32_t i = 0; i < p.parts; i += 32) {
                 uint32_t near = 0;
-                uint8_t code[kCodes];
+                for (uint32_t j = 0; j < 32 && i + j < p.parts; j += kBatch) {
+                    uint8_t code[kBatch];
 #pragma unroll
-                for (uint32_t j = 0; j < kCodes; j++)
-                    code[j] = get(p.far + (slot0 + (i + j < p.parts ? i + j : i)) * kLanes +
-                                  threadIdx.x);
+                    for (uint32_t x = 0; x < kBatch; x++) {
+                        const uint32_t at = i + j + x < p.parts ? i + j + x : i;
+                        code[x] = i < kHeld ? sh.far[at][threadIdx.x]
+                                            : get(p.far + (slot0 + at) * kLanes + threadIdx.x);
+                    }
 #pragma unroll
-                for (uint32_t j = 0; j < kCodes; j++) {
-                    const int b = i + j < p.parts ? parts[i + j].bin : -kNone;
-                    near |= b - 4 * (int)code[j] >= below ? 1u << j : 0u;
+                    for (uint32_t x = 0; x < kBatch; x++) {
+                        const int b = i + j + x < p.parts ? parts[i + j + x].bin : -kNone;
+                        near |= b - 4 * (int)code[x] >= below ? 1u << (j + x) : 0u;
+                    }
                 }
-                while (near) {
-                    const uint32_t at = i + __builtin_ctz(near), first = begin_of(at);
-                    near &= near - 1;
-                    float v[2 * kStrip];
-                    read_tile<DT>(row, first, begin_of(at + 1), 0, v);
-                    answer(sh, ask, big, per, range, v,
-                           [&](int e) { return index_in<DT>(row, first, 0, e); });
-                }
+                answer_tiles<DT>(sh, ask, big, per, range, row, near, [&](uint32_t j) {
+                    return make_uint2(begin_of(i + j), begin_of(i + j + 1));
+                });
             }
         });
     }

@@ -240,6 +240,21 @@ def test_logits_at_the_ends_of_the_range(dev, scale):
     check(dev, x, [0.2, 0.9, 0.5, 0.7], few=0.3, temperature=np.float32(scale))
 
 
+@pytest.mark.parametrize("dtype,step", [(F32, 2.0 ** -149), (BF16, 2.0 ** -133)],
+                         ids=["f32", "bf16"])
+@pytest.mark.parametrize("steps", [0.5, 2.0, 300.0])
+def test_temperatures_of_a_few_of_the_least_steps(dev, dtype, step, steps):
+    """Logits that are small multiples of a type's least number, and temperatures to
+    match them: what lies between two bins' edges then holds no f32."""
+    rng = np.random.default_rng(11)
+    rows = 8
+    x = np.round(rng.standard_normal((rows, 20000)) * 3 * steps) * step
+    t = max(step * steps, 2.0 ** -149)
+    check(dev, x.astype(np.float32), rng.random(rows), dtype, few=0.3, temperature=t,
+          top_p=[1, 0.9, 0.5, 1, 0.8, 1, 1, 0.95], top_k=[0, 0, 0, 700, 50, 1, 0, 0],
+          min_p=[0, 0, 0, 0, 0, 0, 0.1, 0.01])
+
+
 def test_far_from_zero(dev):
     """Weights go by the distance to the largest, however far from zero both are."""
     rng = np.random.default_rng(17)
