@@ -95,6 +95,12 @@ struct NoPaths {};
 struct DraftWork {
     uint32_t tiles, steps;
 };
+// Sums of them.  They stay below kTooMany for offsets that ascend; where entries share
+// rows they may not, and no step is taken then.
+constexpr uint32_t kTooMany = 0xffffffffu;
+__device__ __forceinline__ uint32_t more_steps(uint32_t x, uint32_t y) {
+    return x + y < x ? kTooMany : x + y;
+}
 template <int KT>
 __device__ __forceinline__ DraftWork work_of(const Attention& a, uint32_t len, uint32_t nodes,
                                              int tokens) {
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
-            if (lane >= d) v += up;
+            if (lane >= d) v = TREE ? more_steps(v, up) : v + up;
         }
         cut.lane_sum = v;
         cut.tiles = lane_value(v, 63);
@@ -225,6 +231,10 @@ __global__ __launch_bounds__(256, QT == 1 && DIM <= 128 ? 2 : 1) void paged_pref
     uint32_t tile = 0;
     uint32_t u = 0, u_end = 0;           // drafts: the stretch's steps, to go and past
     if constexpr (TREE) {
+        if (cut.tiles == kTooMany) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) report(fault, kFaultDraft);
+            return;
+        }
         const uint32_t even = (uint32_t)(((uint64_t)cut.tiles + splits - 1) / splits);
         cut.chunk = even > kLeastDraft<F32> ? even : kLeastDraft<F32>;
         u = draft_cut<KT>(cut, c, a, tokens, order);

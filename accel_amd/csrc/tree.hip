@@ -33,17 +33,17 @@ __global__ __launch_bounds__(1024) void draft_sums_kernel(KvCache c, Attention a
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d, 64);
-            if (lane >= d) v += up;
+            if (lane >= d) v = more_steps(v, up);
         }
         __syncthreads();
         if (lane == 63) sh[wave] = v;
         __syncthreads();
         uint32_t before = carry;
         for (int w = 0; w < 16; w++) {
-            before += w < wave ? sh[w] : 0u;
-            carry += sh[w];
+            before = w < wave ? more_steps(before, sh[w]) : before;
+            carry = more_steps(carry, sh[w]);
         }
-        if (i < a.n) sums[i] = before + v;
+        if (i < a.n) sums[i] = more_steps(before, v);
     }
 }
 
@@ -63,7 +63,7 @@ constexpr int key_tile(int dim) { return dim <= 128 ? 64 : 32; }
 bool paged_tree_counts(const KvCache& c, const Attention& a) {
     const uint64_t tiles = (uint64_t)a.rows / lines_of(c, a).tokens + a.n;
     const uint64_t steps = ((uint64_t)c.slots << c.shift) / key_tile(c.dim) + 3;
-    return tiles <= 0xffffffffu / steps;
+    return tiles <= (kTooMany - 1) / steps;
 }
 
 hipError_t launch_paged_tree(Device* d, hipStream_t st, const KvCache& c, const Drafts& a,

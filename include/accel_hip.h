@@ -750,7 +750,9 @@ int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q,
  * not finite are as in accel_paged_prefill.  A node without a parent starts a
  * tree of its own.  Rows of a node on whose path a parent is not below its
  * child, of an entry of more than ACCEL_DRAFT_NODES nodes and of one with more
- * nodes than its sequence has positions are zeros, and reported. */
+ * nodes than its sequence has positions are zeros, and reported.  Offsets that do
+ * not ascend leave it open what the rows that entries share hold; where such
+ * entries' work passes 32 bits, nothing is written, and that is reported. */
 int accel_paged_tree_attention(int dev, void* stream, const accel_tensor_t* q,
                                const accel_tensor_t* offsets, const accel_tensor_t* parents,
                                const accel_kv_cache_t* cache, int64_t layer,

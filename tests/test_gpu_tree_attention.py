@@ -187,6 +187,25 @@ def test_bad_pages_are_left_out(dev):
     c.check()
 
 
+@pytest.mark.parametrize("n", [64, 100])
+def test_entries_that_share_rows_past_32_bits_of_work(dev, n):
+    """Offsets that do not ascend: 8 tiles of rows against 2^24 tiles of keys, so often
+    that their number passes 32 bits.  No step of it is taken."""
+    page, slots = 4096, 1 << 18
+    u = lambda x: dev.upload(np.asarray(x, np.uint32), U32)  # noqa: E731
+    c = dev.kv_cache(1, 1, 1, page, 8, 1, slots)
+    c.lens.write(np.array([page * slots], np.uint32))
+    off = np.zeros(n + 1, np.uint32)
+    off[1::2] = 256
+    q = dev.upload(np.zeros((256, 4, 8), np.uint16), BF16)
+    out = dev.upload(np.full((256, 4, 8), 77, np.uint16), BF16)
+    dev.PagedTreeAttention(q, u(off), u(trees([256])), c, out, seqs=u(np.zeros(n)))
+    with pytest.raises(accel_amd.AccelError, match="draft's parents"):
+        dev.sync()
+    assert (out.numpy() == 77).all()
+    c.free()
+
+
 def test_a_report_is_read_once(dev):
     c = Tree(dev, [100], [40])
     c.parents[7] = 7
