@@ -255,13 +255,13 @@ constexpr int kCopies = 8;             // of each bin's word, for lanes that mee
 constexpr int kReach = 736;            // bins below the largest's that count
 constexpr int kFew = 64;               // logits that a wave puts in order
 
-// A bin's word: 2^49 for each logit, and 2^39 (2^(r / 16) - kLeast).  Up to 2^14 of
-// them: the lower sum stays below 2^39 0.0434 2^14 < 2^49.
-constexpr int kUnit = 39, kCount = 49;
+// A bin's word: 2^49 for each logit, and 2^38 (2^(r / 16) - kLeast).  Up to 30720 of
+// them: their number is below 2^15 and the lower sum below 2^38 0.0434 30720 < 2^49.
+constexpr int kUnit = 38, kCount = 49;
 constexpr double kLeast = 1002.0 / 1024;               // below 2^(-1 / 32)
 constexpr uint64_t kLeastUnits = 1002ull << (kUnit - 10);
 constexpr uint64_t kRest = (1ull << kCount) - 1;
-constexpr uint32_t kMostEach = 1u << 14;
+constexpr uint32_t kMostEach = 30720;
 
 // 2^(r / 16), by the fifth power of its series: off by (ln 2 / 32)^6 / 720 = 2^-42.7 of
 // it for |r| <= 1/2.  `one` is the series' first number.
@@ -275,7 +275,7 @@ __device__ __forceinline__ double sixteenth_of(double r, double one) {
     q = __builtin_fma(q, r, c1);
     return __builtin_fma(q, r, one);
 }
-// A logit's bin, its place r in it and its part of the bin's word, rounded by 2^-40.
+// A logit's bin, its place r in it and its part of the bin's word, rounded by 2^-39.
 // Bins have to be the same wherever they are asked for, so no sum is fused here that is
 // not written so.
 struct Binned {
@@ -286,7 +286,7 @@ struct Binned {
 __device__ __forceinline__ Binned binned(float x, double per) {
 #pragma clang fp contract(off)
     constexpr double kMagic = 6755399441055744.0;      // 3 * 2^51: the sum's low word is whole
-    constexpr double kBase = 8192.0;                   // its last place is 2^-39
+    constexpr double kBase = 16384.0;                  // its last place is 2^-38
     const double e = (double)x * per;
     const double t = e + kMagic;
     const double r = e - (t - kMagic);
@@ -299,7 +299,7 @@ __device__ __forceinline__ Binned binned(float x, double per) {
 __device__ __forceinline__ double bins_per(const Rules& r) {
     return uniform(16 * 1.44269504088896340736 / r.temperature);
 }
-// A weight, or a sum of them, in units of 2^-39 of 2^(bin / 16), exact.
+// A weight, or a sum of them, in units of 2^-38 of 2^(bin / 16), exact.
 __device__ __forceinline__ uint64_t units(uint64_t count, uint64_t rest) {
     return count * kLeastUnits + rest;
 }
@@ -1110,7 +1110,7 @@ __device__ __forceinline__ void give_first(const Sampling& s, uint32_t row, uint
 // Rows of up to kTiles tiles, a workgroup each, two workgroups a CU.  Of each tile of a
 // lane it is kept how far its largest logit is from the window's top, so a second look
 // goes only to what may hold something near a border.
-constexpr int kTiles = 16;
+constexpr int kTiles = 30;             // what LDS holds beside another workgroup
 constexpr int kTile = 2 * kStrip;
 constexpr int kFar = 255;              // below the window; nearer ones are 253 at most
 static_assert(kTiles * kTile * kLanes / kCopies <= kMostEach, "a word's count and sum");
@@ -1200,7 +1200,7 @@ __global__ __launch_bounds__(kLanes, 4) void sample_whole_kernel(Sampling s, uin
     if (!done) draw_slowly<DT>(sh.slow, s, r, rules, top);
 }
 
-// Longer rows, and too few rows to fill the chip: a workgroup a part of up to one tile.
+// Longer rows, and too few rows to fill the chip: a workgroup a tile of a row.
 // The last of a row's parts to end adds up their bins and goes on as above.
 constexpr int kBatch = 8;             // parts whose words are asked for at once
 constexpr int kMostParts = ACCEL_SAMPLE_WIDTH / (kTile * kLanes) + kBatch;
@@ -1391,7 +1391,12 @@ hipError_t launch(Device* d, hipStream_t st, const Sampling& s, int* status) {
     const uint32_t blocks = (s.width + E - 1) / E + 1;
     constexpr uint32_t kMost = kTile / E * kLanes;
     const uint32_t least = (blocks + kMost - 1) / kMost;
-    if (least <= 1 || (least <= kTiles && s.rows >= (uint32_t)d->cu_count)) {
+    // A row's workgroup takes 20 us and 1.45 a tile.  A workgroup a tile takes 24 to 27 us
+    // whatever the width, as long as all run at once (rows of 16 tiles, us: one 43 whole
+    // and 27 in parts, 16 46 and 32, 32 46 and 43, 64 48 and 71; of 8 tiles one 30 and 23;
+    // of 4 one 24 and 24, 32 26 and 26).
+    if (least <= 4 ||
+        (least <= kTiles && (uint64_t)s.rows * least > 2 * (uint32_t)d->cu_count)) {
         // a grid's lanes are counted in 32 bits
         constexpr uint32_t kRows = 1u << 22;
         for (uint32_t first = 0; first < s.rows; first += kRows) {
@@ -1400,12 +1405,8 @@ hipError_t launch(Device* d, hipStream_t st, const Sampling& s, int* status) {
         }
         return hipGetLastError();
     }
-    uint32_t parts = 2 * (uint32_t)d->cu_count / s.rows;
-    const uint32_t most = (blocks + kMost / 2 - 1) / (kMost / 2);
-    parts = parts < most ? parts : most;
-    parts = parts > least ? parts : least;
     Parts p{};
-    p.blocks = (blocks + parts - 1) / parts;
+    p.blocks = (blocks + least - 1) / least;
     p.parts = (blocks + p.blocks - 1) / p.blocks;
     // launches of up to 64 MiB of rings, and of as many rows as there are tickets
     uint32_t rows = (64u << 20) / (p.parts * kRing * 8);

@@ -3,7 +3,7 @@
 A token may differ only where a border lies nearer to a running sum than the sums'
 roundings.  A weight is 2^(i / 16) 2^(r / 16): the exponent's product is off by
 2^-53 of up to 2^17, 2^-36 sixteenths of a power of two or 2^-40.5 of the weight,
-the series by 2^-42.7 and its rounding by 2^-40, together less than 2^-38.9; a row that
+the series by 2^-42.7 and its rounding by 2^-39, together less than 2^-38.4; a row that
 is weighed otherwise has weights rounded by 2^-46 of the largest for each of up to 2^17
 logits.  A sum's share is off by no more than its weights', plus that, and the sums of
 bins by 2^-52 a step of 10.  The oracle's margin (a share of the whole) is held against
