@@ -1,7 +1,10 @@
 // What follows the attention of drafts: the walk down a tree along the tokens that
 // were sampled, and the accepted nodes' keys and values moved up behind their
-// context.  Both are chains of a few dependent reads; the second's bytes are those
-// of the rows that move, in every layer.
+// context.  Both are chains of a few dependent reads (a walk 2.2 us, of 256 trees of up
+// to 64 nodes 4.2); the second's bytes are those of the rows that move, in every layer
+// (8 of up to 64 nodes of 48 sequences, 16 layers, 8 heads of 128: 20 MB read and written
+// together in 7.8 us after a plan of 3.7).  A launch of its own for the plan: whether a
+// sequence is served, and its pages shared, has to be known before the first row moves.
 #include <hip/hip_runtime.h>
 
 #include "internal.hpp"

@@ -16,6 +16,14 @@
 // Bins are absolute, not relative to the row's largest, so one pass is enough: a ring
 // of 1024 bins (64 factors of two), set by the first logits seen.  Weights below 2^-46
 // of the largest are left out.
+//
+// What bounds it: for many rows issue, 29 VALU instructions a logit and one atomic on
+// LDS, of eight copies of a bin (512 rows of 128000 in f32 88 to 118 us, 262 MB at 2.2 to
+// 3 TB/s; digit by digit of the keys, four looks a border, it was 1689).  A row's chain
+// after its pass, some 20 us of barriers and a look, no other workgroup fills where all
+// rows run at once.  For few rows that chain: one row of 128000 26 us, 64 of 100003 in
+// bf16 47; nearly flat ones, with hundreds of logits in a border's bin and two more looks
+// a border, 17 of 32001 in f16 56.
 #include <hip/hip_runtime.h>
 
 #include "internal.hpp"
@@ -255,13 +263,13 @@ constexpr int kCopies = 8;             // of each bin's word, for lanes that mee
 constexpr int kReach = 736;            // bins below the largest's that count
 constexpr int kFew = 64;               // logits that a wave puts in order
 
-// A bin's word: 2^49 for each logit, and 2^38 (2^(r / 16) - kLeast).  Up to 30720 of
-// them: their number is below 2^15 and the lower sum below 2^38 0.0434 30720 < 2^49.
+// A bin's word: 2^49 for each logit, and 2^38 (2^(r / 16) - kLeast).  Up to 30 2^10
+// of them: their number is below 2^15 and the lower sum below 2^38 0.0434 30 2^10 < 2^49.
 constexpr int kUnit = 38, kCount = 49;
 constexpr double kLeast = 1002.0 / 1024;               // below 2^(-1 / 32)
 constexpr uint64_t kLeastUnits = 1002ull << (kUnit - 10);
 constexpr uint64_t kRest = (1ull << kCount) - 1;
-constexpr uint32_t kMostEach = 30720;
+constexpr uint32_t kMostEach = 30 << 10;
 
 // 2^(r / 16), by the fifth power of its series: off by (ln 2 / 32)^6 / 720 = 2^-42.7 of
 // it for |r| <= 1/2.  `one` is the series' first number.

@@ -4,10 +4,18 @@
 //
 // Here the rows are few and the contexts long and uneven, so the work is cut evenly
 // whatever the lengths: the steps (a tile of keys against a tile of rows) of all drafts
-// in one line a key-value head, a workgroup an equal stretch of a head's line.  Eight
-// waves a workgroup, keys and values read once for up to 256 rows, were tried and left:
-// 16 to 64 nodes over 32 contexts of 300 to 8000 took 217 us instead of 222, 9 drafts
-// seen through a window of 333 28.6 instead of 24.7.
+// in one line a key-value head, a workgroup an equal stretch of a head's line (16 to 64
+// nodes over 32 contexts of 300 to 8000, 32/8 heads of 128 in bf16: 193 us, 243 with the
+// prompts' shares).
+//
+// What bounds it: issue, as the prompts (those trees run at 460 TFLOP/s, the prompts at
+// 600; 16 of 64 nodes after 4096 at 570, the keys' bytes are half of the time); for one
+// small tree the chain before its first keys (4.7 us), a busy wave's steps (2 us each) and
+// joins (4.2 each).
+// Tried and left: eight waves a workgroup, keys and values read once for up to 256 rows
+// (the batch above 217 us instead of 222 call upon call, 9 drafts seen through a window of
+// 333 28.6 instead of 24.7); three tiles of keys on their way instead of one (219 and 214);
+// values read some products ahead, pages asked for beside the parents (the same).
 #include <hip/hip_runtime.h>
 
 #include "prompts.hpp"

@@ -28,9 +28,9 @@
  * []uint16", internal/kernels/differential_darwin_test.go:242-244).
  *
  * Workspace.  Kernels that reduce across workgroups (the decode product's
- * K split, the joins of paged attention), the grouped products (segment
- * offsets, tile lists) and the paged cache's planning use a per-device
- * workspace owned by the library.  Two operator calls that run
+ * K split, the joins of paged attention, sampling's rows in parts), the
+ * grouped products (segment offsets, tile lists) and the paged cache's
+ * planning use a per-device workspace owned by the library.  Two operator calls that run
  * concurrently on different streams of one device race on it; serialize
  * them or use one stream per device.  The workspace grows on demand outside
  * graph capture; a call that would need it to grow on a capturing stream is
