@@ -22,8 +22,8 @@
 // 3 TB/s; digit by digit of the keys, four looks a border, it was 1689).  A row's chain
 // after its pass, some 20 us of barriers and a look, no other workgroup fills where all
 // rows run at once.  For few rows that chain: one row of 128000 26 us, 64 of 100003 in
-// bf16 47; nearly flat ones, with hundreds of logits in a border's bin and two more looks
-// a border, 17 of 32001 in f16 56.
+// bf16 49; nearly flat ones, with hundreds of logits in a border's bin and another look a
+// border, 17 of 32001 in f16 51.
 #include <hip/hip_runtime.h>
 
 #include "internal.hpp"
