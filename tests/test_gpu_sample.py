@@ -122,6 +122,22 @@ def test_a_large_vocabulary(dev, dtype):
     check(dev, rng.standard_normal((rows, 262147)) * 3, rng.random(rows), dtype, few=0.15, **kw)
 
 
+@types
+@pytest.mark.parametrize("std", [0.05, 0.5, 2.0])
+@pytest.mark.parametrize("rows,width", [(16, 45001), (110, 45001), (16, 230003), (20, 230003),
+                                        (16, 300007)])
+def test_long_rows_whole_and_in_parts(dev, dtype, std, rows, width):
+    """6, 29 and 37 tiles a row, on both sides of where rows are cut, with many logits
+    and with few near the borders."""
+    rng = np.random.default_rng(rows + width)
+    pick = np.arange(rows) % len(SETTINGS)
+    kw = {k: [SETTINGS[i].get(k, d) for i in pick]
+          for k, d in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))}
+    x = (rng.standard_normal((rows, width), np.float32) * std).astype(np.float32)
+    x[1::4, width // 3:width // 3 + 9000] = -np.inf
+    check(dev, x, rng.random(rows), dtype, few=0.15, **kw)
+
+
 def test_a_very_large_row(dev):
     rng = np.random.default_rng(9)
     check(dev, rng.standard_normal((2, (1 << 22) + 3)) * 3, [0.3, 0.6], few=1.0,
@@ -363,5 +379,13 @@ def test_calls_repeat_themselves(dev):
     for _ in range(4):
         again = draw(dev, x, u, top_p=0.9)
         assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+    # rows in parts, whichever of them ends last
+    x = rng.standard_normal((5, 150001)) * 1.5
+    first = draw(dev, x, u[:5], top_p=0.9)
+    for _ in range(4):
+        again = draw(dev, x, u[:5], top_p=0.9)
+        assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+    x = rng.standard_normal((40, 30011)) * 1.5
+    first = draw(dev, x, u, top_p=0.9)
     # the logarithms are asked for or not
     assert np.array_equal(draw(dev, x, u, top_p=0.9, logprobs=False)[0], first[0])

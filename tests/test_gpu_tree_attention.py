@@ -92,6 +92,15 @@ def test_groups(dev, q, kv, heads, kv_heads):
     Tree(dev, [85, 150], [45, 10], heads=heads, kv_heads=kv_heads, q=q, kv=kv, seed=heads).check()
 
 
+@pytest.mark.parametrize("q,kv", [(F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("n", [2, 66])
+def test_more_heads_than_workgroups(dev, q, kv, n):
+    """A key-value head's whole line is one workgroup's then, and none of it is cut."""
+    nodes = [5, 33] if n == 2 else [3] * 65 + [40]
+    Tree(dev, [m + 30 + i % 7 for i, m in enumerate(nodes)], nodes, heads=600, kv_heads=600,
+         dim=8, q=q, kv=kv).check(window=0 if n == 2 else 20)
+
+
 @pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 4096])
 def test_pages(dev, page):
     Tree(dev, [page + 9, 2 * page, 40], [9, 30 if page > 8 else 16, 40], page=page,
