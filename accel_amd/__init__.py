@@ -137,6 +137,7 @@ class SamplingDesc(ctypes.Structure):
 
 NO_TOKEN = 0xffffffff
 DRAFT_NODES = 256
+DRAFT_REFUSED = 0xfffffffe
 
 QFMT_AWQ, QFMT_GPTQ, QFMT_GPTQ_V2 = 1, 2, 3
 

@@ -43,10 +43,9 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(
         const Rows r = rows_of(offsets, rows, i);
         uint32_t* out = path + (size_t)i * width;
         uint32_t count = 0, last = ACCEL_KV_NONE;
-        if (r.count > ACCEL_DRAFT_NODES) {
-            if (lane == 0)
-                __hip_atomic_fetch_or(fault, kFaultDraft, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_SYSTEM);
+        const bool refused = r.count > ACCEL_DRAFT_NODES;
+        if (refused) {
+            if (lane == 0) report(fault, kFaultDraft);
         } else if (r.count) {
             uint32_t token[kEach], parent[kEach], drawn[kEach];
 #pragma unroll
@@ -77,7 +76,9 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(
                 at = found;
             }
         }
-        for (uint32_t c = count + lane; c < width; c += 64) out[c] = ACCEL_KV_NONE;
+        // a count of 0 alone would have the keep take all of the sequence's nodes back
+        for (uint32_t c = count + lane; c < width; c += 64)
+            out[c] = refused && c == 0 ? ACCEL_DRAFT_REFUSED : ACCEL_KV_NONE;
         if (lane == 0) {
             counts[i] = count;
             next[i] = last;
@@ -122,7 +123,8 @@ __global__ __launch_bounds__(64) void kv_keep_plan_kernel(KvCache c, const uint3
                 wrong = kFaultKvSequence;
             } else if (len > cap || nodes > len) {
                 wrong = kFaultKvPage;
-            } else if (count > width || count > nodes) {
+            } else if (count > width || count > nodes ||
+                       (count == 0 && path[(size_t)i * width] == ACCEL_DRAFT_REFUSED)) {
                 wrong = kFaultDraft;
             } else {
                 const uint32_t first = len - nodes;

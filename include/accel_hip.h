@@ -798,7 +798,10 @@ int accel_sample(int dev, void* stream, const accel_tensor_t* logits, const acce
  * ACCEL_KV_NONE; counts (u32 [n]) how many; next (u32 [n]) the token sampled at
  * the last, the sequence's new token, whose key and value the next step appends.
  * ACCEL_NO_TOKEN ends a walk.  An entry without nodes has count 0 and next
- * ACCEL_NO_TOKEN, and so has one of more than ACCEL_DRAFT_NODES, which is reported. */
+ * ACCEL_NO_TOKEN, and so has one of more than ACCEL_DRAFT_NODES, which is reported
+ * and whose path begins with ACCEL_DRAFT_REFUSED: accel_kv_keep leaves its sequence
+ * as it is. */
+#define ACCEL_DRAFT_REFUSED 0xfffffffeu
 int accel_tree_accept(int dev, void* stream, const accel_tensor_t* tokens,
                       const accel_tensor_t* parents, const accel_tensor_t* offsets,
                       const accel_tensor_t* sampled, accel_tensor_t* path,
@@ -809,8 +812,9 @@ int accel_tree_accept(int dev, void* stream, const accel_tensor_t* tokens,
  * that path[i] (u32 [n, width]) names, ascending from 0 at the first of them.  In
  * every layer their keys and values move up to follow each other, the length becomes
  * that of what is left, and pages past it are given back.  A count of 0 takes all of
- * those positions back.  Left as it is and reported is an entry whose path does not
- * ascend, names a position past the last or is shorter than its count; one of more
+ * those positions back, unless the path begins with ACCEL_DRAFT_REFUSED.  Left as it is
+ * and reported is an entry with such a path; one whose path does not ascend, names a
+ * position past the last or is shorter than its count; one of more
  * positions than its sequence has, or with no page where a row moves; one that would
  * move a row into a page that another sequence has too; a sequence index outside the
  * cache; and one of two entries with one sequence (not specified which).

@@ -9,6 +9,7 @@ import numpy as np
 
 NONE = 0xffffffff
 NODES = 256
+REFUSED = 0xfffffffe
 
 
 def line_of(parents, t):
@@ -118,6 +119,7 @@ def accept(tokens, parents, offsets, sampled, width):
         first, m = int(offsets[i]), int(offsets[i + 1]) - int(offsets[i])
         if m > NODES:
             left_out.append(i)
+            path[i, 0] = REFUSED
         if m <= 0 or m > NODES:
             continue
         at = 0
@@ -150,6 +152,7 @@ def keep(pages, path, counts, offsets, seqs=None):
         L = int(pages.lens[s]) - m
         p = [int(x) for x in path[i][:k]]
         ok = k <= min(m, len(path[i])) and all(t < m for t in p)
+        ok = ok and (k > 0 or int(path[i][0]) != REFUSED)
         ok = ok and all(a < b for a, b in zip(p, p[1:]))
         if ok:
             for c, t in enumerate(p):

@@ -1,0 +1,52 @@
+"""What a step over drafts does to the cache where something in it cannot be served:
+each call against its restatement (oracle/draft_np.py, oracle/kvcache_np.py), whole
+state compared bit for bit."""
+import numpy as np
+import pytest
+
+import accel_amd
+from accel_amd import KV_NONE, NO_TOKEN
+from oracle import draft_np
+from test_gpu_draft import Keeps, run_accept
+from test_gpu_tree_attention import trees
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("width", [1, 9, 300])
+def test_a_draft_that_the_walk_refuses_is_left_by_the_keep(dev, width):
+    """The walk's outputs go to the keep as they are: sequences whose draft is too large
+    stay as they were, and the others are served."""
+    rng = np.random.default_rng(width)
+    nodes, seqs = [257, 9, 0, 300, 256], [0, 1, 2, 4, 5]
+    off = np.concatenate([[0], np.cumsum(nodes)]).astype(np.uint32)
+    b = Keeps(dev, pages=200, sequences=7, slots=60)
+    b.reserve([40, 10, 21, 8, 33, 3, 50])
+    b.reserve(nodes, seqs)
+    before = b.m.lens.copy(), b.m.tables.copy()
+    T = int(off[-1])
+    token, par, drawn = rng.integers(0, 2, T), trees(nodes, 1), rng.integers(0, 2, T)
+    ins, outs = run_accept(dev, token, par, off, drawn, width)
+    dev.KVKeep(b.c, outs[0], outs[1], b.u32(off), b.u32(seqs))
+    path, counts, nxt, refused = draft_np.accept(token, par, off, drawn, width)
+    assert refused == [0, 3]
+    draft_np.keep(b.m, path, counts, off, seqs)
+    assert b.m.left_out == [0, 3]
+    b.settle()
+    for got, want in zip(outs, (path, counts, nxt)):
+        assert np.array_equal(got.numpy(), want)
+    assert nxt[0] == nxt[3] == NO_TOKEN
+    for s in (0, 4):
+        assert b.m.lens[s] == before[0][s] and (b.m.tables[s] == before[1][s]).all()
+    assert b.m.lens[1] < before[0][1] and b.m.lens[2] == 21
+    for x in ins + outs:
+        x.free()
+
+
+def test_a_count_of_zero_takes_back_more_than_a_draft(dev):
+    """As the header says of it, whatever else the path holds."""
+    b = Keeps(dev, pages=200, sequences=3, slots=60)
+    b.reserve([20, 30, 40])
+    b.reserve([300, 257, 5])
+    b.keep([[KV_NONE, 7], [0, 0], [3, 2]], [0, 0, 0], [300, 257, 5])
+    assert b.m.lens.tolist() == [20, 30, 40]
