@@ -24,7 +24,7 @@ void clear_error();
 // instead of producing its result.
 constexpr uint32_t kFaultWaitGaveUp = 1u;     // a split-K hand-off's bounded wait ran out
 constexpr uint32_t kFaultKvRoom = 2u;         // no free page, or no slot left in a table
-constexpr uint32_t kFaultKvPage = 4u;         // no page where a position is read or written
+constexpr uint32_t kFaultKvPage = 4u;         // no page where a position is read, or none of its own where written
 constexpr uint32_t kFaultKvSequence = 8u;     // a sequence or page index that cannot be served
 constexpr uint32_t kFaultDraft = 16u;         // a draft whose parents or sizes cannot be served
 constexpr uint32_t kFaultKv = kFaultKvRoom | kFaultKvPage | kFaultKvSequence | kFaultDraft;

@@ -301,15 +301,18 @@ __device__ __forceinline__ void append_item(const KvCache& c, size_t layer_elems
         return;
     }
     const uint32_t chunks = c.dim >> 3, h = part / chunks, d = (part - h * chunks) * 8;
+    // A sequence that was shortened may end in a page that a branch has too: no row is
+    // stored there.  Asked for beside the row, which is as far away.
+    const uint32_t names = c.refs[page];
     const size_t from = ((size_t)row * c.heads + h) * c.dim + d;
     const size_t to = layer_elems +
                       ((((size_t)page * c.heads + h) << c.shift) + (pos & ((1u << c.shift) - 1))) *
                           c.dim + d;
+    u32x4 out[2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const void* src = x ? v : k;
-        uint16_t* dst = (x ? c.values : c.keys) + to;
-        u32x4 o;
+        u32x4& o = out[x];
         if (dtype == ACCEL_F32) {
             const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(src) + from);
             const u32x4 a = p[0], b = p[1];
@@ -329,8 +332,13 @@ __device__ __forceinline__ void append_item(const KvCache& c, size_t layer_elems
                            (uint32_t)narrow(widen((uint16_t)(o[j] >> 16), !c.bf16), c.bf16) << 16;
             }
         }
-        *reinterpret_cast<u32x4*>(dst) = o;
     }
+    if (names > 1) {
+        report(fault, kFaultKvPage);
+        return;
+    }
+    *reinterpret_cast<u32x4*>(c.keys + to) = out[0];
+    *reinterpret_cast<u32x4*>(c.values + to) = out[1];
 }
 __global__ __launch_bounds__(256) void kv_append_kernel(KvCache c, size_t layer_elems,
                                                         const void* k, const void* v,

@@ -189,11 +189,12 @@ int take_fault(Device* d) {
     } known[] = {
         {kFaultWaitGaveUp, "a split-K hand-off's bounded wait gave up"},
         {kFaultKvRoom, "a key-value pool had no free page, or a table no slot left"},
-        {kFaultKvPage, "a key-value table names no page for a position read or written"},
+        {kFaultKvPage, "a key-value table names no page for a position read or written, or one "
+                       "that another sequence has too for a position written"},
         {kFaultKvSequence, "a sequence or page index cannot be served"},
         {kFaultDraft, "a draft's parents, its path or its size cannot be served"},
     };
-    char what[320] = "";
+    char what[512] = "";
     uint32_t rest = f;
     for (const auto& k : known) {
         if (!(f & k.bit)) continue;

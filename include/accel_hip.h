@@ -647,8 +647,8 @@ int accel_kv_reserve(int dev, void* stream, const accel_kv_cache_t* cache,
  * positions of sequence seqs[i], as accel_kv_reserve left its length.  offsets
  * u32 [n+1], ascending from 0; NULL: one row an entry, n = T.  seqs u32 [n];
  * NULL: i.  Rows past the last offset and rows of ACCEL_KV_NONE are skipped.
- * A position before the sequence's first, or without a page, is skipped and
- * reported.  Of two entries with one sequence it is not specified whose rows
+ * A position before the sequence's first, without a page, or in a page that another
+ * sequence has too, is skipped and reported.  Of two entries with one sequence it is not specified whose rows
  * stay. */
 int accel_kv_append(int dev, void* stream, const accel_kv_cache_t* cache, int64_t layer,
                     const accel_tensor_t* k, const accel_tensor_t* v,
@@ -664,7 +664,7 @@ int accel_kv_append(int dev, void* stream, const accel_kv_cache_t* cache, int64_
  * skipped.  Parents are read as they were before the call.  A parent's slot
  * without a page (accel_kv_trim) has none in the branch.  Rows of positions that
  * a parent has reserved are appended before it branches: a later row of either
- * would be in a page that both have. */
+ * would be in a page that both have, where accel_kv_append stores nothing. */
 int accel_kv_fork(int dev, void* stream, const accel_kv_cache_t* cache,
                   const accel_tensor_t* parents, const accel_tensor_t* children);
 
@@ -818,7 +818,9 @@ int accel_tree_accept(int dev, void* stream, const accel_tensor_t* tokens,
  * positions than its sequence has, or with no page where a row moves; one that would
  * move a row into a page that another sequence has too; a sequence index outside the
  * cache; and one of two entries with one sequence (not specified which).
- * ACCEL_KV_NONE is skipped. */
+ * ACCEL_KV_NONE is skipped.  A sequence may be left with an end inside a page that
+ * another has too.  accel_kv_append stores nothing there: to grow, it branches
+ * (accel_kv_fork copies that page) and the branch goes on in its place. */
 int accel_kv_keep(int dev, void* stream, const accel_kv_cache_t* cache,
                   const accel_tensor_t* seqs, const accel_tensor_t* offsets,
                   const accel_tensor_t* path, const accel_tensor_t* counts);

@@ -67,7 +67,7 @@ class Pages:
             for t in range(offsets[i], min(offsets[i + 1], len(k))):
                 pos = int(self.lens[s]) - int(offsets[i + 1]) + t
                 page = self.tables[s, pos // self.page_size] if pos >= 0 else NONE
-                if page >= self.pages:
+                if page >= self.pages or self.refs[page] > 1:
                     self.left_out.append(t)
                     continue
                 self.keys[layer, page, :, pos % self.page_size] = k[t]

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import accel_amd
-from accel_amd import KV_NONE, NO_TOKEN
+from accel_amd import BF16, KV_NONE, NO_TOKEN
 from oracle import draft_np
 from test_gpu_draft import Keeps, run_accept
 from test_gpu_tree_attention import trees
@@ -50,3 +50,46 @@ def test_a_count_of_zero_takes_back_more_than_a_draft(dev):
     b.reserve([300, 257, 5])
     b.keep([[KV_NONE, 7], [0, 0], [3, 2]], [0, 0, 0], [300, 257, 5])
     assert b.m.lens.tolist() == [20, 30, 40]
+
+
+class Lives(Keeps):
+    def append(self, layer, new, seqs, rows):
+        off = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+        shape = (int(off[-1]), self.m.keys.shape[2], self.m.keys.shape[4])
+        k, v = (rows.integers(0, 1 << 14, shape).astype(np.uint16) for _ in range(2))
+        self.m.append(layer, k, v, seqs, off)
+        self.dev.KVAppend(self.c, layer, self.dev.upload(k, BF16), self.dev.upload(v, BF16),
+                          self.u32(seqs), self.u32(off))
+        self.settle()
+
+
+def test_a_shortened_sequence_does_not_write_over_its_branch(dev):
+    """A sequence that a keep ends inside a page that its branch has too: rows appended
+    there would be the branch's, so they are left out and reported, those of the next
+    pages and of other sequences stored.  As a branch of its own it grows."""
+    rng = np.random.default_rng(4)
+    b = Lives(dev, layers=2, pages=60, sequences=5, slots=9)
+    b.reserve([32, 0, 10, 0, 0])
+    b.fork([0], [1])
+    b.keep([[0]], [0], [13], [0])                    # 19 left: the third page is both's
+    assert b.m.lens.tolist() == [19, 32, 10, 0, 0]
+    b.reserve([11, 0, 3, 0, 0])
+    held = b.m.keys[:, b.m.tables[1, 2]].copy()
+    for layer in range(2):
+        b.m.left_out = []
+        b.append(layer, [11, 3], [0, 2], rng)
+    assert (b.m.keys[:, b.m.tables[1, 2]] == held).all()
+    # positions 24 to 29 lie in a page of its own
+    b.append(0, [6], [0], rng)
+    b.keep([[0]], [0], [11], [0])
+    b.fork([0], [3])
+    b.free([0])
+    b.reserve([0, 0, 0, 12, 0])
+    for layer in range(2):
+        b.append(layer, [12], [3], rng)
+    # and so does a sequence whose branch is gone
+    b.keep([[0]], [0], [5], [1])
+    b.fork([1], [4])
+    b.free([4])
+    b.reserve([0, 4, 0, 0, 0])
+    b.append(1, [4], [1], rng)
