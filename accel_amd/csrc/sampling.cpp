@@ -71,6 +71,9 @@ ACCEL_API int accel_sample(int dev, void* stream, const accel_tensor_t* logits,
             return rc;
     }
     if (rows && !logits->data) return refuse(op, "the logits are missing");
+    // rows are read in blocks of 16 bytes, from whichever of a block's numbers they begin at
+    if ((uintptr_t)logits->data % (logits->dtype == ACCEL_F32 ? 4 : 2))
+        return refuse(op, "the logits must start at an address aligned to their type");
     Device* d = device(dev);
     if (!d) return ACCEL_E_NO_DEVICE;
     if ((rc = begin_submission(d)) != ACCEL_OK || rows == 0) return rc;

@@ -774,8 +774,8 @@ typedef struct accel_sampling {
 /* What a row without a logit past -infinity gives. */
 #define ACCEL_NO_TOKEN 0xffffffffu
 
-/* A token of each row of logits [rows, width] (or [width]), f32, f16 or bf16.  A
- * row's logits are put in order, the larger first, of equal ones the lower index
+/* A token of each row of logits [rows, width] (or [width]), f32, f16 or bf16, at any
+ * address aligned to their type.  A row's logits are put in order, the larger first, of equal ones the lower index
  * first; logit x has the weight exp((x - the largest) / temperature).  top_k keeps
  * the first k; top_p of those the fewest first ones whose weights reach top_p of
  * theirs; min_p those whose weight is min_p or more (1 and more: those of weight 1).
