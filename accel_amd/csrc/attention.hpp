@@ -201,37 +201,6 @@ __device__ __forceinline__ Rows rows_of(const Attention& a, int i) {
     return {lo, hi > lo ? hi - lo : 0};
 }
 
-// The entries' tiles summed up, for more entries than a wave has lanes:
-// sums[i] = tiles of entries 0 .. i, of keys (tokens 0) or of so many of a
-// prompt's tokens.  One workgroup.
-__global__ __launch_bounds__(1024) void paged_sums_kernel(KvCache c, Attention a, uint32_t tokens,
-                                                          uint32_t* sums, uint32_t* fault) {
-    __shared__ uint32_t sh[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t carry = 0;
-    for (int base = 0; base < a.n; base += 1024) {
-        const int i = base + threadIdx.x;
-        uint32_t v = 0;
-        if (i < a.n)
-            v = tokens ? (rows_of(a, i).count + tokens - 1) / tokens
-                       : span_of(a, held_by(c, a, i, fault).len).tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t up = __shfl_up(v, d, 64);
-            if (lane >= d) v += up;
-        }
-        __syncthreads();
-        if (lane == 63) sh[wave] = v;
-        __syncthreads();
-        uint32_t before = carry;
-        for (int w = 0; w < 16; w++) {
-            before += w < wave ? sh[w] : 0u;
-            carry += sh[w];
-        }
-        if (i < a.n) sums[i] = before + v;
-    }
-}
-
 // Where the line of tiles is cut.  Up to 64 entries: what is known of an entry
 // is in the lane of its number, read once; more: in memory, the tiles summed up
 // by the launch before.
