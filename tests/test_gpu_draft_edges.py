@@ -8,7 +8,7 @@ import accel_amd
 from accel_amd import BF16, KV_NONE, NO_TOKEN
 from oracle import draft_np
 from test_gpu_draft import Keeps, run_accept
-from test_gpu_tree_attention import trees
+from test_gpu_tree_attention import Tree, trees
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,15 @@ def test_a_shortened_sequence_does_not_write_over_its_branch(dev):
     b.free([4])
     b.reserve([0, 4, 0, 0, 0])
     b.append(1, [4], [1], rng)
+
+
+@pytest.mark.parametrize("n", [1025, 2100, 4200])
+def test_more_drafts_than_a_pass_over_them(dev, n):
+    """Their steps are summed up 1024 at a time, and found again 64 ways a step: twice
+    past 4096."""
+    rng = np.random.default_rng(n)
+    new = [int(x) for x in rng.integers(0, 4, n)]
+    c = Tree(dev, [int(m + x) for m, x in zip(new, rng.integers(0, 12, n))], new, heads=2,
+             kv_heads=1, dim=16, page=8)
+    c.check()
+    c.check(window=5, sinks=1)
