@@ -78,7 +78,9 @@ __host__ __device__ inline int prompt_tokens(int group) { return kRows / prompt_
 // node sees the context and, of the nodes, those on its path to its root; it stands
 // for the position of its depth behind the context.  All rows see the same keys up
 // to the context's end, so only the tiles past it look at the paths: a bit for each
-// of up to kDraft nodes, made by a lane a node that walks up its parents in LDS.
+// of up to kDraft nodes, made by a lane a node that walks up its parents in LDS, two
+// dependent reads an ancestor (after 500, bf16, one chain of 64 nodes 30.7 us and a tree
+// of two to four children a node 22.6, of 256 nodes 67 and 29).
 constexpr int kDraft = ACCEL_DRAFT_NODES;
 struct Paths {
     // words of a node's bits, and as many past them as a tile reads; an odd stride,
@@ -139,8 +141,9 @@ __device__ __forceinline__ DraftPlace place_of(const Cut& k, const KvCache& c, c
 // A cut this near to a tile of rows' first or last step moves there: a piece of it costs
 // its queries' way in and its part's way out, some two steps.
 constexpr uint32_t kNearDraft = 2;
-// Steps that are worth a workgroup and a join (9 drafts of 1 to 100 nodes seen through a
-// window of 333, f16: 29.8 us with one, 24.4 with two, 31.0 with four).
+// Steps that are worth a workgroup and a join, measured with 1, 2, 3, 4 and 8: 9 drafts of
+// 1 to 100 nodes seen through a window of 333, f16, 30.1, 25.1, 25.1, 31.2 and 49.2 us; 8
+// nodes after 500, bf16, 17.6, 17.1, 18.5, 16.9 and 20.7.
 template <bool F32>
 constexpr uint32_t kLeastDraft = F32 ? 1 : 2;
 template <int KT>

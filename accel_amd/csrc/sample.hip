@@ -11,7 +11,10 @@
 // Sums over bins then say in which bins the borders of k, p, m and u lie.  Where those
 // hold up to 64 logits together, one more look gathers them, and a wave puts them in
 // order and finds the borders.  Otherwise the borders are found one by one, each bin
-// cut into 1024 by another histogram first if it holds more than 64.
+// cut into 1024 by another histogram first if it holds more than 64.  Rows past what
+// that serves (has_bins, kMostEach, kFew) go digit by digit of their keys, many passes of
+// one workgroup: a row of 128000 near 60 below zero at a temperature of 0.005 in 960 us,
+// 512 of them in 2000.
 //
 // Bins are absolute, not relative to the row's largest, so one pass is enough: a ring
 // of 1024 bins (64 factors of two), set by the first logits seen.  Weights below 2^-46
@@ -22,8 +25,9 @@
 // 3 TB/s; digit by digit of the keys, four looks a border, it was 1689).  A row's chain
 // after its pass, some 20 us of barriers and a look, no other workgroup fills where all
 // rows run at once.  For few rows that chain: one row of 128000 26 us, 64 of 100003 in
-// bf16 49; nearly flat ones, with hundreds of logits in a border's bin and another look a
-// border, 17 of 32001 in f16 51.
+// bf16 48 to 53; nearly flat ones, with hundreds of logits in a border's bin and another
+// look a border, 17 of 32001 in f16 51.  At a temperature of 0 only the largest is looked
+// for: 512 rows of 128000 in 63 us (4.2 TB/s), one in 12.
 #include <hip/hip_runtime.h>
 
 #include "internal.hpp"
@@ -1425,7 +1429,8 @@ hipError_t launch(Device* d, hipStream_t st, const Sampling& s, int* status) {
     // A row's workgroup takes 20 us and 1.45 a tile.  A workgroup a tile takes 24 to 27 us
     // whatever the width, as long as all run at once (rows of 16 tiles, us: one 43 whole
     // and 27 in parts, 16 46 and 32, 32 46 and 43, 64 48 and 71; of 8 tiles one 30 and 23;
-    // of 4 one 24 and 24, 32 26 and 26).
+    // of 4 one 24 and 24, 32 26 and 26).  Rows of more tiles than LDS has bytes for go in
+    // parts however many they are (bf16: 300 of 262144 724 us, 300 of 245000 whole 125).
     if (least <= 4 ||
         (least <= kTiles && (uint64_t)s.rows * least > 2 * (uint32_t)d->cu_count)) {
         // a grid's lanes are counted in 32 bits

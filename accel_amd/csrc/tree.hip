@@ -10,8 +10,11 @@
 //
 // What bounds it: issue, as the prompts (those trees run at 460 TFLOP/s, the prompts at
 // 600; 16 of 64 nodes after 4096 at 570, the keys' bytes are half of the time); for one
-// small tree the chain before its first keys (4.7 us), a busy wave's steps (2 us each) and
-// joins (4.2 each).
+// small tree a chain.  8 nodes after 56 positions, one step, are 10.7 us, each further
+// step of the one busy wave 1.4 to 1.5, a join 2.3 (8 steps, two pieces of four: 17.3).
+// Past 128 dims one workgroup a CU, and registers spill: 16 trees of 16 to 64 nodes after
+// 300 to 4000, 16/4 heads of 256 in bf16 104 us (32/8 heads of 128, as many products, 72),
+// in f32 214 over bf16 and 173 over f16 (106 and 103).
 // Tried and left: eight waves a workgroup, keys and values read once for up to 256 rows
 // (the batch above 217 us instead of 222 call upon call, 9 drafts seen through a window of
 // 333 28.6 instead of 24.7); three tiles of keys on their way instead of one (219 and 214);

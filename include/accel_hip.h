@@ -637,7 +637,10 @@ int accel_kv_clear(int dev, void* stream, const accel_kv_cache_t* cache);
  * entry for which the pool or the table has no room is left unchanged and
  * reported, and those after it are served as if it were not there; unchanged
  * and reported are also the second of two entries with one sequence and a
- * sequence index outside the cache.  ACCEL_KV_NONE is skipped. */
+ * sequence index outside the cache.  ACCEL_KV_NONE is skipped.  A step that goes
+ * on after such a report lays its rows over the last positions that a sequence
+ * left unchanged holds (accel_kv_append), and accel_kv_keep takes them back: such
+ * a sequence is freed and filled anew. */
 int accel_kv_reserve(int dev, void* stream, const accel_kv_cache_t* cache,
                      const accel_tensor_t* seqs, const accel_tensor_t* grow);
 
@@ -740,7 +743,8 @@ int accel_paged_prefill(int dev, void* stream, const accel_tensor_t* q,
  * from 0); parents (u32 [T]) gives each row's parent as a number in its entry,
  * below its own, or ACCEL_KV_NONE.  Their keys and values lie in the cache in
  * the rows' order, at the sequence's last m positions (accel_kv_reserve and
- * accel_kv_append put them there). */
+ * accel_kv_append put them there).  accel_kv_trim goes by the length, and nodes stand
+ * before the places where they lie: it is called after accel_kv_keep. */
 #define ACCEL_DRAFT_NODES 256
 
 /* Attention of drafts' nodes: node t of a sequence with L positions before its
@@ -783,9 +787,12 @@ typedef struct accel_sampling {
  * at which the weights' running sum passes u (f32 [rows], in [0, 1): what is outside,
  * or no number, counts as the nearest, 0) times the sum of all that are kept;
  * logprobs (f32 [rows], or NULL) is the logarithm of its weight's share of that sum.
- * Weights and sums are of 64 bits and do not depend on an order, so a call gives the
- * same tokens whatever runs beside it; a weight below 2^-46 of a row's largest may
- * count as 0 (rows of up to 2^17; a bit less a doubling past that).  A NaN counts
+ * Weights are right to 2^-38 of themselves and to 2^-46 of a row's largest (rows of up
+ * to 2^17; a bit less a doubling past that), below which they may count as 0; sums of
+ * them are of 64 bits and do not depend on an order, so a call gives the same tokens
+ * whatever runs beside it.  Rows whose largest logit is 5600 temperatures and more from
+ * zero, and those of more than 30000 logits within a 23rd of a temperature, take
+ * tens of times as long as others.  A NaN counts
  * as -infinity, which is never kept; of infinite logits each has the weight 1 and all
  * others 0.  Rows are independent of each other. */
 int accel_sample(int dev, void* stream, const accel_tensor_t* logits, const accel_tensor_t* u,
