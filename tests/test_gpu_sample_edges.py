@@ -6,8 +6,10 @@ import math
 import numpy as np
 import pytest
 
+import accel_amd
 from accel_amd import BF16, F16, F32
 from oracle import draft_np
+from test_gpu_kv_pages import narrow
 from test_gpu_sample import SETTINGS, check, draw, types
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +110,34 @@ def test_rows_of_millions(dev, dtype, opt):
         assert margin > slack
         assert got[r] == token
         assert abs(lp[r] - share) <= 2.0 ** -24 * abs(share) + 4 * slack
+
+
+@pytest.mark.parametrize("rows,width", [(260, 1 << 24), (140000, 32001)])
+def test_logits_past_32_bits(dev, rows, width):
+    """More than 2^32 logits, in parts and whole: the first and the last rows give what
+    they give alone, bit for bit (the others are whatever memory held, at a temperature of
+    0)."""
+    rng = np.random.default_rng(23)
+    some = [0, rows - 2, rows - 1]
+    x = (rng.standard_normal((3, width), np.float32) * 3).astype(np.float32)
+    u = rng.random(3).astype(np.float32)
+    kw = dict(temperature=[0.8, 0.8, 0.9], top_k=[40, 0, 0], top_p=[0.9, 1.0, 0.8])
+    want = draw(dev, x, u, BF16, **kw)
+    logits = dev.alloc((rows, width), BF16)
+    bits = narrow(x, BF16)
+    for i, r in enumerate(some):
+        accel_amd._check(accel_amd.lib().accel_hip_write(
+            dev.index, logits.ptr, r * width * 2, bits[i].ctypes.data, bits[i].nbytes))
+    full = {k: np.zeros(rows, np.float32) for k in ("u", "temperature", "top_p", "lp")}
+    full["top_k"], full["token"] = np.zeros(rows, np.uint32), np.zeros(rows, np.uint32)
+    full["u"][some] = u
+    for k, v in kw.items():
+        full[k][some] = v
+    b = {k: dev.upload(v) for k, v in full.items()}
+    dev.Sample(logits, b["u"], b["token"], b["lp"], temperature=b["temperature"],
+               top_k=b["top_k"], top_p=b["top_p"])
+    dev.sync()
+    assert np.array_equal(b["token"].numpy()[some], want[0])
+    assert np.array_equal(b["lp"].numpy()[some], want[1])
+    for x in [logits, *b.values()]:
+        x.free()
